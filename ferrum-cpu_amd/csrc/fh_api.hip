@@ -134,6 +134,10 @@ int fh_counter_area(fh_ctx* ctx, size_t bytes, void** out) {
     return zeroed_area(ctx, &ctx->counters, &ctx->counters_bytes, bytes, "the GEMM's per-tile counters", out);
 }
 
+int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out) {
+    return zeroed_area(ctx, &ctx->kv4, &ctx->kv4_bytes, bytes, "the 4-bit cache's workspace", out);
+}
+
 // Every entry point works on the context's device.
 // (hipSetDevice only when needed, so calls stay legal under stream capture.)
 static hipError_t on_device(int device) {
@@ -229,6 +233,7 @@ void fh_ctx_destroy(fh_ctx* ctx) {
     if (ctx->ws) (void)hipFree(ctx->ws);
     if (ctx->sync) (void)hipFree(ctx->sync);
     if (ctx->counters) (void)hipFree(ctx->counters);
+    if (ctx->kv4) (void)hipFree(ctx->kv4);
     if (ctx->act) (void)hipFree(ctx->act);
     if (ctx->io) (void)hipFree(ctx->io);
     if (ctx->pin) (void)hipHostFree(ctx->pin);
@@ -1009,6 +1014,152 @@ int fh_gqa_attention_rope_decode_async(fh_ctx* ctx, float* d_qkv, size_t ld, siz
     return fh_launch_gqa_attention_rope_decode(ctx, d_qkv, ld, rows, n_heads, n_kv, head_dim, d_k_cache, d_v_cache,
                                                capacity, d_pos, max_pos, rope_dim, base, rope_type, d_freq_factors,
                                                linear_factor, d_out);
+}
+
+// ---- the 4-bit cache -----------------------------------------------------------
+
+static int kv4_check_cache(fh_ctx* ctx, const std::string& who, const fh_kv4_cache* c) {
+    if (!c) return fh_fail(ctx, FH_ERR_INVALID, who + ": cache is NULL");
+    if (!c->k || !c->k_d || !c->v || !c->v_d) return fh_fail(ctx, FH_ERR_INVALID, who + ": a plane of the cache is NULL");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->k_d) |
+                           reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->v_d);
+    if (bits % 16 != 0) return fh_fail(ctx, FH_ERR_INVALID, who + ": a plane of the cache is not 16-byte aligned");
+    if (c->seqs == 0 || c->n_kv == 0) return fh_fail(ctx, FH_ERR_INVALID, who + ": the cache has no sequences or heads");
+    if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128)
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": head width " + std::to_string(c->head_dim) + " is not 32, 64 or 128");
+    if (c->capacity == 0 || c->capacity % 8 != 0)
+        return fh_fail(ctx, FH_ERR_INVALID,
+                       who + ": capacity " + std::to_string(c->capacity) + " is not a positive multiple of 8");
+    if (c->seqs > 65535 || c->n_kv > 65535 || c->capacity > 0x7FFFFF00u ||
+        c->seqs * c->n_kv > 0x7FFFFFFFu / (c->head_dim * 2) || c->seqs * c->n_kv * c->capacity > (size_t(1) << 36))
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": a dimension is too large");
+    return FH_OK;
+}
+
+// The rows' arguments; *max_rows becomes total / seqs where the sequences have equal parts.
+static int kv4_check_rows(fh_ctx* ctx, const std::string& who, const fh_kv4_cache* c, size_t ld, size_t heads_wide,
+                          size_t total, size_t n_heads, const uint32_t* off, size_t* max_rows) {
+    if (n_heads == 0 || n_heads % c->n_kv != 0)
+        return fh_fail(ctx, FH_ERR_DIM, "n_heads " + std::to_string(n_heads) + " must be a multiple of n_kv_heads " +
+                                            std::to_string(c->n_kv));
+    if (n_heads > 65535 || total > 0x7FFFFFFFu / n_heads)
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": a dimension is too large");
+    if (ld < heads_wide * c->head_dim)
+        return fh_fail(ctx, FH_ERR_DIM, who + ": ld is below the heads' " + std::to_string(heads_wide * c->head_dim) +
+                                            " floats");
+    if (!off) {
+        if (total % c->seqs != 0)
+            return fh_fail(ctx, FH_ERR_DIM, who + ": " + std::to_string(total) + " rows do not divide over " +
+                                                std::to_string(c->seqs) + " sequences");
+        *max_rows = total / c->seqs;
+    } else {
+        *max_rows = std::min(*max_rows, total);
+    }
+    return FH_OK;
+}
+
+int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_qkv, size_t ld, size_t total,
+                        size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                        const uint32_t* d_pos, size_t rope_dim, float base, int rope_type,
+                        const float* d_freq_factors, float linear_factor, float* d_q) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    int rc = kv4_check_cache(ctx, "fh_kv4_append", cache);
+    if (rc) return rc;
+    rc = kv4_check_rows(ctx, "fh_kv4_append", cache, ld, n_heads + 2 * cache->n_kv, total, n_heads, d_off, &max_rows);
+    if (rc) return rc;
+    if (rope_dim > cache->head_dim || rope_dim % 2 != 0)
+        return fh_fail(ctx, FH_ERR_DIM, "rope_dim " + std::to_string(rope_dim) + " must be even and \u2264 head_dim " +
+                                            std::to_string(cache->head_dim));
+    if (rope_dim && (!(linear_factor > 0.0f) || !std::isfinite(linear_factor)))
+        return fh_fail(ctx, FH_ERR_DIM, "RoPE scaling factors must be finite and > 0");
+    if (rope_dim && rope_type != FH_ROPE_NORM && rope_type != FH_ROPE_NEOX)
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_append: unknown rope_type " + std::to_string(rope_type));
+    if (total == 0 || max_rows == 0) return FH_OK;
+    if (!d_qkv) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_append: qkv is NULL");
+    if (d_q == d_qkv) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_append: q must not be qkv");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_kv4_append(ctx, *cache, d_qkv, ld, total, n_heads, d_off, max_rows, d_len, d_pos, rope_dim, base,
+                                rope_type, d_freq_factors, linear_factor, d_q);
+}
+
+static int kv4_check_score(fh_ctx* ctx, const std::string& who, const fh_attn_score* s) {
+    if (s && !(s->softcap >= 0.0f && std::isfinite(s->softcap)))
+        return fh_fail(ctx, FH_ERR_INVALID, who + ": softcap must be finite and not negative");
+    return FH_OK;
+}
+
+int fh_kv4_attention_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
+                           size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                           size_t max_keys, const fh_attn_score* score, float* d_out, float* d_lse) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    int rc = kv4_check_cache(ctx, "fh_kv4_attention", cache);
+    if (rc == FH_OK)
+        rc = kv4_check_rows(ctx, "fh_kv4_attention", cache, ld, n_heads, total, n_heads, d_off, &max_rows);
+    if (rc == FH_OK) rc = kv4_check_score(ctx, "fh_kv4_attention", score);
+    if (rc) return rc;
+    if (total == 0 || max_rows == 0) return FH_OK;
+    if (!d_q || !d_out) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_attention: q or out is NULL");
+    if (d_out == d_q) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_attention: out must not be q");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_kv4_attention(ctx, *cache, d_q, ld, total, n_heads, d_off, max_rows, d_len, max_keys, score,
+                                   d_out, d_lse);
+}
+
+int fh_kv4_weigh_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
+                       size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len, size_t max_keys,
+                       const fh_attn_score* score, const float* d_lse) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    int rc = kv4_check_cache(ctx, "fh_kv4_weigh", cache);
+    if (rc == FH_OK) rc = kv4_check_rows(ctx, "fh_kv4_weigh", cache, ld, n_heads, total, n_heads, d_off, &max_rows);
+    if (rc == FH_OK) rc = kv4_check_score(ctx, "fh_kv4_weigh", score);
+    if (rc) return rc;
+    if (!cache->weight) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_weigh: the cache has no weight plane");
+    if (total == 0 || max_rows == 0 || max_keys == 0) return FH_OK;
+    if (!d_q || !d_lse) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_weigh: q or lse is NULL");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_kv4_weigh(ctx, *cache, d_q, ld, total, n_heads, d_off, max_rows, d_len, max_keys, score, d_lse);
+}
+
+int fh_kv4_evict_async(fh_ctx* ctx, const fh_kv4_cache* src, const fh_kv4_cache* dst, const uint32_t* d_len,
+                       size_t max_len, size_t keep, size_t recent, uint32_t* d_new_len) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    int rc = kv4_check_cache(ctx, "fh_kv4_evict", src);
+    if (rc == FH_OK) rc = kv4_check_cache(ctx, "fh_kv4_evict", dst);
+    if (rc) return rc;
+    if (src->seqs != dst->seqs || src->n_kv != dst->n_kv || src->head_dim != dst->head_dim)
+        return fh_fail(ctx, FH_ERR_DIM, "fh_kv4_evict: the caches differ in sequences, heads or head width");
+    if (keep > dst->capacity)
+        return fh_fail(ctx, FH_ERR_DIM, "fh_kv4_evict: keep " + std::to_string(keep) + " is above the capacity " +
+                                            std::to_string(dst->capacity) + " of the cache written to");
+    if (keep == 0 || recent > keep)
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_evict: keep must be positive and recent at most keep");
+    if (!src->weight) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_evict: the cache has no weight plane");
+    if (!d_len || !d_new_len) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_evict: len or new_len is NULL");
+    if (src->k == dst->k || src->v == dst->v || src->k_d == dst->k_d || src->v_d == dst->v_d ||
+        src->weight == dst->weight || (src->pos && src->pos == dst->pos))
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_evict: the caches share a plane");
+    if (src->seqs * src->n_kv * ((keep + 63) / 64) > 0x7FFFFFFFu)
+        return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_evict: more than 2^31 - 1 workgroups");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_kv4_evict(ctx, *src, *dst, d_len, max_len, keep, recent, d_new_len);
+}
+
+int fh_kv4_read_async(fh_ctx* ctx, const fh_kv4_cache* cache, const uint32_t* d_first, size_t rows, float* d_k,
+                      float* d_v) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    const int rc = kv4_check_cache(ctx, "fh_kv4_read", cache);
+    if (rc) return rc;
+    if (rows == 0) return FH_OK;
+    if (!d_k || !d_v) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_read: k or v is NULL");
+    if (rows > 0x7FFFFFFFu || cache->seqs * cache->n_kv * rows > (size_t(1) << 32))
+        return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_read: more than 2^32 head rows");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_kv4_read(ctx, *cache, d_first, rows, d_k, d_v);
 }
 
 int fh_swiglu_async(fh_ctx* ctx, const float* d_g, const float* d_u, size_t rows, size_t n, size_t ld, float* d_out) {

@@ -37,6 +37,10 @@ struct fh_ctx {
     // generation tags there must never be reset behind its back.
     void* counters = nullptr;
     size_t counters_bytes = 0;
+    // The 4-bit cache's attention: arrival counters (left at zero) and partial
+    // sums of keys split over workgroups.  Allocated once, at its only size.
+    void* kv4 = nullptr;
+    size_t kv4_bytes = 0;
     // Grow-on-demand activation staging (a LayerNorm output feeding a
     // linear), separate from ws, which the linear itself may use.
     void* act = nullptr;
@@ -113,6 +117,8 @@ int fh_act_area(fh_ctx* ctx, size_t bytes, void** out);
 int fh_sync_area(fh_ctx* ctx, size_t bytes, void** out);
 // The same for ctx->counters.
 int fh_counter_area(fh_ctx* ctx, size_t bytes, void** out);
+// The same for ctx->kv4.
+int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out);
 // Round up to a multiple of 256 bytes.
 static inline size_t fh_align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -233,6 +239,19 @@ int fh_launch_rope(fh_ctx* ctx, float* x, size_t rows, size_t ld, size_t n_heads
 int fh_launch_swiglu(fh_ctx* ctx, const float* g, const float* u, size_t rows, size_t n, size_t ld, float* out);
 int fh_launch_embed_rows(fh_ctx* ctx, const float* tok_w, size_t vocab, size_t d, const uint32_t* tokens, size_t rows,
                          float* out);
+// The 4-bit cache (fh_kv4.hip), arguments as the entry points' and checked there.
+int fh_launch_kv4_append(fh_ctx* ctx, const fh_kv4_cache& c, const float* qkv, size_t ld, size_t total, size_t n_heads,
+                         const uint32_t* off, size_t max_rows, const uint32_t* len, const uint32_t* pos,
+                         size_t rope_dim, float base, int rope_type, const float* ff, float linear, float* q);
+int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size_t ld, size_t total, size_t n_heads,
+                            const uint32_t* off, size_t max_rows, const uint32_t* len, size_t max_keys,
+                            const fh_attn_score* sc, float* out, float* lse);
+int fh_launch_kv4_weigh(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size_t ld, size_t total, size_t n_heads,
+                        const uint32_t* off, size_t max_rows, const uint32_t* len, size_t max_keys,
+                        const fh_attn_score* sc, const float* lse);
+int fh_launch_kv4_read(fh_ctx* ctx, const fh_kv4_cache& c, const uint32_t* first, size_t rows, float* k, float* v);
+int fh_launch_kv4_evict(fh_ctx* ctx, const fh_kv4_cache& src, const fh_kv4_cache& dst, const uint32_t* len,
+                        size_t max_len, size_t keep, size_t recent, uint32_t* new_len);
 int fh_launch_dequant(fh_ctx* ctx, const uint8_t* raw, size_t n, float* out);
 int fh_launch_block_dots(fh_ctx* ctx, const fh_q8_0* w, const int8_t* qx, size_t m,
                          int32_t* dots);

@@ -57,6 +57,7 @@ EXPORTS = (
     "fh_gguf_tensor_info", "fh_gguf_tensor_data", "fh_gguf_meta_type", "fh_gguf_meta_u64", "fh_gguf_meta_f64",
     "fh_gguf_meta_str", "fh_gguf_meta_array_data", "fh_gguf_read_f32", "fh_gguf_upload_q8_0",
     "fh_qweight_upload", "fh_qweight_free", "fh_qlinear_async",
+    "fh_kv4_append_async", "fh_kv4_attention_async", "fh_kv4_weigh_async", "fh_kv4_evict_async", "fh_kv4_read_async",
 )
 
 
@@ -127,6 +128,47 @@ class GPT2Block(C.Structure):
 
     _fields_ = [(n, C.c_void_p) for n in ("qkv", "out", "up", "down", "qkv_b", "out_b", "up_b", "down_b", "ln1_g",
                                            "ln1_b", "ln2_g", "ln2_b", "k_cache", "v_cache")]
+
+
+class KV4Cache(C.Structure):
+    """fh_kv4_cache: the device planes of one layer's 4-bit key/value cache for
+    `seqs` sequences (their layout: include/ferrum_hip.h).  The planes are torch
+    tensors (kept alive here) or device addresses; pos and weight may be None.
+    KV4Cache.alloc makes the planes."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k", "k_d", "v", "v_d", "pos", "weight")] + \
+        [(n, C.c_size_t) for n in ("seqs", "n_kv", "head_dim", "capacity")]
+
+    def __init__(self, seqs: int, n_kv: int, head_dim: int, capacity: int, k, k_d, v, v_d, pos=None, weight=None):
+        planes = (k, k_d, v, v_d, pos, weight)
+        super().__init__(*(_ptr(p) for p in planes), seqs, n_kv, head_dim, capacity)
+        self.planes = dict(zip(("k", "k_d", "v", "v_d", "pos", "weight"), planes))
+
+    @classmethod
+    def alloc(cls, seqs: int, n_kv: int, head_dim: int, capacity: int, tracked: bool = False) -> "KV4Cache":
+        """Zeroed planes of at least `capacity` positions (rounded up to a
+        multiple of 8); tracked: with the pos and weight planes."""
+        import torch
+
+        cap = -(-capacity // 8) * 8
+        zeros = lambda dt, *shape: torch.zeros((seqs, n_kv, *shape), dtype=dt, device="cuda")  # noqa: E731
+        levels = lambda: zeros(torch.uint8, cap * head_dim // 2)  # noqa: E731
+        scales = lambda: zeros(torch.float16, cap // 8, head_dim // 32, 8)  # noqa: E731
+        return cls(seqs, n_kv, head_dim, cap, levels(), scales(), levels(), scales(),
+                   zeros(torch.int32, cap) if tracked else None, zeros(torch.float32, cap) if tracked else None)
+
+
+class AttnScore(C.Structure):
+    """fh_attn_score: score options of the 4-bit cache's attention.  softcap > 0
+    caps scores with a tanh; slopes [n_heads] subtracts slope * distance (the rows'
+    positions: pos [total], None = their cache rows); row r sees cache rows
+    first[r] <= j < end[r] (None: 0 and its own + 1).  Tensors are kept alive here."""
+
+    _fields_ = [("softcap", C.c_float)] + [(n, C.c_void_p) for n in ("slopes", "pos", "first", "end")]
+
+    def __init__(self, softcap: float = 0.0, slopes=None, pos=None, first=None, end=None):
+        super().__init__(float(softcap), _ptr(slopes), _ptr(pos), _ptr(first), _ptr(end))
+        self.tensors = (slopes, pos, first, end)
 
 
 _lib = None
@@ -234,6 +276,12 @@ def lib():
         L.fh_qweight_free.argtypes = [vp]
         L.fh_qweight_free.restype = None
         L.fh_qlinear_async.argtypes = [vp, vp, vp, sz, sz, vp, sz, vp]
+        kv, sc = C.POINTER(KV4Cache), C.POINTER(AttnScore)
+        L.fh_kv4_append_async.argtypes = [vp, kv, vp, sz, sz, sz, vp, sz, vp, vp, sz, f32, i32, vp, f32, vp]
+        L.fh_kv4_attention_async.argtypes = [vp, kv, vp, sz, sz, sz, vp, sz, vp, sz, sc, vp, vp]
+        L.fh_kv4_weigh_async.argtypes = [vp, kv, vp, sz, sz, sz, vp, sz, vp, sz, sc, vp]
+        L.fh_kv4_evict_async.argtypes = [vp, kv, kv, vp, sz, sz, sz, vp]
+        L.fh_kv4_read_async.argtypes = [vp, kv, vp, sz, vp, vp]
         _lib = L
     return _lib
 
@@ -1104,6 +1152,47 @@ def gqa_attention_rope_decode_async(ctx: Context, qkv, ld: int, rows: int, n_hea
                                                        _ptr(k_cache), _ptr(v_cache), capacity, _ptr(pos), max_pos,
                                                        rope_dim, base, rope_type, _ptr(freq_factors), linear_factor,
                                                        _ptr(out)))
+
+
+def kv4_append_async(ctx: Context, cache: KV4Cache, qkv, ld: int, total: int, n_heads: int, off, max_rows: int, len_,
+                     pos=None, rope_dim: int = 0, base: float = 10000.0, rope_type: int = ROPE_NEOX, freq_factors=None,
+                     linear_factor: float = 1.0, q=None):
+    """Appends `total` rows of q|k|v to a 4-bit cache: q and k rotated (rope_dim >
+    0) at pos, k and v quantised to cache rows len_[s] + t, the rotated q to q
+    [total, n_heads * head_dim].  Sequence s has rows off[s] .. off[s + 1] - 1
+    (off None: total / seqs each)."""
+    ctx.check(lib().fh_kv4_append_async(ctx.h, cache, _ptr(qkv), ld, total, n_heads, _ptr(off), max_rows, _ptr(len_),
+                                        _ptr(pos), rope_dim, base, rope_type, _ptr(freq_factors), linear_factor,
+                                        _ptr(q)))
+
+
+def kv4_attention_async(ctx: Context, cache: KV4Cache, q, ld: int, total: int, n_heads: int, off, max_rows: int, len_,
+                        max_keys: int, score, out, lse=None):
+    """Attention of appended rows over a 4-bit cache, single tokens or prompts:
+    out [total, n_heads * head_dim], and with lse [total, n_heads] the log-sum-exp
+    of each row's scores.  score: an AttnScore or None.  max_keys bounds the cache
+    rows in use, the call's own rows included."""
+    ctx.check(lib().fh_kv4_attention_async(ctx.h, cache, _ptr(q), ld, total, n_heads, _ptr(off), max_rows, _ptr(len_),
+                                           max_keys, score, _ptr(out), _ptr(lse)))
+
+
+def kv4_weigh_async(ctx: Context, cache: KV4Cache, q, ld: int, total: int, n_heads: int, off, max_rows: int, len_,
+                    max_keys: int, score, lse):
+    """Adds each key's attention weight from these rows to the cache's weight
+    plane; the arguments and lse of the kv4_attention_async call before it."""
+    ctx.check(lib().fh_kv4_weigh_async(ctx.h, cache, _ptr(q), ld, total, n_heads, _ptr(off), max_rows, _ptr(len_),
+                                       max_keys, score, _ptr(lse)))
+
+
+def kv4_evict_async(ctx: Context, src: KV4Cache, dst: KV4Cache, len_, max_len: int, keep: int, recent: int, new_len):
+    """Writes to dst what stays of src: per kv head, of a sequence longer than
+    `keep`, the last `recent` rows and the heaviest others, in order."""
+    ctx.check(lib().fh_kv4_evict_async(ctx.h, src, dst, _ptr(len_), max_len, keep, recent, _ptr(new_len)))
+
+
+def kv4_read_async(ctx: Context, cache: KV4Cache, first, rows: int, k, v):
+    """Cache rows first[s] .. + rows - 1 as f32, in the f32 cache's layout."""
+    ctx.check(lib().fh_kv4_read_async(ctx.h, cache, _ptr(first), rows, _ptr(k), _ptr(v)))
 
 
 def swiglu_async(ctx: Context, g, u, rows: int, n: int, ld: int, out):

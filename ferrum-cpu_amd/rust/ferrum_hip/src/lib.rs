@@ -46,6 +46,31 @@ pub mod sys {
     pub struct fh_qweight {
         _p: [u8; 0],
     }
+    /// A 4-bit key/value cache's device planes (include/ferrum_hip.h has their layout).
+    #[repr(C)]
+    #[derive(Clone, Copy)]
+    pub struct fh_kv4_cache {
+        pub k: *mut u8,
+        pub k_d: *mut u16,
+        pub v: *mut u8,
+        pub v_d: *mut u16,
+        pub pos: *mut u32,
+        pub weight: *mut f32,
+        pub seqs: usize,
+        pub n_kv: usize,
+        pub head_dim: usize,
+        pub capacity: usize,
+    }
+    /// Score options of `fh_kv4_attention_async`.
+    #[repr(C)]
+    #[derive(Clone, Copy)]
+    pub struct fh_attn_score {
+        pub softcap: f32,
+        pub d_slopes: *const f32,
+        pub d_pos: *const u32,
+        pub d_first: *const u32,
+        pub d_end: *const u32,
+    }
     #[repr(C)]
     pub struct fh_gguf {
         _p: [u8; 0],
@@ -145,6 +170,11 @@ pub mod sys {
         pub fn fh_rope_async(ctx: *mut fh_ctx, d_x: *mut f32, rows: usize, ld: usize, n_heads: usize, head_dim: usize, rope_dim: usize, d_pos: *const u32, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32) -> c_int;
         pub fn fh_gqa_attention_decode_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, rows: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, capacity: usize, d_pos: *const u32, max_pos: usize, d_out: *mut f32) -> c_int;
         pub fn fh_gqa_attention_rope_decode_async(ctx: *mut fh_ctx, d_qkv: *mut f32, ld: usize, rows: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, capacity: usize, d_pos: *const u32, max_pos: usize, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
+        pub fn fh_kv4_append_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_q: *mut f32) -> c_int;
+        pub fn fh_kv4_attention_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_q: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, score: *const fh_attn_score, d_out: *mut f32, d_lse: *mut f32) -> c_int;
+        pub fn fh_kv4_weigh_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_q: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, score: *const fh_attn_score, d_lse: *const f32) -> c_int;
+        pub fn fh_kv4_evict_async(ctx: *mut fh_ctx, src: *const fh_kv4_cache, dst: *const fh_kv4_cache, d_len: *const u32, max_len: usize, keep: usize, recent: usize, d_new_len: *mut u32) -> c_int;
+        pub fn fh_kv4_read_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_first: *const u32, rows: usize, d_k: *mut f32, d_v: *mut f32) -> c_int;
         pub fn fh_swiglu_async(ctx: *mut fh_ctx, d_g: *const f32, d_u: *const f32, rows: usize, n: usize, ld: usize, d_out: *mut f32) -> c_int;
         pub fn fh_embed_rows_async(ctx: *mut fh_ctx, d_tok_w: *const f32, vocab: usize, d: usize, d_tokens: *const u32, rows: usize, d_out: *mut f32) -> c_int;
         pub fn fh_embed_rows_pos_async(ctx: *mut fh_ctx, d_token_w: *const f32, d_pos_w: *const f32, vocab: usize, max_seq: usize, d: usize, d_tokens: *const u32, d_pos: *const u32, rows: usize, d_hist: *mut u32, hist_stride: usize, d_out: *mut f32) -> c_int;

@@ -435,6 +435,109 @@ int fh_attention_prefill_seqs_async(fh_ctx* ctx, const float* d_qkv, float* d_k_
                                     size_t seq_stride, size_t capacity, size_t d, size_t heads, size_t pos0,
                                     size_t rows, size_t seqs, float* d_out);
 
+/* ---- a key/value cache held in 4 bits ----------------------------------------
+ * KvCache (layer/transformer.rs:15-56) and Attention::forward_one (llm.rs:285-358)
+ * with keys and values in 4 bits: 0.5625 bytes a channel where the f32 cache
+ * takes 4.  No reference counterpart for the format, the score options, the
+ * weights and the eviction.
+ *
+ * A block of 32 channels x of one head row is a scale d and 32 levels: with m
+ * the first channel of largest magnitude, d = f16(m / -8) (finite values beyond
+ * f16 get +-65504; a block with an infinity or NaN gets d = NaN), levels
+ * clamp(rint(x / d), -8, 7) + 8 with ties to even, 8 where d = 0; the block
+ * stands for d * (level - 8).
+ *
+ * The planes of one layer's cache, in the caller's device memory.  For each
+ * (sequence, kv head), sequence-major, `capacity` positions (a multiple of 8):
+ *   k    head_dim / 2 bytes a position: word (g, b), g < 4, b < head_dim / 32, at
+ *        word g * head_dim / 32 + b holds channel 32 b + 8 g + i in bits 4i;
+ *   v    2-byte units [position / 8][n][p][position % 8]: head_dim >= 64: n < 16,
+ *        p < head_dim / 64, bits 8h + 4e are channel 64 p + 32 h + 2 n + e;
+ *        head_dim 32: n < 8, no p, bits 8h + 4e are channel 16 h + 2 n + e;
+ *   k_d, v_d  f16 [position / 8][block][position % 8];
+ *   pos    nullable: each key's position in its text, [capacity] u32 (NULL: its
+ *        cache row; they differ once rows have been evicted);
+ *   weight nullable: the attention weight each key has drawn so far, [capacity].
+ * k, k_d, v and v_d are 16-byte aligned.  head_dim 32, 64 or 128, else FH_ERR_LIMIT.
+ * Rows that no call has appended may hold anything. */
+typedef struct {
+    uint8_t* k;
+    uint16_t* k_d;
+    uint8_t* v;
+    uint16_t* v_d;
+    uint32_t* pos;
+    float* weight;
+    size_t seqs, n_kv, head_dim, capacity;
+} fh_kv4_cache;
+/* Score options of fh_kv4_attention_async, all nullable / off at zero.  With x the
+ * scaled score of a query row and a key:
+ *   softcap > 0: x = softcap * tanh(x / softcap);
+ *   d_slopes [n_heads]: x - slope * |position of the row - position of the key|,
+ *     the row's from d_pos [total] (NULL: its cache row), the key's from the
+ *     cache's pos;
+ *   d_first, d_end [total]: the row sees cache rows first <= j < end, cut to the
+ *     rows that are there (NULL: 0, and the row's own cache row + 1).  A document
+ *     mask is first = its document's start; a sliding window of w, first = row + 1 -
+ *     w; a prefix whose rows see each other, end = max(row + 1, the prefix's end). */
+typedef struct {
+    float softcap;
+    const float* d_slopes;
+    const uint32_t* d_pos;
+    const uint32_t* d_first;
+    const uint32_t* d_end;
+} fh_attn_score;
+/* Rows of these calls.  `total` rows belong to the cache's sequences: rows d_off[s]
+ * .. d_off[s + 1] - 1 to sequence s (d_off [seqs + 1], at most max_rows rows each;
+ * rows past that and rows outside all sequences are left as they are), or with
+ * d_off NULL total / seqs to each, in order.  d_len [seqs] (NULL: 0) is the number of
+ * cache rows in use before them: row t of sequence s is cache row d_len[s] + t.  A
+ * decode step is one row per sequence, a prompt many. */
+/* Appends the rows' keys and values: d_qkv row r is [q (n_heads heads) | k (n_kv) |
+ * v (n_kv)] at r * ld.  rope_dim > 0 rotates q and k first, as fh_rope_async does
+ * (the same angles; sine, cosine and products in 64 bits, so within an f32
+ * rounding of it) at position d_pos[r] (NULL: the cache row).  q goes to d_q [total,
+ * n_heads * head_dim] (NULL: nowhere); d_qkv is left as it is.  The cache's pos
+ * and weight rows are set to the position and 0.  Rows that would lie past the
+ * capacity are not stored.  Errors as fh_rope_async's and
+ * fh_gqa_attention_decode_async's. */
+int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_qkv, size_t ld, size_t total,
+                        size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                        const uint32_t* d_pos, size_t rope_dim, float base, int rope_type,
+                        const float* d_freq_factors, float linear_factor, float* d_q);
+/* Attention of the rows (already appended) over the cache: query head h of row r
+ * at d_q + r * ld + h * head_dim, with kv head h / (n_heads / n_kv), scale
+ * 1 / sqrt(head_dim), softmax over the keys it sees.  d_out [total, n_heads *
+ * head_dim]; d_lse (nullable) [total, n_heads] gets the log of the sum of
+ * exp(score).  A row that sees nothing gets 0 and -inf.  max_keys bounds the cache
+ * rows in use after the call's rows (it sizes the launch); a row whose cache row is at or past
+ * max_keys or the capacity gets NaN.  Within 1e-5 of float64 over the cache's
+ * values.  The context's workspace for it is allocated once and never moves;
+ * calls of one context must not overlap, replayed graphs included. */
+int fh_kv4_attention_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
+                           size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                           size_t max_keys, const fh_attn_score* score, float* d_out, float* d_lse);
+/* Adds to the cache's weight of every key what the rows' query heads gave it:
+ * exp(score - lse) over rows and heads of its kv head, d_lse as
+ * fh_kv4_attention_async wrote it for the same arguments. */
+int fh_kv4_weigh_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
+                       size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len, size_t max_keys,
+                       const fh_attn_score* score, const float* d_lse);
+/* Cuts every (sequence, kv head) of src whose sequence has more than `keep` rows
+ * (d_len [seqs], cut to max_len and the capacity) to the last `recent` and the
+ * (keep - recent) of largest weight among the others (equal weights: the first; a
+ * NaN counts as largest), and writes the rows that stay, in order, to dst, whose
+ * rows from there on are left as they are; shorter sequences are copied.  dst is
+ * another cache of the same seqs, n_kv and head_dim with capacity >= keep; its pos
+ * and weight planes, where it has them, get src's.  d_new_len [seqs] (it may be
+ * d_len) gets min(length, keep). */
+int fh_kv4_evict_async(fh_ctx* ctx, const fh_kv4_cache* src, const fh_kv4_cache* dst, const uint32_t* d_len,
+                       size_t max_len, size_t keep, size_t recent, uint32_t* d_new_len);
+/* Cache rows d_first[s] (NULL: 0) .. + rows - 1 of every sequence as f32, in the f32
+ * caches' layout: d_k, d_v [seqs, rows, n_kv * head_dim].  Rows past the capacity
+ * are NaN. */
+int fh_kv4_read_async(fh_ctx* ctx, const fh_kv4_cache* cache, const uint32_t* d_first, size_t rows, float* d_k,
+                      float* d_v);
+
 /* ---- a batched decode step's residual adds and norms, fused into the linears ---
  * The block of forward_with_cache (layer/transformer.rs:221-294; Llama:
  * LlamaBlock::forward_one, llm.rs:445-456) adds each projection to the

@@ -1,0 +1,664 @@
+"""The 4-bit key/value cache (fh_kv4_*) against its definitions in float64
+(kv4_ref): the bytes that append writes, attention for single tokens and prompts
+under every score option, the weights, the eviction, and their refusals."""
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(4, 4, 32), (14, 2, 64), (12, 12, 64), (32, 8, 128), (40, 2, 64), (5, 1, 128)]
+
+
+def gpu(a, dtype=None):
+    import torch
+
+    return torch.from_numpy(np.ascontiguousarray(a if dtype is None else np.asarray(a, dtype))).cuda()
+
+
+def ints(values):
+    return gpu(np.asarray(values, np.uint32).view(np.int32))
+
+
+class Box:
+    """A cache whose unused rows hold the worst that memory can: NaN and huge
+    scales.  Rows below `lens` hold quantised normals, kept here as float64."""
+
+    def __init__(self, seqs, n_kv, hd, cap, lens, seed, tracked=False, k_std=1.0, v_std=1.0):
+        import ferrum_hip
+        import torch
+
+        rng = np.random.default_rng(seed)
+        self.seqs, self.n_kv, self.hd, self.cap, self.lens = seqs, n_kv, hd, cap, list(lens)
+        nb = hd // 32
+        kp, vp = (rng.integers(0, 256, (seqs, n_kv, cap * hd // 2), dtype=np.uint8) for _ in range(2))
+        junk = np.array([0x7E00, 0x7BFF, 0xFC00, 0xFBFF, 0x7C00, 0xFE01], np.uint16)
+        kd, vd = (rng.choice(junk, (seqs, n_kv, cap // 8, nb, 8)).view(np.float16) for _ in range(2))
+        self.k, self.v = (np.zeros((seqs, n_kv, cap, hd)) for _ in range(2))
+        self.vstep = np.zeros((seqs, n_kv, cap, hd))
+        self.kstep = np.zeros((seqs, n_kv, cap, hd))
+        for s in range(seqs):
+            n = min(self.lens[s], cap)
+            for h in range(n_kv):
+                for plane, sc, val, std, step, isv in ((kp, kd, self.k, k_std, self.kstep, False),
+                                                       (vp, vd, self.v, v_std, self.vstep, True)):
+                    x = (rng.standard_normal((n, hd)) * std * np.exp(0.3 * rng.standard_normal(hd))).astype(np.float32)
+                    d, q = ref.quantise(x)
+                    new, nd = ref.pack(d, q, cap, isv)
+                    key, ch = np.arange(n), np.arange(nb)
+                    val[s, h, :n] = ref.values(d, q)
+                    step[s, h, :n] = np.abs(np.repeat(d.astype(np.float64), 32, axis=1))
+                    sc[s, h][key[:, None] // 8, ch[None], key[:, None] % 8] = d
+                    if isv:  # (positions share no byte, but an octet's bytes interleave)
+                        used = np.zeros(cap * hd // 2, bool)
+                        one = np.full((n, hd), 15, np.uint8)
+                        used = ref.pack(d, one, cap, True)[0] != 0
+                        plane[s, h][used] = new[used]
+                    else:
+                        plane[s, h, :n * hd // 2] = new[:n * hd // 2]
+        self.pos = np.tile(np.arange(cap, dtype=np.int32), (seqs, n_kv, 1)) if tracked else None
+        self.weight = rng.random((seqs, n_kv, cap)).astype(np.float32) if tracked else None
+        planes = [gpu(kp), gpu(kd), gpu(vp), gpu(vd)]
+        self.c = ferrum_hip.KV4Cache(seqs, n_kv, hd, cap, *planes, gpu(self.pos) if tracked else None,
+                                     gpu(self.weight) if tracked else None)
+        torch.cuda.synchronize()
+
+    def plane(self, name):
+        p = self.c.planes[name]
+        return None if p is None else p.cpu().numpy()
+
+
+def rows_of(lens, news):
+    off = np.concatenate([[0], np.cumsum(news)])
+    return off, [(s, off[s] + t, lens[s] + t, t) for s in range(len(news)) for t in range(news[s])]
+
+
+def check_attention(box, q, lens, news, out, lse, first=None, end=None, softcap=0.0, slopes=None, qpos=None,
+                    weight=None):
+    """Each output within its own bound.  With a_j = sum_c |q_c| 8 step_jc / sqrt(hd) (what
+    a score's partial sums can reach; plus the distance term, plus the cap) a score has at
+    most 8 roundings of 2^-24 of a_j, so a weight is off by 2^-21 a_j and, with the
+    normaliser, an output by 2^-21 sum_j p_j (a_j + mean a) 8 step_j; the weights' own
+    roundings (exp2 2^-23, scale 2^-24, two f16 terms 2^-22) and the sums' (4 a tile of at
+    most twice the mass; 64 tiles add up as sqrt) give 2^-18 of the mass sum_j p_j 8 step_j."""
+    n_heads, hd = q.shape[1], q.shape[2]
+    group = n_heads // box.n_kv
+    total_w = np.zeros((box.seqs, box.n_kv, box.cap))
+    tol_w = np.zeros_like(total_w)
+    _, places = rows_of(lens, news)
+    for s, row, at, t in places:
+        keys = min(lens[s] + news[s], box.cap)
+        lo = 0 if first is None else int(first[row])
+        hi = min(at + 1 if end is None else int(end[row]), keys)
+        if at >= keys:
+            assert np.isnan(out[row]).all() and (lse is None or np.isnan(lse[row]).all())
+            continue
+        kp = None if box.pos is None else box.pos[s].astype(np.int64)
+        o, z, w = ref.attention(q[row:row + 1], box.k[s], box.v[s], [lo], [hi], softcap, slopes,
+                                None if slopes is None else [at if qpos is None else qpos[row]], kp)
+        if lo >= hi:
+            assert (out[row] == 0).all() and (lse is None or (lse[row] == -np.inf).all())
+            continue
+        for h in range(n_heads):
+            g, qa = h // group, np.abs(q[row, h]).astype(np.float64)
+            a = 8 * box.kstep[s, g, lo:hi] @ qa / np.sqrt(hd)
+            score = box.k[s, g, lo:hi] @ q[row, h].astype(np.float64) / np.sqrt(hd)
+            if softcap:
+                score = softcap * np.tanh(score / softcap)
+                a = a + softcap * (np.abs(score) > 0.4 * softcap) + np.abs(score)
+            if slopes is not None:
+                here = np.arange(lo, hi) if kp is None else kp[g, lo:hi]
+                far = slopes[h] * np.abs((at if qpos is None else int(qpos[row])) - here)
+                score, a = score - far, a + np.abs(far)
+            p = np.exp(score - z[0, h])
+            abar = (p * a).sum()
+            mass = p @ (8 * box.vstep[s, g, lo:hi])
+            tol = 2.0 ** -21 * ((p * (a + abar)) @ (8 * box.vstep[s, g, lo:hi])) + 2.0 ** -18 * mass
+            err = np.abs(out[row, h] - o[0, h])
+            assert (err <= tol).all(), (s, row, h, float((err / tol).max()))
+            if lse is not None:
+                assert abs(lse[row, h] - z[0, h]) <= 2.0 ** -21 * abar + 2.0 ** -20 * (1 + abs(z[0, h]))
+            total_w[s, g, lo:hi] += p
+            tol_w[s, g, lo:hi] += p * (2.0 ** -21 * (a + abar) + 2.0 ** -20 * (1 + abs(z[0, h])))
+    if weight is not None:
+        want = box.weight.astype(np.float64) + total_w
+        # (one rounding of the stored sum, sqrt(columns) of the columns' own)
+        tol = tol_w + 2.0 ** -21 * total_w + 2.0 ** -23 * want
+        assert (np.abs(weight - want) <= tol).all(), float((np.abs(weight - want) / np.maximum(tol, 1e-300)).max())
+
+
+def attend(fh, box, n_heads, lens, news, seed, use_off, masks=None, softcap=0.0, slopes=None, qpos=None, weigh=False,
+           max_keys=None, ld_pad=0, tail=0):
+    import ferrum_hip
+    import torch
+
+    rng = np.random.default_rng(seed)
+    total, hd = sum(news) + tail, box.hd
+    q = rng.standard_normal((total, n_heads, hd)).astype(np.float32)
+    ld = n_heads * hd + ld_pad
+    qb = np.full((total, ld), np.nan, np.float32)
+    qb[:, :n_heads * hd] = q.reshape(total, -1)
+    off, _ = rows_of(lens, news)
+    first, end = (None, None) if masks is None else masks
+    pad = lambda x: None if x is None else ints(list(x) + [0] * tail)  # noqa: E731
+    out = torch.full((total, n_heads * hd), 7.0, device="cuda")
+    lse = torch.full((total, n_heads), 7.0, device="cuda")
+    sc = ferrum_hip.AttnScore(softcap, None if slopes is None else gpu(slopes, np.float32), pad(qpos), pad(first), pad(end))
+    mk = max(a + b for a, b in zip(lens, news)) if max_keys is None else max_keys
+    args = (fh, box.c, gpu(qb), ld, total, n_heads, ints(off) if use_off else None, max(news), ints(lens), mk, sc)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_attention_async(*args, out, lse)
+    if weigh:
+        ferrum_hip.kv4_weigh_async(*args, lse)
+    fh.sync()
+    o, z = out.cpu().numpy(), lse.cpu().numpy()
+    if tail:
+        assert (o[-tail:] == 7).all() and (z[-tail:] == 7).all()
+        o, z, q = o[:-tail], z[:-tail], q[:-tail]
+    check_attention(box, q, lens, news, o.reshape(-1, n_heads, hd), z, first, end, softcap,
+                    None if slopes is None else np.asarray(slopes, np.float32), qpos,
+                    box.plane("weight") if weigh else None)
+    return o
+
+
+# ---- append and read ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
+@pytest.mark.parametrize("lens,news", [([0], [1]), ([7, 0, 8, 3], [1, 1, 1, 1]), ([5, 0], [30, 30]), ([3, 8, 20], [0, 17, 4])])
+@pytest.mark.parametrize("rope", [None, "norm", "neox", "part"])
+def test_append_writes_the_formats_bytes(fh, n_heads, n_kv, hd, lens, news, rope):
+    import ferrum_hip
+    import torch
+
+    rng = np.random.default_rng(sum(lens) + hd)
+    cap, seqs, total = 40, len(lens), sum(news)
+    box = Box(seqs, n_kv, hd, cap, lens, 1, tracked=True)
+    before = {n: box.plane(n).copy() for n in ("k", "k_d", "v", "v_d", "pos", "weight")}
+    wide = (n_heads + 2 * n_kv) * hd
+    x = rng.standard_normal((total, n_heads + 2 * n_kv, hd)).astype(np.float32)
+    if rope is None and total:  # blocks at the edges of the format
+        e = x[0, n_heads:, :32]
+        e[0] = 0
+        e[-1] = np.where(np.arange(32) % 2, 2.0, -2.0)
+        if n_kv > 1:
+            e[1] = np.arange(32) * 0.5 - 8
+            e[-2] = 3e6
+        if total > 2:
+            x[1, n_heads, 5] = np.inf
+            x[1, n_heads + n_kv, hd - 1] = np.nan
+            x[2, n_heads:] *= np.float32(1e-7)
+    off, places = rows_of(lens, news)
+    pos = rng.integers(0, 5000, total)
+    rd = 0 if rope is None else hd // 2 if rope == "part" else hd
+    ff = rng.uniform(0.5, 2, rd // 2).astype(np.float32) if rope == "part" else None
+    lin = 2.0 if rope == "part" else 1.0
+    buf = np.full((total, wide + 3), np.nan, np.float32)
+    buf[:, :wide] = x.reshape(total, wide)
+    q = torch.full((total, n_heads * hd), float("nan"), device="cuda")
+    uniform = len(set(news)) == 1
+    args = (gpu(buf), wide + 3, total, n_heads, None if uniform else ints(off), max(news), ints(lens), ints(pos), rd, 1e4,
+            ferrum_hip.ROPE_NORM if rope == "norm" else ferrum_hip.ROPE_NEOX, None if ff is None else gpu(ff), lin, q)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_append_async(fh, box.c, *args)
+    fh.sync()
+    turned = ref.rotate(x[:, :n_heads + n_kv], pos, rd, 1e4, rope != "norm", ff, lin)
+    k, v = turned[:, n_heads:].astype(np.float32), x[:, n_heads + n_kv:]
+    got_q = q.cpu().numpy().reshape(total, n_heads, hd)
+    assert np.allclose(got_q, turned[:, :n_heads], rtol=2.0 ** -23, atol=2.0 ** -45)  # one f32 rounding of a float64 result
+    after = {n: box.plane(n) for n in before}
+    touched = {n: np.zeros(before[n].shape, bool) for n in before}
+    (dk, qk), (dv, qv) = ref.quantise(k), ref.quantise(v)
+    for s, row, at, _ in places:
+        if at >= cap:
+            continue
+        for h in range(n_kv):
+            for name, lev, sc, isv in (("k", qk, dk, False), ("v", qv, dv, True)):
+                _, gq, gd = ref.unpack(after[name][s, h], after[name + "_d"][s, h], hd, [at], isv)
+                assert np.array_equal(gq[0], lev[row, h]), (name, s, row, h)
+                assert np.array_equal(gd[0].view(np.uint16) & 0x7FFF, sc[row, h].view(np.uint16) & 0x7FFF)
+                assert np.array_equal(np.isnan(gd[0]) | (gd[0] == sc[row, h]), np.ones(hd // 32, bool))
+                place = ref.v_place if isv else ref.k_place
+                for c in range(hd):
+                    touched[name][s, h, place(at, c, hd)[0]] = True
+                touched[name + "_d"][s, h, at // 8, :, at % 8] = True
+            assert after["pos"][s, h, at] == pos[row] and after["weight"][s, h, at] == 0
+            touched["pos"][s, h, at] = touched["weight"][s, h, at] = True
+    for n in before:  # every other byte as it was
+        keep = ~touched[n]
+        a, b = (z.view(np.uint16) if z.dtype == np.float16 else z for z in (after[n], before[n]))
+        assert np.array_equal(a[keep], b[keep]), n
+
+
+def test_append_past_the_capacity_stores_what_fits(fh):
+    import ferrum_hip
+    import torch
+
+    box = Box(2, 1, 64, 16, [12, 16], 3, tracked=True)
+    x = np.random.default_rng(0).standard_normal((16, 3 * 64)).astype(np.float32)
+    old = box.plane("k").copy()
+    q = torch.zeros((16, 64), device="cuda")
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_append_async(fh, box.c, gpu(x), 192, 16, 1, None, 8, ints([12, 16]), q=q)
+    fh.sync()
+    new = box.plane("k")
+    assert np.array_equal(old[0, 0, :12 * 32], new[0, 0, :12 * 32]) and np.array_equal(old[1], new[1])
+    _, lev, _ = ref.unpack(new[0, 0], box.plane("k_d")[0, 0], 64, range(12, 16), False)
+    assert np.array_equal(lev, ref.quantise(x[:4, 64:128])[1])
+    assert np.array_equal(q.cpu().numpy(), x[:, :64])  # no rotation: q as it is, for every row
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
+def test_read_gives_the_values_the_blocks_stand_for(fh, n_heads, n_kv, hd):
+    import ferrum_hip
+    import torch
+
+    box = Box(3, n_kv, hd, 24, [24, 24, 24], 9)
+    first, rows = [0, 5, 20], 7
+    k, v = (torch.zeros((3, rows, n_kv * hd), device="cuda") for _ in range(2))
+    f = ints(first)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_read_async(fh, box.c, f, rows, k, v)
+    fh.sync()
+    for got, want in ((k, box.k), (v, box.v)):
+        got = got.cpu().numpy().reshape(3, rows, n_kv, hd)
+        for s in range(3):
+            n = min(rows, 24 - first[s])
+            assert np.array_equal(got[s, :n], want[s, :, first[s]:first[s] + n].transpose(1, 0, 2).astype(np.float32))
+            assert np.isnan(got[s, n:]).all()
+
+
+# ---- attention ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
+@pytest.mark.parametrize("lens", [[0], [1], [31, 32, 33], [7, 0, 300, 64, 255]])
+def test_decode(fh, n_heads, n_kv, hd, lens):
+    cap = -(-(max(lens) + 1) // 8) * 8
+    box = Box(len(lens), n_kv, hd, cap, [n + 1 for n in lens], 4)
+    attend(fh, box, n_heads, lens, [1] * len(lens), 5, False)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", [(14, 2, 64), (4, 4, 32), (8, 2, 128)])
+def test_decode_of_long_rows_splits_the_keys(fh, n_heads, n_kv, hd):
+    lens = [2500, 9, 1777]
+    box = Box(3, n_kv, hd, 2504, [n + 1 for n in lens], 6, tracked=True)
+    attend(fh, box, n_heads, lens, [1] * 3, 7, False, weigh=True)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
+@pytest.mark.parametrize("lens,news", [([0], [2]), ([0], [45]), ([13, 0, 40], [3, 70, 1]), ([0, 5], [0, 33])])
+def test_prompts(fh, n_heads, n_kv, hd, lens, news):
+    cap = -(-max(a + b for a, b in zip(lens, news)) // 8) * 8
+    box = Box(len(lens), n_kv, hd, cap, [a + b for a, b in zip(lens, news)], 8, tracked=True)
+    attend(fh, box, n_heads, lens, news, 9, True, weigh=True, ld_pad=5, tail=3)
+
+
+def test_many_rows_take_a_wave_each(fh):
+    """Enough columns for the form in which each wave has its own."""
+    lens, news = [3, 0, 17, 8], [90, 130, 64, 77]
+    box = Box(4, 8, 64, 136, [a + b for a, b in zip(lens, news)], 18, tracked=True)
+    attend(fh, box, 32, lens, news, 19, True, weigh=True)
+
+
+def masks_of(kind, lens, news, rng):
+    first, end = [], []
+    for at, new in zip(lens, news):
+        for t in range(new):
+            row = at + t
+            if kind == "window":
+                f, e = max(0, row - 9), row + 1
+            elif kind == "documents":
+                f, e = at + t // 11 * 11, row + 1
+            elif kind == "prefix":
+                f, e = 0, max(row + 1, at + new // 2)
+            elif kind == "holes":  # some rows see nothing, some one key
+                f, e = [(0, row + 1), (row, row + 1), (5, 5), (row + 1, row), (0, 1)][t % 5]
+            else:  # beyond what is there
+                f, e = int(rng.integers(0, 5)), 0xFFFFFFFF if t % 2 else at + new + 50
+            first.append(f)
+            end.append(e)
+    return first, end
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", [(14, 2, 64), (4, 4, 32), (8, 2, 128)])
+@pytest.mark.parametrize("kind", ["window", "documents", "prefix", "holes", "beyond"])
+@pytest.mark.parametrize("rows", ["one", "many"])
+def test_masks(fh, n_heads, n_kv, hd, kind, rows):
+    lens, news = ([70, 3, 33], [1, 1, 1]) if rows == "one" else ([20, 0, 7], [40, 77, 9])
+    box = Box(3, n_kv, hd, 80, [a + b for a, b in zip(lens, news)], 10, tracked=True)
+    attend(fh, box, n_heads, lens, news, 11, rows == "many", masks_of(kind, lens, news, np.random.default_rng(1)), weigh=True)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", [(14, 2, 64), (4, 4, 32), (8, 2, 128)])
+@pytest.mark.parametrize("softcap", [0.0, 2.0, 30.0])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("rows", ["one", "many"])
+def test_caps_and_biases(fh, n_heads, n_kv, hd, softcap, biased, rows):
+    lens, news = ([170, 3], [1, 1]) if rows == "one" else ([20, 0], [40, 67])
+    box = Box(2, n_kv, hd, 176, [a + b for a, b in zip(lens, news)], 12, tracked=True)
+    slopes = 2.0 ** (-8.0 * np.arange(1, n_heads + 1) / n_heads) if biased else None
+    attend(fh, box, n_heads, lens, news, 13, rows == "many", softcap=softcap, slopes=slopes, weigh=True)
+
+
+def test_bias_goes_by_positions_not_rows(fh):
+    """A cache whose rows are no longer their positions (as after an eviction)."""
+    box = Box(2, 2, 64, 104, [100, 61], 14, tracked=True)
+    box.pos = np.sort(np.random.default_rng(3).integers(0, 900, box.pos.shape), axis=2).astype(np.int32)
+    box.c.planes["pos"].copy_(gpu(box.pos))
+    slopes = 2.0 ** (-8.0 * np.arange(1, 15) / 14)
+    attend(fh, box, 14, [99, 60], [1, 1], 15, False, slopes=slopes, qpos=[950, 901], weigh=True)
+
+
+@pytest.mark.parametrize("k_std,v_std", [(1e-3, 1e-4), (8.0, 1e3), (1.0, 3e4)])
+def test_scales_far_from_one(fh, k_std, v_std):
+    lens = [600, 33]
+    box = Box(2, 2, 128, 608, [n + 1 for n in lens], 16, k_std=k_std, v_std=v_std)
+    attend(fh, box, 8, lens, [1, 1], 17, False)
+
+
+def test_one_large_value_among_small_ones(fh):
+    """The weights' f16 range follows the largest value scale; the others keep their bits."""
+    import torch
+
+    lens = [300]
+    box = Box(1, 1, 64, 304, [301], 20)
+    d = box.plane("v_d").copy()
+    d[0, 0, 10, 1, 3] = np.float16(900.0)  # key 83, block 1
+    box.vstep[0, 0, 83, 32:] = 900.0
+    old = box.v[0, 0, 83, 32:].copy()
+    lev, _, _ = ref.unpack(box.plane("v")[0, 0], d[0, 0], 64, [83], True)
+    box.v[0, 0, 83, 32:] = lev[0, 32:]
+    assert not np.array_equal(old, lev[0, 32:])
+    box.c.planes["v_d"].copy_(gpu(d))
+    torch.cuda.synchronize()
+    attend(fh, box, 7, lens, [1], 21, False)
+
+
+def test_rows_beyond_the_bounds_are_nan_and_nothing_else_is(fh):
+    import ferrum_hip
+    import torch
+
+    box = Box(3, 2, 64, 32, [32, 32, 10], 22)
+    q = torch.randn((3, 14 * 64), device="cuda")
+    out = torch.zeros_like(q)
+    lens = ints([32, 0xFFFFFFFF, 9])  # at the capacity, far past it, inside
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_attention_async(fh, box.c, q, 14 * 64, 3, 14, None, 1, lens, 64, None, out)
+    fh.sync()
+    o = out.cpu().numpy()
+    assert np.isnan(o[:2]).all() and np.isfinite(o[2]).all()
+    ferrum_hip.kv4_attention_async(fh, box.c, q, 14 * 64, 3, 14, None, 1, ints([8, 9, 7]), 9, None, out)
+    fh.sync()
+    o = out.cpu().numpy()
+    assert np.isfinite(o[0]).all() and np.isnan(o[1]).all() and np.isfinite(o[2]).all()
+
+
+def test_offsets_that_decrease_or_run_out_stay_inside(fh):
+    import ferrum_hip
+    import torch
+
+    box = Box(3, 2, 64, 32, [8, 8, 8], 23)
+    q = torch.randn((6, 14 * 64), device="cuda")
+    out = torch.full_like(q, 7.0)
+    off = ints([2, 1, 900, 0xFFFFFFFF])  # nothing; rows 1 .. 5; nothing (behind the end)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_attention_async(fh, box.c, q, 14 * 64, 6, 14, off, 4, None, 32, None, out)
+    fh.sync()
+    o = out.cpu().numpy()
+    assert (o[0] == 7).all() and (o[5] == 7).all()  # (max_rows 4: rows 1 .. 4)
+    assert np.isfinite(o[1:5]).all() and (o[1:5] != 7).any()
+
+
+def test_a_nan_key_reaches_only_the_rows_that_see_it(fh):
+    import ferrum_hip
+    import torch
+
+    for name in ("k_d", "v_d"):
+        box = Box(1, 2, 64, 64, [60], 24)
+        box.c.planes[name][0, 0, 5, 1, 0] = float("nan")  # key 40 of head 0
+        q = torch.randn((20, 14 * 64), device="cuda")
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        ferrum_hip.kv4_attention_async(fh, box.c, q, 14 * 64, 20, 14, None, 20, ints([30]), 64, None, out)
+        fh.sync()
+        o = out.cpu().numpy().reshape(20, 14, 64)
+        assert np.isfinite(o[:10]).all() and np.isfinite(o[10:, 7:]).all()
+        assert np.isnan(o[10:, :7]).any(axis=(1, 2)).all()
+
+
+# ---- eviction -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
+@pytest.mark.parametrize("lens,keep,recent", [([30, 5, 17], 16, 4), ([200, 64, 65], 64, 0), ([200, 150, 90], 70, 70),
+                                              ([33], 1, 0), ([1500, 1500], 1100, 100)])
+def test_evict(fh, n_heads, n_kv, hd, lens, keep, recent):
+    import ferrum_hip
+    import torch
+
+    cap, kcap = -(-max(lens) // 8) * 8, -(-keep // 8) * 8
+    box = Box(len(lens), n_kv, hd, cap, lens, 30, tracked=True)
+    w = box.weight
+    w[:, :, ::3] = 0.25  # ties: the first ones stay
+    w[:, 0, 4] = np.nan
+    w[:, 0, 6], w[:, 0, 7] = 0.0, -0.0
+    box.pos = (box.pos * 3 + 1).astype(np.int32)
+    box.c.planes["weight"].copy_(gpu(w))
+    box.c.planes["pos"].copy_(gpu(box.pos))
+    to = Box(len(lens), n_kv, hd, kcap, [0] * len(lens), 31, tracked=True)
+    names = ("k", "k_d", "v", "v_d", "pos", "weight")
+    before = {n: to.plane(n).copy() for n in names}
+    src = {n: box.plane(n).copy() for n in names}
+    ln = ints(lens)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_evict_async(fh, box.c, to.c, ln, max(lens), keep, recent, ln)
+    fh.sync()
+    assert list(ln.cpu().numpy()) == [min(n, keep) for n in lens]
+    after = {n: to.plane(n) for n in names}
+    for n in names:
+        assert np.array_equal(src[n].view(np.uint8), box.plane(n).view(np.uint8)), n  # the source is read only
+    for s, n in enumerate(lens):
+        for h in range(n_kv):
+            kept = ref.evict(w[s, h], n, keep, recent)
+            m = len(kept)
+            assert m == min(n, keep)
+            assert np.array_equal(after["pos"][s, h, :m], box.pos[s, h, kept])
+            assert np.array_equal(after["weight"][s, h, :m].view(np.uint32), w[s, h, kept].view(np.uint32))
+            for name, isv in (("k", False), ("v", True)):
+                _, lev, sc = ref.unpack(after[name][s, h], after[name + "_d"][s, h], hd, range(m), isv)
+                _, lw, sw = ref.unpack(src[name][s, h], src[name + "_d"][s, h], hd, kept, isv)
+                assert np.array_equal(lev, lw) and np.array_equal(sc.view(np.uint16), sw.view(np.uint16))
+                if m < kcap:
+                    _, lev, sc = ref.unpack(after[name][s, h], after[name + "_d"][s, h], hd, range(m, kcap), isv)
+                    _, lw, sw = ref.unpack(before[name][s, h], before[name + "_d"][s, h], hd, range(m, kcap), isv)
+                    assert np.array_equal(lev, lw) and np.array_equal(sc.view(np.uint16), sw.view(np.uint16))
+
+
+# ---- together -------------------------------------------------------------------
+
+
+def test_a_run_of_them_together(fh):
+    """A prompt, its weights, an eviction and decode steps over what is left: the
+    attention of every step is that of the rows that a float64 account keeps."""
+    import ferrum_hip
+    import torch
+
+    n_heads, n_kv, hd, keep, recent, prompt = 14, 2, 64, 40, 8, 60
+    rng = np.random.default_rng(40)
+    caches = [ferrum_hip.KV4Cache.alloc(1, n_kv, hd, 72, tracked=True) for _ in range(2)]
+    wide = (n_heads + 2 * n_kv) * hd
+    k, v = [np.zeros((0, hd)) for _ in range(n_kv)], [np.zeros((0, hd)) for _ in range(n_kv)]
+    ln, at = torch.zeros(1, dtype=torch.int32, device="cuda"), 0
+    for rows in [prompt] + [1] * 6:
+        x = rng.standard_normal((rows, n_heads + 2 * n_kv, hd)).astype(np.float32)
+        pos = np.arange(at, at + rows)
+        qkv, q = gpu(x.reshape(rows, wide)), torch.empty((rows, n_heads * hd), device="cuda")
+        out, lse, p = torch.empty_like(q), torch.empty((rows, n_heads), device="cuda"), ints(pos)
+        torch.cuda.synchronize()
+        used = int(ln.item())
+        ferrum_hip.kv4_append_async(fh, caches[0], qkv, wide, rows, n_heads, None, rows, ln, p, hd, 1e6, 1, None, 1.0, q)
+        args = (fh, caches[0], q, n_heads * hd, rows, n_heads, None, rows, ln, used + rows, None)
+        ferrum_hip.kv4_attention_async(*args, out, lse)
+        ferrum_hip.kv4_weigh_async(*args, lse)
+        fh.sync()
+        turned = ref.rotate(x[:, :n_heads + n_kv], pos, hd, 1e6, True)
+        for h in range(n_kv):
+            k[h] = np.concatenate([k[h], ref.values(*ref.quantise(turned[:, n_heads + h].astype(np.float32)))])
+            v[h] = np.concatenate([v[h], ref.values(*ref.quantise(x[:, n_heads + n_kv + h]))])
+        o, _, _ = ref.attention(turned[:, :n_heads].astype(np.float32), np.stack(k), np.stack(v), [0] * rows,
+                                used + np.arange(rows) + 1)
+        got = out.cpu().numpy().reshape(o.shape)
+        # (1e-5 of the values' size: every score here is below 2^4, see check_attention)
+        assert np.abs(got - o).max() <= 1e-5 * np.abs(np.stack(v)).max()
+        ln += rows
+        at += rows
+        torch.cuda.synchronize()
+        if int(ln.item()) > keep:
+            w = caches[0].planes["weight"].cpu().numpy()
+            n = int(ln.item())
+            ferrum_hip.kv4_evict_async(fh, caches[0], caches[1], ln, n, keep, recent, ln)
+            fh.sync()
+            caches.reverse()
+            for h in range(n_kv):
+                stay = ref.evict(w[0, h], n, keep, recent)
+                k[h], v[h] = k[h][stay], v[h][stay]
+        torch.cuda.synchronize()
+
+
+def test_captured_calls_replay_as_they_ran(fh):
+    import ferrum_hip
+    import torch
+
+    rng = np.random.default_rng(50)
+    lens = [900, 17, 333]
+    n_heads, n_kv, hd = 14, 2, 64
+    box = Box(3, n_kv, hd, 904, [n + 1 for n in lens], 51, tracked=True)
+    wide = (n_heads + 2 * n_kv) * hd
+    x = gpu(rng.standard_normal((3, wide)).astype(np.float32))
+    q, out = torch.empty((3, n_heads * hd), device="cuda"), torch.empty((3, n_heads * hd), device="cuda")
+    lse, ln = torch.empty((3, n_heads), device="cuda"), ints(lens)
+    weight = box.c.planes["weight"].clone()
+
+    def calls():
+        ferrum_hip.kv4_append_async(fh, box.c, x, wide, 3, n_heads, None, 1, ln, None, hd, 1e6, 1, None, 1.0, q)
+        args = (fh, box.c, q, n_heads * hd, 3, n_heads, None, 1, ln, 901, None)
+        ferrum_hip.kv4_attention_async(*args, out, lse)
+        ferrum_hip.kv4_weigh_async(*args, lse)
+
+    torch.cuda.synchronize()
+    calls()  # (the workspace exists from here on)
+    fh.sync()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    try:
+        with torch.cuda.graph(g, stream=s):
+            fh.set_stream(torch.cuda.current_stream().cuda_stream)
+            calls()
+    finally:
+        fh.set_stream(None)
+    seen = []
+    for i in range(4):
+        for how in (g.replay, calls):
+            box.c.planes["weight"].copy_(weight)
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            how()
+            torch.cuda.synchronize()
+            fh.sync()
+            seen.append((out.cpu().numpy().view(np.uint32).copy(), box.plane("weight").view(np.uint32).copy()))
+    assert np.isfinite(seen[0][0].view(np.float32)).all()
+    assert all(np.array_equal(a, seen[0][0]) and np.array_equal(b, seen[0][1]) for a, b in seen)
+
+
+def test_two_contexts_on_two_streams_at_once(fh):
+    import ferrum_hip
+    import torch
+
+    box = Box(2, 2, 128, 2048, [2048, 2048], 60)
+    q = [torch.randn((2, 8 * 128), device="cuda") for _ in range(2)]
+    lens = ints([2047, 1500])
+    want, got = [torch.empty_like(a) for a in q], [torch.zeros_like(a) for a in q]
+    torch.cuda.synchronize()
+    for a, o in zip(q, want):
+        ferrum_hip.kv4_attention_async(fh, box.c, a, 1024, 2, 8, None, 1, lens, 2048, None, o)
+    fh.sync()
+    with ferrum_hip.Context(0) as c1, ferrum_hip.Context(0) as c2:
+        for _ in range(20):
+            for c, a, o in zip((c1, c2), q, got):
+                ferrum_hip.kv4_attention_async(c, box.c, a, 1024, 2, 8, None, 1, lens, 2048, None, o)
+        c1.sync()
+        c2.sync()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+
+
+# ---- refusals -------------------------------------------------------------------
+
+
+def test_refusals(fh):
+    import ferrum_hip as F
+    import torch
+
+    ok = F.KV4Cache.alloc(2, 2, 64, 32, tracked=True)
+    bare = F.KV4Cache.alloc(2, 2, 64, 32)
+    q, out = torch.zeros((2, 8 * 64), device="cuda"), torch.zeros((2, 4 * 64), device="cuda")
+    ln = ints([0, 0])
+    p = ok.planes
+
+    def att(cache=ok, q=q, ld=512, total=2, heads=4, off=None, rows=1, score=None, out=out):
+        return lambda: F.kv4_attention_async(fh, cache, q, ld, total, heads, off, rows, ln, 32, score, out)
+
+    def cache(**kw):
+        a = dict(seqs=2, n_kv=2, head_dim=64, capacity=32, k=p["k"], k_d=p["k_d"], v=p["v"], v_d=p["v_d"])
+        a.update(kw)
+        return F.KV4Cache(**a)
+
+    cases = [
+        (F.FH_ERR_INVALID, "cache is NULL", att(cache=None)),
+        (F.FH_ERR_INVALID, "plane of the cache is NULL", att(cache=cache(v_d=None))),
+        (F.FH_ERR_INVALID, "16-byte aligned", att(cache=cache(k=p["k"].data_ptr() + 8))),
+        (F.FH_ERR_INVALID, "no sequences", att(cache=cache(seqs=0))),
+        (F.FH_ERR_LIMIT, "head width 96", att(cache=cache(head_dim=96))),
+        (F.FH_ERR_INVALID, "multiple of 8", att(cache=cache(capacity=12))),
+        (F.FH_ERR_INVALID, "multiple of 8", att(cache=cache(capacity=0))),
+        (F.FH_ERR_LIMIT, "too large", att(cache=cache(capacity=1 << 40))),
+        (F.FH_ERR_DIM, "multiple of n_kv_heads", att(heads=3)),
+        (F.FH_ERR_DIM, "multiple of n_kv_heads", att(heads=0)),
+        (F.FH_ERR_DIM, "ld is below", att(ld=255)),
+        (F.FH_ERR_DIM, "do not divide", att(total=3)),
+        (F.FH_ERR_LIMIT, "too large", att(total=1 << 40)),
+        (F.FH_ERR_INVALID, "q or out is NULL", att(q=None)),
+        (F.FH_ERR_INVALID, "q or out is NULL", att(out=None)),
+        (F.FH_ERR_INVALID, "must not be q", att(out=q)),
+        (F.FH_ERR_INVALID, "softcap", att(score=F.AttnScore(-1.0))),
+        (F.FH_ERR_INVALID, "softcap", att(score=F.AttnScore(float("nan")))),
+        (F.FH_ERR_INVALID, "no weight plane", lambda: F.kv4_weigh_async(fh, bare, q, 512, 2, 4, None, 1, ln, 32, None, out)),
+        (F.FH_ERR_INVALID, "lse is NULL", lambda: F.kv4_weigh_async(fh, ok, q, 512, 2, 4, None, 1, ln, 32, None, None)),
+        (F.FH_ERR_DIM, "ld is below", lambda: F.kv4_append_async(fh, ok, q, 511, 2, 4, None, 1, ln)),
+        (F.FH_ERR_DIM, "rope_dim", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, rope_dim=66)),
+        (F.FH_ERR_DIM, "rope_dim", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, rope_dim=7)),
+        (F.FH_ERR_INVALID, "rope_type", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, rope_dim=8, rope_type=5)),
+        (F.FH_ERR_DIM, "RoPE scaling", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, rope_dim=8, linear_factor=0.0)),
+        (F.FH_ERR_INVALID, "must not be qkv", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, q=q)),
+        (F.FH_ERR_INVALID, "qkv is NULL", lambda: F.kv4_append_async(fh, ok, None, 512, 2, 4, None, 1, ln)),
+        (F.FH_ERR_INVALID, "no weight plane", lambda: F.kv4_evict_async(fh, bare, ok, ln, 32, 8, 0, ln)),
+        (F.FH_ERR_INVALID, "share a plane", lambda: F.kv4_evict_async(fh, ok, ok, ln, 32, 8, 0, ln)),
+        (F.FH_ERR_DIM, "above the capacity", lambda: F.kv4_evict_async(fh, ok, bare, ln, 32, 33, 0, ln)),
+        (F.FH_ERR_DIM, "caches differ", lambda: F.kv4_evict_async(fh, ok, F.KV4Cache.alloc(2, 1, 64, 32), ln, 32, 8, 0, ln)),
+        (F.FH_ERR_INVALID, "keep must be", lambda: F.kv4_evict_async(fh, ok, bare, ln, 32, 0, 0, ln)),
+        (F.FH_ERR_INVALID, "keep must be", lambda: F.kv4_evict_async(fh, ok, bare, ln, 32, 8, 9, ln)),
+        (F.FH_ERR_INVALID, "len or new_len", lambda: F.kv4_evict_async(fh, ok, bare, None, 32, 8, 0, ln)),
+        (F.FH_ERR_INVALID, "k or v is NULL", lambda: F.kv4_read_async(fh, ok, None, 4, None, out)),
+        (F.FH_ERR_LIMIT, "2^32", lambda: F.kv4_read_async(fh, ok, None, 1 << 40, out, out)),
+    ]
+    for code, text, call in cases:
+        with pytest.raises(F.FerrumHipError, match=text.replace("^", r"\^")) as e:
+            call()
+        assert e.value.code == code, text
+    # empty calls are valid
+    F.kv4_append_async(fh, ok, None, 512, 0, 4, None, 0, ln)
+    F.kv4_attention_async(fh, ok, None, 512, 0, 4, None, 0, ln, 32, None, None)
+    F.kv4_weigh_async(fh, ok, None, 512, 0, 4, None, 0, ln, 32, None, None)
+    F.kv4_read_async(fh, ok, None, 0, None, None)
+    fh.sync()
