@@ -1225,6 +1225,11 @@ class LlamaDevice:
     output.weight).  Each row's token and position live on the device
     (self.tokens, self.pos), so a step can be captured in one graph.
 
+    cfg["kv"] = "q4" holds the caches in 4 bits (KV4Cache; head_dim 32, 64 or
+    128): prompts can then be fed at once (prefill_async), self.used counts each
+    row's cache rows beside its position, and with cfg["kv_tracked"] every step
+    adds up the weight each cached key draws, for evict_async to make room by.
+
     from_weights takes numpy arrays keyed as a GGUF file names them
     (gguf/llama.rs:171-340): token_embd (Q8_0 bytes [vocab, d]), output
     (optional, Q8_0 [vocab, d]), output_norm [d], and per block i
@@ -1257,6 +1262,16 @@ class LlamaDevice:
         self.z = torch.empty((B, self.vocab), device=dev)
         self.tokens = torch.zeros(B, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
+        self.kv, self.tracked = c.get("kv", "f32"), bool(c.get("kv_tracked", False))
+        if self.kv not in ("f32", "q4"):
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice: cache type {self.kv!r} is not 'f32' or 'q4'")
+        if self.kv == "q4":
+            if self.hd not in (32, 64, 128):
+                raise FerrumHipError(FH_ERR_LIMIT, f"LlamaDevice: a 4-bit cache needs head width 32, 64 or 128, not {self.hd}")
+            self.q = torch.empty((B, self.q_dim), device=dev)
+            self.lse = torch.empty((B, self.nh), device=dev) if self.tracked else None
+            self.used = torch.zeros(B, dtype=torch.int32, device=dev)  # cache rows in use, as pos until rows are evicted
+            self.spare = None
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
         self.fused = 3 <= B <= 64 and self.d % 32 == 0
@@ -1267,6 +1282,8 @@ class LlamaDevice:
     def _alloc_cache(self):
         import torch
 
+        if self.kv == "q4":
+            return KV4Cache.alloc(self.rows, self.nkv, self.hd, self.cap, self.tracked), None
         n = self.rows * self.cap * self.kv_dim
         return torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
 
@@ -1303,7 +1320,8 @@ class LlamaDevice:
         return m
 
     @classmethod
-    def from_gguf(cls, ctx: Context, path, rows: int = 1, capacity=None) -> "LlamaDevice":
+    def from_gguf(cls, ctx: Context, path, rows: int = 1, capacity=None, kv: str = "f32",
+                  kv_tracked: bool = False) -> "LlamaDevice":
         """A llama / qwen2 GGUF read as Gguf::load_llama_prec(None) reads it
         (gguf/llama.rs:171-340; the checks, llama_gguf_plan): rope type by
         architecture (NORM for llama, NEOX for qwen2), the metadata defaults,
@@ -1313,13 +1331,15 @@ class LlamaDevice:
         concatenation: Q8_0 rows stay Q8_0 bytes; a group holding an F32 / F16
         matrix becomes one F32 weight, the Q8_0 rows expanded exactly).  Each
         row's KV cache holds `capacity` positions (default: the file's
-        context_length)."""
+        context_length), in f32 or 4 bits (kv, kv_tracked: the class's
+        cfg["kv"], cfg["kv_tracked"])."""
         import torch
 
         with GGUFFile(path) as g:
             cfg, mats, tied = llama_gguf_plan(g)
             if capacity is not None:
                 cfg["context"] = int(capacity)
+            cfg["kv"], cfg["kv_tracked"] = kv, kv_tracked
             m = cls(ctx, cfg, rows)
             d = m.d
             f = lambda name: torch.from_numpy(np.ascontiguousarray(g.read_f32(ctx, name), np.float32).ravel()).cuda()  # noqa: E731
@@ -1428,9 +1448,13 @@ class LlamaDevice:
         block, six with SwiGLU in the gate|up GEMM, one fewer again where the
         attention rotates q and k itself); otherwise each RmsNorm is a launch
         of its own (nine).  The head counts as one call (a wide head at more
-        than 32 rows takes one launch per 32 rows)."""
+        than 32 rows takes one launch per 32 rows).  A 4-bit cache takes two
+        launches per block where the f32 one takes RoPE and attention, three
+        when it keeps the keys' weights."""
         per = (6 if all(b.get("glu") for b in self.blocks) else 7) if self.fused else 9
-        if self.fused and self._rope_in_attention():
+        if self.kv == "q4":
+            per += self.tracked
+        elif self.fused and self._rope_in_attention():
             per -= 1
         return 1 + per * self.layers + 2 + (1 if self.fused else 0)
 
@@ -1452,22 +1476,120 @@ class LlamaDevice:
         if self.rows != 1:
             raise FerrumHipError(FH_ERR_INVALID, "forward_one drives a single-row LlamaDevice")
         nxt = getattr(self, "next_pos", 0)
-        if nxt >= self.cap:
+        used = getattr(self, "next_used", 0) if self.kv == "q4" else nxt
+        if used >= self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
         self.ctx.sync()
         self.tokens.fill_(int(token))
         self.pos.fill_(nxt)
+        if self.kv == "q4":
+            self.used.fill_(used)
+            self.next_used = used + 1
         torch.cuda.current_stream().synchronize()
         self.feed_async(nxt)
         self.next_pos = nxt + 1
         self.ctx.sync()
         return self.z[0].cpu().numpy()
 
+    def _attend4_async(self, b, qkv, total: int, off, max_rows: int, pos, max_keys: int, q, att, lse):
+        """A block's attention over its 4-bit cache: append (with RoPE), attend,
+        and add up the keys' weights where they are tracked."""
+        ctx, c = self.ctx, b["k"]
+        kv4_append_async(ctx, c, qkv, self.qkv_dim, total, self.nh, off, max_rows, self.used, pos, self.rope_dim,
+                         self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear, q)
+        args = (ctx, c, q, self.q_dim, total, self.nh, off, max_rows, self.used, max_keys, None)
+        kv4_attention_async(*args, att, lse)
+        if self.tracked:
+            kv4_weigh_async(*args, lse)
+
+    def prefill_async(self, tokens, lens):
+        """Feeds lens[r] >= 1 tokens of every row r at once (a 4-bit cache only):
+        tokens holds the rows' ids one after the other, on the device; row r's go
+        to positions self.pos[r] .. and cache rows self.used[r] .. .  The scores
+        of each row's last token land in self.z; positions are not advanced.
+        Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
+        read on the host, so the call waits for the stream."""
+        import torch
+
+        if self.kv != "q4":
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async needs the 4-bit cache (cfg['kv'] = 'q4')")
+        ctx, d, B = self.ctx, self.d, self.rows
+        n = np.asarray(lens, np.int64)
+        if n.shape != (B,) or (n < 1).any():
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {B} lengths of at least 1")
+        total, most = int(n.sum()), int(n.max())
+        if tokens.numel() != total:
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {tokens.numel()} tokens for {total} places")
+        ctx.sync()
+        torch.cuda.synchronize()
+        max_keys = int((self.used.cpu().numpy().astype(np.int64) + n).max())
+        if max_keys > self.cap:
+            raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
+        dev, ends = "cuda", np.cumsum(n)
+        off = torch.from_numpy(np.concatenate([[0], ends]).astype(np.int32)).to(dev)
+        rep = torch.from_numpy(n).to(dev)
+        first = torch.repeat_interleave(off[:-1].long(), rep)
+        pos = (torch.repeat_interleave(self.pos, rep) + torch.arange(total, device=dev) - first).to(torch.int32)
+        x, x2, h, proj = (torch.empty((total, d), device=dev) for _ in range(4))
+        qkv, q, att = (torch.empty((total, w), device=dev) for w in (self.qkv_dim, self.q_dim, self.q_dim))
+        gu, mid = torch.empty((total, 2 * self.ffn), device=dev), torch.empty((total, self.ffn), device=dev)
+        lse = torch.empty((total, self.nh), device=dev) if self.tracked else None
+        torch.cuda.synchronize()
+        embed_rows_async(ctx, self.tok_w, self.vocab, d, tokens, total, x)
+        cur, other = x, x2
+        for i, b in enumerate(self.blocks):
+            if i == 0:
+                rmsnorm_async(ctx, cur, None, None, total, d, b["attn_norm"], self.eps, h)
+            else:
+                rmsnorm_async(ctx, cur, proj, other, total, d, b["attn_norm"], self.eps, h)
+                cur, other = other, cur
+            qkv_b = b.get("qkv_b")
+            linear_forward_async(ctx, b["qkv"], h, total, d, qkv_b, 0 if qkv_b is None else self.qkv_dim, qkv)
+            self._attend4_async(b, qkv, total, off, most, pos, max_keys, q, att, lse)
+            linear_forward_async(ctx, b["o"], att, total, self.q_dim, None, 0, proj)
+            rmsnorm_async(ctx, cur, proj, other, total, d, b["ffn_norm"], self.eps, h)
+            cur, other = other, cur
+            linear_forward_async(ctx, b["gate_up"], h, total, d, None, 0, gu)
+            if b.get("glu"):  # gate and up rows lie interleaved by 32: each 64 outputs are a row of 32 of them
+                swiglu_async(ctx, gu, gu.view(-1)[32:], total * self.ffn // 32, 32, 64, mid)
+            else:
+                swiglu_async(ctx, gu, gu[:, self.ffn:], total, self.ffn, 2 * self.ffn, mid)
+            linear_forward_async(ctx, b["down"], mid, total, self.ffn, None, 0, proj)
+        rmsnorm_async(ctx, cur, proj, other, total, d, self.out_norm, self.eps, h)
+        ctx.sync()
+        last = h[torch.from_numpy(ends - 1).to(dev)].contiguous()
+        torch.cuda.synchronize()
+        linear_forward_async(ctx, self.head, last, B, d, None, 0, self.z)
+        self._keep = last  # alive until the stream has used it
+
+    def evict_async(self, keep: int, recent: int):
+        """Cuts every row's caches that hold more than `keep` keys to the last
+        `recent` and the heaviest others (kv4_evict_async, per layer and kv head),
+        and self.used with them; positions stay.  Each layer's cache changes places
+        with a spare one: capture steps again after it.  Needs cfg["kv_tracked"]."""
+        import torch
+
+        if self.kv != "q4" or not self.tracked:
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.evict_async needs a tracked 4-bit cache")
+        if self.spare is None:
+            self.spare = self._alloc_cache()[0]
+            self._cut = torch.empty_like(self.used)
+            torch.cuda.synchronize()
+        for i, b in enumerate(self.blocks):
+            last = i == self.layers - 1  # (the lengths change once every layer has read them)
+            kv4_evict_async(self.ctx, b["k"], self.spare, self.used, self.cap, keep, recent,
+                            self.used if last else self._cut)
+            b["k"], self.spare = self.spare, b["k"]
+        if hasattr(self, "next_used"):
+            self.next_used = min(self.next_used, keep)
+
     def feed_async(self, max_pos: int):
         """One decode step of every row: token self.tokens[r] at position
         self.pos[r] (both on the device; max_pos bounds the positions).  The
-        head's scores land in self.z; positions are not advanced."""
+        head's scores land in self.z; positions are not advanced.  (A 4-bit cache:
+        at cache row self.used[r], which is not advanced either.)"""
         ctx, d, B = self.ctx, self.d, self.rows
+        max_keys = min(max_pos + 1, self.cap)
         embed_rows_async(ctx, self.tok_w, self.vocab, d, self.tokens, B, self.x)
         if self.fused:
             # x is updated in place by the o and down projections, which leave
@@ -1482,9 +1604,12 @@ class LlamaDevice:
                 else:
                     linear_normed_async(ctx, b["qkv"], x, B, d, st, b["attn_norm"], None, self.eps, True, qkv_b,
                                         0 if qkv_b is None else self.qkv_dim, self.qkv)
-                gqa_attention_rope_decode_async(ctx, self.qkv, self.qkv_dim, B, self.nh, self.nkv, self.hd, b["k"],
-                                                b["v"], self.cap, self.pos, max_pos, self.rope_dim, self.rope_base,
-                                                self.rope_type, self.rope_freqs, self.rope_linear, self.att)
+                if self.kv == "q4":
+                    self._attend4_async(b, self.qkv, B, None, 1, self.pos, max_keys, self.q, self.att, self.lse)
+                else:
+                    gqa_attention_rope_decode_async(ctx, self.qkv, self.qkv_dim, B, self.nh, self.nkv, self.hd, b["k"],
+                                                    b["v"], self.cap, self.pos, max_pos, self.rope_dim, self.rope_base,
+                                                    self.rope_type, self.rope_freqs, self.rope_linear, self.att)
                 linear_residual_async(ctx, b["o"], self.att, B, self.q_dim, None, 0, x, x, st)
                 if b.get("glu"):
                     linear_normed_async(ctx, b["gate_up"], x, B, d, st, b["ffn_norm"], None, self.eps, True, None, 0,
@@ -1506,10 +1631,13 @@ class LlamaDevice:
                 cur, other = other, cur
             qkv_b = b.get("qkv_b")  # (None: a file without q/k/v biases, whose linears are bias-free)
             linear_forward_async(ctx, b["qkv"], self.h, B, d, qkv_b, 0 if qkv_b is None else self.qkv_dim, self.qkv)
-            rope_async(ctx, self.qkv, B, self.qkv_dim, self.nh + self.nkv, self.hd, self.rope_dim, self.pos,
-                       self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear)
-            gqa_attention_decode_async(ctx, self.qkv, self.qkv_dim, B, self.nh, self.nkv, self.hd, b["k"], b["v"],
-                                       self.cap, self.pos, max_pos, self.att)
+            if self.kv == "q4":
+                self._attend4_async(b, self.qkv, B, None, 1, self.pos, max_keys, self.q, self.att, self.lse)
+            else:
+                rope_async(ctx, self.qkv, B, self.qkv_dim, self.nh + self.nkv, self.hd, self.rope_dim, self.pos,
+                           self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear)
+                gqa_attention_decode_async(ctx, self.qkv, self.qkv_dim, B, self.nh, self.nkv, self.hd, b["k"], b["v"],
+                                           self.cap, self.pos, max_pos, self.att)
             linear_forward_async(ctx, b["o"], self.att, B, self.q_dim, None, 0, self.proj)
             rmsnorm_async(ctx, cur, self.proj, other, B, d, b["ffn_norm"], self.eps, self.h)
             cur, other = other, cur
