@@ -1030,7 +1030,7 @@ static int kv4_check_cache(fh_ctx* ctx, const std::string& who, const fh_kv4_cac
     if (c->capacity == 0 || c->capacity % 8 != 0)
         return fh_fail(ctx, FH_ERR_INVALID,
                        who + ": capacity " + std::to_string(c->capacity) + " is not a positive multiple of 8");
-    if (c->seqs > 65535 || c->n_kv > 65535 || c->capacity > 0x7FFFFF00u ||
+    if (c->seqs > 65535 || c->n_kv > 65535 || c->capacity > (size_t(1) << 25) ||
         c->seqs * c->n_kv > 0x7FFFFFFFu / (c->head_dim * 2) || c->seqs * c->n_kv * c->capacity > (size_t(1) << 36))
         return fh_fail(ctx, FH_ERR_LIMIT, who + ": a dimension is too large");
     return FH_OK;

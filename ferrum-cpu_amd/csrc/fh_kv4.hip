@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 
 namespace {
 
@@ -123,7 +124,7 @@ __device__ __forceinline__ void load_k(const Planes& p, int cap, int tile, int l
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         // (a tile's end past the capacity reads the last row again; the mask drops it)
-        const uint8_t* a = p.k + static_cast<size_t>(min(key + 4 * h, cap - 1)) * (HD / 2) + g * (4 * NB);
+        const uint8_t* a = p.k + (static_cast<uint32_t>(min(key + 4 * h, cap - 1)) * (HD / 2) + g * (4 * NB));
         if constexpr (NB == 4) {
             const u32x4 w = *reinterpret_cast<const u32x4*>(a);
 #pragma unroll
@@ -136,9 +137,9 @@ __device__ __forceinline__ void load_k(const Planes& p, int cap, int tile, int l
             k[h][0] = *reinterpret_cast<const uint32_t*>(a);
         }
     }
-    const size_t o = min(tile * 4 + g, cap / 8 - 1);
+    const uint32_t o = min(tile * 4 + g, cap / 8 - 1);
 #pragma unroll
-    for (int b = 0; b < NB; b++) kd[b] = *reinterpret_cast<const u32x4*>(p.kd + (o * NB + b) * 8);
+    for (int b = 0; b < NB; b++) kd[b] = *reinterpret_cast<const u32x4*>(p.kd + o * (NB * 8) + b * 8);
 }
 
 template <int HD>
@@ -146,15 +147,14 @@ __device__ __forceinline__ void load_tile(const Planes& p, int cap, int tile, in
     constexpr int NB = Shape<HD>::NB, N = Shape<HD>::N, BP = Shape<HD>::BP;
     load_k<HD>(p, cap, tile, lane, t.k, t.kd);
     const int g = lane >> 4, n = lane & 15, last = cap / 8 - 1;
-    const size_t o = min(tile * 4 + g, last);
+    const uint32_t o = min(tile * 4 + g, last), vo = o * (N * BP * 16) + n % N * (BP * 16), so = o * (NB * 8);
 #pragma unroll
-    for (int i = 0; i < BP; i++)
-        t.v[i] = *reinterpret_cast<const u32x4*>(p.v + ((o * N + n % N) * BP + i) * 16);
+    for (int i = 0; i < BP; i++) t.v[i] = *reinterpret_cast<const u32x4*>(p.v + vo + i * 16);
 #pragma unroll
-    for (int b = 0; b < NB; b++) t.vd[b] = *reinterpret_cast<const u32x4*>(p.vd + (o * NB + b) * 8);
+    for (int b = 0; b < NB; b++) t.vd[b] = *reinterpret_cast<const u32x4*>(p.vd + so + b * 8);
     const int i = lane % (16 * NB);
-    const size_t ox = min(tile * 4 + i / (4 * NB), last);
-    t.vx = *reinterpret_cast<const uint32_t*>(p.vd + ox * (NB * 8) + i % (4 * NB) * 2);
+    const uint32_t ox = min(tile * 4 + i / (4 * NB), last);
+    t.vx = *reinterpret_cast<const uint32_t*>(p.vd + (ox * (NB * 8) + i % (4 * NB) * 2));
 }
 
 __device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -162,6 +162,16 @@ __device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, ui
 }
 __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// A constant that the compiler does not know: it then keeps a product or a mask with it in
+// the one instruction that takes it (v_fma_mix_f32, v_and_or_b32).
+__device__ __forceinline__ float hidden(float c) {
+    asm("" : "+v"(c));
+    return c;
+}
+__device__ __forceinline__ uint32_t hidden(uint32_t c) {
+    asm("" : "+v"(c));
+    return c;
 }
 // Four levels of each 16-bit half of a word as f16 operands, level - 8 as itself:
 // under the exponent of 1024 a nibble of bits 0 .. 3 is 1024 + level, one of bits 4
@@ -172,7 +182,7 @@ __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
 // those 23 bits, 1e-5 of the result.)
 template <int E>
 __device__ __forceinline__ uint32_t levels2(uint32_t w) {
-    const uint32_t x = ((E & 2 ? w >> 8 : w) & (E & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+    const uint32_t x = ((E & 2 ? w >> 8 : w) & (E & 1 ? 0x00F000F0u : 0x000F000Fu)) | hidden(0x64006400u);
     const half2v v = __builtin_bit_cast(half2v, x);
     const _Float16 sixteenth = static_cast<_Float16>(0.0625f);
     const half2v r = E & 1 ? __builtin_elementwise_fma(v, half2v{sixteenth, sixteenth}, half2v{-72, -72})
@@ -190,36 +200,76 @@ __device__ __forceinline__ float half_at(const u32x4& w, int i) {
     return fh_h2f(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
 }
 // Two f32 as a pair of f16 and what that leaves, each rounded to nearest: 22 bits in all.
-// (The values are kept from the compiler's view: it would form a product's hi in one
-// mixed-precision instruction, with one rounding, and lo from the twice rounded one.)
+// (The values and the pair are kept from the compiler's view: it would form a product's
+// hi in one mixed-precision instruction, with one rounding, and lo from the twice rounded
+// one, or the pair twice over.)
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     asm("" : "+v"(a), "+v"(b));
     const half2v h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
-    const half2v l = {static_cast<_Float16>(a - static_cast<float>(h[0])),
-                      static_cast<_Float16>(b - static_cast<float>(h[1]))};
     hi = __builtin_bit_cast(uint32_t, h);
+    asm("" : "+v"(hi));
+    const half2v k = __builtin_bit_cast(half2v, hi);
+    const float minus = hidden(-1.0f);
+    const half2v l = {static_cast<_Float16>(fmaf(static_cast<float>(k[0]), minus, a)),
+                      static_cast<_Float16>(fmaf(static_cast<float>(k[1]), minus, b))};
     lo = __builtin_bit_cast(uint32_t, l);
 }
+// A lane's value with those of the other three lane groups (its column's other keys).
+struct Pair {
+    float a, b;
+};
+__device__ __forceinline__ Pair halves(float v) {  // of the wave, each in every lane
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const uint32_t a = r[0], b = r[1];
+    return {__uint_as_float(a), __uint_as_float(b)};
+}
+__device__ __forceinline__ Pair rows16(float v) {  // of each half
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const uint32_t a = r[0], b = r[1];
+    return {__uint_as_float(a), __uint_as_float(b)};
+}
 __device__ __forceinline__ float across_groups_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    Pair p = halves(v);
+    p = rows16(fmaxf(p.a, p.b));
+    return fmaxf(p.a, p.b);
 }
 __device__ __forceinline__ float across_groups_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    Pair p = halves(v);
+    p = rows16(p.a + p.b);
+    return p.a + p.b;
+}
+// Over the 16 lanes of a group.
+__device__ __forceinline__ int group_min(int v) {
+    v = min(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false));
+    return min(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false));
 }
 
-// c tanh(x / c).  Up to 0.6 a polynomial (least maximum error over [0, 0.36] of
-// tanh(y) / y in y^2: 2.4e-9), past it 1 - 2 / (1 + e^2y), whose rounding is then
-// no larger than the result's own.
-__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
-    const float y = x * inv_cap, a = fabsf(y), z = y * y;
-    const float p = fmaf(fmaf(fmaf(fmaf(fmaf(-0.005863219499588013f, z, 0.020763587206602097f), z,
-                                        -0.05377184599637985f), z, 0.13331729173660278f), z, -0.3333328366279602f), z,
-                         1.0f) * y;
-    const float t = copysignf(
-        1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * (2.0f * kLog2e))), y);
-    return cap * (a < 0.6f ? p : t);
+// Eight scores x, in units of `unit`, capped: cap tanh(x unit / cap), in the same units.
+// Up to 0.6 a polynomial (least maximum error over [0, 0.36] of tanh(y) / y in y^2:
+// 2.4e-9), past it, where a wave has such scores, 1 - 2 / (1 + e^2y), whose rounding
+// is then no larger than the result's own.
+__device__ __forceinline__ void cap_scores(float (&x)[8], float cap, float unit) {
+    const float in = unit / cap;
+    float y[8], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        y[j] = x[j] * in;
+        top = fmaxf(top, fabsf(y[j]));
+        const float z = y[j] * y[j];
+        x[j] *= fmaf(fmaf(fmaf(fmaf(fmaf(-0.005863219499588013f, z, 0.020763587206602097f), z, -0.05377184599637985f), z,
+                               0.13331729173660278f), z, -0.3333328366279602f), z, 1.0f);
+    }
+    if (__any(top > 0.6f)) {
+        const float out = cap / unit;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float a = fabsf(y[j]);
+            const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * (2.0f * kLog2e)));
+            x[j] = a > 0.6f ? copysignf(out * t, y[j]) : x[j];
+        }
+    }
 }
 
 // One of the 16 query columns of a wave: column c of a (sequence, kv head) is
@@ -258,6 +308,7 @@ __device__ __forceinline__ void column_place(const AttnArgs& a, const Rows& r, i
 }
 
 // The column's query: lane group g holds channels 8 g .. 8 g + 7 of every block,
+// (a column that is not the call's: row 0's, whose result goes nowhere)
 // scaled so that the largest of the row is in [2^13, 2^14) (f16 then has 2^-39
 // of it as its last place).
 template <int HD>
@@ -272,8 +323,8 @@ __device__ __forceinline__ void column_query(const AttnArgs& a, int lane, Column
         const f32x4 u = *reinterpret_cast<const f32x4u*>(q + 32 * b), v = *reinterpret_cast<const f32x4u*>(q + 32 * b + 4);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            x[b][i] = col.on ? u[i] : 0.0f;
-            x[b][4 + i] = col.on ? v[i] : 0.0f;
+            x[b][i] = u[i];
+            x[b][4 + i] = v[i];
             top = fmaxf(top, fmaxf(fabsf(x[b][i]), fabsf(x[b][4 + i])));
         }
     }
@@ -307,25 +358,22 @@ __device__ __forceinline__ void scores(const uint32_t (&k)[2][Shape<HD>::NB], co
     }
 }
 
-// Scores in the exponent's unit (log2), options applied.
+// Options applied: scores then in the exponent's unit (log2), as they were without any.
 template <int HD, bool MODS>
 __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD>& col, const uint32_t* kpos, int key0,
                                               float (&s)[8]) {
     if constexpr (MODS) {
-        const float inv = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[j] *= col.factor;
+        if (a.softcap > 0.0f) cap_scores(s, a.softcap, 1.0f);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            float x = s[j] * col.factor;
-            if (a.softcap > 0.0f) x = capped(x, a.softcap, inv);
             if (a.slopes) {
                 const int kp = kpos ? static_cast<int>(kpos[min(key0 + j, a.c.cap - 1)]) : key0 + j;
-                x = fmaf(-col.slope, static_cast<float>(abs(col.qpos - kp)), x);
+                s[j] = fmaf(-col.slope, static_cast<float>(abs(col.qpos - kp)), s[j]);
             }
-            s[j] = x * kLog2e;
+            s[j] *= kLog2e;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) s[j] *= col.factor * kLog2e;
     }
 }
 
@@ -375,23 +423,24 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
         if (kx < seen_lo || kx >= seen_hi) vx &= 0xFFFF0000u;
         if (kx + 1 < seen_lo || kx + 1 >= seen_hi) vx &= 0x0000FFFFu;
     }
-    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    const float f = MODS ? 1.0f : col.factor * kLog2e;
+    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * f;
     const uint32_t vm = max(vx & 0x7FFFu, (vx >> 16) & 0x7FFFu);
     if (__any(top > z.limit || vm > z.vbits)) {
-        int v = static_cast<int>(vm);
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m, 64));
+        int v = -group_min(-static_cast<int>(vm));
+        v = max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+                max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
         v = max(v, static_cast<int>(z.vbits)) >> 10;
         const int vexp = min(v, 30) - 14;
         const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + static_cast<float>(10 - z.vexp),
                               across_groups_max(top));
         const float base = m == -FLT_MAX ? -FLT_MAX : m + static_cast<float>(vexp - 10);
-        const float f = __builtin_amdgcn_exp2f(z.base - base);
-        z.l *= f;
+        const float k = __builtin_amdgcn_exp2f(z.base - base);
+        z.l *= k;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            z.o[b][0] *= f;
-            z.o[b][1] *= f;
+            z.o[b][0] *= k;
+            z.o[b][1] *= k;
         }
         z.base = base;
         z.limit = m == -FLT_MAX ? -FLT_MAX : m + 4.0f;
@@ -400,14 +449,15 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
     }
     float p[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(s[j] - z.base);
+    for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], f, -z.base));
     z.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    const float zero = hidden(0.0f);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float x = p[2 * i] * half_at(t.vd[b], 2 * i), y = p[2 * i + 1] * half_at(t.vd[b], 2 * i + 1);
+            float x = fmaf(p[2 * i], half_at(t.vd[b], 2 * i), zero), y = fmaf(p[2 * i + 1], half_at(t.vd[b], 2 * i + 1), zero);
             if constexpr (MASKED) {
                 x = seen[2 * i] ? x : 0.0f;
                 y = seen[2 * i + 1] ? y : 0.0f;
@@ -451,17 +501,10 @@ __device__ __forceinline__ void column_range(bool on, int first, int wide, int& 
     hi = wide ? first + wide : 0;
     flo = on ? first : 0;
     fhi = on ? first + wide : 0x7FFFFFFF;
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-        lo = min(lo, __shfl_xor(lo, m, 64));
-        hi = max(hi, __shfl_xor(hi, m, 64));
-        flo = max(flo, __shfl_xor(flo, m, 64));
-        fhi = min(fhi, __shfl_xor(fhi, m, 64));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    flo = __builtin_amdgcn_readfirstlane(flo);
-    fhi = __builtin_amdgcn_readfirstlane(fhi);
+    lo = __builtin_amdgcn_readfirstlane(group_min(lo));
+    hi = -__builtin_amdgcn_readfirstlane(group_min(-hi));
+    flo = -__builtin_amdgcn_readfirstlane(group_min(-flo));
+    fhi = __builtin_amdgcn_readfirstlane(group_min(fhi));
 }
 
 // Channels 32 b + 8 g .. + 7 of a column, from its sums.
@@ -475,17 +518,17 @@ __device__ __forceinline__ void channels(const Sums<HD>& z, int b, float factor,
 }
 
 // Attention of 16 columns by one workgroup: the four waves take every fourth tile
-// of the workgroup's share of the keys (KEYS), or each its own 16 columns.
-template <int HD, bool MODS, bool KEYS>
+// of the workgroup's share of the keys.
+template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, LD = HD + 4;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     int id = static_cast<int>(blockIdx.x);
-    const int split = KEYS ? id % a.splits : 0;
-    if (KEYS) id /= a.splits;
-    const int unit = id;  // of the arrival counters
-    const int ct = KEYS ? id % a.col_tiles : id % a.col_tiles * 4 + wave;
-    id /= a.col_tiles;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int unit = id, heads = a.c.seqs * a.c.n_kv;
+    const int ct = a.col_tiles - 1 - id / heads;  // (the longest rows first)
+    id %= heads;
     const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     if (static_cast<uint64_t>(ct) * 16 >= static_cast<uint64_t>(r.count) * a.group) return;
@@ -499,106 +542,442 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     Sums<HD> z;
     clear<HD>(z);
     const int t_lo = lo < hi ? lo / 32 : 0, tiles = lo < hi ? (hi + 31) / 32 - t_lo : 0;
-    if constexpr (!KEYS) {
-        walk<HD, MODS>(a, p, lane, col, kpos, t_lo, t_lo + tiles, 1, flo, fhi, lo, hi, z);
-        const float l = across_groups_sum(z.l);
-        if (!col.on) return;
-        float* out = a.out + (static_cast<size_t>(col.row) * a.n_heads + col.head) * HD + g * 8;
-        const float f = col.bad ? __builtin_nanf("") : l == 0.0f ? 0.0f : 1.0f / l;
+    const int t0 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+    const int t1 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, lo, hi, z);
+    // join the waves
+    __shared__ float so[4][16][LD], sb[4][16], sl[4][16];
+    __shared__ int last;
+    const float l = across_groups_sum(z.l);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            float x[8];
-            channels<HD>(z, b, f, x);
+    for (int b = 0; b < NB; b++) {
+        float x[8];
+        channels<HD>(z, b, 1.0f, x);
+        *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g]) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g + 4]) = f32x4{x[4], x[5], x[6], x[7]};
+    }
+    if (g == 0) {
+        sb[wave][n] = z.base;
+        sl[wave][n] = l;
+    }
+    __syncthreads();
+    constexpr int PER = HD / 16;  // channels of a column that a thread joins
+    const int cj = threadIdx.x >> 4, ch = (threadIdx.x & 15) * PER;
+    float base = fmaxf(fmaxf(sb[0][cj], sb[1][cj]), fmaxf(sb[2][cj], sb[3][cj]));
+    float sum = 0.0f, x[PER];
 #pragma unroll
-            for (int i = 0; i < 8; i++) out[32 * b + i] = x[i];
-        }
-        if (a.lse && g == 0)
-            a.lse[static_cast<size_t>(col.row) * a.n_heads + col.head] =
-                col.bad ? __builtin_nanf("") : (z.base + log2f(l)) * kLn2;
-        return;
-    } else {
-        const int t0 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-        const int t1 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-        walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, lo, hi, z);
-        // join the waves
-        __shared__ float so[4][16][LD], sb[4][16], sl[4][16];
-        __shared__ int last;
-        const float l = across_groups_sum(z.l);
+    for (int i = 0; i < PER; i++) x[i] = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            float x[8];
-            channels<HD>(z, b, 1.0f, x);
-            *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g]) = f32x4{x[0], x[1], x[2], x[3]};
-            *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g + 4]) = f32x4{x[4], x[5], x[6], x[7]};
+    for (int w = 0; w < 4; w++) {
+        const float f = __builtin_amdgcn_exp2f(sb[w][cj] - base);
+        sum = fmaf(sl[w][cj], f, sum);
+#pragma unroll
+        for (int i = 0; i < PER; i++) x[i] = fmaf(so[w][cj][ch + i], f, x[i]);
+    }
+    const uint32_t c = static_cast<uint32_t>(ct) * 16 + cj;
+    Column<HD> mine;  // (its place only)
+    column_place<HD, false>(a, r, kv, c, mine);
+    if (a.splits > 1) {
+        float* part = a.part + (static_cast<size_t>(unit) * a.splits * 16 + cj) * (HD + 2);
+        float* to = part + static_cast<size_t>(split) * 16 * (HD + 2);
+        if (mine.on) {
+            if (ch == 0) {
+                __hip_atomic_store(to, base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(to + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                __hip_atomic_store(to + 2 + ch + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        if (g == 0) {
-            sb[wave][n] = z.base;
-            sl[wave][n] = l;
-        }
+        // Every thread's coherent stores complete before the arrival count moves.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        constexpr int PER = HD / 16;  // channels of a column that a thread joins
-        const int cj = threadIdx.x >> 4, ch = (threadIdx.x & 15) * PER;
-        float base = fmaxf(fmaxf(sb[0][cj], sb[1][cj]), fmaxf(sb[2][cj], sb[3][cj]));
-        float sum = 0.0f, x[PER];
+        if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0)
+            __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!mine.on) return;
+        base = -FLT_MAX;
+        for (int i = 0; i < a.splits; i++)
+            base = fmaxf(base, __hip_atomic_load(part + static_cast<size_t>(i) * 16 * (HD + 2), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT));
+        sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; i++) x[i] = 0.0f;
+        for (int sp = 0; sp < a.splits; sp++) {
+            const float* from = part + static_cast<size_t>(sp) * 16 * (HD + 2);
+            const float f = __builtin_amdgcn_exp2f(
+                __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - base);
+            sum = fmaf(__hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f, sum);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float f = __builtin_amdgcn_exp2f(sb[w][cj] - base);
-            sum = fmaf(sl[w][cj], f, sum);
-#pragma unroll
-            for (int i = 0; i < PER; i++) x[i] = fmaf(so[w][cj][ch + i], f, x[i]);
+            for (int i = 0; i < PER; i++)
+                x[i] = fmaf(__hip_atomic_load(from + 2 + ch + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f,
+                            x[i]);
         }
-        const uint32_t c = static_cast<uint32_t>(ct) * 16 + cj;
-        Column<HD> mine;  // (its place only)
-        column_place<HD, false>(a, r, kv, c, mine);
-        if (a.splits > 1) {
-            float* part = a.part + (static_cast<size_t>(unit) * a.splits * 16 + cj) * (HD + 2);
-            float* to = part + static_cast<size_t>(split) * 16 * (HD + 2);
-            if (mine.on) {
-                if (ch == 0) {
-                    __hip_atomic_store(to, base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(to + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!mine.on) return;
+    float* out = a.out + (static_cast<size_t>(mine.row) * a.n_heads + mine.head) * HD + ch;
+    const float f = mine.bad ? __builtin_nanf("") : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < PER; i++) out[i] = x[i] * f;
+    if (a.lse && ch == 0)
+        a.lse[static_cast<size_t>(mine.row) * a.n_heads + mine.head] =
+            mine.bad ? __builtin_nanf("") : (base + log2f(sum)) * kLn2;
+}
+
+// ---- attention of many columns --------------------------------------------------
+
+// What is staged of 32 keys, as the matrix cores take it: fragments [lane][8 f16].
+template <int HD>
+struct Stage {
+    uint32_t k[2][Shape<HD>::NB][2][64][4];  // keys as MFMA rows 0 .. 15 and 16 .. 31, by block and f16 term
+    uint32_t v[Shape<HD>::NB][2][2][64][4];  // values, by block, channel parity and f16 term
+};
+// Per key of four tiles: 2^e and 2^-e, e the largest exponent of its scales (of values:
+// under vexp), and the bits of a scale to take: none of a key that nobody sees
+// or that holds a NaN, whose 2^e is then NaN.
+struct Factors {
+    float up[4][32], down[4][32];
+    uint16_t ok[4][32];
+};
+template <int HD>
+struct Room {
+    Stage<HD> stage[2];
+    Factors k, v;
+    int range[2], vbits[4];
+};
+
+// One thread's share of a tile on its way to LDS.
+template <int HD>
+struct Load {
+    static constexpr int W = HD == 128 ? 2 : 1;  // words of keys
+    uint32_t k[W];
+    uint16_t kd[W];
+    u32x4 v, vd;
+    uint16_t d[Shape<HD>::NB];  // a key's scales, two tiles ahead (threads 0 .. 31 values', 32 .. 63 keys')
+};
+
+// A thread stages the levels of one key (MFMA row n of half h), channels 8 g .. + 7 of
+// blocks kb .. kb + W - 1; and of octet g the nibbles at ve (head width 128: both) of
+// the 2-byte units of lane n in block vb.
+template <int HD>
+struct Part {
+    static constexpr int NB = Shape<HD>::NB, BP = Shape<HD>::BP, W = Load<HD>::W;
+    int n, g, h, kb, vb, ve;
+    bool on;
+    __device__ __forceinline__ explicit Part(int tid) {
+        n = tid & 15;
+        g = tid >> 4 & 3;
+        h = tid >> 6 & 1;
+        kb = (tid >> 7) * W;
+        vb = HD == 128 ? tid >> 6 : HD == 64 ? tid >> 6 & 1 : 0;
+        ve = HD == 128 ? 0 : HD == 64 ? tid >> 7 : tid >> 6 & 1;
+        on = HD >= 64 || tid < 128;
+    }
+    __device__ __forceinline__ int key() const { return 8 * (n >> 2) + (n & 3) + 4 * h; }
+    __device__ __forceinline__ int unit() const { return HD >= 64 ? n * BP + vb / 2 : n & 7; }
+    __device__ __forceinline__ int shift() const { return HD >= 64 ? vb % 2 * 8 : (n >> 3) * 8; }
+};
+
+template <int HD>
+__device__ __forceinline__ void load_part(const Planes& p, int cap, int tile, const Part<HD>& w, Load<HD>& t) {
+    constexpr int NB = Shape<HD>::NB, VU = HD / 4;
+    if (!w.on) return;
+    // (a tile's end past the capacity reads the last rows again; they weigh nothing)
+    const uint32_t key = min(tile * 32 + w.key(), cap - 1), o = min(tile * 4 + w.g, cap / 8 - 1);
+    const uint8_t* a = p.k + static_cast<size_t>(key * (HD / 2) + (w.g * NB + w.kb) * 4);
+    if constexpr (HD == 128) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(a);
+        t.k[0] = x[0];
+        t.k[1] = x[1];
+    } else {
+        t.k[0] = *reinterpret_cast<const uint32_t*>(a);
+    }
+#pragma unroll
+    for (int i = 0; i < Load<HD>::W; i++) t.kd[i] = p.kd[key / 8 * (NB * 8) + (w.kb + i) * 8 + key % 8];
+    t.v = *reinterpret_cast<const u32x4*>(p.v + (o * VU + w.unit()) * 16);
+    t.vd = *reinterpret_cast<const u32x4*>(p.vd + (o * NB + w.vb) * 8);
+}
+
+__device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
+__device__ __forceinline__ uint32_t bits(half2v x) { return __builtin_bit_cast(uint32_t, x); }
+
+// level * scale in f16 and what that leaves, both exact: 15 bits.
+__device__ __forceinline__ void times_scale(uint32_t level, half2v scale, uint32_t& hi, uint32_t& lo) {
+    const half2v x = as_half2(level), h = x * scale;
+    hi = bits(h);
+    lo = bits(__builtin_elementwise_fma(x, scale, -h));
+}
+template <int HD, int I>
+__device__ __forceinline__ void store_values(const Part<HD>& w, const u32x4& v, const uint32_t (&d)[4], Stage<HD>& st) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) times_scale(levels2<I>(v[i] >> w.shift()), as_half2(d[i]), hi[i], lo[i]);
+    const int lane = w.g * 16 + w.n;
+    *reinterpret_cast<u32x4*>(st.v[w.vb][I][0][lane]) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+    *reinterpret_cast<u32x4*>(st.v[w.vb][I][1][lane]) = u32x4{lo[0], lo[1], lo[2], lo[3]};
+}
+
+template <int HD>
+__device__ __forceinline__ void store_part(int tile, const Part<HD>& w, const Load<HD>& t, const Factors& fk,
+                                           const Factors& fv, float vdown, Stage<HD>& st) {
+    if (!w.on) return;
+    const int lane = w.g * 16 + w.n, f = tile & 3, key = w.key();
+#pragma unroll
+    for (int i = 0; i < Load<HD>::W; i++) {
+        const _Float16 x = static_cast<_Float16>(fh_h2f(t.kd[i] & fk.ok[f][key]) * fk.down[f][key]);
+        const half2v sc = {x, x};
+        uint32_t hi[4], lo[4];
+        times_scale(levels2<0>(t.k[i]), sc, hi[0], lo[0]);
+        times_scale(levels2<1>(t.k[i]), sc, hi[1], lo[1]);
+        times_scale(levels2<2>(t.k[i]), sc, hi[2], lo[2]);
+        times_scale(levels2<3>(t.k[i]), sc, hi[3], lo[3]);
+        *reinterpret_cast<u32x4*>(st.k[w.h][w.kb + i][0][lane]) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+        *reinterpret_cast<u32x4*>(st.k[w.h][w.kb + i][1][lane]) = u32x4{lo[0], lo[1], lo[2], lo[3]};
+    }
+    const u32x4 ok = *reinterpret_cast<const u32x4*>(&fv.ok[f][8 * w.g]);
+    uint32_t d[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const half2v x = as_half2(t.vd[i] & ok[i]);
+        const half2v y = {static_cast<_Float16>(static_cast<float>(x[0]) * (fv.down[f][8 * w.g + 2 * i] * vdown)),
+                          static_cast<_Float16>(static_cast<float>(x[1]) * (fv.down[f][8 * w.g + 2 * i + 1] * vdown))};
+        d[i] = bits(y);
+    }
+    if constexpr (HD == 128) {
+        store_values<HD, 0>(w, t.v, d, st);
+        store_values<HD, 1>(w, t.v, d, st);
+    } else {
+        if (w.ve) store_values<HD, 1>(w, t.v, d, st);
+        else store_values<HD, 0>(w, t.v, d, st);
+    }
+}
+
+constexpr int kPromptTiles = 2;  // tiles of 16 columns of a wave
+
+// Attention of 128 columns of one (sequence, kv head): four waves with 32
+// columns each walk the same keys, 32 at a time, expanded once into LDS for all
+// of them: keys and values as level * scale in two exact f16 terms, so that
+// neither a score nor a weight takes its scale block by block, and every product
+// of an f32 operand (two terms as well) is three matrix products, the lowest left
+// out (2^-22).  The range of f16 is each key's own (2^-e here, 2^e on its score or
+// weight; values under their block's largest exponent over all the keys), so
+// nothing loses bits beside a larger key or block.
+template <int HD, bool MODS>
+__global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
+    constexpr int NB = Shape<HD>::NB, CT = kPromptTiles;
+    extern __shared__ __align__(16) char smem[];
+    Room<HD>& room = *reinterpret_cast<Room<HD>*>(smem);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int heads = a.c.seqs * a.c.n_kv;
+    const int id = static_cast<int>(blockIdx.x) % heads;
+    const int ct0 = (a.col_tiles - 1 - static_cast<int>(blockIdx.x) / heads) * 4 * CT;  // (the longest rows first)
+    const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
+    if (static_cast<uint64_t>(ct0) * 16 >= static_cast<uint64_t>(r.count) * a.group) return;
+    Column<HD> col[CT];
+    int lo = 0x7FFFFFFF, hi = 0, flo = 0, fhi = 0x7FFFFFFF;
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        column_place<HD, MODS>(a, r, kv, static_cast<uint32_t>(ct0 + wave * CT + c) * 16 + n, col[c]);
+        int x, y, fx, fy;
+        column_range(col[c].on, col[c].first, col[c].wide, x, y, fx, fy);
+        lo = min(lo, x);
+        hi = max(hi, y);
+        flo = max(flo, fx);
+        fhi = min(fhi, fy);
+    }
+    if (tid == 0) {
+        room.range[0] = 0x7FFFFFFF;
+        room.range[1] = 0;
+    }
+    if (tid < 4) room.vbits[tid] = 0;
+    __syncthreads();
+    if (lane == 0) {
+        atomicMin(&room.range[0], lo);
+        atomicMax(&room.range[1], hi);
+    }
+    __syncthreads();
+    const int glo = room.range[0], ghi = room.range[1];
+    const int t0 = glo < ghi ? glo / 32 : 0, t1 = glo < ghi ? (ghi + 31) / 32 : 0;
+    const Planes p = planes_of<HD>(a.c, s, kv);
+    const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + (static_cast<size_t>(s) * a.c.n_kv + kv) * a.c.cap : nullptr;
+    const Part<HD> part(tid);
+    Load<HD> ld;
+    const auto load_scales = [&](int tile) {
+        const uint32_t key = min(tile * 32 + (tid & 31), a.c.cap - 1);
+        const uint16_t* from = (tid < 32 ? p.vd : p.kd) + key / 8 * (NB * 8) + key % 8;
+#pragma unroll
+        for (int b = 0; b < NB; b++) ld.d[b] = from[b * 8];
+    };
+    if (t0 < t1) {
+        load_part<HD>(p, a.c.cap, t0, part, ld);
+        // the largest exponent of each block's value scales
+        uint32_t m = 0;
+        for (int i = t0 * 4 * NB + tid; i < min(t1 * 4, a.c.cap / 8) * NB; i += kThreads) {  // (NB divides kThreads: one block a thread)
+            const u32x4 w = *reinterpret_cast<const u32x4*>(p.vd + static_cast<size_t>(i) * 8);
+            const int k0 = i / NB * 8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t x = w[j >> 1] >> (16 * (j & 1)) & 0x7FFFu;
+                m = k0 + j >= glo && k0 + j < ghi && x < 0x7C00u ? max(m, x) : m;
+            }
+        }
+        atomicMax(&room.vbits[tid % NB], static_cast<int>(m));
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) column_query<HD>(a, lane, col[c]);
+    __syncthreads();
+    int vexp[NB];
+    float vdown = 1.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        vexp[b] = min(__builtin_amdgcn_readfirstlane(room.vbits[b]) >> 10, 30) - 14;
+        vdown = part.vb == b ? ldexpf(1.0f, -vexp[b]) : vdown;
+    }
+    const auto key_factors = [&](int tile) {  // of key tid % 32, from ld.d
+        int e = -64;
+        bool fine = true;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int x = ld.d[b] >> 10 & 31;
+            fine = fine && x < 31;
+            e = max(e, x - 14 - (tid < 32 ? vexp[b] : 0));
+        }
+        const int key = tile * 32 + (tid & 31);
+        const bool seen = key >= glo && key < ghi;
+        e = fine && seen ? e : 0;
+        Factors& f = tid < 32 ? room.v : room.k;
+        f.up[tile & 3][tid & 31] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
+        f.down[tile & 3][tid & 31] = ldexpf(1.0f, -e);
+        f.ok[tile & 3][tid & 31] = fine && seen ? 0xFFFF : 0;
+    };
+    f32x4 o[CT][NB][2];
+    float l[CT], base[CT], limit[CT], unit_of[CT];  // unit_of: log2 units of a score's own
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        l[c] = 0.0f;
+        base[c] = limit[c] = -FLT_MAX;
+        unit_of[c] = MODS && a.slopes ? kLog2e : col[c].factor * kLog2e;
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[c][b][0] = o[c][b][1] = f32x4{0, 0, 0, 0};
+    }
+    if (t0 < t1) {
+        if (tid < 64) {
+            load_scales(t0);
+            key_factors(t0);
+            load_scales(t0 + 1);
+            key_factors(t0 + 1);
+        }
+        __syncthreads();
+        store_part<HD>(t0, part, ld, room.k, room.v, vdown, room.stage[t0 & 1]);
+    }
+    for (int t = t0; t < t1; t++) {
+        __syncthreads();
+        if (t + 1 < t1) load_part<HD>(p, a.c.cap, t + 1, part, ld);
+        if (tid < 64) load_scales(t + 2);
+        const Stage<HD>& st = room.stage[t & 1];
+        if (t * 32 < hi && t * 32 + 32 > lo) {
+            f32x4 d[CT][2];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const half8 kh = *reinterpret_cast<const half8*>(st.k[h][b][0][lane]);
+                    const half8 kl = *reinterpret_cast<const half8*>(st.k[h][b][1][lane]);
+#pragma unroll
+                    for (int c = 0; c < CT; c++)
+                        d[c][h] = mfma(kh, col[c].hi[b], mfma(kh, col[c].lo[b], mfma(kl, col[c].hi[b],
+                                       b == 0 ? f32x4{0, 0, 0, 0} : d[c][h])));
                 }
+            const bool full = t * 32 >= flo && t * 32 + 32 <= fhi;
+            const int key0 = t * 32 + 8 * g;
+            half8 ph[CT], pl[CT];
+            const float *kup = room.k.up[t & 3] + 8 * g, *vup = room.v.up[t & 3] + 8 * g;
 #pragma unroll
-                for (int i = 0; i < PER; i++)
-                    __hip_atomic_store(to + 2 + ch + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int c = 0; c < CT; c++) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = d[c][j >> 2][j & 3] * kup[j];
+                if constexpr (MODS) {
+                    if (a.softcap > 0.0f) cap_scores(x, a.softcap, col[c].factor);
+                    if (a.slopes) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int kp = kpos ? static_cast<int>(kpos[min(key0 + j, a.c.cap - 1)]) : key0 + j;
+                            x[j] = fmaf(-col[c].slope, static_cast<float>(abs(col[c].qpos - kp)), x[j] * col[c].factor);
+                        }
+                    }
+                }
+                if (!full) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (!(static_cast<uint32_t>(key0 + j - col[c].first) < static_cast<uint32_t>(col[c].wide)))
+                            x[j] = -INFINITY;
+                }
+                const float f = unit_of[c];
+                const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * f;
+                if (__any(top > limit[c])) {
+                    const float m = fmaxf(base[c] == -FLT_MAX ? -FLT_MAX : base[c] + 10.0f, across_groups_max(top));
+                    const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, k = __builtin_amdgcn_exp2f(base[c] - nb);
+                    l[c] *= k;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        o[c][b][0] *= k;
+                        o[c][b][1] *= k;
+                    }
+                    base[c] = nb;
+                    limit[c] = m == -FLT_MAX ? -FLT_MAX : m + 4.0f;
+                }
+                uint32_t hw[4], lw[4];
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float u = __builtin_amdgcn_exp2f(fmaf(x[2 * j], f, -base[c])),
+                                v = __builtin_amdgcn_exp2f(fmaf(x[2 * j + 1], f, -base[c]));
+                    sum += u + v;
+                    float uw = u * vup[2 * j], vw = v * vup[2 * j + 1];
+                    if (!full) {  // (a NaN of a key that this row does not see stays out)
+                        uw = x[2 * j] == -INFINITY ? 0.0f : uw;
+                        vw = x[2 * j + 1] == -INFINITY ? 0.0f : vw;
+                    }
+                    split2(uw, vw, hw[j], lw[j]);
+                }
+                l[c] += sum;
+                ph[c] = as_half8(hw[0], hw[1], hw[2], hw[3]);
+                pl[c] = as_half8(lw[0], lw[1], lw[2], lw[3]);
             }
-            // Every thread's coherent stores complete before the arrival count moves.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
-            __syncthreads();
-            if (!last) return;
-            if (threadIdx.x == 0)
-                __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (!mine.on) return;
-            base = -FLT_MAX;
-            for (int i = 0; i < a.splits; i++)
-                base = fmaxf(base, __hip_atomic_load(part + static_cast<size_t>(i) * 16 * (HD + 2), __ATOMIC_RELAXED,
-                                                     __HIP_MEMORY_SCOPE_AGENT));
-            sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; i++) x[i] = 0.0f;
-            for (int sp = 0; sp < a.splits; sp++) {
-                const float* from = part + static_cast<size_t>(sp) * 16 * (HD + 2);
-                const float f = __builtin_amdgcn_exp2f(
-                    __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - base);
-                sum = fmaf(__hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f, sum);
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < PER; i++)
-                    x[i] = fmaf(__hip_atomic_load(from + 2 + ch + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f,
-                                x[i]);
-            }
+                for (int e = 0; e < 2; e++) {
+                    const half8 vh = *reinterpret_cast<const half8*>(st.v[b][e][0][lane]);
+                    const half8 vl = *reinterpret_cast<const half8*>(st.v[b][e][1][lane]);
+#pragma unroll
+                    for (int c = 0; c < CT; c++)
+                        o[c][b][e] = mfma(vh, ph[c], mfma(vh, pl[c], mfma(vl, ph[c], o[c][b][e])));
+                }
         }
-        if (!mine.on) return;
-        float* out = a.out + (static_cast<size_t>(mine.row) * a.n_heads + mine.head) * HD + ch;
-        const float f = mine.bad ? __builtin_nanf("") : sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (t + 1 < t1) store_part<HD>(t + 1, part, ld, room.k, room.v, vdown, room.stage[(t + 1) & 1]);
+        if (tid < 64) key_factors(t + 2);
+    }
+    // Each lane has 8 channels of every block of its columns: 32 b + 8 g + i at o[b][i & 1][i >> 1] * 2^vexp[b].
 #pragma unroll
-        for (int i = 0; i < PER; i++) out[i] = x[i] * f;
-        if (a.lse && ch == 0)
-            a.lse[static_cast<size_t>(mine.row) * a.n_heads + mine.head] =
-                mine.bad ? __builtin_nanf("") : (base + log2f(sum)) * kLn2;
+    for (int c = 0; c < CT; c++) l[c] = across_groups_sum(l[c]);
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        if (!col[c].on) continue;
+        float* out = a.out + (static_cast<size_t>(col[c].row) * a.n_heads + col[c].head) * HD + g * 8;
+        const float f = col[c].bad ? __builtin_nanf("") : l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) out[32 * b + i] = o[c][b][i & 1][i >> 1] * ldexpf(f, vexp[b]);
+        if (a.lse && g == 0)
+            a.lse[static_cast<size_t>(col[c].row) * a.n_heads + col[c].head] =
+                col[c].bad ? __builtin_nanf("") : (base[c] + log2f(l[c])) * kLn2;
     }
 }
 
@@ -631,13 +1010,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh(AttnArgs a) {
         if (!__any(col.wide && col.first < tile * 32 + 32 && col.first + col.wide > tile * 32)) continue;
         column_query<HD>(a, lane, col);
         const float lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
+        const float f = MODS ? 1.0f : col.factor * kLog2e;
         float x[8];
         scores<HD>(k, kd, col, x);
         finish_scores<HD, MODS>(a, col, kpos, key0, x);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             acc[j] += static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide)
-                          ? __builtin_amdgcn_exp2f(x[j] - lse) : 0.0f;
+                          ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse)) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -661,48 +1041,124 @@ struct AppendArgs {
     const float* qkv;
     size_t ld;
     uint32_t total, max_rows;
-    int n_heads, hd, octets, heads;  // heads: kv heads of a workgroup, with their query heads
+    int n_heads, octets, heads;  // heads: kv heads of a workgroup, with their query heads
     const uint32_t *off, *len, *pos;
-    int rope_dim, neox;
+    int rope_dim, neox, quads;  // quads: every four channels from a multiple of 4 are 16-byte aligned, and so are their partners
     float base, linear;
     const float* ff;
     float* q;
 };
 
-// apply_rope's rotation (llm.rs:146-175, the angle of RopeScaling::angle, llm.rs:118-121, in
-// 32 bits as there) with sine, cosine and products in 64 bits: a key's channel goes on to the
-// border between two levels, where its last bit decides.
-__device__ __forceinline__ float rope_angle(uint32_t pos, int i, const AppendArgs& a) {
+// The frequency of pair i and the angle at a position: apply_rope's (llm.rs:146-175, RopeScaling::angle,
+// llm.rs:118-121), in 32 bits as there.
+__device__ __forceinline__ float rope_frequency(int i, const AppendArgs& a) {
+    return static_cast<float>(pow(static_cast<double>(a.base), -2.0 * i / static_cast<double>(a.rope_dim)));
+}
+__device__ __forceinline__ float rope_angle(uint32_t pos, int i, float freq, const AppendArgs& a) {
 #pragma clang fp contract(off)
-    const float freq =
-        static_cast<float>(pow(static_cast<double>(a.base), -2.0 * i / static_cast<double>(a.rope_dim)));
     const float f = a.ff ? a.ff[i] : 1.0f;
     return static_cast<float>(static_cast<int>(pos)) * freq / f * (1.0f / a.linear);
 }
 
-// One channel of a head row, rotated where it is one of the first rope_dim.
-__device__ __forceinline__ float rotated(const float* x, int ch, const AppendArgs& a, const double2* turn) {
+// Four channels from ch (a multiple of 4) of a head row, rotated where they are
+// among the first rope_dim: angles in 32 bits as fh_rope_async's, sine, cosine
+// and products in 64, since a key's channel goes on to the border between two
+// levels, where its last bit decides.
+__device__ __forceinline__ f32x4 rotated4(const float* x, int ch, const AppendArgs& a, const double2* turn) {
 #pragma clang fp contract(off)
-    const float own = x[ch];
-    if (ch >= a.rope_dim) return own;
     const int half = a.rope_dim / 2;
-    const bool second = a.neox ? ch >= half : ch & 1;
-    const int i = a.neox ? (second ? ch - half : ch) : ch >> 1;
-    const double other = x[a.neox ? (second ? ch - half : ch + half) : ch ^ 1];
-    const double2 t = turn[i];  // (cosine, sine)
-    return static_cast<float>(second ? other * t.y + own * t.x : own * t.x - other * t.y);
+    float own[4], other[4];
+    const bool second = ch >= half;
+    if (a.quads) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(x + ch);
+        f32x4 v = f32x4{u[1], u[0], u[3], u[2]};
+        if (a.neox && ch < a.rope_dim) v = *reinterpret_cast<const f32x4*>(x + (second ? ch - half : ch + half));
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            own[k] = u[k];
+            other[k] = v[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int c = ch + k;
+            own[k] = x[c];
+            other[k] = c < a.rope_dim ? x[a.neox ? (c >= half ? c - half : c + half) : c ^ 1] : 0.0f;
+        }
+    }
+    f32x4 y;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int c = ch + k;
+        y[k] = own[k];
+        if (c < a.rope_dim) {
+            const bool hi = a.neox ? c >= half : c & 1;
+            const double2 t = turn[a.neox ? (hi ? c - half : c) : c >> 1];  // (cosine, sine)
+            const double u = own[k], v = other[k];
+            y[k] = static_cast<float>(hi ? v * t.y + u * t.x : u * t.x - v * t.y);
+        }
+    }
+    return y;
+}
+
+// Exchange within eight consecutive lanes.
+__device__ __forceinline__ float max8(float v) {
+    v = fmaxf(v, fh::dpp<0xB1>(v));
+    v = fmaxf(v, fh::dpp<0x4E>(v));
+    return fmaxf(v, fh::dpp<0x141>(v));
+}
+__device__ __forceinline__ int min8(int v) {
+    v = min(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false));
+    return min(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false));
+}
+
+// The scale (f16 bits) and levels of a block whose channels 4 l .. 4 l + 3 lane l of
+// eight holds: nibbles of channels 0, 1 (bits 0 .. 7) and 2, 3 (8 .. 15) of the lane's four.
+__device__ __forceinline__ void quantise4(const f32x4& x, uint16_t& scale, uint32_t& levels) {
+    const int l = threadIdx.x & 7;
+    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    const bool fine = fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY && fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY;
+    top = max8(fine ? top : INFINITY);
+    int at = 127;  // 2 * (first channel of that magnitude) + its sign
+#pragma unroll
+    for (int k = 3; k >= 0; k--)
+        if (fabsf(x[k]) == top) at = 2 * (4 * l + k) + (x[k] < 0.0f);
+    at = min8(at);
+    const float m = at & 1 ? -top : top;
+    const bool odd = !(top < INFINITY);
+    _Float16 dh = static_cast<_Float16>(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
+    if (odd) dh = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7E00));
+    const float d = static_cast<float>(dh), inv = __builtin_amdgcn_rcpf(d), lim = 0.5f * fabsf(d);
+    const bool flat = odd || d == 0.0f;
+    levels = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        // the nearest level, ties to even: from an approximate quotient, put right by the
+        // remainder, which one FMA gives exactly
+        float t = rintf(x[k] * inv);
+        const float rest = fmaf(-t, d, x[k]), over = fabsf(rest) - lim;
+        const bool odd_t = static_cast<int>(t) & 1;
+        if (over > 0.0f || (over == 0.0f && odd_t)) t += (rest > 0.0f) == (d > 0.0f) ? 1.0f : -1.0f;
+        const uint32_t q = flat ? 8u : static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(t, -8.0f), 7.0f)) + 8);
+        levels |= q << (4 * k);
+    }
+    scale = __builtin_bit_cast(uint16_t, dh);
 }
 
 // The eight cache rows of one octet: rotate and store their queries, quantise
-// their keys and values.  A wave's halves each take one block of 32 channels.
+// their keys and values, eight lanes a block.
+template <int HD>
 __global__ void __launch_bounds__(kThreads) k_kv4_append(AppendArgs a) {
-    extern __shared__ char smem[];
-    const int hd = a.hd, nb = hd / 32, vn = hd >= 64 ? 16 : 8, bp = hd >= 64 ? hd / 64 : 1, half = a.rope_dim / 2;
-    double2* turn = reinterpret_cast<double2*>(smem);  // [8][half]
-    uint8_t* kl = reinterpret_cast<uint8_t*>(turn + 8 * half);  // [heads][8][hd / 2]
-    uint8_t* vl = kl + a.heads * 4 * hd;                        // [heads][vn][bp][8][2]
-    uint16_t* kdl = reinterpret_cast<uint16_t*>(vl + a.heads * 4 * hd);  // [heads][nb][8]
-    uint16_t* vdl = kdl + a.heads * nb * 8;
+    constexpr int NB = Shape<HD>::NB, VN = Shape<HD>::N, BP = Shape<HD>::BP, KW = HD / 8, VU = HD / 4;
+    extern __shared__ __align__(16) char smem[];
+    const int half = a.rope_dim / 2;
+    double2* turn = reinterpret_cast<double2*>(smem);           // [8][half]
+    uint8_t* kl = reinterpret_cast<uint8_t*>(turn + 8 * half);  // [heads][8][HD / 2]
+    uint8_t* vl = kl + a.heads * 4 * HD;                        // [heads][VN][BP][8][2]
+    uint16_t* kdl = reinterpret_cast<uint16_t*>(vl + a.heads * 4 * HD);  // [heads][NB][8]
+    uint16_t* vdl = kdl + a.heads * NB * 8;
+    float* freq = reinterpret_cast<float*>(vdl + a.heads * NB * 8);  // [half]
     const int h0 = static_cast<int>(blockIdx.y) * a.heads, heads = min(a.heads, a.c.n_kv - h0);
     const int group = a.n_heads / a.c.n_kv;
     const int s = static_cast<int>(blockIdx.x) / a.octets;
@@ -714,86 +1170,97 @@ __global__ void __launch_bounds__(kThreads) k_kv4_append(AppendArgs a) {
     if (j0 >= j1) return;
     const uint32_t row0 = r.begin + static_cast<uint32_t>(oct * 8 + j0 - r.at);  // the call's row of j0
     const bool store = oct < static_cast<uint64_t>(a.c.cap / 8);
-    for (int i = threadIdx.x; i < (j1 - j0) * half; i += kThreads) {
-        const int j = j0 + i / half;
-        const uint32_t row = row0 + (j - j0);
-        const uint32_t pos = a.pos ? a.pos[row] : static_cast<uint32_t>(oct * 8 + j);
-        double sn, cs;
-        sincos(static_cast<double>(rope_angle(pos, i % half, a)), &sn, &cs);
-        turn[j * half + i % half] = make_double2(cs, sn);
+    if (half) {
+        for (int i = threadIdx.x; i < half; i += kThreads) freq[i] = rope_frequency(i, a);
+        __syncthreads();
+        for (int i = threadIdx.x; i < (j1 - j0) * half; i += kThreads) {
+            const int j = j0 + i / half;
+            const uint32_t row = row0 + (j - j0);
+            const uint32_t pos = a.pos ? a.pos[row] : static_cast<uint32_t>(oct * 8 + j);
+            double sn, cs;
+            sincos(static_cast<double>(rope_angle(pos, i % half, freq[i % half], a)), &sn, &cs);
+            turn[j * half + i % half] = make_double2(cs, sn);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (a.q) {
-        const int wide = heads * group * hd;
-        for (int i = threadIdx.x; i < (j1 - j0) * wide; i += kThreads) {
-            const int jj = i / wide, c = i - jj * wide + h0 * group * hd;
+        constexpr int PER = HD / 4;
+        const int wide = heads * group * PER;
+        for (int jj = 0; jj < j1 - j0; jj++) {
             const size_t row = row0 + jj;
-            a.q[row * (a.n_heads * hd) + c] =
-                rotated(a.qkv + row * a.ld + c / hd * hd, c % hd, a, turn + (j0 + jj) * half);
+            const float* x = a.qkv + row * a.ld + static_cast<size_t>(h0) * group * HD;
+            float* y = a.q + (row * a.n_heads + static_cast<size_t>(h0) * group) * HD;
+            for (int u = threadIdx.x; u < wide; u += kThreads) {
+                const f32x4 v = rotated4(x + u / PER * HD, u % PER * 4, a, turn + (j0 + jj) * half);
+                if (a.quads) *reinterpret_cast<f32x4*>(y + u * 4) = v;
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; k++) y[u * 4 + k] = v[k];
+            }
         }
     }
     if (!store) return;
-    const int side = threadIdx.x >> 5, i = threadIdx.x & 31, blocks = heads * nb;
-    for (int u = side; u < (j1 - j0) * blocks * 2; u += kThreads / 32) {
-        const int jj = u / (blocks * 2), v = u % 2, hb = u / 2 % blocks, h = hb / nb, b = hb % nb, j = j0 + jj;
-        const size_t row = row0 + jj;
-        const float* x = a.qkv + row * a.ld + static_cast<size_t>(a.n_heads + (v ? a.c.n_kv : 0) + h0 + h) * hd;
-        const float y = v ? x[32 * b + i] : rotated(x, 32 * b + i, a, turn + j * half);
-        float top = fabsf(y);
+    const int l = threadIdx.x & 7, blocks = heads * NB;
+    for (int jj = 0; jj < j1 - j0; jj++) {
+        const int j = j0 + jj;
+        const float* x = a.qkv + (row0 + jj) * a.ld + static_cast<size_t>(a.n_heads + h0) * HD;
+        // (the eight lanes of a block leave the loop together, which is all that the exchange needs)
+        for (int u = threadIdx.x >> 3; u < blocks * 2; u += kThreads / 8) {
+            const bool v = u >= blocks;
+            const int hb = v ? u - blocks : u, h = hb / NB, b = hb % NB;
+            const float* xh = x + static_cast<size_t>((v ? a.c.n_kv : 0) + h) * HD;
+            f32x4 y;
+            if (v) {
+                if (a.quads) y = *reinterpret_cast<const f32x4*>(xh + 32 * b + 4 * l);
+                else
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 32));
-        const int up = threadIdx.x & 32;  // this half's place in the wave
-        const uint32_t odd = static_cast<uint32_t>(__ballot(!(fabsf(y) < INFINITY)) >> up);
-        const uint32_t tops = static_cast<uint32_t>(__ballot(fabsf(y) == top) >> up);
-        const float m = __shfl(y, tops ? __ffs(tops) - 1 : 0, 32);
-        _Float16 dh = static_cast<_Float16>(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
-        if (odd) dh = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7E00));
-        const float d = static_cast<float>(dh);
-        int level = 8;
-        if (!odd && d != 0.0f) {
-            // the nearest level, ties to even: the quotient's own rounding can hide on which side
-            // of a border the exact one lies, which the remainder (exact in one FMA) tells
-            float t = rintf(y / d);
-            const float rest = fmaf(-t, d, y);
-            if (fabsf(rest) > 0.5f * fabsf(d)) t += (rest > 0.0f) == (d > 0.0f) ? 1.0f : -1.0f;
-            level = static_cast<int>(fminf(fmaxf(t, -8.0f), 7.0f)) + 8;
+                    for (int k = 0; k < 4; k++) y[k] = xh[32 * b + 4 * l + k];
+            } else {
+                y = rotated4(xh, 32 * b + 4 * l, a, turn + j * half);
+            }
+            uint16_t scale;
+            uint32_t lev;
+            quantise4(y, scale, lev);
+            if (v) {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int n = 2 * l + k;
+                    const int at8 = HD >= 64 ? (n * BP + b / 2) * 16 + b % 2 : n % VN * 16 + n / VN;
+                    vl[h * 4 * HD + at8 + j * 2] = static_cast<uint8_t>(lev >> (8 * k));
+                }
+            } else {
+                *reinterpret_cast<uint16_t*>(kl + (h * 8 + j) * (HD / 2) + ((l >> 1) * NB + b) * 4 + (l & 1) * 2) =
+                    static_cast<uint16_t>(lev);
+            }
+            if (l == 0) (v ? vdl : kdl)[(h * NB + b) * 8 + j] = scale;
         }
-        const int two = level | __shfl_xor(level, 1, 32) << 4;  // (the even lane's)
-        if ((i & 1) == 0) {
-            if (v) vl[(((h * vn + (i >> 1) % vn) * bp + (hd >= 64 ? b >> 1 : 0)) * 8 + j) * 2 +
-                      (hd >= 64 ? b & 1 : i >> 4)] = static_cast<uint8_t>(two);
-            else kl[(h * 8 + j) * (hd / 2) + ((i >> 3) * nb + b) * 4 + (i & 7) / 2] = static_cast<uint8_t>(two);
-        }
-        if (i == 0) (v ? vdl : kdl)[(h * nb + b) * 8 + j] = __builtin_bit_cast(uint16_t, dh);
     }
     __syncthreads();
     const size_t plane = static_cast<size_t>(s) * a.c.n_kv + h0;
     // keys: words of whole rows
-    const int kw = hd / 8;
-    for (int u = threadIdx.x; u < heads * 8 * kw; u += kThreads) {
-        const int h = u / (8 * kw), j = u / kw % 8, w = u % kw;
+    for (int u = threadIdx.x; u < heads * 8 * KW; u += kThreads) {
+        const int h = u / (8 * KW), j = u / KW % 8, w = u % KW;
         if (j >= j0 && j < j1)
-            reinterpret_cast<uint32_t*>(a.c.k + ((plane + h) * a.c.cap + oct * 8 + j) * (hd / 2))[w] =
-                reinterpret_cast<const uint32_t*>(kl)[(h * 8 + j) * kw + w];
+            reinterpret_cast<uint32_t*>(a.c.k + ((plane + h) * a.c.cap + oct * 8 + j) * (HD / 2))[w] =
+                reinterpret_cast<const uint32_t*>(kl)[u];
     }
     // values and scales: 2-byte units, eight keys side by side, at once where all eight are new
-    const int vu = hd / 4;
     const bool whole = j0 == 0 && j1 == 8;
-    const int rows8 = heads * (vu + 2 * nb);
+    const int rows8 = heads * (VU + 2 * NB);
     for (int u = threadIdx.x; u < rows8 * (whole ? 1 : 8); u += kThreads) {
-        const int j = whole ? 0 : u % 8, q = whole ? u : u / 8, h = q / (vu + 2 * nb), w = q % (vu + 2 * nb);
+        const int j = whole ? 0 : u % 8, q = whole ? u : u / 8, h = q / (VU + 2 * NB), w = q % (VU + 2 * NB);
         const size_t o = (plane + h) * (a.c.cap / 8) + oct;
         const uint16_t* from;
         uint16_t* to;
-        if (w < vu) {
-            from = reinterpret_cast<const uint16_t*>(vl) + (h * vu + w) * 8;
-            to = reinterpret_cast<uint16_t*>(a.c.v) + (o * vu + w) * 8;
-        } else if (w < vu + nb) {
-            from = kdl + (h * nb + w - vu) * 8;
-            to = a.c.kd + (o * nb + w - vu) * 8;
+        if (w < VU) {
+            from = reinterpret_cast<const uint16_t*>(vl) + (h * VU + w) * 8;
+            to = reinterpret_cast<uint16_t*>(a.c.v) + (o * VU + w) * 8;
+        } else if (w < VU + NB) {
+            from = kdl + (h * NB + w - VU) * 8;
+            to = a.c.kd + (o * NB + w - VU) * 8;
         } else {
-            from = vdl + (h * nb + w - vu - nb) * 8;
-            to = a.c.vd + (o * nb + w - vu - nb) * 8;
+            from = vdl + (h * NB + w - VU - NB) * 8;
+            to = a.c.vd + (o * NB + w - VU - NB) * 8;
         }
         if (whole) *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(from);
         else if (j >= j0 && j < j1) to[j] = from[j];
@@ -809,42 +1276,40 @@ __global__ void __launch_bounds__(kThreads) k_kv4_append(AppendArgs a) {
 
 // ---- read back ----------------------------------------------------------------
 
-// Rows first[s] .. + rows - 1 of every head as f32 rows of n_kv * hd, the f32
-// cache's layout.  One thread: one 4-byte word of keys (8 channels), or one
-// 2-byte unit of values (4 channels).
+// Rows first[s] .. + rows - 1 of every head as f32 rows of n_kv * HD, the f32
+// cache's layout.  One thread: four channels of a key and of its value, so that
+// a wave's stores are whole lines.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_kv4_read(Cache c, const uint32_t* __restrict__ first, uint32_t rows,
                                                       float* __restrict__ ko, float* __restrict__ vo) {
-    constexpr int NB = Shape<HD>::NB, BP = Shape<HD>::BP, KW = HD / 8, VU = HD / 4;
+    constexpr int NB = Shape<HD>::NB, N = Shape<HD>::N, BP = Shape<HD>::BP, VU = HD / 4, PER = HD / 4;
+    const int s = static_cast<int>(blockIdx.y);
     const size_t id = blockIdx.x * static_cast<size_t>(kThreads) + threadIdx.x;
-    const size_t per = static_cast<size_t>(c.n_kv) * (KW + VU);
-    if (id >= per * rows * c.seqs) return;
-    const int u = static_cast<int>(id % (KW + VU)), h = static_cast<int>(id / (KW + VU) % c.n_kv);
-    const uint32_t t = static_cast<uint32_t>(id / per % rows);
-    const int s = static_cast<int>(id / per / rows);
+    const size_t head = id / PER;  // (row, kv head)
+    if (head >= static_cast<size_t>(rows) * c.n_kv) return;
+    const uint32_t t = static_cast<uint32_t>(head / c.n_kv);
+    const int h = static_cast<int>(head - static_cast<size_t>(t) * c.n_kv), ch = static_cast<int>(id % PER) * 4;
     const uint64_t key = static_cast<uint64_t>(first ? first[s] : 0) + t;
     const bool ok = key < static_cast<uint64_t>(c.cap);
-    const size_t plane = (static_cast<size_t>(s) * c.n_kv + h) * c.cap, at = ok ? key : 0;
-    const size_t row = (static_cast<size_t>(s) * rows + t) * c.n_kv + h;
-    if (u < KW) {
-        const int b = u >> 2, g = u & 3;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + (plane + at) * (HD / 2) + (g * NB + b) * 4);
-        const float d = ok ? fh_h2f(c.kd[((plane + at) / 8 * NB + b) * 8 + at % 8]) : __builtin_nanf("");
-        float* to = ko + row * HD + 32 * b + 8 * g;
+    const size_t at = (static_cast<size_t>(s) * c.n_kv + h) * c.cap + (ok ? key : 0), oct = at / 8, j = at % 8;
+    const int b = ch / 32, g = ch % 32 / 8, n = ch % 32 / 2;
+    const uint32_t kw = *reinterpret_cast<const uint16_t*>(c.k + at * (HD / 2) + (g * NB + b) * 4 + ch % 8 / 2);
+    const uint8_t* v = c.v + oct * (VU * 16) + j * 2;
+    const uint32_t v0 = v[HD >= 64 ? (n * BP + b / 2) * 16 + b % 2 : n % N * 16 + n / N];
+    const uint32_t v1 = v[HD >= 64 ? ((n + 1) * BP + b / 2) * 16 + b % 2 : (n + 1) % N * 16 + (n + 1) / N];
+    const float kd = ok ? fh_h2f(c.kd[(oct * NB + b) * 8 + j]) : __builtin_nanf("");
+    const float vd = ok ? fh_h2f(c.vd[(oct * NB + b) * 8 + j]) : __builtin_nanf("");
+    const uint32_t vw = v0 | v1 << 8;
+    const size_t to = (static_cast<size_t>(s) * rows * c.n_kv + head) * HD + ch;
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    f32x4u x, y;
 #pragma unroll
-        for (int i = 0; i < 8; i++) to[i] = static_cast<float>(static_cast<int>(w >> (4 * i) & 15) - 8) * d;
-    } else {
-        const int v = u - KW, n = v / BP, pair = v % BP;
-        const uint32_t w = reinterpret_cast<const uint16_t*>(c.v)[((plane + at) / 8 * VU + n * BP + pair) * 8 + at % 8];
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            const int b = HD >= 64 ? 2 * pair + y : 0, ch = HD >= 64 ? 32 * b + 2 * n : 2 * (n + 8 * y);
-            const float d = ok ? fh_h2f(c.vd[((plane + at) / 8 * NB + b) * 8 + at % 8]) : __builtin_nanf("");
-            float* to = vo + row * HD + ch;
-            to[0] = static_cast<float>(static_cast<int>(w >> (8 * y) & 15) - 8) * d;
-            to[1] = static_cast<float>(static_cast<int>(w >> (8 * y + 4) & 15) - 8) * d;
-        }
+    for (int i = 0; i < 4; i++) {
+        x[i] = static_cast<float>(static_cast<int>(kw >> (4 * i) & 15) - 8) * kd;
+        y[i] = static_cast<float>(static_cast<int>(vw >> (4 * i) & 15) - 8) * vd;
     }
+    *reinterpret_cast<f32x4u*>(ko + to) = x;
+    *reinterpret_cast<f32x4u*>(vo + to) = y;
 }
 
 // ---- eviction -----------------------------------------------------------------
@@ -856,16 +1321,37 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr int kSelect = 1024;
+}  // namespace
+
+namespace fh {
+// The sum over a wave, in every lane.
+__device__ __forceinline__ uint32_t wave_count(uint32_t u) {
+    int v = static_cast<int>(u);
+    v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false);
+    return static_cast<uint32_t>((__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+                                 (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48)));
+}
+}  // namespace fh
+
+namespace {
+
+constexpr int kSelect = 1024, kHeld = 16;  // threads, and weights that each keeps in registers
 
 // Which rows of a (sequence, kv head) stay: the last `recent` and the heaviest
 // of the others up to `keep`, in order; idx gets their cache rows, *count how
-// many.  Four passes of an 8-bit radix select find the lightest weight that
-// stays and how many of its equals do (the first ones); a last pass writes.
+// many.  The lightest weight that stays is found a bit at a time by counting
+// (a histogram's atomics would queue: weights crowd into few leading digits),
+// from registers up to 16384 rows.  Row k * 1024 + t is thread t's k-th, so places follow from
+// counts per (k, wave).
 __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t* __restrict__ len, uint32_t max_len,
                                                        uint32_t keep, uint32_t recent, uint32_t* __restrict__ idx,
                                                        uint32_t* __restrict__ counts) {
-    __shared__ uint32_t hist[256], wsum[2][kSelect / 64], pick[2];
+    constexpr int W = kSelect / 64;
+    __shared__ __align__(16) uint32_t tally[2][W];
+    __shared__ uint32_t slot[kHeld * W], base;
     const int s = static_cast<int>(blockIdx.x) / c.n_kv;
     const uint32_t n = min(min(len[s], max_len), static_cast<uint32_t>(c.cap));
     uint32_t* to = idx + static_cast<size_t>(blockIdx.x) * keep;
@@ -875,87 +1361,113 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
         for (uint32_t i = tid; i < n; i += kSelect) to[i] = i;
         return;
     }
-    const uint32_t free = n - recent;
-    uint32_t want = keep - recent;  // of the free rows; less than `free`
+    const uint32_t free = n - recent, want = keep - recent;  // `want` of the free rows stay
+    for (uint32_t i = tid; i < recent; i += kSelect) to[want + i] = free + i;
+    if (want == 0) return;
     const float* w = c.weight + static_cast<size_t>(blockIdx.x) * c.cap;
-    uint32_t prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < free; i += kSelect) {
-            const uint32_t o = ordered(w[i]);
-            if ((o & mask) == prefix) atomicAdd(&hist[o >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {
-            // from the heaviest digit down: the one at which the count reaches `want`
-            uint32_t h[4], sum = 0;
+    uint32_t held[kHeld];
 #pragma unroll
-            for (int i = 0; i < 4; i++) sum += h[i] = hist[255 - (lane * 4 + i)];
-            uint32_t upto = sum;
-            for (int m = 1; m < 64; m <<= 1) {
-                const uint32_t v = __shfl_up(upto, m, 64);
-                if (lane >= m) upto += v;
+    for (int k = 0; k < kHeld; k++) {
+        const uint32_t i = k * kSelect + tid;
+        held[k] = i < free ? ordered(w[i]) : 0;  // (0 is below every weight's number: -NaN has none of its own)
+    }
+    // the largest `cut` that at least `want` rows reach, a bit at a time; done once it is `want` exactly
+    uint32_t cut = 0;
+    for (int bit = 31, turn = 0; bit >= 0; bit--, turn ^= 1) {
+        const uint32_t t = cut | 1u << bit;
+        uint32_t have = 0;
+#pragma unroll
+        for (int k = 0; k < kHeld; k++)
+            if (static_cast<uint32_t>(k * kSelect) < free) have += held[k] >= t;
+        for (uint32_t i = kHeld * kSelect + tid; i < free; i += kSelect) have += ordered(w[i]) >= t;
+        have = fh::wave_count(have);
+        if (lane == 0) tally[turn][wave] = have;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int v = 0; v < W; v += 4) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(&tally[turn][v]);
+            all += (x[0] + x[1]) + (x[2] + x[3]);
+        }
+        if (all >= want) cut = t;
+        if (all == want) break;
+    }
+    // rows above `cut` all stay, and the first of those at `cut` that bring them to `want`
+    uint32_t above = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; k++) above += __popcll(__ballot(held[k] > cut));
+    for (uint32_t i0 = kHeld * kSelect; i0 < free; i0 += kSelect)
+        above += __popcll(__ballot(i0 + tid < free && ordered(w[i0 + tid]) > cut));
+    __syncthreads();
+    if (lane == 0) tally[0][wave] = above;
+    __syncthreads();
+    uint32_t ties = want;
+    for (int v = 0; v < W; v++) ties -= tally[0][v];
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    uint32_t equal = 0, kept = 0;  // before the chunk at hand
+    for (uint32_t c0 = 0; c0 < free; c0 += kHeld * kSelect) {
+        if (c0) {
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {
+                const uint32_t i = c0 + k * kSelect + tid;
+                held[k] = i < free ? ordered(w[i]) : 0;
             }
-            uint32_t before = upto - sum;
-            for (int i = 0; i < 4; i++) {
-                if (before < want && before + h[i] >= want) {
-                    pick[0] = 255 - (lane * 4 + i);
-                    pick[1] = want - before;
+        }
+        // twice: places among the equals, then among the rows that stay
+        uint32_t stay = 0;
+#pragma unroll
+        for (int pass = 0; pass < 2; pass++) {
+            uint64_t votes[kHeld];
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {
+                const bool in = c0 + k * kSelect + tid < free;
+                votes[k] = __ballot(pass == 0 ? in && held[k] == cut : (stay >> k & 1) != 0);
+                if (lane == 0) slot[k * W + wave] = __popcll(votes[k]);
+            }
+            __syncthreads();
+            if (wave == 0) {  // exclusive sums over the 256 counts, four a lane
+                uint32_t v[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[i] = sum;
+                    sum += slot[lane * 4 + i];
                 }
-                before += h[i];
+                uint32_t upto = sum;
+#pragma unroll
+                for (int m = 1; m < 64; m <<= 1) {
+                    const uint32_t x = __shfl_up(upto, m, 64);
+                    if (lane >= m) upto += x;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) slot[lane * 4 + i] = v[i] + upto - sum;
+                if (lane == 63) base = upto;
             }
-            if (want == 0 && lane == 0) {
-                pick[0] = 255;
-                pick[1] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {
+                const uint32_t place = slot[k * W + wave] + __popcll(votes[k] & below), i = c0 + k * kSelect + tid;
+                if (pass == 0) {
+                    const bool in = i < free;
+                    if (in && (held[k] > cut || (held[k] == cut && equal + place < ties))) stay |= 1u << k;
+                } else if (stay >> k & 1) {
+                    to[kept + place] = i;
+                }
             }
+            if (pass == 0) equal += base;
+            else kept += base;
+            __syncthreads();
         }
-        __syncthreads();
-        prefix |= pick[0] << shift;
-        want = pick[1];
-        mask |= 255u << shift;
-        __syncthreads();
     }
-    // `want` of the rows that weigh exactly `prefix` stay
-    uint32_t kept = 0, equal = 0;
-    const bool none = keep == recent;
-    for (uint32_t i0 = 0; i0 < free; i0 += kSelect) {
-        const uint32_t i = i0 + tid;
-        const uint32_t o = i < free ? ordered(w[i]) : 0;
-        const bool eq = !none && i < free && o == prefix, gt = !none && i < free && o > prefix;
-        const uint64_t below = (uint64_t(1) << lane) - 1;
-        const uint64_t beq = __ballot(eq);
-        if (lane == 0) wsum[0][wave] = __popcll(beq);
-        __syncthreads();
-        uint32_t rank = equal + __popcll(beq & below), alleq = 0;
-        for (int v = 0; v < kSelect / 64; v++) {
-            if (v < wave) rank += wsum[0][v];
-            alleq += wsum[0][v];
-        }
-        const bool stay = gt || (eq && rank < want);
-        const uint64_t bst = __ballot(stay);
-        if (lane == 0) wsum[1][wave] = __popcll(bst);
-        __syncthreads();
-        uint32_t place = kept + __popcll(bst & below), all = 0;
-        for (int v = 0; v < kSelect / 64; v++) {
-            if (v < wave) place += wsum[1][v];
-            all += wsum[1][v];
-        }
-        if (stay) to[place] = i;
-        kept += all;
-        equal += alleq;
-        __syncthreads();
-    }
-    for (uint32_t i = tid; i < recent; i += kSelect) to[keep - recent + i] = free + i;
 }
 
-// Moves the rows that stay.  A workgroup: 64 rows of one (sequence, kv head).
+// Moves the rows that stay.  A workgroup: 64 rows of one (sequence, kv head),
+// keys in 16-byte pieces of a row, values and scales eight rows' units at once.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_kv4_move(Cache c, Cache d, uint32_t keep, int chunks,
                                                       const uint32_t* __restrict__ idx,
                                                       const uint32_t* __restrict__ counts,
                                                       uint32_t* __restrict__ new_len) {
-    constexpr int NB = Shape<HD>::NB, VU = HD / 4, KP = HD / 32 * 4;  // KP: words of a key row
+    constexpr int NB = Shape<HD>::NB, VU = HD / 4, KP = HD / 32;  // KP: 16-byte pieces of a key row
     const int sh = static_cast<int>(blockIdx.x) / chunks, ck = static_cast<int>(blockIdx.x) % chunks;
     const uint32_t n = counts[sh], r0 = static_cast<uint32_t>(ck) * 64;
     if (ck == 0 && threadIdx.x == 0 && sh % c.n_kv == 0) new_len[sh / c.n_kv] = n;
@@ -965,21 +1477,40 @@ __global__ void __launch_bounds__(kThreads) k_kv4_move(Cache c, Cache d, uint32_
     if (threadIdx.x < 64) src[threadIdx.x] = idx[static_cast<size_t>(sh) * keep + r0 + min(static_cast<int>(threadIdx.x), rows - 1)];
     __syncthreads();
     const size_t from = static_cast<size_t>(sh) * c.cap, to = static_cast<size_t>(sh) * d.cap;
-    const uint32_t* ks = reinterpret_cast<const uint32_t*>(c.k);
-    uint32_t* kt = reinterpret_cast<uint32_t*>(d.k);
     for (int u = threadIdx.x; u < rows * KP; u += kThreads)
-        kt[(to + r0 + u / KP) * KP + u % KP] = ks[(from + src[u / KP]) * KP + u % KP];
-    // eight rows side by side: 2-byte units of the values and the scales
-    for (int u = threadIdx.x; u < (VU + 2 * NB) * 64; u += kThreads) {
-        const int j = u % 8, w = u / 8 % (VU + 2 * NB), o = u / (8 * (VU + 2 * NB)), row = o * 8 + j;
-        if (row >= rows) continue;
-        const uint32_t r = src[row];
-        const size_t fo = from / 8 + r / 8, tu = to / 8 + r0 / 8 + o;
-        if (w < VU)
-            reinterpret_cast<uint16_t*>(d.v)[(tu * VU + w) * 8 + j] =
-                reinterpret_cast<const uint16_t*>(c.v)[(fo * VU + w) * 8 + r % 8];
-        else if (w < VU + NB) d.kd[(tu * NB + w - VU) * 8 + j] = c.kd[(fo * NB + w - VU) * 8 + r % 8];
-        else d.vd[(tu * NB + w - VU - NB) * 8 + j] = c.vd[(fo * NB + w - VU - NB) * 8 + r % 8];
+        reinterpret_cast<u32x4*>(d.k)[(to + r0 + u / KP) * KP + u % KP] =
+            reinterpret_cast<const u32x4*>(c.k)[(from + src[u / KP]) * KP + u % KP];
+    for (int u = threadIdx.x; u < (VU + 2 * NB) * 8; u += kThreads) {
+        const int w = u % (VU + 2 * NB), o = u / (VU + 2 * NB);
+        if (o * 8 >= rows) break;
+        const uint16_t* sp;
+        uint16_t* tp;
+        int wide;  // units of an octet
+        if (w < VU) {
+            sp = reinterpret_cast<const uint16_t*>(c.v) + w * 8;
+            tp = reinterpret_cast<uint16_t*>(d.v) + w * 8;
+            wide = VU;
+        } else {
+            const bool k = w < VU + NB;
+            const int x = (k ? w - VU : w - VU - NB) * 8;
+            sp = (k ? c.kd : c.vd) + x;
+            tp = (k ? d.kd : d.vd) + x;
+            wide = NB;
+        }
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t r = src[o * 8 + j];  // (rows past the end repeat the last)
+            v[j] = sp[(from / 8 + r / 8) * (wide * 8) + r % 8];
+        }
+        tp += (to / 8 + r0 / 8 + o) * (wide * 8);
+        if (o * 8 + 8 <= rows) {
+            *reinterpret_cast<u32x4*>(tp) = u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (o * 8 + j < rows) tp[j] = static_cast<uint16_t>(v[j]);
+        }
     }
     if (threadIdx.x < rows) {
         const uint32_t r = src[threadIdx.x];
@@ -997,17 +1528,18 @@ Cache device_cache(const fh_kv4_cache& c) {
 // kUnits of them, each 16 columns of HD + 2 floats, behind one arrival counter
 // each.  One area of this size for the context's life, so a graph that was
 // captured with it never loses it to a larger call.
-constexpr size_t kUnits = 2048;
+constexpr size_t kUnits = 1024;
 constexpr size_t kPartBytes = kUnits * 16 * (128 + 2) * sizeof(float);
 
 template <int HD, bool MODS>
-void launch_attention(fh_ctx* ctx, const AttnArgs& a, bool keys, size_t grid) {
-    if (keys)
-        hipLaunchKernelGGL((k_kv4_attention<HD, MODS, true>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
-                           ctx->stream, a);
-    else
-        hipLaunchKernelGGL((k_kv4_attention<HD, MODS, false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
-                           ctx->stream, a);
+void launch_attention(fh_ctx* ctx, const AttnArgs& a, bool prompt, size_t grid) {
+    const dim3 g(static_cast<unsigned>(grid));
+    if (prompt) {
+        if constexpr (HD >= 64)
+            hipLaunchKernelGGL((k_kv4_prompt<HD, MODS>), g, dim3(kThreads), sizeof(Room<HD>), ctx->stream, a);
+    } else {
+        hipLaunchKernelGGL((k_kv4_attention<HD, MODS>), g, dim3(kThreads), 0, ctx->stream, a);
+    }
 }
 
 AttnArgs attn_args(const fh_kv4_cache& c, const float* q, size_t ld, size_t total, size_t n_heads, const uint32_t* off,
@@ -1046,7 +1578,6 @@ int fh_launch_kv4_append(fh_ctx* ctx, const fh_kv4_cache& c, const float* qkv, s
     a.total = static_cast<uint32_t>(total);
     a.max_rows = static_cast<uint32_t>(max_rows);
     a.n_heads = static_cast<int>(n_heads);
-    a.hd = static_cast<int>(c.head_dim);
     a.octets = static_cast<int>((max_rows + 14) / 8);  // a block of rows touches that many at most
     a.off = off;
     a.len = len;
@@ -1058,9 +1589,16 @@ int fh_launch_kv4_append(fh_ctx* ctx, const fh_kv4_cache& c, const float* qkv, s
     a.ff = ff;
     a.q = q;
     a.heads = static_cast<int>(std::min<size_t>(c.n_kv, 8));
-    const size_t lds = 8 * (rope_dim / 2) * sizeof(double2) + a.heads * (8 * c.head_dim + c.head_dim / 32 * 8 * 2 * 2);
+    a.quads = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q)) % 16 == 0 &&
+              (rope_type != FH_ROPE_NEOX || rope_dim % 8 == 0) && rope_dim % 4 == 0;
+    const size_t lds = 8 * (rope_dim / 2) * sizeof(double2) + rope_dim / 2 * sizeof(float) +
+                       a.heads * (8 * c.head_dim + c.head_dim / 32 * 8 * 2 * 2);
     const dim3 grid(static_cast<unsigned>(c.seqs * a.octets), static_cast<unsigned>((c.n_kv + a.heads - 1) / a.heads));
-    hipLaunchKernelGGL(k_kv4_append, grid, dim3(kThreads), lds, ctx->stream, a);
+    switch (c.head_dim) {
+        case 32: hipLaunchKernelGGL((k_kv4_append<32>), grid, dim3(kThreads), lds, ctx->stream, a); break;
+        case 64: hipLaunchKernelGGL((k_kv4_append<64>), grid, dim3(kThreads), lds, ctx->stream, a); break;
+        default: hipLaunchKernelGGL((k_kv4_append<128>), grid, dim3(kThreads), lds, ctx->stream, a); break;
+    }
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
@@ -1072,11 +1610,20 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     a.out = out;
     a.lse = lse;
     const size_t cols = max_rows * a.group, tiles16 = (cols + 15) / 16, key_tiles = (a.max_keys + 31) / 32;
-    const size_t units = c.seqs * c.n_kv * tiles16;
-    const bool keys = units < 4 * static_cast<size_t>(ctx->num_cus);
-    size_t grid;
-    if (keys) {
+    // Many columns share each key's expansion (128 to a workgroup) where that still fills the
+    // GPU twice over, so that one workgroup's barriers hide behind another's work.  us, at 8
+    // x 500 rows of 32 and 8 heads of width 128 (1024 such workgroups): 77, and 129 by 16
+    // columns; at 1 x 1000 (256): 80 and 59; 8 x 1001 rows of 14 and 2 heads of width 64 (880):
+    // 80 and 99.  At width 32 a key's expansion costs less than its sharing.
+    const size_t shared = c.seqs * c.n_kv * ((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
+    const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus);
+    size_t grid = shared;
+    if (prompt) {
+        a.col_tiles = static_cast<int>((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
+        a.splits = 1;
+    } else {
         a.col_tiles = static_cast<int>(tiles16);
+        const size_t units = c.seqs * c.n_kv * tiles16;
         size_t splits = std::max<size_t>(1, 2 * ctx->num_cus / units);
         splits = std::min(splits, std::max<size_t>(1, key_tiles / 8));
         if (units * splits > kUnits) splits = 1;
@@ -1089,17 +1636,13 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
             a.counters = static_cast<unsigned*>(area);
             a.part = reinterpret_cast<float*>(a.counters + kUnits);
         }
-    } else {
-        a.col_tiles = static_cast<int>((tiles16 + 3) / 4);
-        a.splits = 1;
-        grid = c.seqs * c.n_kv * a.col_tiles;
     }
     if (grid > 0x7FFFFFFF) return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_attention: more than 2^31 - 1 workgroups");
     const bool mods = a.softcap > 0.0f || a.slopes;
     switch (c.head_dim) {
-        case 32: mods ? launch_attention<32, true>(ctx, a, keys, grid) : launch_attention<32, false>(ctx, a, keys, grid); break;
-        case 64: mods ? launch_attention<64, true>(ctx, a, keys, grid) : launch_attention<64, false>(ctx, a, keys, grid); break;
-        default: mods ? launch_attention<128, true>(ctx, a, keys, grid) : launch_attention<128, false>(ctx, a, keys, grid); break;
+        case 32: mods ? launch_attention<32, true>(ctx, a, prompt, grid) : launch_attention<32, false>(ctx, a, prompt, grid); break;
+        case 64: mods ? launch_attention<64, true>(ctx, a, prompt, grid) : launch_attention<64, false>(ctx, a, prompt, grid); break;
+        default: mods ? launch_attention<128, true>(ctx, a, prompt, grid) : launch_attention<128, false>(ctx, a, prompt, grid); break;
     }
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
@@ -1136,8 +1679,8 @@ int fh_launch_kv4_weigh(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size
 
 int fh_launch_kv4_read(fh_ctx* ctx, const fh_kv4_cache& c, const uint32_t* first, size_t rows, float* k, float* v) {
     const Cache d = device_cache(c);
-    const size_t n = c.seqs * rows * c.n_kv * (c.head_dim / 8 + c.head_dim / 4);
-    const dim3 grid(static_cast<unsigned>((n + kThreads - 1) / kThreads));
+    const size_t n = rows * c.n_kv * (c.head_dim / 4);
+    const dim3 grid(static_cast<unsigned>((n + kThreads - 1) / kThreads), static_cast<unsigned>(c.seqs));
     const uint32_t r = static_cast<uint32_t>(rows);
     switch (c.head_dim) {
         case 32: hipLaunchKernelGGL((k_kv4_read<32>), grid, dim3(kThreads), 0, ctx->stream, d, first, r, k, v); break;

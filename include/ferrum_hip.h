@@ -458,7 +458,8 @@ int fh_attention_prefill_seqs_async(fh_ctx* ctx, const float* d_qkv, float* d_k_
  *   pos    nullable: each key's position in its text, [capacity] u32 (NULL: its
  *        cache row; they differ once rows have been evicted);
  *   weight nullable: the attention weight each key has drawn so far, [capacity].
- * k, k_d, v and v_d are 16-byte aligned.  head_dim 32, 64 or 128, else FH_ERR_LIMIT.
+ * k, k_d, v and v_d are 16-byte aligned.  head_dim 32, 64 or 128 and a capacity of
+ * at most 2^25, else FH_ERR_LIMIT.
  * Rows that no call has appended may hold anything. */
 typedef struct {
     uint8_t* k;
