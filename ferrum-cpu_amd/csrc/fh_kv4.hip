@@ -312,22 +312,28 @@ __device__ __forceinline__ void column_place(const AttnArgs& a, const Rows& r, i
 // scaled so that the largest of the row is in [2^13, 2^14) (f16 then has 2^-39
 // of it as its last place).
 template <int HD>
-__device__ __forceinline__ void column_query(const AttnArgs& a, int lane, Column<HD>& col) {
-    constexpr int NB = Shape<HD>::NB;
+__device__ __forceinline__ void load_query(const AttnArgs& a, int lane, const Column<HD>& col,
+                                           float (&x)[Shape<HD>::NB][8]) {
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     const float* q = a.q + static_cast<size_t>(col.row) * a.ld + static_cast<size_t>(col.head) * HD + (lane >> 4) * 8;
-    float x[NB][8];
-    float top = 0.0f;
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
+    for (int b = 0; b < Shape<HD>::NB; b++) {
         const f32x4 u = *reinterpret_cast<const f32x4u*>(q + 32 * b), v = *reinterpret_cast<const f32x4u*>(q + 32 * b + 4);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[b][i] = u[i];
             x[b][4 + i] = v[i];
-            top = fmaxf(top, fmaxf(fabsf(x[b][i]), fabsf(x[b][4 + i])));
         }
     }
+}
+template <int HD>
+__device__ __forceinline__ void split_query(const AttnArgs& a, const float (&x)[Shape<HD>::NB][8], Column<HD>& col) {
+    constexpr int NB = Shape<HD>::NB;
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[b][i]));
     top = across_groups_max(top);
     const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
@@ -339,6 +345,12 @@ __device__ __forceinline__ void column_query(const AttnArgs& a, int lane, Column
         col.lo[b] = as_half8(l[0], l[1], l[2], l[3]);
     }
     col.factor = ldexpf(a.scale, e - 14);
+}
+template <int HD>
+__device__ __forceinline__ void column_query(const AttnArgs& a, int lane, Column<HD>& col) {
+    float x[Shape<HD>::NB][8];
+    load_query<HD>(a, lane, col, x);
+    split_query<HD>(a, x, col);
 }
 
 // The scores of 32 keys and 16 columns: lane (g, n) gets keys 8 g + j of column n.
@@ -982,42 +994,70 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
 }
 
 // Adds to each key's weight what every (query row, head of its group) gave it.
-// A wave holds 32 keys; COLS: the workgroup's waves share one tile and take every
-// fourth tile of columns, else each has a tile of its own.
+// COLS: a workgroup has 32 keys, and its eight waves take every eighth tile of 16
+// columns; else (a single tile of columns) each of four waves has 32 keys of its own.
 template <int HD, bool MODS, bool COLS>
-__global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh(AttnArgs a) {
-    constexpr int NB = Shape<HD>::NB;
-    __shared__ float red[4][32];
+__global__ void __launch_bounds__(COLS ? 512 : 256, 2) k_kv4_weigh(AttnArgs a) {
+    constexpr int NB = Shape<HD>::NB, WAVES = COLS ? 8 : 4, per = COLS ? 1 : 4;
+    __shared__ float red[WAVES][32];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int per = COLS ? 1 : 4, groups = (static_cast<int>((min(a.max_keys, static_cast<uint32_t>(a.c.cap)) + 31) / 32) +
-                                            per - 1) / per;
-    int id = static_cast<int>(blockIdx.x);
-    const int tile = COLS ? id % groups : id % groups * 4 + wave;
-    id /= groups;
-    const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
+    const int limit = static_cast<int>(min(a.max_keys, static_cast<uint32_t>(a.c.cap)));
+    const int heads = a.c.seqs * a.c.n_kv;
+    const int first = static_cast<int>(blockIdx.x) / heads * per, tile = first + (COLS ? 0 : wave);  // (the most seen keys first)
+    const int id = static_cast<int>(blockIdx.x) % heads, kv = id % a.c.n_kv, s = id / a.c.n_kv;
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     const Planes p = planes_of<HD>(a.c, s, kv);
-    const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + (static_cast<size_t>(s) * a.c.n_kv + kv) * a.c.cap : nullptr;
+    const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + static_cast<size_t>(id) * a.c.cap : nullptr;
     const int key0 = tile * 32 + 8 * g;
-    uint32_t k[2][NB];
+    half8 lv[2][NB];
     u32x4 kd[NB];
-    load_k<HD>(p, a.c.cap, tile, lane, k, kd);
+    {
+        uint32_t k[2][NB];
+        load_k<HD>(p, a.c.cap, tile, lane, k, kd);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) lv[h][b] = k_levels(k[h][b]);
+    }
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const uint64_t cols = static_cast<uint64_t>(r.count) * a.group;
-    for (uint64_t c0 = COLS ? wave * 16 : 0; c0 < cols; c0 += COLS ? 64 : 16) {
-        Column<HD> col;
-        column_place<HD, MODS>(a, r, kv, static_cast<uint32_t>(c0) + n, col);
-        if (!__any(col.wide && col.first < tile * 32 + 32 && col.first + col.wide > tile * 32)) continue;
-        column_query<HD>(a, lane, col);
-        const float lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
-        const float f = MODS ? 1.0f : col.factor * kLog2e;
+    const uint32_t cols = r.count * a.group;  // (below 2^31: total * n_heads is)
+    // The next tile of columns that sees some of these keys, its queries on their way.
+    Column<HD> col;
+    float raw[NB][8], lse = 0.0f;
+    const auto seek = [&](uint32_t c) {
+        for (; c < cols; c += COLS ? WAVES * 16 : 16) {
+            column_place<HD, MODS>(a, r, kv, c + n, col);
+            if (__any(col.wide && col.first < tile * 32 + 32 && col.first + col.wide > tile * 32)) {
+                load_query<HD>(a, lane, col, raw);
+                lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
+                break;
+            }
+        }
+        return c;
+    };
+    uint32_t c = seek(COLS ? wave * 16 : 0);
+    while (c < cols) {
+        Column<HD> now = col;
+        const float lse_now = lse;
+        split_query<HD>(a, raw, now);
+        c = seek(c + (COLS ? WAVES * 16 : 16));
         float x[8];
-        scores<HD>(k, kd, col, x);
-        finish_scores<HD, MODS>(a, col, kpos, key0, x);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const f32x4 d = mfma(lv[h][b], now.hi[b], mfma(lv[h][b], now.lo[b], f32x4{0, 0, 0, 0}));
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    x[4 * h + i] = b == 0 ? half_at(kd[b], 4 * h + i) * d[i]
+                                          : fmaf(half_at(kd[b], 4 * h + i), d[i], x[4 * h + i]);
+            }
+        finish_scores<HD, MODS>(a, now, kpos, key0, x);
+        const float f = MODS ? 1.0f : now.factor * kLog2e;
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            acc[j] += static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide)
-                          ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse)) : 0.0f;
+            acc[j] += static_cast<uint32_t>(key0 + j - now.first) < static_cast<uint32_t>(now.wide)
+                          ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse_now)) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -1027,11 +1067,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh(AttnArgs a) {
     __syncthreads();
     const int t = threadIdx.x & 31, w = threadIdx.x >> 5;
     if (w >= per) return;
-    const int key = (COLS ? tile : tile - wave + w) * 32 + t;
-    const uint64_t keys = min(static_cast<uint64_t>(min(a.max_keys, static_cast<uint32_t>(a.c.cap))), r.at + r.count);
-    if (static_cast<uint64_t>(key) >= keys) return;
-    float* to = a.c.weight + (static_cast<size_t>(s) * a.c.n_kv + kv) * a.c.cap + key;
-    *to += COLS ? (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]) : red[w][t];
+    const int key = (first + w) * 32 + t;
+    if (key >= limit || static_cast<uint64_t>(key) >= r.at + r.count) return;
+    float* to = a.c.weight + static_cast<size_t>(id) * a.c.cap + key;
+    float sum = red[w][t];
+    if constexpr (COLS)
+        sum = ((red[0][t] + red[1][t]) + (red[2][t] + red[3][t])) + ((red[4][t] + red[5][t]) + (red[6][t] + red[7][t]));
+    *to += sum;
 }
 
 // ---- append -------------------------------------------------------------------
@@ -1324,15 +1366,15 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 }  // namespace
 
 namespace fh {
-// The sum over a wave, in every lane.
-__device__ __forceinline__ uint32_t wave_count(uint32_t u) {
-    int v = static_cast<int>(u);
-    v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);
-    v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
-    v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false);
-    v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false);
-    return static_cast<uint32_t>((__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
-                                 (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48)));
+// The sum over a wave's lanes up to each.
+__device__ __forceinline__ uint32_t wave_upto(uint32_t u) {
+    uint32_t v = u;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t x = __shfl_up(v, m, 64);
+        if (static_cast<int>(threadIdx.x & 63) >= m) v += x;
+    }
+    return v;
 }
 }  // namespace fh
 
@@ -1342,16 +1384,15 @@ constexpr int kSelect = 1024, kHeld = 16;  // threads, and weights that each kee
 
 // Which rows of a (sequence, kv head) stay: the last `recent` and the heaviest
 // of the others up to `keep`, in order; idx gets their cache rows, *count how
-// many.  The lightest weight that stays is found a bit at a time by counting
-// (a histogram's atomics would queue: weights crowd into few leading digits),
-// from registers up to 16384 rows.  Row k * 1024 + t is thread t's k-th, so places follow from
+// many.  The lightest weight that stays is found by a radix select of 8-bit digits,
+// from registers up to 16384 rows (a bit at a time by counting, without atomics, the
+// 32 rounds of barriers cost more: 21 us, and 30 at 16384 rows).  Row k * 1024 + t is thread t's k-th, so places follow from
 // counts per (k, wave).
 __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t* __restrict__ len, uint32_t max_len,
                                                        uint32_t keep, uint32_t recent, uint32_t* __restrict__ idx,
                                                        uint32_t* __restrict__ counts) {
     constexpr int W = kSelect / 64;
-    __shared__ __align__(16) uint32_t tally[2][W];
-    __shared__ uint32_t slot[kHeld * W], base;
+    __shared__ uint32_t hist[256], pick[2], slot[kHeld * W], base;
     const int s = static_cast<int>(blockIdx.x) / c.n_kv;
     const uint32_t n = min(min(len[s], max_len), static_cast<uint32_t>(c.cap));
     uint32_t* to = idx + static_cast<size_t>(blockIdx.x) * keep;
@@ -1371,38 +1412,41 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
         const uint32_t i = k * kSelect + tid;
         held[k] = i < free ? ordered(w[i]) : 0;  // (0 is below every weight's number: -NaN has none of its own)
     }
-    // the largest `cut` that at least `want` rows reach, a bit at a time; done once it is `want` exactly
-    uint32_t cut = 0;
-    for (int bit = 31, turn = 0; bit >= 0; bit--, turn ^= 1) {
-        const uint32_t t = cut | 1u << bit;
-        uint32_t have = 0;
+    // the largest `cut` that at least `want` rows reach, 8 bits at a time
+    uint32_t cut = 0, mask = 0, left = want;  // `left` of the rows that agree with `cut` so far
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kHeld; k++)
-            if (static_cast<uint32_t>(k * kSelect) < free) have += held[k] >= t;
-        for (uint32_t i = kHeld * kSelect + tid; i < free; i += kSelect) have += ordered(w[i]) >= t;
-        have = fh::wave_count(have);
-        if (lane == 0) tally[turn][wave] = have;
-        __syncthreads();
-        uint32_t all = 0;
-#pragma unroll
-        for (int v = 0; v < W; v += 4) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(&tally[turn][v]);
-            all += (x[0] + x[1]) + (x[2] + x[3]);
+            if (static_cast<uint32_t>(k * kSelect + tid) < free && (held[k] & mask) == cut)
+                atomicAdd(&hist[held[k] >> shift & 255], 1u);
+        for (uint32_t i = kHeld * kSelect + tid; i < free; i += kSelect) {
+            const uint32_t o = ordered(w[i]);
+            if ((o & mask) == cut) atomicAdd(&hist[o >> shift & 255], 1u);
         }
-        if (all >= want) cut = t;
-        if (all == want) break;
-    }
-    // rows above `cut` all stay, and the first of those at `cut` that bring them to `want`
-    uint32_t above = 0;
+        __syncthreads();
+        if (wave == 0) {
+            // from the heaviest digit down: the one at which the count reaches `left`
+            uint32_t h[4], sum = 0;
 #pragma unroll
-    for (int k = 0; k < kHeld; k++) above += __popcll(__ballot(held[k] > cut));
-    for (uint32_t i0 = kHeld * kSelect; i0 < free; i0 += kSelect)
-        above += __popcll(__ballot(i0 + tid < free && ordered(w[i0 + tid]) > cut));
-    __syncthreads();
-    if (lane == 0) tally[0][wave] = above;
-    __syncthreads();
-    uint32_t ties = want;
-    for (int v = 0; v < W; v++) ties -= tally[0][v];
+            for (int i = 0; i < 4; i++) sum += h[i] = hist[255 - (lane * 4 + i)];
+            uint32_t before = fh::wave_upto(sum) - sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (before < left && before + h[i] >= left) {
+                    pick[0] = 255 - (lane * 4 + i);
+                    pick[1] = left - before;
+                }
+                before += h[i];
+            }
+        }
+        __syncthreads();
+        cut |= pick[0] << shift;
+        left = pick[1];
+        mask |= 255u << shift;
+    }
+    // rows above `cut` all stay, and the first `left` of those at it
     const uint64_t below = (uint64_t(1) << lane) - 1;
     uint32_t equal = 0, kept = 0;  // before the chunk at hand
     for (uint32_t c0 = 0; c0 < free; c0 += kHeld * kSelect) {
@@ -1432,12 +1476,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
                     v[i] = sum;
                     sum += slot[lane * 4 + i];
                 }
-                uint32_t upto = sum;
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const uint32_t x = __shfl_up(upto, m, 64);
-                    if (lane >= m) upto += x;
-                }
+                const uint32_t upto = fh::wave_upto(sum);
 #pragma unroll
                 for (int i = 0; i < 4; i++) slot[lane * 4 + i] = v[i] + upto - sum;
                 if (lane == 63) base = upto;
@@ -1448,7 +1487,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
                 const uint32_t place = slot[k * W + wave] + __popcll(votes[k] & below), i = c0 + k * kSelect + tid;
                 if (pass == 0) {
                     const bool in = i < free;
-                    if (in && (held[k] > cut || (held[k] == cut && equal + place < ties))) stay |= 1u << k;
+                    if (in && (held[k] > cut || (held[k] == cut && equal + place < left))) stay |= 1u << k;
                 } else if (stay >> k & 1) {
                     to[kept + place] = i;
                 }
@@ -1651,7 +1690,7 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
 template <int HD, bool MODS>
 static void launch_weigh(fh_ctx* ctx, const AttnArgs& a, bool cols, size_t grid) {
     if (cols)
-        hipLaunchKernelGGL((k_kv4_weigh<HD, MODS, true>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
+        hipLaunchKernelGGL((k_kv4_weigh<HD, MODS, true>), dim3(static_cast<unsigned>(grid)), dim3(512), 0,
                            ctx->stream, a);
     else
         hipLaunchKernelGGL((k_kv4_weigh<HD, MODS, false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
