@@ -90,16 +90,16 @@ __device__ __forceinline__ Rows rows_of(const uint32_t* off, const uint32_t* len
     return r;
 }
 
-// One lane's share of 32 keys of a cache: lane (g, n) = (lane / 16, lane % 16)
-// holds key rows 8 (n / 4) + n % 4 and + 4 as MFMA rows, and of the eight keys
-// 8 g .. 8 g + 7 their scales and its output channels' value levels.
+// One lane's share of 32 keys of a cache on its way: lane (g, n) = (lane / 16, lane %
+// 16) holds key rows 8 (n / 4) + n % 4 and + 4 as MFMA rows and its output channels'
+// value levels of the eight keys 8 g .. 8 g + 7; and one 64th of the tile's scales
+// (lanes 0 .. 31 the keys', 32 .. 63 the values'), which go through LDS to the
+// lanes that want them: loaded as wanted, each would come 16 times over.
 template <int HD>
 struct Tile {
     uint32_t k[2][Shape<HD>::NB];
-    u32x4 kd[Shape<HD>::NB];
     u32x4 v[Shape<HD>::BP];
-    u32x4 vd[Shape<HD>::NB];
-    uint32_t vx;  // two scales of the tile's values, for their exponent
+    uint32_t sc[HD == 128 ? 2 : 1];
 };
 
 struct Planes {
@@ -116,8 +116,7 @@ __device__ __forceinline__ Planes planes_of(const Cache& c, int s, int kv) {
 }
 
 template <int HD>
-__device__ __forceinline__ void load_k(const Planes& p, int cap, int tile, int lane, uint32_t (&k)[2][Shape<HD>::NB],
-                                       u32x4 (&kd)[Shape<HD>::NB]) {
+__device__ __forceinline__ void load_k(const Planes& p, int cap, int tile, int lane, uint32_t (&k)[2][Shape<HD>::NB]) {
     constexpr int NB = Shape<HD>::NB;
     const int g = lane >> 4, n = lane & 15;
     const int key = tile * 32 + 8 * (n >> 2) + (n & 3);
@@ -137,24 +136,34 @@ __device__ __forceinline__ void load_k(const Planes& p, int cap, int tile, int l
             k[h][0] = *reinterpret_cast<const uint32_t*>(a);
         }
     }
-    const uint32_t o = min(tile * 4 + g, cap / 8 - 1);
+}
+template <int HD>
+__device__ __forceinline__ void load_kd(const Planes& p, int cap, int tile, int lane, u32x4 (&kd)[Shape<HD>::NB]) {
+    const uint32_t o = min(tile * 4 + (lane >> 4), cap / 8 - 1);
 #pragma unroll
-    for (int b = 0; b < NB; b++) kd[b] = *reinterpret_cast<const u32x4*>(p.kd + o * (NB * 8) + b * 8);
+    for (int b = 0; b < Shape<HD>::NB; b++)
+        kd[b] = *reinterpret_cast<const u32x4*>(p.kd + o * (Shape<HD>::NB * 8) + b * 8);
 }
 
 template <int HD>
-__device__ __forceinline__ void load_tile(const Planes& p, int cap, int tile, int lane, Tile<HD>& t) {
+__device__ __forceinline__ void load_tile(const Planes& p, const uint16_t* scales, int cap, int tile, int lane, Tile<HD>& t) {
     constexpr int NB = Shape<HD>::NB, N = Shape<HD>::N, BP = Shape<HD>::BP;
-    load_k<HD>(p, cap, tile, lane, t.k, t.kd);
+    load_k<HD>(p, cap, tile, lane, t.k);
     const int g = lane >> 4, n = lane & 15, last = cap / 8 - 1;
-    const uint32_t o = min(tile * 4 + g, last), vo = o * (N * BP * 16) + n % N * (BP * 16), so = o * (NB * 8);
+    const uint32_t vo = min(tile * 4 + g, last) * (N * BP * 16) + n % N * (BP * 16);
 #pragma unroll
     for (int i = 0; i < BP; i++) t.v[i] = *reinterpret_cast<const u32x4*>(p.v + vo + i * 16);
-#pragma unroll
-    for (int b = 0; b < NB; b++) t.vd[b] = *reinterpret_cast<const u32x4*>(p.vd + so + b * 8);
-    const int i = lane % (16 * NB);
-    const uint32_t ox = min(tile * 4 + i / (4 * NB), last);
-    t.vx = *reinterpret_cast<const uint32_t*>(p.vd + (ox * (NB * 8) + i % (4 * NB) * 2));
+    // eight lanes an octet, NB scales each, as they lie
+    const uint16_t* a = scales + (min(tile * 4 + (lane >> 3 & 3), last) * (8 * NB) + (lane & 7) * NB);
+    if constexpr (NB == 4) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(a);
+        t.sc[0] = w[0];
+        t.sc[1] = w[1];
+    } else if constexpr (NB == 2) {
+        t.sc[0] = *reinterpret_cast<const uint32_t*>(a);
+    } else {
+        t.sc[0] = *a;
+    }
 }
 
 __device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -413,31 +422,53 @@ __device__ __forceinline__ void clear(Sums<HD>& z) {
 
 // One tile of 32 keys into the sums.  The weights times their block's value
 // scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that as
-// their last place, so none of them loses bits to f16's range.
+// their last place, so none of them loses bits to f16's range.  swap: the wave's
+// LDS room for a tile's scales.
 template <int HD, bool MODS, bool MASKED>
 __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int tile, int lane, const Column<HD>& col,
-                                     const uint32_t* kpos, int seen_lo, int seen_hi, Sums<HD>& z) {
+                                     const uint32_t* kpos, int seen_lo, int seen_hi, uint16_t* swap, Sums<HD>& z) {
     constexpr int NB = Shape<HD>::NB;
     const int g = lane >> 4, n = lane & 15, key0 = tile * 32 + 8 * g;
+    // (a wave's LDS instructions run in order: only the compiler has to be held)
+    if constexpr (NB == 4) *reinterpret_cast<u32x2*>(swap + lane * 4) = u32x2{t.sc[0], t.sc[1]};
+    else if constexpr (NB == 2) *reinterpret_cast<uint32_t*>(swap + lane * 2) = t.sc[0];
+    else swap[lane] = static_cast<uint16_t>(t.sc[0]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    u32x4 kd[NB], vd[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        kd[b] = *reinterpret_cast<const u32x4*>(swap + (g * NB + b) * 8);
+        vd[b] = *reinterpret_cast<const u32x4*>(swap + ((4 + g) * NB + b) * 8);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     float s[8];
-    scores<HD>(t.k, t.kd, col, s);
+    scores<HD>(t.k, kd, col, s);
     finish_scores<HD, MODS>(a, col, kpos, key0, s);
     bool seen[8];
-    uint32_t vx = t.vx;
     if constexpr (MASKED) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             seen[j] = static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide);
             s[j] = seen[j] ? s[j] : -INFINITY;
         }
-        // (scales of keys that no column sees may hold anything)
-        const int i = lane % (16 * NB), kx = tile * 32 + i / (4 * NB) * 8 + i % 4 * 2;
-        if (kx < seen_lo || kx >= seen_hi) vx &= 0xFFFF0000u;
-        if (kx + 1 < seen_lo || kx + 1 >= seen_hi) vx &= 0x0000FFFFu;
     }
+    uint32_t vm = 0;  // the largest of this lane's value scales, as bits
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        uint32_t x = t.sc[i >> 1] >> (16 * (i & 1)) & 0x7FFFu;
+        if constexpr (MASKED) {  // (scales of keys that no column sees may hold anything)
+            const int key = tile * 32 + (lane >> 3 & 3) * 8 + (lane & 7) * NB % 8 + i;
+            x = key >= seen_lo && key < seen_hi ? x : 0;
+        }
+        vm = max(vm, x);
+    }
+    vm = lane < 32 ? 0 : vm;
     const float f = MODS ? 1.0f : col.factor * kLog2e;
     const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * f;
-    const uint32_t vm = max(vx & 0x7FFFu, (vx >> 16) & 0x7FFFu);
     if (__any(top > z.limit || vm > z.vbits)) {
         int v = -group_min(-static_cast<int>(vm));
         v = max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
@@ -469,7 +500,7 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float x = fmaf(p[2 * i], half_at(t.vd[b], 2 * i), zero), y = fmaf(p[2 * i + 1], half_at(t.vd[b], 2 * i + 1), zero);
+            float x = fmaf(p[2 * i], half_at(vd[b], 2 * i), zero), y = fmaf(p[2 * i + 1], half_at(vd[b], 2 * i + 1), zero);
             if constexpr (MASKED) {
                 x = seen[2 * i] ? x : 0.0f;
                 y = seen[2 * i + 1] ? y : 0.0f;
@@ -488,21 +519,30 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
     }
 }
 
+// The columns' queries against tiles t0, t0 + stride, .. below t1, the next two on their way
+// while one is worked on.
 template <int HD, bool MODS>
-__device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lane, const Column<HD>& col,
+__device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lane, Column<HD>& col,
                                      const uint32_t* kpos, int t0, int t1, int stride, int full_lo, int full_hi,
-                                     int seen_lo, int seen_hi, Sums<HD>& z) {
+                                     int seen_lo, int seen_hi, uint16_t* swap, Sums<HD>& z) {
     if (t0 >= t1) return;
-    Tile<HD> cur;
-    load_tile<HD>(p, a.c.cap, t0, lane, cur);
-    for (int t = t0; t < t1; t += stride) {
-        Tile<HD> next;
-        load_tile<HD>(p, a.c.cap, min(t + stride, t1 - 1), lane, next);
+    const uint16_t* scales = lane < 32 ? p.kd : p.vd;
+    Tile<HD> even, odd;
+    load_tile<HD>(p, scales, a.c.cap, t0, lane, even);
+    load_tile<HD>(p, scales, a.c.cap, min(t0 + stride, t1 - 1), lane, odd);
+    column_query<HD>(a, lane, col);  // (its loads wait beside the tiles')
+    const auto work = [&](const Tile<HD>& tile, int t) {
         if (t * 32 >= full_lo && t * 32 + 32 <= full_hi)
-            step<HD, MODS, false>(a, cur, t, lane, col, kpos, seen_lo, seen_hi, z);
+            step<HD, MODS, false>(a, tile, t, lane, col, kpos, seen_lo, seen_hi, swap, z);
         else
-            step<HD, MODS, true>(a, cur, t, lane, col, kpos, seen_lo, seen_hi, z);
-        cur = next;
+            step<HD, MODS, true>(a, tile, t, lane, col, kpos, seen_lo, seen_hi, swap, z);
+    };
+    for (int t = t0; t < t1; t += 2 * stride) {
+        work(even, t);
+        if (t + stride >= t1) break;
+        load_tile<HD>(p, scales, a.c.cap, min(t + 2 * stride, t1 - 1), lane, even);
+        work(odd, t + stride);
+        load_tile<HD>(p, scales, a.c.cap, min(t + 3 * stride, t1 - 1), lane, odd);
     }
 }
 
@@ -529,6 +569,16 @@ __device__ __forceinline__ void channels(const Sums<HD>& z, int b, float factor,
     }
 }
 
+// Two floats of memory that other workgroups read and write, 8-byte aligned.
+__device__ __forceinline__ void store2(float* to, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, make_float2(a, b)), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load2(const float* from) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(from)),
+                                                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 // Attention of 16 columns by one workgroup: the four waves take every fourth tile
 // of the workgroup's share of the keys.
 template <int HD, bool MODS>
@@ -548,7 +598,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     column_place<HD, MODS>(a, r, kv, static_cast<uint32_t>(ct) * 16 + n, col);
     int lo, hi, flo, fhi;
     column_range(col.on, col.first, col.wide, lo, hi, flo, fhi);
-    column_query<HD>(a, lane, col);
     const Planes p = planes_of<HD>(a.c, s, kv);
     const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + (static_cast<size_t>(s) * a.c.n_kv + kv) * a.c.cap : nullptr;
     Sums<HD> z;
@@ -556,9 +605,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     const int t_lo = lo < hi ? lo / 32 : 0, tiles = lo < hi ? (hi + 31) / 32 - t_lo : 0;
     const int t0 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
     const int t1 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, lo, hi, z);
+    __shared__ __align__(16) float so[4][16][LD];
+    __shared__ float sb[4][16], sl[4][16];
+    // (a wave's room for scales is in its own part of the sums')
+    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, lo, hi, reinterpret_cast<uint16_t*>(so[wave]), z);
     // join the waves
-    __shared__ float so[4][16][LD], sb[4][16], sl[4][16];
     __shared__ int last;
     const float l = across_groups_sum(z.l);
 #pragma unroll
@@ -590,16 +641,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     Column<HD> mine;  // (its place only)
     column_place<HD, false>(a, r, kv, c, mine);
     if (a.splits > 1) {
-        float* part = a.part + (static_cast<size_t>(unit) * a.splits * 16 + cj) * (HD + 2);
-        float* to = part + static_cast<size_t>(split) * 16 * (HD + 2);
+        constexpr int PL = HD + 2;
+        float* part = a.part + static_cast<size_t>(unit) * a.splits * 16 * PL;
         if (mine.on) {
-            if (ch == 0) {
-                __hip_atomic_store(to, base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(to + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            float* to = part + (static_cast<size_t>(split) * 16 + cj) * PL;
+            if (ch == 0) store2(to, base, sum);
 #pragma unroll
-            for (int i = 0; i < PER; i++)
-                __hip_atomic_store(to + 2 + ch + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int i = 0; i < PER; i += 2) store2(to + 2 + ch + i, x[i], x[i + 1]);
         }
         // Every thread's coherent stores complete before the arrival count moves.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -609,23 +657,68 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
         if (!last) return;
         if (threadIdx.x == 0)
             __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (!mine.on) return;
+        // Sixteen threads a column; with fewer than 16 columns they also share out the
+        // splits (each eight at a time, their loads in flight together), and join in LDS.
+        const int cols = min(16, static_cast<int>(r.count * a.group - static_cast<uint32_t>(ct) * 16));
+        const int lanes = cols > 8 ? 16 : cols > 4 ? 8 : cols > 2 ? 4 : cols, sets = 16 / lanes;
+        const int jc = cj % lanes, set = cj / lanes;
         base = -FLT_MAX;
-        for (int i = 0; i < a.splits; i++)
-            base = fmaxf(base, __hip_atomic_load(part + static_cast<size_t>(i) * 16 * (HD + 2), __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT));
         sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; i++) x[i] = 0.0f;
-        for (int sp = 0; sp < a.splits; sp++) {
-            const float* from = part + static_cast<size_t>(sp) * 16 * (HD + 2);
-            const float f = __builtin_amdgcn_exp2f(
-                __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - base);
-            sum = fmaf(__hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f, sum);
+        if (jc < cols) {
+            constexpr int R = 8;
+            for (int s0 = set; s0 < a.splits; s0 += R * sets) {
+                float2 st[R], v[R][PER / 2];
 #pragma unroll
-            for (int i = 0; i < PER; i++)
-                x[i] = fmaf(__hip_atomic_load(from + 2 + ch + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), f,
-                            x[i]);
+                for (int i = 0; i < R; i++) {
+                    const float* from = part + (static_cast<size_t>(min(s0 + i * sets, a.splits - 1)) * 16 + jc) * PL;
+                    st[i] = load2(from);
+#pragma unroll
+                    for (int k = 0; k < PER / 2; k++) v[i][k] = load2(from + 2 + ch + 2 * k);
+                }
+                float m = base;
+#pragma unroll
+                for (int i = 0; i < R; i++) m = fmaxf(m, st[i].x);  // (repeats of the last change nothing)
+                const float k0 = __builtin_amdgcn_exp2f(base - m);
+                base = m;
+                sum *= k0;
+#pragma unroll
+                for (int k = 0; k < PER; k++) x[k] *= k0;
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    const float f = s0 + i * sets < a.splits ? __builtin_amdgcn_exp2f(st[i].x - m) : 0.0f;
+                    sum = fmaf(st[i].y, f, sum);
+#pragma unroll
+                    for (int k = 0; k < PER / 2; k++) {
+                        x[2 * k] = fmaf(v[i][k].x, f, x[2 * k]);
+                        x[2 * k + 1] = fmaf(v[i][k].y, f, x[2 * k + 1]);
+                    }
+                }
+            }
+        }
+        if (sets > 1) {
+            float(*sx)[LD] = so[0];
+#pragma unroll
+            for (int i = 0; i < PER; i++) sx[cj][ch + i] = x[i];
+            if (ch == 0) {
+                sb[0][cj] = base;
+                sl[0][cj] = sum;
+            }
+            __syncthreads();
+            if (cj < cols) {
+                base = -FLT_MAX;
+                for (int i = 0; i < sets; i++) base = fmaxf(base, sb[0][cj + i * lanes]);
+                sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; i++) x[i] = 0.0f;
+                for (int q = 0; q < sets; q++) {
+                    const float f = __builtin_amdgcn_exp2f(sb[0][cj + q * lanes] - base);
+                    sum = fmaf(sl[0][cj + q * lanes], f, sum);
+#pragma unroll
+                    for (int i = 0; i < PER; i++) x[i] = fmaf(sx[cj + q * lanes][ch + i], f, x[i]);
+                }
+            }
         }
     }
     if (!mine.on) return;
@@ -1013,7 +1106,8 @@ __global__ void __launch_bounds__(COLS ? 512 : 256, 2) k_kv4_weigh(AttnArgs a) {
     u32x4 kd[NB];
     {
         uint32_t k[2][NB];
-        load_k<HD>(p, a.c.cap, tile, lane, k, kd);
+        load_k<HD>(p, a.c.cap, tile, lane, k);
+        load_kd<HD>(p, a.c.cap, tile, lane, kd);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -1655,7 +1749,9 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     // columns; at 1 x 1000 (256): 80 and 59; 8 x 1001 rows of 14 and 2 heads of width 64 (880):
     // 80 and 99.  At width 32 a key's expansion costs less than its sharing.
     const size_t shared = c.seqs * c.n_kv * ((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
-    const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus);
+    // (and only with three quarters of those columns in use: its cost is a workgroup's.)
+    const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus) &&
+                        4 * tiles16 * c.seqs * c.n_kv >= 3 * 4 * kPromptTiles * shared;
     size_t grid = shared;
     if (prompt) {
         a.col_tiles = static_cast<int>((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
@@ -1663,8 +1759,12 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     } else {
         a.col_tiles = static_cast<int>(tiles16);
         const size_t units = c.seqs * c.n_kv * tiles16;
-        size_t splits = std::max<size_t>(1, 2 * ctx->num_cus / units);
-        splits = std::min(splits, std::max<size_t>(1, key_tiles / 8));
+        // Keys of few columns are dealt over workgroups until the GPU has two each, but to no more
+        // than the root of their tiles (the last workgroup joins them all: at 1 x 32767 keys of 14 and 2
+        // heads of width 64, 32 take 12.9 us, 128 16.2; at 1 x 4000, 12 8.5 us and 8 9.4).
+        size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(ctx->num_cus) / units);
+        splits = std::min(splits, std::max<size_t>(1, key_tiles / 4));
+        splits = std::min(splits, static_cast<size_t>(std::ceil(std::sqrt(static_cast<double>(key_tiles)))));
         if (units * splits > kUnits) splits = 1;
         a.splits = static_cast<int>(splits);
         grid = units * splits;
