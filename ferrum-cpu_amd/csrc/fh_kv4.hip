@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -1179,7 +1180,7 @@ struct AppendArgs {
     uint32_t total, max_rows;
     int n_heads, octets, heads;  // heads: kv heads of a workgroup, with their query heads
     const uint32_t *off, *len, *pos;
-    int rope_dim, neox, quads;  // quads: every four channels from a multiple of 4 are 16-byte aligned, and so are their partners
+    int rope_dim, neox;
     float base, linear;
     const float* ff;
     float* q;
@@ -1196,41 +1197,45 @@ __device__ __forceinline__ float rope_angle(uint32_t pos, int i, float freq, con
     return static_cast<float>(static_cast<int>(pos)) * freq / f * (1.0f / a.linear);
 }
 
-// Four channels from ch (a multiple of 4) of a head row, rotated where they are
-// among the first rope_dim: angles in 32 bits as fh_rope_async's, sine, cosine
-// and products in 64, since a key's channel goes on to the border between two
-// levels, where its last bit decides.
-__device__ __forceinline__ f32x4 rotated4(const float* x, int ch, const AppendArgs& a, const double2* turn) {
-#pragma clang fp contract(off)
+// Four channels from ch (a multiple of 4) of a head row and those they are rotated with.
+struct Quad {
+    f32x4 own, other;
+};
+template <bool QUADS>  // 16-byte accesses
+__device__ __forceinline__ Quad load_quad(const float* x, int ch, bool turned, const AppendArgs& a) {
     const int half = a.rope_dim / 2;
-    float own[4], other[4];
-    const bool second = ch >= half;
-    if (a.quads) {
-        const f32x4 u = *reinterpret_cast<const f32x4*>(x + ch);
-        f32x4 v = f32x4{u[1], u[0], u[3], u[2]};
-        if (a.neox && ch < a.rope_dim) v = *reinterpret_cast<const f32x4*>(x + (second ? ch - half : ch + half));
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            own[k] = u[k];
-            other[k] = v[k];
-        }
+    Quad q;
+    if constexpr (QUADS) {
+        const bool apart = turned && a.neox && ch < a.rope_dim;
+        q.own = *reinterpret_cast<const f32x4*>(x + ch);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(x + (!apart ? ch : ch >= half ? ch - half : ch + half));
+        q.other = apart ? v : f32x4{v[1], v[0], v[3], v[2]};
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int c = ch + k;
-            own[k] = x[c];
-            other[k] = c < a.rope_dim ? x[a.neox ? (c >= half ? c - half : c + half) : c ^ 1] : 0.0f;
+            q.own[k] = x[c];
+            q.other[k] = turned && c < a.rope_dim ? x[a.neox ? (c >= half ? c - half : c + half) : c ^ 1] : 0.0f;
         }
     }
-    f32x4 y;
+    return q;
+}
+// Rotated where they are among the first rope_dim: angles in 32 bits as
+// fh_rope_async's, sine, cosine and products in 64, since a key's channel goes on
+// to the border between two levels, where its last bit decides.
+template <bool QUADS>
+__device__ __forceinline__ f32x4 rotate_quad(const Quad& q, int ch, const AppendArgs& a, const double2* turn) {
+#pragma clang fp contract(off)
+    const int half = a.rope_dim / 2;
+    f32x4 y = q.own;
+    if (QUADS && ch >= a.rope_dim) return y;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const int c = ch + k;
-        y[k] = own[k];
-        if (c < a.rope_dim) {
+        if (QUADS || c < a.rope_dim) {
             const bool hi = a.neox ? c >= half : c & 1;
             const double2 t = turn[a.neox ? (hi ? c - half : c) : c >> 1];  // (cosine, sine)
-            const double u = own[k], v = other[k];
+            const double u = q.own[k], v = q.other[k];
             y[k] = static_cast<float>(hi ? v * t.y + u * t.x : u * t.x - v * t.y);
         }
     }
@@ -1284,8 +1289,8 @@ __device__ __forceinline__ void quantise4(const f32x4& x, uint16_t& scale, uint3
 
 // The eight cache rows of one octet: rotate and store their queries, quantise
 // their keys and values, eight lanes a block.
-template <int HD>
-__global__ void __launch_bounds__(kThreads) k_kv4_append(AppendArgs a) {
+template <int HD, bool QUADS>
+__global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
     constexpr int NB = Shape<HD>::NB, VN = Shape<HD>::N, BP = Shape<HD>::BP, KW = HD / 8, VU = HD / 4;
     extern __shared__ __align__(16) char smem[];
     const int half = a.rope_dim / 2;
@@ -1320,40 +1325,54 @@ __global__ void __launch_bounds__(kThreads) k_kv4_append(AppendArgs a) {
         __syncthreads();
     }
     if (a.q) {
-        constexpr int PER = HD / 4;
-        const int wide = heads * group * PER;
-        for (int jj = 0; jj < j1 - j0; jj++) {
-            const size_t row = row0 + jj;
-            const float* x = a.qkv + row * a.ld + static_cast<size_t>(h0) * group * HD;
-            float* y = a.q + (row * a.n_heads + static_cast<size_t>(h0) * group) * HD;
-            for (int u = threadIdx.x; u < wide; u += kThreads) {
-                const f32x4 v = rotated4(x + u / PER * HD, u % PER * 4, a, turn + (j0 + jj) * half);
-                if (a.quads) *reinterpret_cast<f32x4*>(y + u * 4) = v;
+        // four quads a thread on their way at once
+        constexpr int PER = HD / 4, R = 4;
+        const int wide = heads * group * PER, all = (j1 - j0) * wide;
+        for (int u0 = threadIdx.x; u0 < all; u0 += R * kThreads) {
+            Quad q[R];
+            int jj[R], u[R];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int v = min(u0 + i * kThreads, all - 1);
+                jj[i] = v / wide;
+                u[i] = v - jj[i] * wide;
+                q[i] = load_quad<QUADS>(a.qkv + (row0 + jj[i]) * a.ld + static_cast<size_t>(h0) * group * HD + u[i] / PER * HD,
+                                 u[i] % PER * 4, true, a);
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (u0 + i * kThreads >= all) continue;
+                const f32x4 v = rotate_quad<QUADS>(q[i], u[i] % PER * 4, a, turn + (j0 + jj[i]) * half);
+                float* y = a.q + ((row0 + jj[i]) * static_cast<size_t>(a.n_heads) + static_cast<size_t>(h0) * group) * HD + u[i] * 4;
+                if constexpr (QUADS) *reinterpret_cast<f32x4*>(y) = v;
                 else
 #pragma unroll
-                    for (int k = 0; k < 4; k++) y[u * 4 + k] = v[k];
+                    for (int k = 0; k < 4; k++) y[k] = v[k];
             }
         }
     }
     if (!store) return;
     const int l = threadIdx.x & 7, blocks = heads * NB;
-    for (int jj = 0; jj < j1 - j0; jj++) {
-        const int j = j0 + jj;
-        const float* x = a.qkv + (row0 + jj) * a.ld + static_cast<size_t>(a.n_heads + h0) * HD;
-        // (the eight lanes of a block leave the loop together, which is all that the exchange needs)
-        for (int u = threadIdx.x >> 3; u < blocks * 2; u += kThreads / 8) {
+    constexpr int R = 4;
+    const int per = 2 * blocks, all = (j1 - j0) * per;
+    for (int u0 = threadIdx.x >> 3; u0 < all; u0 += R * (kThreads / 8)) {
+        Quad q[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int w = min(u0 + i * (kThreads / 8), all - 1), jj = w / per, u = w - jj * per;
+            const bool v = u >= blocks;
+            const int hb = v ? u - blocks : u;
+            q[i] = load_quad<QUADS>(a.qkv + (row0 + jj) * a.ld + static_cast<size_t>(a.n_heads + h0 + (v ? a.c.n_kv : 0) + hb / NB) * HD,
+                             hb % NB * 32 + 4 * l, !v, a);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            // (the eight lanes of a block leave together, which is all that their exchange needs)
+            const int w = u0 + i * (kThreads / 8), jj = w / per, u = w - jj * per, j = j0 + jj;
+            if (w >= all) break;
             const bool v = u >= blocks;
             const int hb = v ? u - blocks : u, h = hb / NB, b = hb % NB;
-            const float* xh = x + static_cast<size_t>((v ? a.c.n_kv : 0) + h) * HD;
-            f32x4 y;
-            if (v) {
-                if (a.quads) y = *reinterpret_cast<const f32x4*>(xh + 32 * b + 4 * l);
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) y[k] = xh[32 * b + 4 * l + k];
-            } else {
-                y = rotated4(xh, 32 * b + 4 * l, a, turn + j * half);
-            }
+            const f32x4 y = v ? q[i].own : rotate_quad<QUADS>(q[i], 32 * b + 4 * l, a, turn + j * half);
             uint16_t scale;
             uint32_t lev;
             quantise4(y, scale, lev);
@@ -1444,8 +1463,8 @@ __global__ void __launch_bounds__(kThreads) k_kv4_read(Cache c, const uint32_t* 
         x[i] = static_cast<float>(static_cast<int>(kw >> (4 * i) & 15) - 8) * kd;
         y[i] = static_cast<float>(static_cast<int>(vw >> (4 * i) & 15) - 8) * vd;
     }
-    *reinterpret_cast<f32x4u*>(ko + to) = x;
-    *reinterpret_cast<f32x4u*>(vo + to) = y;
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4u*>(ko + to));
+    __builtin_nontemporal_store(y, reinterpret_cast<f32x4u*>(vo + to));
 }
 
 // ---- eviction -----------------------------------------------------------------
@@ -1512,9 +1531,11 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kHeld; k++)
+        for (int k = 0; k < kHeld; k++) {
+            if (static_cast<uint32_t>(k * kSelect) >= free) continue;
             if (static_cast<uint32_t>(k * kSelect + tid) < free && (held[k] & mask) == cut)
                 atomicAdd(&hist[held[k] >> shift & 255], 1u);
+        }
         for (uint32_t i = kHeld * kSelect + tid; i < free; i += kSelect) {
             const uint32_t o = ordered(w[i]);
             if ((o & mask) == cut) atomicAdd(&hist[o >> shift & 255], 1u);
@@ -1558,6 +1579,8 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
             uint64_t votes[kHeld];
 #pragma unroll
             for (int k = 0; k < kHeld; k++) {
+                votes[k] = 0;
+                if (c0 + k * kSelect >= free) continue;
                 const bool in = c0 + k * kSelect + tid < free;
                 votes[k] = __ballot(pass == 0 ? in && held[k] == cut : (stay >> k & 1) != 0);
                 if (lane == 0) slot[k * W + wave] = __popcll(votes[k]);
@@ -1568,7 +1591,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     v[i] = sum;
-                    sum += slot[lane * 4 + i];
+                    sum += c0 + (lane / 4) * kSelect < free ? slot[lane * 4 + i] : 0;  // (k = lane / 4)
                 }
                 const uint32_t upto = fh::wave_upto(sum);
 #pragma unroll
@@ -1578,6 +1601,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kHeld; k++) {
+                if (c0 + k * kSelect >= free) continue;
                 const uint32_t place = slot[k * W + wave] + __popcll(votes[k] & below), i = c0 + k * kSelect + tid;
                 if (pass == 0) {
                     const bool in = i < free;
@@ -1721,16 +1745,22 @@ int fh_launch_kv4_append(fh_ctx* ctx, const fh_kv4_cache& c, const float* qkv, s
     a.linear = linear;
     a.ff = ff;
     a.q = q;
-    a.heads = static_cast<int>(std::min<size_t>(c.n_kv, 8));
-    a.quads = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q)) % 16 == 0 &&
+    a.heads = static_cast<int>(std::min<size_t>(c.n_kv, 2));  // (8 x 1000 rows of 32 and 8 heads: 67 us, by eights 78)
+    // 16-byte accesses: every four channels from a multiple of 4 are aligned, and so are their partners
+    const bool quads = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q)) % 16 == 0 &&
               (rope_type != FH_ROPE_NEOX || rope_dim % 8 == 0) && rope_dim % 4 == 0;
     const size_t lds = 8 * (rope_dim / 2) * sizeof(double2) + rope_dim / 2 * sizeof(float) +
                        a.heads * (8 * c.head_dim + c.head_dim / 32 * 8 * 2 * 2);
     const dim3 grid(static_cast<unsigned>(c.seqs * a.octets), static_cast<unsigned>((c.n_kv + a.heads - 1) / a.heads));
+    const auto go = [&](auto width) {
+        constexpr int HD = decltype(width)::value;
+        if (quads) hipLaunchKernelGGL((k_kv4_append<HD, true>), grid, dim3(kThreads), lds, ctx->stream, a);
+        else hipLaunchKernelGGL((k_kv4_append<HD, false>), grid, dim3(kThreads), lds, ctx->stream, a);
+    };
     switch (c.head_dim) {
-        case 32: hipLaunchKernelGGL((k_kv4_append<32>), grid, dim3(kThreads), lds, ctx->stream, a); break;
-        case 64: hipLaunchKernelGGL((k_kv4_append<64>), grid, dim3(kThreads), lds, ctx->stream, a); break;
-        default: hipLaunchKernelGGL((k_kv4_append<128>), grid, dim3(kThreads), lds, ctx->stream, a); break;
+        case 32: go(std::integral_constant<int, 32>{}); break;
+        case 64: go(std::integral_constant<int, 64>{}); break;
+        default: go(std::integral_constant<int, 128>{}); break;
     }
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
