@@ -1088,41 +1088,137 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
 }
 
 // Adds to each key's weight what every (query row, head of its group) gave it.
-// COLS: a workgroup has 32 keys, and its eight waves take every eighth tile of 16
-// columns; else (a single tile of columns) each of four waves has 32 keys of its own.
-template <int HD, bool MODS, bool COLS>
-__global__ void __launch_bounds__(COLS ? 512 : 256, 2) k_kv4_weigh(AttnArgs a) {
-    constexpr int NB = Shape<HD>::NB, WAVES = COLS ? 8 : 4, per = COLS ? 1 : 4;
-    __shared__ float red[WAVES][32];
+// Two forms: k_kv4_weigh_step for a single tile of 16 columns, whose queries are
+// split once for all the keys that a wave walks, and k_kv4_weigh_prompt.
+
+// The score of 32 keys and 16 columns as weights, added to acc.
+template <int HD, bool MODS, typename Scales>
+__device__ __forceinline__ void add_weights(const AttnArgs& a, const half8 (&lv)[2][Shape<HD>::NB], const Scales& scales,
+                                            const Column<HD>& col, float lse, const uint32_t* kpos, int key0,
+                                            float (&acc)[8]) {
+    float x[8];
+#pragma unroll
+    for (int b = 0; b < Shape<HD>::NB; b++) {
+        const u32x4 kd = scales(b);  // of the lane's eight keys
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f32x4 d = mfma(lv[h][b], col.hi[b], mfma(lv[h][b], col.lo[b], f32x4{0, 0, 0, 0}));
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[4 * h + j] = b == 0 ? half_at(kd, 4 * h + j) * d[j] : fmaf(half_at(kd, 4 * h + j), d[j], x[4 * h + j]);
+        }
+    }
+    finish_scores<HD, MODS>(a, col, kpos, key0, x);
+    const float f = MODS ? 1.0f : col.factor * kLog2e;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        acc[j] += static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide)
+                      ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse)) : 0.0f;
+}
+
+// A workgroup: every fourth tile of its share of the keys to a wave, the next on its way.
+template <int HD, bool MODS>
+__global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
+    constexpr int NB = Shape<HD>::NB;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int limit = static_cast<int>(min(a.max_keys, static_cast<uint32_t>(a.c.cap)));
-    const int heads = a.c.seqs * a.c.n_kv;
-    const int first = static_cast<int>(blockIdx.x) / heads * per, tile = first + (COLS ? 0 : wave);  // (the most seen keys first)
-    const int id = static_cast<int>(blockIdx.x) % heads, kv = id % a.c.n_kv, s = id / a.c.n_kv;
+    const int split = static_cast<int>(blockIdx.x) % a.splits, id = static_cast<int>(blockIdx.x) / a.splits;
+    const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
+    Column<HD> col;
+    column_place<HD, MODS>(a, r, kv, n, col);
+    int lo, hi, flo, fhi;
+    column_range(col.on, col.first, col.wide, lo, hi, flo, fhi);
+    if (lo >= hi) return;
+    const int first = lo / 32, tiles = (hi + 31) / 32 - first;
+    const int t1 = first + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    int t = first + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits) + wave;
+    if (t >= t1) return;
+    const Planes p = planes_of<HD>(a.c, s, kv);
+    const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + static_cast<size_t>(id) * a.c.cap : nullptr;
+    float* weight = a.c.weight + static_cast<size_t>(id) * a.c.cap;
+    uint32_t k[2][NB];
+    u32x4 kd[NB];
+    load_k<HD>(p, a.c.cap, t, lane, k);
+    load_kd<HD>(p, a.c.cap, t, lane, kd);
+    column_query<HD>(a, lane, col);
+    const float lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
+    for (; t < t1; t += 4) {
+        half8 lv[2][NB];
+        u32x4 sc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            lv[0][b] = k_levels(k[0][b]);
+            lv[1][b] = k_levels(k[1][b]);
+            sc[b] = kd[b];
+        }
+        const int next = min(t + 4, t1 - 1);
+        load_k<HD>(p, a.c.cap, next, lane, k);
+        load_kd<HD>(p, a.c.cap, next, lane, kd);
+        const int key = t * 32 + 8 * g + (n & 7);  // (lanes n and n + 8 have the same; n < 8 add it)
+        const bool mine = n < 8 && key >= lo && key < hi;
+        const float old = mine ? weight[key] : 0.0f;
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        add_weights<HD, MODS>(a, lv, [&](int b) { return sc[b]; }, col, lse, kpos, t * 32 + 8 * g, acc);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float v = fh::group_sum<16>(acc[j]);
+            sum = (n & 7) == j ? v : sum;
+        }
+        if (mine) weight[key] = old + sum;
+    }
+}
+
+// A workgroup has 32 KT keys, in every one of its eight waves, which take every eighth
+// tile of 16 columns of the workgroup's share (of `splits`; their sums then go to a.part
+// and k_kv4_add_weights adds them up in order).
+constexpr int kWeighTiles = 2;  // KT
+
+template <int HD, bool MODS>
+__global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
+    constexpr int NB = Shape<HD>::NB, WAVES = 8, KT = kWeighTiles;
+    __shared__ float red[WAVES][KT * 32];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int limit = static_cast<int>(a.max_keys), heads = a.c.seqs * a.c.n_kv;
+    int id = static_cast<int>(blockIdx.x);
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int tile = id / heads * KT;  // (the most seen keys first)
+    id %= heads;
+    const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     const Planes p = planes_of<HD>(a.c, s, kv);
     const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + static_cast<size_t>(id) * a.c.cap : nullptr;
-    const int key0 = tile * 32 + 8 * g;
-    half8 lv[2][NB];
-    u32x4 kd[NB];
-    {
+    __shared__ u32x4 kd[KT][NB][4];  // (in registers they would crowd the queries on their way out)
+    half8 lv[KT][2][NB];
+    float acc[KT][8];
+    if (threadIdx.x < KT * NB * 4) {
+        const int i = threadIdx.x / (NB * 4), b = threadIdx.x / 4 % NB, o = threadIdx.x % 4;
+        kd[i][b][o] = *reinterpret_cast<const u32x4*>(
+            p.kd + (static_cast<uint32_t>(min((tile + i) * 4 + o, a.c.cap / 8 - 1)) * (NB * 8) + b * 8));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KT; i++) {
         uint32_t k[2][NB];
-        load_k<HD>(p, a.c.cap, tile, lane, k);
-        load_kd<HD>(p, a.c.cap, tile, lane, kd);
+        load_k<HD>(p, a.c.cap, tile + i, lane, k);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int b = 0; b < NB; b++) lv[h][b] = k_levels(k[h][b]);
+            for (int b = 0; b < NB; b++) lv[i][h][b] = k_levels(k[h][b]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[i][j] = 0.0f;
     }
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const uint32_t cols = r.count * a.group;  // (below 2^31: total * n_heads is)
+    const uint32_t cols = r.count * a.group, tiles = (cols + 15) / 16;  // (below 2^31: total * n_heads is)
+    const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits) * 16;
+    const uint32_t c1 = min(cols, static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits) * 16);
     // The next tile of columns that sees some of these keys, its queries on their way.
     Column<HD> col;
     float raw[NB][8], lse = 0.0f;
     const auto seek = [&](uint32_t c) {
-        for (; c < cols; c += COLS ? WAVES * 16 : 16) {
+        for (; c < c1; c += WAVES * 16) {
             column_place<HD, MODS>(a, r, kv, c + n, col);
-            if (__any(col.wide && col.first < tile * 32 + 32 && col.first + col.wide > tile * 32)) {
+            if (__any(col.wide && col.first < (tile + KT) * 32 && col.first + col.wide > tile * 32)) {
                 load_query<HD>(a, lane, col, raw);
                 lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
                 break;
@@ -1130,45 +1226,43 @@ __global__ void __launch_bounds__(COLS ? 512 : 256, 2) k_kv4_weigh(AttnArgs a) {
         }
         return c;
     };
-    uint32_t c = seek(COLS ? wave * 16 : 0);
-    while (c < cols) {
+    uint32_t c = seek(c0 + wave * 16);
+    while (c < c1) {
         Column<HD> now = col;
         const float lse_now = lse;
         split_query<HD>(a, raw, now);
-        c = seek(c + (COLS ? WAVES * 16 : 16));
-        float x[8];
+        c = seek(c + WAVES * 16);
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const f32x4 d = mfma(lv[h][b], now.hi[b], mfma(lv[h][b], now.lo[b], f32x4{0, 0, 0, 0}));
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    x[4 * h + i] = b == 0 ? half_at(kd[b], 4 * h + i) * d[i]
-                                          : fmaf(half_at(kd[b], 4 * h + i), d[i], x[4 * h + i]);
-            }
-        finish_scores<HD, MODS>(a, now, kpos, key0, x);
-        const float f = MODS ? 1.0f : now.factor * kLog2e;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            acc[j] += static_cast<uint32_t>(key0 + j - now.first) < static_cast<uint32_t>(now.wide)
-                          ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse_now)) : 0.0f;
+        for (int i = 0; i < KT; i++)
+            add_weights<HD, MODS>(a, lv[i], [&](int b) { return kd[i][b][g]; }, now, lse_now, kpos, (tile + i) * 32 + 8 * g,
+                                  acc[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float v = fh::group_sum<16>(acc[j]);
-        if (n == 0) red[wave][8 * g + j] = v;
-    }
+    for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float v = fh::group_sum<16>(acc[i][j]);
+            if (n == 0) red[wave][i * 32 + 8 * g + j] = v;
+        }
     __syncthreads();
-    const int t = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (w >= per) return;
-    const int key = (first + w) * 32 + t;
-    if (key >= limit || static_cast<uint64_t>(key) >= r.at + r.count) return;
-    float* to = a.c.weight + static_cast<size_t>(id) * a.c.cap + key;
-    float sum = red[w][t];
-    if constexpr (COLS)
-        sum = ((red[0][t] + red[1][t]) + (red[2][t] + red[3][t])) + ((red[4][t] + red[5][t]) + (red[6][t] + red[7][t]));
-    *to += sum;
+    const int t = threadIdx.x, key = tile * 32 + t;
+    if (t >= KT * 32 || key >= limit || static_cast<uint64_t>(key) >= r.at + r.count) return;
+    const float sum =
+        ((red[0][t] + red[1][t]) + (red[2][t] + red[3][t])) + ((red[4][t] + red[5][t]) + (red[6][t] + red[7][t]));
+    if (a.splits > 1) a.part[(static_cast<size_t>(split) * heads + id) * limit + key] = sum;
+    else a.c.weight[static_cast<size_t>(id) * a.c.cap + key] += sum;
+}
+
+__global__ void __launch_bounds__(kThreads) k_kv4_add_weights(AttnArgs a) {
+    const uint32_t heads = static_cast<uint32_t>(a.c.seqs) * a.c.n_kv;
+    const size_t i = blockIdx.x * static_cast<size_t>(kThreads) + threadIdx.x, all = static_cast<size_t>(heads) * a.max_keys;
+    if (i >= all) return;
+    const uint32_t id = static_cast<uint32_t>(i / a.max_keys), key = static_cast<uint32_t>(i % a.max_keys);
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, static_cast<int>(id) / a.c.n_kv);
+    if (key >= r.at + r.count) return;
+    float sum = 0.0f;
+    for (int s = 0; s < a.splits; s++) sum += a.part[s * all + i];
+    a.c.weight[static_cast<size_t>(id) * a.c.cap + key] += sum;
 }
 
 // ---- append -------------------------------------------------------------------
@@ -1818,13 +1912,41 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
 }
 
 template <int HD, bool MODS>
-static void launch_weigh(fh_ctx* ctx, const AttnArgs& a, bool cols, size_t grid) {
-    if (cols)
-        hipLaunchKernelGGL((k_kv4_weigh<HD, MODS, true>), dim3(static_cast<unsigned>(grid)), dim3(512), 0,
+static int launch_weigh(fh_ctx* ctx, AttnArgs& a, size_t tiles16) {
+    const size_t heads = static_cast<size_t>(a.c.seqs) * a.c.n_kv, tiles = (a.max_keys + 31) / 32;
+    const size_t room = 4 * static_cast<size_t>(ctx->num_cus);
+    if (tiles16 == 1) {
+        // workgroups of at least four tiles, and no more than four to a CU
+        const size_t splits = std::max<size_t>(1, std::min(room / heads, tiles / 4));
+        a.splits = static_cast<int>(splits);
+        hipLaunchKernelGGL((k_kv4_weigh_step<HD, MODS>), dim3(static_cast<unsigned>(heads * splits)), dim3(kThreads), 0,
                            ctx->stream, a);
-    else
-        hipLaunchKernelGGL((k_kv4_weigh<HD, MODS, false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
+        FH_HIP(ctx, hipGetLastError());
+        return FH_OK;
+    }
+    // Few workgroups share out the columns too, until there are four for each CU (the first
+    // keys are seen by the most rows, so that many even out) or no more than two tiles a wave.
+    constexpr size_t KT = kWeighTiles;
+    const size_t groups = (tiles + KT - 1) / KT;
+    const size_t splits = std::max<size_t>(1, std::min(room / (heads * groups), tiles16 / 16));
+    const size_t grid = heads * groups * splits;
+    if (grid > 0x7FFFFFFF) return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_weigh: more than 2^31 - 1 workgroups");
+    a.splits = static_cast<int>(splits);
+    if (splits > 1) {
+        void* ws = nullptr;
+        const int rc = fh_workspace(ctx, splits * heads * a.max_keys * sizeof(float), &ws);
+        if (rc) return rc;
+        a.part = static_cast<float*>(ws);
+    }
+    hipLaunchKernelGGL((k_kv4_weigh_prompt<HD, MODS>), dim3(static_cast<unsigned>(grid)), dim3(512), 0, ctx->stream, a);
+    FH_HIP(ctx, hipGetLastError());
+    if (splits > 1) {
+        const size_t n = heads * a.max_keys;
+        hipLaunchKernelGGL(k_kv4_add_weights, dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)), dim3(kThreads), 0,
                            ctx->stream, a);
+        FH_HIP(ctx, hipGetLastError());
+    }
+    return FH_OK;
 }
 
 int fh_launch_kv4_weigh(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size_t ld, size_t total, size_t n_heads,
@@ -1832,18 +1954,13 @@ int fh_launch_kv4_weigh(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size
                         const fh_attn_score* sc, const float* lse) {
     AttnArgs a = attn_args(c, q, ld, total, n_heads, off, max_rows, len, max_keys, sc);
     a.lse_in = lse;
-    const bool cols = max_rows * a.group > 16;
-    const size_t tiles = (a.max_keys + 31) / 32, groups = cols ? tiles : (tiles + 3) / 4;
-    const size_t grid = c.seqs * c.n_kv * groups;
-    if (grid > 0x7FFFFFFF) return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_weigh: more than 2^31 - 1 workgroups");
+    const size_t tiles16 = (max_rows * a.group + 15) / 16;
     const bool mods = a.softcap > 0.0f || a.slopes;
     switch (c.head_dim) {
-        case 32: mods ? launch_weigh<32, true>(ctx, a, cols, grid) : launch_weigh<32, false>(ctx, a, cols, grid); break;
-        case 64: mods ? launch_weigh<64, true>(ctx, a, cols, grid) : launch_weigh<64, false>(ctx, a, cols, grid); break;
-        default: mods ? launch_weigh<128, true>(ctx, a, cols, grid) : launch_weigh<128, false>(ctx, a, cols, grid); break;
+        case 32: return mods ? launch_weigh<32, true>(ctx, a, tiles16) : launch_weigh<32, false>(ctx, a, tiles16);
+        case 64: return mods ? launch_weigh<64, true>(ctx, a, tiles16) : launch_weigh<64, false>(ctx, a, tiles16);
+        default: return mods ? launch_weigh<128, true>(ctx, a, tiles16) : launch_weigh<128, false>(ctx, a, tiles16);
     }
-    FH_HIP(ctx, hipGetLastError());
-    return FH_OK;
 }
 
 int fh_launch_kv4_read(fh_ctx* ctx, const fh_kv4_cache& c, const uint32_t* first, size_t rows, float* k, float* v) {
