@@ -138,6 +138,30 @@ int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out) {
     return zeroed_area(ctx, &ctx->kv4, &ctx->kv4_bytes, bytes, "the 4-bit cache's workspace", out);
 }
 
+int fh_kv4_room(fh_ctx* ctx, size_t bytes, void** out) {
+    if (ctx->kv4_room_bytes < bytes) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        FH_HIP(ctx, hipStreamIsCapturing(ctx->stream, &cs));
+        if (cs != hipStreamCaptureStatusNone)
+            return fh_fail(ctx, FH_ERR_INVALID,
+                           "the 4-bit cache's workspace must grow, which cannot happen during graph capture: "
+                           "run the same call once outside capture first");
+        bytes = fh_align256(std::max(bytes, 2 * ctx->kv4_room_bytes));
+        void* room = nullptr;
+        FH_HIP(ctx, hipMalloc(&room, bytes));
+        try {
+            if (ctx->kv4_room) ctx->kv4_old.push_back(ctx->kv4_room);
+        } catch (const std::bad_alloc&) {
+            (void)hipFree(room);
+            return fh_fail(ctx, FH_ERR_OOM, "out of host memory");
+        }
+        ctx->kv4_room = room;
+        ctx->kv4_room_bytes = bytes;
+    }
+    *out = ctx->kv4_room;
+    return FH_OK;
+}
+
 // Every entry point works on the context's device.
 // (hipSetDevice only when needed, so calls stay legal under stream capture.)
 static hipError_t on_device(int device) {
@@ -234,6 +258,8 @@ void fh_ctx_destroy(fh_ctx* ctx) {
     if (ctx->sync) (void)hipFree(ctx->sync);
     if (ctx->counters) (void)hipFree(ctx->counters);
     if (ctx->kv4) (void)hipFree(ctx->kv4);
+    if (ctx->kv4_room) (void)hipFree(ctx->kv4_room);
+    for (void* p : ctx->kv4_old) (void)hipFree(p);
     if (ctx->act) (void)hipFree(ctx->act);
     if (ctx->io) (void)hipFree(ctx->io);
     if (ctx->pin) (void)hipHostFree(ctx->pin);
@@ -1078,6 +1104,8 @@ int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q
     if (total == 0 || max_rows == 0) return FH_OK;
     if (!d_qkv) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_append: qkv is NULL");
     if (d_q == d_qkv) return fh_fail(ctx, FH_ERR_INVALID, "fh_kv4_append: q must not be qkv");
+    if (cache->seqs * ((max_rows + 14) / 8) > 0x7FFFFFFFu)
+        return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_append: more than 2^31 - 1 workgroups");
     FH_ON_DEVICE(ctx);
     return fh_launch_kv4_append(ctx, *cache, d_qkv, ld, total, n_heads, d_off, max_rows, d_len, d_pos, rope_dim, base,
                                 rope_type, d_freq_factors, linear_factor, d_q);

@@ -15,6 +15,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "../../include/ferrum_hip.h"
 
@@ -41,6 +42,12 @@ struct fh_ctx {
     // sums of keys split over workgroups.  Allocated once, at its only size.
     void* kv4 = nullptr;
     size_t kv4_bytes = 0;
+    // Room for its other calls (evicted rows' indices, a prompt's partial weights).
+    // Grows to at least twice its size, and what it grows out of is kept until the
+    // context ends: a graph that was captured with it may still be replayed.
+    void* kv4_room = nullptr;
+    size_t kv4_room_bytes = 0;
+    std::vector<void*> kv4_old;
     // Grow-on-demand activation staging (a LayerNorm output feeding a
     // linear), separate from ws, which the linear itself may use.
     void* act = nullptr;
@@ -119,6 +126,8 @@ int fh_sync_area(fh_ctx* ctx, size_t bytes, void** out);
 int fh_counter_area(fh_ctx* ctx, size_t bytes, void** out);
 // The same for ctx->kv4.
 int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out);
+// Make sure ctx->kv4_room holds at least `bytes`; refused under capture where it must grow.
+int fh_kv4_room(fh_ctx* ctx, size_t bytes, void** out);
 // Round up to a multiple of 256 bytes.
 static inline size_t fh_align256(size_t b) { return (b + 255) & ~(size_t)255; }
 

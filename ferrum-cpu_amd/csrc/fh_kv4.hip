@@ -29,6 +29,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -400,34 +401,31 @@ __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD
 }
 
 // What a wave has of its 16 columns: the sums of e = 2^(score - base) (l, each lane
-// its own keys') and of e * value (o).
+// its own keys') and of e * value (o).  base is 10 below the largest of score + E so
+// far, 2^E being above the key's value scales: what counts is not how large a weight
+// is but how large its product, so that a row whose keys have small values is as
+// exact beside a row, or a key of no weight, with large ones.
 template <int HD>
 struct Sums {
     f32x4 o[Shape<HD>::NB][2];
-    float l, base, limit;  // base = running maximum - 10 + vexp; scores up to limit = base + 14 - vexp keep it
-    int vexp;              // 2^vexp is above every value scale so far
-    uint32_t vbits;        // f16 bits that such a scale may have
+    float l, base;
 };
 
 template <int HD>
 __device__ __forceinline__ void clear(Sums<HD>& z) {
 #pragma unroll
-    for (int b = 0; b < Shape<HD>::NB; b++) {
-        z.o[b][0] = z.o[b][1] = f32x4{0, 0, 0, 0};
-    }
+    for (int b = 0; b < Shape<HD>::NB; b++) z.o[b][0] = z.o[b][1] = f32x4{0, 0, 0, 0};
     z.l = 0.0f;
-    z.base = z.limit = -FLT_MAX;
-    z.vexp = 0;
-    z.vbits = 0;
+    z.base = -FLT_MAX;
 }
 
 // One tile of 32 keys into the sums.  The weights times their block's value
 // scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that as
-// their last place, so none of them loses bits to f16's range.  swap: the wave's
-// LDS room for a tile's scales.
+// their last place, which is 2^-35 of the row's largest.  swap: the wave's LDS
+// room for a tile's scales.
 template <int HD, bool MODS, bool MASKED>
 __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int tile, int lane, const Column<HD>& col,
-                                     const uint32_t* kpos, int seen_lo, int seen_hi, uint16_t* swap, Sums<HD>& z) {
+                                     const uint32_t* kpos, uint16_t* swap, Sums<HD>& z) {
     constexpr int NB = Shape<HD>::NB;
     const int g = lane >> 4, n = lane & 15, key0 = tile * 32 + 8 * g;
     // (a wave's LDS instructions run in order: only the compiler has to be held)
@@ -457,28 +455,23 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
             s[j] = seen[j] ? s[j] : -INFINITY;
         }
     }
-    uint32_t vm = 0;  // the largest of this lane's value scales, as bits
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        uint32_t x = t.sc[i >> 1] >> (16 * (i & 1)) & 0x7FFFu;
-        if constexpr (MASKED) {  // (scales of keys that no column sees may hold anything)
-            const int key = tile * 32 + (lane >> 3 & 3) * 8 + (lane & 7) * NB % 8 + i;
-            x = key >= seen_lo && key < seen_hi ? x : 0;
-        }
-        vm = max(vm, x);
-    }
-    vm = lane < 32 ? 0 : vm;
     const float f = MODS ? 1.0f : col.factor * kLog2e;
-    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * f;
-    if (__any(top > z.limit || vm > z.vbits)) {
-        int v = -group_min(-static_cast<int>(vm));
-        v = max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-                max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-        v = max(v, static_cast<int>(z.vbits)) >> 10;
-        const int vexp = min(v, 30) - 14;
-        const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + static_cast<float>(10 - z.vexp),
-                              across_groups_max(top));
-        const float base = m == -FLT_MAX ? -FLT_MAX : m + static_cast<float>(vexp - 10);
+    // 1024 + the exponent field of each key's largest scale, as f16
+    u32x4 e;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        u16x2 m = __builtin_bit_cast(u16x2, vd[0][i] & 0x7C007C00u);
+#pragma unroll
+        for (int b = 1; b < NB; b++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, vd[b][i] & 0x7C007C00u));
+        e[i] = __builtin_bit_cast(uint32_t, m >> 10) | 0x64006400u;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = fmaxf(top, fmaf(s[j], f, half_at(e, j)));
+    top -= 1024.0f + 14.0f;  // (the scale is below 2^(field - 14))
+    if (__any(top > z.base + 14.0f)) {
+        const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + 10.0f, across_groups_max(top));
+        const float base = m == -FLT_MAX ? -FLT_MAX : m - 10.0f;
         const float k = __builtin_amdgcn_exp2f(z.base - base);
         z.l *= k;
 #pragma unroll
@@ -487,9 +480,6 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
             z.o[b][1] *= k;
         }
         z.base = base;
-        z.limit = m == -FLT_MAX ? -FLT_MAX : m + 4.0f;
-        z.vexp = vexp;
-        z.vbits = v >= 30 ? 0x7FFFu : static_cast<uint32_t>(v << 10 | 0x3FF);
     }
     float p[8];
 #pragma unroll
@@ -525,7 +515,7 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
 template <int HD, bool MODS>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lane, Column<HD>& col,
                                      const uint32_t* kpos, int t0, int t1, int stride, int full_lo, int full_hi,
-                                     int seen_lo, int seen_hi, uint16_t* swap, Sums<HD>& z) {
+                                     uint16_t* swap, Sums<HD>& z) {
     if (t0 >= t1) return;
     const uint16_t* scales = lane < 32 ? p.kd : p.vd;
     Tile<HD> even, odd;
@@ -534,9 +524,9 @@ __device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lan
     column_query<HD>(a, lane, col);  // (its loads wait beside the tiles')
     const auto work = [&](const Tile<HD>& tile, int t) {
         if (t * 32 >= full_lo && t * 32 + 32 <= full_hi)
-            step<HD, MODS, false>(a, tile, t, lane, col, kpos, seen_lo, seen_hi, swap, z);
+            step<HD, MODS, false>(a, tile, t, lane, col, kpos, swap, z);
         else
-            step<HD, MODS, true>(a, tile, t, lane, col, kpos, seen_lo, seen_hi, swap, z);
+            step<HD, MODS, true>(a, tile, t, lane, col, kpos, swap, z);
     };
     for (int t = t0; t < t1; t += 2 * stride) {
         work(even, t);
@@ -609,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     __shared__ __align__(16) float so[4][16][LD];
     __shared__ float sb[4][16], sl[4][16];
     // (a wave's room for scales is in its own part of the sums')
-    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, lo, hi, reinterpret_cast<uint16_t*>(so[wave]), z);
+    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, reinterpret_cast<uint16_t*>(so[wave]), z);
     // join the waves
     __shared__ int last;
     const float l = across_groups_sum(z.l);
@@ -740,18 +730,18 @@ struct Stage {
     uint32_t k[2][Shape<HD>::NB][2][64][4];  // keys as MFMA rows 0 .. 15 and 16 .. 31, by block and f16 term
     uint32_t v[Shape<HD>::NB][2][2][64][4];  // values, by block, channel parity and f16 term
 };
-// Per key of four tiles: 2^e and 2^-e, e the largest exponent of its scales (of values:
-// under vexp), and the bits of a scale to take: none of a key that nobody sees
-// or that holds a NaN, whose 2^e is then NaN.
+// Per key of four tiles: e, the largest exponent of its scales (values' under vexp; of keys
+// as 2^e), 2^-e, and the bits of a scale to take: none of a key that nobody sees or that
+// holds a NaN.  Such a NaN is in a key's 2^e; values' are told by nan.
 struct Factors {
-    float up[4][32], down[4][32];
+    float e[4][32], down[4][32];
     uint16_t ok[4][32];
 };
 template <int HD>
 struct Room {
     Stage<HD> stage[2];
     Factors k, v;
-    int range[2], vbits[4];
+    int nan[4], range[2], vbits[4];
 };
 
 // One thread's share of a tile on its way to LDS.
@@ -867,9 +857,10 @@ constexpr int kPromptTiles = 2;  // tiles of 16 columns of a wave
 // of them: keys and values as level * scale in two exact f16 terms, so that
 // neither a score nor a weight takes its scale block by block, and every product
 // of an f32 operand (two terms as well) is three matrix products, the lowest left
-// out (2^-22).  The range of f16 is each key's own (2^-e here, 2^e on its score or
-// weight; values under their block's largest exponent over all the keys), so
-// nothing loses bits beside a larger key or block.
+// out (2^-22).  The range of f16 is each key's own: 2^-e here, 2^e on its score or
+// weight, values under their block's largest exponent over all the keys.  The
+// running maximum is that of score + e, so that a row of keys with small values
+// has all the bits that it has where no other row sees larger ones.
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, CT = kPromptTiles;
@@ -955,16 +946,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         const bool seen = key >= glo && key < ghi;
         e = fine && seen ? e : 0;
         Factors& f = tid < 32 ? room.v : room.k;
-        f.up[tile & 3][tid & 31] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
+        const uint64_t nans = __ballot(!fine && seen);
+        if (tid < 32) f.e[tile & 3][tid & 31] = static_cast<float>(e);
+        else f.e[tile & 3][tid & 31] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
+        if (tid == 0) room.nan[tile & 3] = static_cast<uint32_t>(nans) != 0;
         f.down[tile & 3][tid & 31] = ldexpf(1.0f, -e);
         f.ok[tile & 3][tid & 31] = fine && seen ? 0xFFFF : 0;
     };
     f32x4 o[CT][NB][2];
-    float l[CT], base[CT], limit[CT], unit_of[CT];  // unit_of: log2 units of a score's own
+    float l[CT], base[CT], unit_of[CT];  // unit_of: log2 units of a score's own
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         l[c] = 0.0f;
-        base[c] = limit[c] = -FLT_MAX;
+        base[c] = -FLT_MAX;
         unit_of[c] = MODS && a.slopes ? kLog2e : col[c].factor * kLog2e;
 #pragma unroll
         for (int b = 0; b < NB; b++) o[c][b][0] = o[c][b][1] = f32x4{0, 0, 0, 0};
@@ -1000,7 +994,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
             const bool full = t * 32 >= flo && t * 32 + 32 <= fhi;
             const int key0 = t * 32 + 8 * g;
             half8 ph[CT], pl[CT];
-            const float *kup = room.k.up[t & 3] + 8 * g, *vup = room.v.up[t & 3] + 8 * g;
+            const bool nan = room.nan[t & 3] != 0;
+            const uint16_t* ok = room.v.ok[t & 3] + 8 * g;
+            const float *kup = room.k.e[t & 3] + 8 * g, *ve = room.v.e[t & 3] + 8 * g,
+                        *vdown8 = room.v.down[t & 3] + 8 * g;
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 float x[8];
@@ -1023,10 +1020,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
                             x[j] = -INFINITY;
                 }
                 const float f = unit_of[c];
-                const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * f;
-                if (__any(top > limit[c])) {
-                    const float m = fmaxf(base[c] == -FLT_MAX ? -FLT_MAX : base[c] + 10.0f, across_groups_max(top));
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fmaf(x[j], f, ve[j]));
+                if (__any(top > base[c] + 14.0f)) {
+                    // (a whole number, so that e - base is exact)
+                    const float m = fmaxf(base[c] == -FLT_MAX ? -FLT_MAX : base[c] + 10.0f, ceilf(across_groups_max(top)));
                     const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, k = __builtin_amdgcn_exp2f(base[c] - nb);
                     l[c] *= k;
 #pragma unroll
@@ -1035,21 +1034,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
                         o[c][b][1] *= k;
                     }
                     base[c] = nb;
-                    limit[c] = m == -FLT_MAX ? -FLT_MAX : m + 4.0f;
                 }
                 uint32_t hw[4], lw[4];
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float u = __builtin_amdgcn_exp2f(fmaf(x[2 * j], f, -base[c])),
-                                v = __builtin_amdgcn_exp2f(fmaf(x[2 * j + 1], f, -base[c]));
-                    sum += u + v;
-                    float uw = u * vup[2 * j], vw = v * vup[2 * j + 1];
-                    if (!full) {  // (a NaN of a key that this row does not see stays out)
-                        uw = x[2 * j] == -INFINITY ? 0.0f : uw;
-                        vw = x[2 * j + 1] == -INFINITY ? 0.0f : vw;
+                    float u = __builtin_amdgcn_exp2f(fmaf(x[2 * j], f, ve[2 * j] - base[c])),
+                          v = __builtin_amdgcn_exp2f(fmaf(x[2 * j + 1], f, ve[2 * j + 1] - base[c]));
+                    sum = fmaf(u, vdown8[2 * j], sum);
+                    sum = fmaf(v, vdown8[2 * j + 1], sum);
+                    if (nan) {  // (that of a key that this row does not see stays out)
+                        u = ok[2 * j] || x[2 * j] == -INFINITY ? u : __builtin_nanf("");
+                        v = ok[2 * j + 1] || x[2 * j + 1] == -INFINITY ? v : __builtin_nanf("");
                     }
-                    split2(uw, vw, hw[j], lw[j]);
+                    split2(u, v, hw[j], lw[j]);
                 }
                 l[c] += sum;
                 ph[c] = as_half8(hw[0], hw[1], hw[2], hw[3]);
@@ -1934,7 +1932,7 @@ static int launch_weigh(fh_ctx* ctx, AttnArgs& a, size_t tiles16) {
     a.splits = static_cast<int>(splits);
     if (splits > 1) {
         void* ws = nullptr;
-        const int rc = fh_workspace(ctx, splits * heads * a.max_keys * sizeof(float), &ws);
+        const int rc = fh_kv4_room(ctx, splits * heads * a.max_keys * sizeof(float), &ws);
         if (rc) return rc;
         a.part = static_cast<float*>(ws);
     }
@@ -1982,7 +1980,7 @@ int fh_launch_kv4_evict(fh_ctx* ctx, const fh_kv4_cache& src, const fh_kv4_cache
     const Cache c = device_cache(src), d = device_cache(dst);
     const size_t heads = src.seqs * src.n_kv, idx_bytes = fh_align256(heads * keep * sizeof(uint32_t));
     void* ws = nullptr;
-    const int rc = fh_workspace(ctx, idx_bytes + heads * sizeof(uint32_t), &ws);
+    const int rc = fh_kv4_room(ctx, idx_bytes + heads * sizeof(uint32_t), &ws);
     if (rc) return rc;
     uint32_t* idx = static_cast<uint32_t*>(ws);
     uint32_t* counts = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + idx_bytes);

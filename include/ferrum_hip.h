@@ -512,8 +512,10 @@ int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q
  * exp(score).  A row that sees nothing gets 0 and -inf.  max_keys bounds the cache
  * rows in use after the call's rows (it sizes the launch); a row whose cache row is at or past
  * max_keys or the capacity gets NaN.  Within 1e-5 of float64 over the cache's
- * values.  The context's workspace for it is allocated once and never moves;
- * calls of one context must not overlap, replayed graphs included. */
+ * values.  A block that holds a NaN makes NaN of the rows that see it, of its own
+ * channels at least.  The context's workspace for these calls is never freed before the
+ * context ends, so captured graphs stay valid; calls of one context must not
+ * overlap, replayed graphs included. */
 int fh_kv4_attention_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
                            size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
                            size_t max_keys, const fh_attn_score* score, float* d_out, float* d_lse);

@@ -25,7 +25,8 @@ class Box:
     """A cache whose unused rows hold the worst that memory can: NaN and huge
     scales.  Rows below `lens` hold quantised normals, kept here as float64."""
 
-    def __init__(self, seqs, n_kv, hd, cap, lens, seed, tracked=False, k_std=1.0, v_std=1.0):
+    def __init__(self, seqs, n_kv, hd, cap, lens, seed, tracked=False, k_std=1.0, v_std=1.0, repeat=1):
+        """repeat: so many times the sequences given, one set after the other."""
         import ferrum_hip
         import torch
 
@@ -57,6 +58,12 @@ class Box:
                         plane[s, h][used] = new[used]
                     else:
                         plane[s, h, :n * hd // 2] = new[:n * hd // 2]
+        if repeat > 1:
+            again = lambda x: np.tile(x, (repeat,) + (1,) * (x.ndim - 1))  # noqa: E731
+            kp, kd, vp, vd, self.k, self.v, self.kstep, self.vstep = map(
+                again, (kp, kd, vp, vd, self.k, self.v, self.kstep, self.vstep))
+            self.seqs = seqs = seqs * repeat
+            self.lens = self.lens * repeat
         self.pos = np.tile(np.arange(cap, dtype=np.int32), (seqs, n_kv, 1)) if tracked else None
         self.weight = rng.random((seqs, n_kv, cap)).astype(np.float32) if tracked else None
         planes = [gpu(kp), gpu(kd), gpu(vp), gpu(vd)]
@@ -86,41 +93,49 @@ def check_attention(box, q, lens, news, out, lse, first=None, end=None, softcap=
     group = n_heads // box.n_kv
     total_w = np.zeros((box.seqs, box.n_kv, box.cap))
     tol_w = np.zeros_like(total_w)
-    _, places = rows_of(lens, news)
-    for s, row, at, t in places:
+    off, _ = rows_of(lens, news)
+    for s in range(box.seqs):
+        rows = np.arange(off[s], off[s + 1])
+        at = lens[s] + np.arange(news[s])
         keys = min(lens[s] + news[s], box.cap)
-        lo = 0 if first is None else int(first[row])
-        hi = min(at + 1 if end is None else int(end[row]), keys)
-        if at >= keys:
-            assert np.isnan(out[row]).all() and (lse is None or np.isnan(lse[row]).all())
+        lo = np.zeros(news[s], np.int64) if first is None else np.minimum(np.asarray(first, np.int64)[rows], keys)
+        hi = np.minimum(at + 1 if end is None else np.asarray(end, np.int64)[rows], keys)
+        bad = at >= keys
+        none = ~bad & (lo >= hi)
+        assert np.isnan(out[rows[bad]]).all() and (out[rows[none]] == 0).all()
+        if lse is not None:
+            assert np.isnan(lse[rows[bad]]).all() and (lse[rows[none]] == -np.inf).all()
+        ok = ~bad & ~none
+        if not ok.any():
             continue
-        kp = None if box.pos is None else box.pos[s].astype(np.int64)
-        o, z, w = ref.attention(q[row:row + 1], box.k[s], box.v[s], [lo], [hi], softcap, slopes,
-                                None if slopes is None else [at if qpos is None else qpos[row]], kp)
-        if lo >= hi:
-            assert (out[row] == 0).all() and (lse is None or (lse[row] == -np.inf).all())
-            continue
+        rows, lo, hi, at = rows[ok], lo[ok], hi[ok], at[ok]
+        here = np.arange(hi.max())
+        seen = (here >= lo[:, None]) & (here < hi[:, None])
         for h in range(n_heads):
-            g, qa = h // group, np.abs(q[row, h]).astype(np.float64)
-            a = 8 * box.kstep[s, g, lo:hi] @ qa / np.sqrt(hd)
-            score = box.k[s, g, lo:hi] @ q[row, h].astype(np.float64) / np.sqrt(hd)
+            g, x = h // group, q[rows, h].astype(np.float64)
+            k, v = box.k[s, g, :len(here)], box.v[s, g, :len(here)]
+            ks, vs = 8 * box.kstep[s, g, :len(here)], 8 * box.vstep[s, g, :len(here)]
+            score, a = x @ k.T / np.sqrt(hd), np.abs(x) @ ks.T / np.sqrt(hd)
             if softcap:
                 score = softcap * np.tanh(score / softcap)
                 a = a + softcap * (np.abs(score) > 0.4 * softcap) + np.abs(score)
             if slopes is not None:
-                here = np.arange(lo, hi) if kp is None else kp[g, lo:hi]
-                far = slopes[h] * np.abs((at if qpos is None else int(qpos[row])) - here)
-                score, a = score - far, a + np.abs(far)
-            p = np.exp(score - z[0, h])
-            abar = (p * a).sum()
-            mass = p @ (8 * box.vstep[s, g, lo:hi])
-            tol = 2.0 ** -21 * ((p * (a + abar)) @ (8 * box.vstep[s, g, lo:hi])) + 2.0 ** -18 * mass
-            err = np.abs(out[row, h] - o[0, h])
-            assert (err <= tol).all(), (s, row, h, float((err / tol).max()))
+                kp = here if box.pos is None else box.pos[s, g, :len(here)].astype(np.int64)
+                me = at if qpos is None else np.asarray(qpos, np.int64)[rows]
+                far = np.float64(slopes[h]) * np.abs(me[:, None] - kp)
+                score, a = score - far, a + far
+            score = np.where(seen, score, -np.inf)
+            top = score.max(axis=1, keepdims=True)
+            mass = np.exp(score - top).sum(axis=1, keepdims=True)
+            z, p = (top + np.log(mass))[:, 0], np.exp(score - top) / mass
+            abar = (p * a).sum(axis=1, keepdims=True)
+            tol = 2.0 ** -21 * ((p * (a + abar)) @ vs) + 2.0 ** -18 * (p @ vs)
+            err = np.abs(out[rows, h] - p @ v)
+            assert (err <= tol).all(), (s, h, float((err / tol).max()))
             if lse is not None:
-                assert abs(lse[row, h] - z[0, h]) <= 2.0 ** -21 * abar + 2.0 ** -20 * (1 + abs(z[0, h]))
-            total_w[s, g, lo:hi] += p
-            tol_w[s, g, lo:hi] += p * (2.0 ** -21 * (a + abar) + 2.0 ** -20 * (1 + abs(z[0, h])))
+                assert (np.abs(lse[rows, h] - z) <= 2.0 ** -21 * abar[:, 0] + 2.0 ** -20 * (1 + np.abs(z))).all()
+            total_w[s, g, :len(here)] += p.sum(axis=0)
+            tol_w[s, g, :len(here)] += (p * (2.0 ** -21 * (a + abar) + 2.0 ** -20 * (1 + np.abs(z[:, None])))).sum(axis=0)
     if weight is not None:
         want = box.weight.astype(np.float64) + total_w
         # (one rounding of the stored sum, sqrt(columns) of the columns' own)
@@ -168,7 +183,8 @@ def attend(fh, box, n_heads, lens, news, seed, use_off, masks=None, softcap=0.0,
 @pytest.mark.parametrize("n_heads,n_kv,hd", HEADS)
 @pytest.mark.parametrize("lens,news", [([0], [1]), ([7, 0, 8, 3], [1, 1, 1, 1]), ([5, 0], [30, 30]), ([3, 8, 20], [0, 17, 4])])
 @pytest.mark.parametrize("rope", [None, "norm", "neox", "part"])
-def test_append_writes_the_formats_bytes(fh, n_heads, n_kv, hd, lens, news, rope):
+@pytest.mark.parametrize("pad", [0, 3])  # (rows that are 16-byte aligned, and rows that are not)
+def test_append_writes_the_formats_bytes(fh, n_heads, n_kv, hd, lens, news, rope, pad):
     import ferrum_hip
     import torch
 
@@ -194,11 +210,11 @@ def test_append_writes_the_formats_bytes(fh, n_heads, n_kv, hd, lens, news, rope
     rd = 0 if rope is None else hd // 2 if rope == "part" else hd
     ff = rng.uniform(0.5, 2, rd // 2).astype(np.float32) if rope == "part" else None
     lin = 2.0 if rope == "part" else 1.0
-    buf = np.full((total, wide + 3), np.nan, np.float32)
+    buf = np.full((total, wide + pad), np.nan, np.float32)
     buf[:, :wide] = x.reshape(total, wide)
     q = torch.full((total, n_heads * hd), float("nan"), device="cuda")
     uniform = len(set(news)) == 1
-    args = (gpu(buf), wide + 3, total, n_heads, None if uniform else ints(off), max(news), ints(lens), ints(pos), rd, 1e4,
+    args = (gpu(buf), wide + pad, total, n_heads, None if uniform else ints(off), max(news), ints(lens), ints(pos), rd, 1e4,
             ferrum_hip.ROPE_NORM if rope == "norm" else ferrum_hip.ROPE_NEOX, None if ff is None else gpu(ff), lin, q)
     torch.cuda.synchronize()
     ferrum_hip.kv4_append_async(fh, box.c, *args)
@@ -295,11 +311,60 @@ def test_prompts(fh, n_heads, n_kv, hd, lens, news):
     attend(fh, box, n_heads, lens, news, 9, True, weigh=True, ld_pad=5, tail=3)
 
 
-def test_many_rows_take_a_wave_each(fh):
-    """Enough columns for the form in which each wave has its own."""
-    lens, news = [3, 0, 17, 8], [90, 130, 64, 77]
-    box = Box(4, 8, 64, 136, [a + b for a, b in zip(lens, news)], 18, tracked=True)
-    attend(fh, box, 32, lens, news, 19, True, weigh=True)
+# Enough columns (at least 512 workgroups of 128, three quarters of them in use) for the form
+# in which columns share each key's expansion.
+MANY = [(8, 2, 64, 32), (8, 2, 128, 32), (12, 12, 64, 6)]
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,repeat", MANY)
+@pytest.mark.parametrize("kind", ["causal", "documents", "prefix", "holes", "beyond"])
+@pytest.mark.parametrize("options", [False, True])
+def test_many_rows(fh, n_heads, n_kv, hd, repeat, kind, options):
+    lens, news = [0, 41, 7, 130] * repeat, [120, 101, 117, 128] * repeat
+    if n_kv == 12:
+        lens, news = [0, 41, 7, 130] * repeat, [480, 501, 417, 510] * repeat
+    top = max(a + b for a, b in zip(lens, news))
+    box = Box(4, n_kv, hd, -(-top // 8) * 8, [a + b for a, b in zip(lens, news)][:4], 18, repeat=repeat)
+    masks = None if kind == "causal" else masks_of(kind, lens, news, np.random.default_rng(2))
+    slopes = 2.0 ** (-8.0 * np.arange(1, n_heads + 1) / n_heads) if options else None
+    attend(fh, box, n_heads, lens, news, 19, True, masks, softcap=3.0 if options else 0.0, slopes=slopes, ld_pad=4, tail=2)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("repeat", [1, 64])  # (few columns, and many)
+def test_values_far_apart(fh, repeat, hd):
+    """A document of huge keys and values beside one of tiny ones, a NaN in a third, and blocks of
+    very different size: each row has the accuracy of what it sees."""
+    import torch
+
+    n_kv = 2
+    lens, news = [0, 0] * repeat, [96, 96] * repeat
+    box = Box(2, n_kv, hd, 96, [96, 96], 80, repeat=repeat)
+    nb = hd // 32
+    scale = np.ones((96, nb))
+    scale[32:40] = 2.0 ** 12
+    scale[40:64] = 2.0 ** -9
+    scale[:, nb // 2:] *= 2.0 ** -3
+    by = scale.reshape(12, 8, nb).transpose(0, 2, 1)
+    for name, val, step, f in (("k_d", box.k, box.kstep, np.where(by > 1, 4.0, 0.5)), ("v_d", box.v, box.vstep, by)):
+        old = box.plane(name)
+        new = (old.astype(np.float32) * f).astype(np.float16)  # (the smallest are subnormal: rounded again)
+        ratio = np.repeat((new.astype(np.float64) / old.astype(np.float64)).transpose(0, 1, 2, 4, 3).reshape(
+            box.seqs, n_kv, 96, nb), 32, axis=3)
+        val *= ratio
+        step *= np.abs(ratio)
+        if name == "v_d":
+            new[:, :, 9, 0, 3] = np.nan  # key 75
+        box.c.planes[name].copy_(gpu(new))
+    torch.cuda.synchronize()
+    # documents: keys 0 .. 31, 32 .. 39, 40 .. 63, 64 .. 74, and rows of the last see 64 .. 74 too
+    first, end = [], []
+    for s in range(2 * repeat):
+        for t in range(96):
+            f = 0 if t < 32 else 32 if t < 40 else 40 if t < 64 else 64
+            first.append(f)
+            end.append(min(t + 1, 75))
+    attend(fh, box, 8, lens, news, 81, True, (first, end))
 
 
 def masks_of(kind, lens, news, rng):
@@ -426,6 +491,42 @@ def test_a_nan_key_reaches_only_the_rows_that_see_it(fh):
         o = out.cpu().numpy().reshape(20, 14, 64)
         assert np.isfinite(o[:10]).all() and np.isfinite(o[10:, 7:]).all()
         assert np.isnan(o[10:, :7]).any(axis=(1, 2)).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("name", ["k_d", "v_d"])
+def test_a_nan_key_among_many_rows(fh, hd, name):
+    """In every fourth sequence: its neighbours and the rows before it stay as they were, and a NaN
+    among the values is none of the scores'."""
+    import ferrum_hip
+    import torch
+
+    seqs, rows = 128, 64
+    box = Box(4, 2, hd, 64, [64] * 4, 25, repeat=seqs // 4)
+    q = torch.randn((seqs * rows, 8 * hd), device="cuda")
+    outs = []
+    for bad in (False, True):
+        if bad:
+            box.c.planes[name][::4, 0, 5, 1, 0] = float("nan")  # key 40 of head 0
+        out, lse = torch.zeros_like(q), torch.zeros((seqs * rows, 8), device="cuda")
+        torch.cuda.synchronize()
+        ferrum_hip.kv4_attention_async(fh, box.c, q, 8 * hd, seqs * rows, 8, ints(np.arange(seqs + 1) * rows), rows,
+                                       ints([0] * seqs), 64, None, out, lse)
+        fh.sync()
+        outs.append((out.cpu().numpy().reshape(seqs, rows, 8, hd), lse.cpu().numpy().reshape(seqs, rows, 8)))
+    (o, z), (ob, zb) = outs
+    hit = np.zeros((seqs, rows, 8), bool)
+    hit[::4, 40:, :4] = True
+    assert np.isfinite(o).all() and np.array_equal(ob[~hit], o[~hit]) and np.array_equal(zb[~hit], z[~hit])
+    assert np.isnan(ob[hit]).any(axis=-1).all()
+    if name == "k_d":
+        assert np.isnan(zb[hit]).all()
+    else:
+        # The scores are the same bits, but the running maximum goes by the values' exponents too, and a
+        # NaN has none: other powers of two stand before the sums, so exp2's arguments round elsewhere.
+        # Either sum is within 2^-20 of itself (exp2 2^-23 and its argument 2^-22, 64 terms' additions
+        # at most 2^-21 together in sequences of 8, 2 and 4), its log and the product 2^-23 (1 + |z|).
+        assert (np.abs(zb[hit] - z[hit]) <= 2.0 ** -19 + 2.0 ** -22 * (1 + np.abs(z[hit]))).all()
 
 
 # ---- eviction -------------------------------------------------------------------
@@ -571,6 +672,127 @@ def test_captured_calls_replay_as_they_ran(fh):
     assert all(np.array_equal(a, seen[0][0]) and np.array_equal(b, seen[0][1]) for a, b in seen)
 
 
+def test_capture_needs_a_first_run_and_outlives_larger_ones():
+    """On a fresh context the calls that need workspace refuse to be captured; after one
+    run they can be, and a larger call later leaves the captured graph as it was."""
+    import ferrum_hip
+    import torch
+
+    def args(c, box, rows, lens):
+        q = torch.randn((len(lens) * rows, 8 * 128), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+        out, lse = torch.empty_like(q), torch.empty((len(lens) * rows, 8), device="cuda")
+        return (c, box.c, q, 1024, len(lens) * rows, 8, None, rows, ints(lens), max(lens) + rows, None), out, lse
+
+    with ferrum_hip.Context(0) as c:
+        box = Box(1, 2, 128, 1024, [1000], 61, tracked=True)
+        start = box.c.planes["weight"].clone()
+        spare = Box(1, 2, 128, 512, [0], 62, tracked=True)
+        a, out, lse = args(c, box, 100, [900])
+        ln, new = ints([1000]), ints([0])
+
+        def calls():
+            ferrum_hip.kv4_attention_async(*a, out, lse)
+            ferrum_hip.kv4_weigh_async(*a, lse)
+            ferrum_hip.kv4_evict_async(c, box.c, spare.c, ln, 1000, 500, 20, new)
+
+        def capture():
+            g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            refused = []
+            try:
+                with torch.cuda.graph(g, stream=s):
+                    c.set_stream(torch.cuda.current_stream().cuda_stream)
+                    try:
+                        calls()
+                    except ferrum_hip.FerrumHipError as e:
+                        refused.append(e)
+            finally:
+                c.set_stream(None)
+            return g, refused
+
+        torch.cuda.synchronize()
+        _, refused = capture()
+        assert refused and "outside capture first" in refused[0].msg
+        calls()
+        c.sync()
+        box.c.planes["weight"].copy_(start)
+        torch.cuda.synchronize()
+        calls()
+        c.sync()
+        want = [t.clone() for t in (out, box.c.planes["weight"], spare.c.planes["pos"], new)]
+        g, refused = capture()
+        assert not refused
+        big = Box(4, 2, 128, 2048, [2000] * 4, 63, tracked=True)
+        b, out2, lse2 = args(c, big, 300, [1700] * 4)
+        to = Box(4, 2, 128, 1600, [0] * 4, 64, tracked=True)
+        ferrum_hip.kv4_attention_async(*b, out2, lse2)
+        ferrum_hip.kv4_weigh_async(*b, lse2)
+        ferrum_hip.kv4_evict_async(c, big.c, to.c, ints([2000] * 4), 2000, 1600, 20, ints([0] * 4))
+        c.sync()
+        for _ in range(3):
+            box.c.planes["weight"].copy_(start)
+            out.fill_(float("nan"))
+            new.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(want, (out, box.c.planes["weight"], spare.c.planes["pos"], new)))
+
+
+def test_planes_beyond_four_gibibytes(fh):
+    """The last of 20 sequences, whose levels lie past 2^32 bytes of their planes."""
+    import ferrum_hip
+    import torch
+
+    seqs, n_kv, hd, cap, n = 20, 8, 128, 1 << 19, 70
+    small = Box(1, n_kv, hd, 80, [n + 1], 70, tracked=True)
+    nb = hd // 32
+    zeros = lambda dt, *s: torch.zeros((seqs, n_kv, *s), dtype=dt, device="cuda")  # noqa: E731
+    k, v = zeros(torch.uint8, cap * hd // 2), zeros(torch.uint8, cap * hd // 2)
+    assert k.numel() > 2 ** 32
+    kd, vd = zeros(torch.float16, cap // 8, nb, 8), zeros(torch.float16, cap // 8, nb, 8)
+    weight = zeros(torch.float32, cap)
+    p = small.c.planes
+    for big, name in ((k, "k"), (kd, "k_d"), (v, "v"), (vd, "v_d")):
+        big[-1, :, :p[name].shape[2]] = p[name][0]
+    c = ferrum_hip.KV4Cache(seqs, n_kv, hd, cap, k, kd, v, vd, None, weight)
+    one = dict(total=seqs, q=torch.randn((seqs, 32 * hd), device="cuda"))
+    lens = ints([0] * (seqs - 1) + [n])
+    out, lse = torch.empty_like(one["q"]), torch.empty((seqs, 32), device="cuda")
+    ref_out, ref_lse = torch.empty((1, 32 * hd), device="cuda"), torch.empty((1, 32), device="cuda")
+    small.c.planes["weight"].zero_()
+    torch.cuda.synchronize()
+    args = (fh, c, one["q"], 32 * hd, seqs, 32, None, 1, lens, n + 1, None)
+    ferrum_hip.kv4_attention_async(*args, out, lse)
+    ferrum_hip.kv4_weigh_async(*args, lse)
+    args = (fh, small.c, one["q"][-1:], 32 * hd, 1, 32, None, 1, ints([n]), n + 1, None)
+    ferrum_hip.kv4_attention_async(*args, ref_out, ref_lse)
+    ferrum_hip.kv4_weigh_async(*args, ref_lse)
+    rk, rv = (torch.empty((seqs, n, n_kv * hd), device="cuda") for _ in range(2))
+    sk, sv = (torch.empty((1, n, n_kv * hd), device="cuda") for _ in range(2))
+    ferrum_hip.kv4_read_async(fh, c, None, n, rk, rv)
+    ferrum_hip.kv4_read_async(fh, small.c, None, n, sk, sv)
+    fh.sync()
+    # (the two differ in how many workgroups share the keys, by roundings only)
+    assert torch.allclose(out[-1], ref_out[0], rtol=1e-5, atol=1e-5) and torch.allclose(lse[-1], ref_lse[0], rtol=1e-5)
+    assert torch.allclose(weight[-1, :, :n + 1], small.c.planes["weight"][0, :, :n + 1], rtol=1e-5, atol=1e-6)
+    assert torch.equal(rk[-1], sk[0]) and torch.equal(rv[-1], sv[0])
+    x = torch.randn((seqs, (32 + 16) * hd), device="cuda")
+    to = ferrum_hip.KV4Cache.alloc(seqs, n_kv, hd, 64)
+    new = ints([0] * seqs)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_append_async(fh, c, x, 48 * hd, seqs, 32, None, 1, lens)
+    ferrum_hip.kv4_append_async(fh, small.c, x[-1:], 48 * hd, 1, 32, None, 1, ints([n]))
+    weight[-1, :, :n] = torch.rand((n_kv, n), device="cuda")
+    small.c.planes["weight"][0, :, :n] = weight[-1, :, :n]
+    torch.cuda.synchronize()
+    to1 = ferrum_hip.KV4Cache.alloc(1, n_kv, hd, 64)
+    ferrum_hip.kv4_evict_async(fh, c, to, ints([0] * (seqs - 1) + [n + 1]), n + 1, 60, 5, new)
+    ferrum_hip.kv4_evict_async(fh, small.c, to1, ints([n + 1]), n + 1, 60, 5, ints([0]))
+    fh.sync()
+    for name in ("k", "k_d", "v", "v_d"):
+        assert torch.equal(to.planes[name][-1], to1.planes[name][0]), name
+
+
 def test_two_contexts_on_two_streams_at_once(fh):
     import ferrum_hip
     import torch
@@ -642,6 +864,7 @@ def test_refusals(fh):
         (F.FH_ERR_DIM, "RoPE scaling", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, rope_dim=8, linear_factor=0.0)),
         (F.FH_ERR_INVALID, "must not be qkv", lambda: F.kv4_append_async(fh, ok, q, 512, 2, 4, None, 1, ln, q=q)),
         (F.FH_ERR_INVALID, "qkv is NULL", lambda: F.kv4_append_async(fh, ok, None, 512, 2, 4, None, 1, ln)),
+        (F.FH_ERR_LIMIT, "workgroups", lambda: F.kv4_append_async(fh, cache(seqs=65535, n_kv=1), q, 512, 1 << 29, 2, ln, 1 << 29, ln)),
         (F.FH_ERR_INVALID, "no weight plane", lambda: F.kv4_evict_async(fh, bare, ok, ln, 32, 8, 0, ln)),
         (F.FH_ERR_INVALID, "share a plane", lambda: F.kv4_evict_async(fh, ok, ok, ln, 32, 8, 0, ln)),
         (F.FH_ERR_DIM, "above the capacity", lambda: F.kv4_evict_async(fh, ok, bare, ln, 32, 33, 0, ln)),
