@@ -381,6 +381,27 @@ __device__ __forceinline__ void scores(const uint32_t (&k)[2][Shape<HD>::NB], co
     }
 }
 
+// Less slope * distance, of the octet of keys at key0.
+__device__ __forceinline__ void less_distance(const AttnArgs& a, float slope, int qpos, const uint32_t* kpos, int key0,
+                                              float (&x)[8]) {
+    int kp[8];
+    if (kpos) {
+        typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        const u32x4u* from = reinterpret_cast<const u32x4u*>(kpos + min(key0, a.c.cap - 8));
+        const u32x4u u = from[0], v = from[1];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            kp[j] = static_cast<int>(u[j]);
+            kp[4 + j] = static_cast<int>(v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) kp[j] = key0 + j;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = fmaf(-slope, static_cast<float>(abs(qpos - kp[j])), x[j]);
+}
+
 // Options applied: scores then in the exponent's unit (log2), as they were without any.
 template <int HD, bool MODS>
 __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD>& col, const uint32_t* kpos, int key0,
@@ -389,14 +410,9 @@ __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD
 #pragma unroll
         for (int j = 0; j < 8; j++) s[j] *= col.factor;
         if (a.softcap > 0.0f) cap_scores(s, a.softcap, 1.0f);
+        if (a.slopes) less_distance(a, col.slope, col.qpos, kpos, key0, s);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (a.slopes) {
-                const int kp = kpos ? static_cast<int>(kpos[min(key0 + j, a.c.cap - 1)]) : key0 + j;
-                s[j] = fmaf(-col.slope, static_cast<float>(abs(col.qpos - kp)), s[j]);
-            }
-            s[j] *= kLog2e;
-        }
+        for (int j = 0; j < 8; j++) s[j] *= kLog2e;
     }
 }
 
@@ -730,18 +746,25 @@ struct Stage {
     uint32_t k[2][Shape<HD>::NB][2][64][4];  // keys as MFMA rows 0 .. 15 and 16 .. 31, by block and f16 term
     uint32_t v[Shape<HD>::NB][2][2][64][4];  // values, by block, channel parity and f16 term
 };
-// Per key of four tiles: e, the largest exponent of its scales (values' under vexp; of keys
-// as 2^e), 2^-e, and the bits of a scale to take: none of a key that nobody sees or that
-// holds a NaN.  Such a NaN is in a key's 2^e; values' are told by nan.
-struct Factors {
-    float e[4][32], down[4][32];
-    uint16_t ok[4][32];
+// What a column keeps here rather than in registers (which would be spilled).
+struct Place {
+    float unit, factor, slope;  // unit: log2 units of a score, distance off
+    int qpos, first, wide;
+    uint32_t row;   // all ones: not a column of the call
+    uint32_t head;  // the top bit: its row has no place in the cache
 };
+
+// Of four tiles' keys: the block scales under 2^e (0 of a key that nobody sees or that
+// holds a NaN), e being the largest exponent of a key's own; as 2^e of keys (NaN
+// where they hold one), as e and 2^-e of values (under their blocks' exponents).
 template <int HD>
 struct Room {
     Stage<HD> stage[2];
-    Factors k, v;
-    int nan[4], range[2], vbits[4];
+    Place place[128];
+    float kup[4][32], ve[4][32], vdown[4][32];
+    uint16_t d[2][4][Shape<HD>::NB][32];  // of values, of keys
+    uint32_t nan[4];                      // a bit a key whose values hold one
+    int range[2], vbits[4];
 };
 
 // One thread's share of a tile on its way to LDS.
@@ -749,9 +772,8 @@ template <int HD>
 struct Load {
     static constexpr int W = HD == 128 ? 2 : 1;  // words of keys
     uint32_t k[W];
-    uint16_t kd[W];
-    u32x4 v, vd;
-    uint16_t d[Shape<HD>::NB];  // a key's scales, two tiles ahead (threads 0 .. 31 values', 32 .. 63 keys')
+    u32x4 v;
+    uint16_t d[Shape<HD>::NB];  // a key's scales, two tiles ahead (lanes 0 .. 31 of one wave values', the others keys')
 };
 
 // A thread stages the levels of one key (MFMA row n of half h), channels 8 g .. + 7 of
@@ -790,10 +812,7 @@ __device__ __forceinline__ void load_part(const Planes& p, int cap, int tile, co
     } else {
         t.k[0] = *reinterpret_cast<const uint32_t*>(a);
     }
-#pragma unroll
-    for (int i = 0; i < Load<HD>::W; i++) t.kd[i] = p.kd[key / 8 * (NB * 8) + (w.kb + i) * 8 + key % 8];
     t.v = *reinterpret_cast<const u32x4*>(p.v + (o * VU + w.unit()) * 16);
-    t.vd = *reinterpret_cast<const u32x4*>(p.vd + (o * NB + w.vb) * 8);
 }
 
 __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
@@ -806,7 +825,7 @@ __device__ __forceinline__ void times_scale(uint32_t level, half2v scale, uint32
     lo = bits(__builtin_elementwise_fma(x, scale, -h));
 }
 template <int HD, int I>
-__device__ __forceinline__ void store_values(const Part<HD>& w, const u32x4& v, const uint32_t (&d)[4], Stage<HD>& st) {
+__device__ __forceinline__ void store_values(const Part<HD>& w, const u32x4& v, const u32x4& d, Stage<HD>& st) {
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) times_scale(levels2<I>(v[i] >> w.shift()), as_half2(d[i]), hi[i], lo[i]);
@@ -816,13 +835,13 @@ __device__ __forceinline__ void store_values(const Part<HD>& w, const u32x4& v, 
 }
 
 template <int HD>
-__device__ __forceinline__ void store_part(int tile, const Part<HD>& w, const Load<HD>& t, const Factors& fk,
-                                           const Factors& fv, float vdown, Stage<HD>& st) {
+__device__ __forceinline__ void store_part(int tile, const Part<HD>& w, const Load<HD>& t, Room<HD>& room) {
     if (!w.on) return;
-    const int lane = w.g * 16 + w.n, f = tile & 3, key = w.key();
+    const int lane = w.g * 16 + w.n, f = tile & 3;
+    Stage<HD>& st = room.stage[tile & 1];
 #pragma unroll
     for (int i = 0; i < Load<HD>::W; i++) {
-        const _Float16 x = static_cast<_Float16>(fh_h2f(t.kd[i] & fk.ok[f][key]) * fk.down[f][key]);
+        const _Float16 x = __builtin_bit_cast(_Float16, room.d[1][f][w.kb + i][w.key()]);
         const half2v sc = {x, x};
         uint32_t hi[4], lo[4];
         times_scale(levels2<0>(t.k[i]), sc, hi[0], lo[0]);
@@ -832,15 +851,7 @@ __device__ __forceinline__ void store_part(int tile, const Part<HD>& w, const Lo
         *reinterpret_cast<u32x4*>(st.k[w.h][w.kb + i][0][lane]) = u32x4{hi[0], hi[1], hi[2], hi[3]};
         *reinterpret_cast<u32x4*>(st.k[w.h][w.kb + i][1][lane]) = u32x4{lo[0], lo[1], lo[2], lo[3]};
     }
-    const u32x4 ok = *reinterpret_cast<const u32x4*>(&fv.ok[f][8 * w.g]);
-    uint32_t d[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const half2v x = as_half2(t.vd[i] & ok[i]);
-        const half2v y = {static_cast<_Float16>(static_cast<float>(x[0]) * (fv.down[f][8 * w.g + 2 * i] * vdown)),
-                          static_cast<_Float16>(static_cast<float>(x[1]) * (fv.down[f][8 * w.g + 2 * i + 1] * vdown))};
-        d[i] = bits(y);
-    }
+    const u32x4 d = *reinterpret_cast<const u32x4*>(&room.d[0][f][w.vb][8 * w.g]);
     if constexpr (HD == 128) {
         store_values<HD, 0>(w, t.v, d, st);
         store_values<HD, 1>(w, t.v, d, st);
@@ -873,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     if (static_cast<uint64_t>(ct0) * 16 >= static_cast<uint64_t>(r.count) * a.group) return;
-    Column<HD> col[CT];
+    Column<HD> col[CT];  // (their queries alone stay)
     int lo = 0x7FFFFFFF, hi = 0, flo = 0, fhi = 0x7FFFFFFF;
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -903,8 +914,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     const Part<HD> part(tid);
     Load<HD> ld;
     const auto load_scales = [&](int tile) {
-        const uint32_t key = min(tile * 32 + (tid & 31), a.c.cap - 1);
-        const uint16_t* from = (tid < 32 ? p.vd : p.kd) + key / 8 * (NB * 8) + key % 8;
+        const uint32_t key = min(tile * 32 + (lane & 31), a.c.cap - 1);
+        const uint16_t* from = (lane < 32 ? p.vd : p.kd) + key / 8 * (NB * 8) + key % 8;
 #pragma unroll
         for (int b = 0; b < NB; b++) ld.d[b] = from[b * 8];
     };
@@ -924,59 +935,66 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         atomicMax(&room.vbits[tid % NB], static_cast<int>(m));
     }
 #pragma unroll
-    for (int c = 0; c < CT; c++) column_query<HD>(a, lane, col[c]);
+    for (int c = 0; c < CT; c++) {
+        column_query<HD>(a, lane, col[c]);
+        if (g == 0) {
+            const float unit = MODS && a.slopes ? kLog2e : col[c].factor * kLog2e;
+            Place& to = room.place[(wave * CT + c) * 16 + n];
+            to = Place{unit, col[c].factor, MODS ? col[c].slope : 0.0f, MODS ? col[c].qpos : 0, col[c].first, col[c].wide,
+                       col[c].on ? col[c].row : ~0u, static_cast<uint32_t>(col[c].head) | (col[c].bad ? 0x80000000u : 0u)};
+        }
+    }
     __syncthreads();
     int vexp[NB];
-    float vdown = 1.0f;
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-        vexp[b] = min(__builtin_amdgcn_readfirstlane(room.vbits[b]) >> 10, 30) - 14;
-        vdown = part.vb == b ? ldexpf(1.0f, -vexp[b]) : vdown;
-    }
-    const auto key_factors = [&](int tile) {  // of key tid % 32, from ld.d
+    for (int b = 0; b < NB; b++) vexp[b] = min(__builtin_amdgcn_readfirstlane(room.vbits[b]) >> 10, 30) - 14;
+    const auto key_factors = [&](int tile) {  // of key lane % 32, from ld.d
+        const int i = tile & 3, j = lane & 31, key = tile * 32 + j;
         int e = -64;
         bool fine = true;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const int x = ld.d[b] >> 10 & 31;
             fine = fine && x < 31;
-            e = max(e, x - 14 - (tid < 32 ? vexp[b] : 0));
+            e = max(e, x - 14 - (lane < 32 ? vexp[b] : 0));
         }
-        const int key = tile * 32 + (tid & 31);
-        const bool seen = key >= glo && key < ghi;
-        e = fine && seen ? e : 0;
-        Factors& f = tid < 32 ? room.v : room.k;
-        const uint64_t nans = __ballot(!fine && seen);
-        if (tid < 32) f.e[tile & 3][tid & 31] = static_cast<float>(e);
-        else f.e[tile & 3][tid & 31] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
-        if (tid == 0) room.nan[tile & 3] = static_cast<uint32_t>(nans) != 0;
-        f.down[tile & 3][tid & 31] = ldexpf(1.0f, -e);
-        f.ok[tile & 3][tid & 31] = fine && seen ? 0xFFFF : 0;
+        const bool seen = key >= glo && key < ghi, use = fine && seen;
+        e = use ? e : 0;
+        const uint64_t nans = __ballot(seen && !fine);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const float x = ldexpf(fh_h2f(ld.d[b]), -e - (lane < 32 ? vexp[b] : 0));
+            room.d[lane >> 5][i][b][j] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(use ? x : 0.0f));
+        }
+        if (lane < 32) {
+            room.ve[i][j] = static_cast<float>(e);
+            room.vdown[i][j] = ldexpf(1.0f, -e);
+            if (lane == 0) room.nan[i] = static_cast<uint32_t>(nans);
+        } else {
+            room.kup[i][j] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
+        }
     };
     f32x4 o[CT][NB][2];
-    float l[CT], base[CT], unit_of[CT];  // unit_of: log2 units of a score's own
+    float l[CT], base[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         l[c] = 0.0f;
         base[c] = -FLT_MAX;
-        unit_of[c] = MODS && a.slopes ? kLog2e : col[c].factor * kLog2e;
 #pragma unroll
         for (int b = 0; b < NB; b++) o[c][b][0] = o[c][b][1] = f32x4{0, 0, 0, 0};
     }
     if (t0 < t1) {
-        if (tid < 64) {
-            load_scales(t0);
-            key_factors(t0);
-            load_scales(t0 + 1);
-            key_factors(t0 + 1);
+        if (wave < 2) {
+            load_scales(t0 + wave);
+            key_factors(t0 + wave);
         }
         __syncthreads();
-        store_part<HD>(t0, part, ld, room.k, room.v, vdown, room.stage[t0 & 1]);
+        store_part<HD>(t0, part, ld, room);
     }
     for (int t = t0; t < t1; t++) {
         __syncthreads();
         if (t + 1 < t1) load_part<HD>(p, a.c.cap, t + 1, part, ld);
-        if (tid < 64) load_scales(t + 2);
+        if (wave == (t & 3)) load_scales(t + 2);
         const Stage<HD>& st = room.stage[t & 1];
         if (t * 32 < hi && t * 32 + 32 > lo) {
             f32x4 d[CT][2];
@@ -994,38 +1012,38 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
             const bool full = t * 32 >= flo && t * 32 + 32 <= fhi;
             const int key0 = t * 32 + 8 * g;
             half8 ph[CT], pl[CT];
-            const bool nan = room.nan[t & 3] != 0;
-            const uint16_t* ok = room.v.ok[t & 3] + 8 * g;
-            const float *kup = room.k.e[t & 3] + 8 * g, *ve = room.v.e[t & 3] + 8 * g,
-                        *vdown8 = room.v.down[t & 3] + 8 * g;
+            const uint32_t nan = __builtin_amdgcn_readfirstlane(room.nan[t & 3]);
+            const float *kup = room.kup[t & 3] + 8 * g, *ve = room.ve[t & 3] + 8 * g, *vdown = room.vdown[t & 3] + 8 * g;
 #pragma unroll
             for (int c = 0; c < CT; c++) {
+                if (c) asm volatile("" ::: "memory");  // (the factors are read again: registers for them would be spilled)
+                const Place& at = room.place[(wave * CT + c) * 16 + n];
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = d[c][j >> 2][j & 3] * kup[j];
                 if constexpr (MODS) {
-                    if (a.softcap > 0.0f) cap_scores(x, a.softcap, col[c].factor);
+                    if (a.softcap > 0.0f) cap_scores(x, a.softcap, at.factor);
                     if (a.slopes) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int kp = kpos ? static_cast<int>(kpos[min(key0 + j, a.c.cap - 1)]) : key0 + j;
-                            x[j] = fmaf(-col[c].slope, static_cast<float>(abs(col[c].qpos - kp)), x[j] * col[c].factor);
-                        }
+                        for (int j = 0; j < 8; j++) x[j] *= at.factor;
+                        less_distance(a, at.slope, at.qpos, kpos, key0, x);
                     }
                 }
                 if (!full) {
+                    const int before = key0 - at.first, wide = at.wide;
 #pragma unroll
                     for (int j = 0; j < 8; j++)
-                        if (!(static_cast<uint32_t>(key0 + j - col[c].first) < static_cast<uint32_t>(col[c].wide)))
-                            x[j] = -INFINITY;
+                        x[j] = static_cast<uint32_t>(before + j) < static_cast<uint32_t>(wide) ? x[j] : -INFINITY;
                 }
-                const float f = unit_of[c];
+                const float f = at.unit;
                 float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 8; j++) top = fmaxf(top, fmaf(x[j], f, ve[j]));
+                for (int j = 0; j < 8; j++) {
+                    x[j] = fmaf(x[j], f, ve[j]);
+                    top = fmaxf(top, x[j]);
+                }
                 if (__any(top > base[c] + 14.0f)) {
-                    // (a whole number, so that e - base is exact)
-                    const float m = fmaxf(base[c] == -FLT_MAX ? -FLT_MAX : base[c] + 10.0f, ceilf(across_groups_max(top)));
+                    const float m = fmaxf(base[c] == -FLT_MAX ? -FLT_MAX : base[c] + 10.0f, across_groups_max(top));
                     const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, k = __builtin_amdgcn_exp2f(base[c] - nb);
                     l[c] *= k;
 #pragma unroll
@@ -1035,21 +1053,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
                     }
                     base[c] = nb;
                 }
-                uint32_t hw[4], lw[4];
-                float sum = 0.0f;
+                float e[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float u = __builtin_amdgcn_exp2f(fmaf(x[2 * j], f, ve[2 * j] - base[c])),
-                          v = __builtin_amdgcn_exp2f(fmaf(x[2 * j + 1], f, ve[2 * j + 1] - base[c]));
-                    sum = fmaf(u, vdown8[2 * j], sum);
-                    sum = fmaf(v, vdown8[2 * j + 1], sum);
-                    if (nan) {  // (that of a key that this row does not see stays out)
-                        u = ok[2 * j] || x[2 * j] == -INFINITY ? u : __builtin_nanf("");
-                        v = ok[2 * j + 1] || x[2 * j + 1] == -INFINITY ? v : __builtin_nanf("");
-                    }
-                    split2(u, v, hw[j], lw[j]);
+                for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(x[j] - base[c]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) l[c] = fmaf(e[j], vdown[j], l[c]);
+                if (nan) {  // (that of a key that this row does not see stays out)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) e[j] = (nan >> (8 * g + j) & 1) && x[j] != -INFINITY ? __builtin_nanf("") : e[j];
                 }
-                l[c] += sum;
+                uint32_t hw[4], lw[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) split2(e[2 * j], e[2 * j + 1], hw[j], lw[j]);
                 ph[c] = as_half8(hw[0], hw[1], hw[2], hw[3]);
                 pl[c] = as_half8(lw[0], lw[1], lw[2], lw[3]);
             }
@@ -1064,24 +1079,25 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
                         o[c][b][e] = mfma(vh, ph[c], mfma(vh, pl[c], mfma(vl, ph[c], o[c][b][e])));
                 }
         }
-        if (t + 1 < t1) store_part<HD>(t + 1, part, ld, room.k, room.v, vdown, room.stage[(t + 1) & 1]);
-        if (tid < 64) key_factors(t + 2);
+        if (t + 1 < t1) store_part<HD>(t + 1, part, ld, room);
+        if (wave == (t & 3)) key_factors(t + 2);
     }
     // Each lane has 8 channels of every block of its columns: 32 b + 8 g + i at o[b][i & 1][i >> 1] * 2^vexp[b].
 #pragma unroll
     for (int c = 0; c < CT; c++) l[c] = across_groups_sum(l[c]);
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        if (!col[c].on) continue;
-        float* out = a.out + (static_cast<size_t>(col[c].row) * a.n_heads + col[c].head) * HD + g * 8;
-        const float f = col[c].bad ? __builtin_nanf("") : l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+        const Place at = room.place[(wave * CT + c) * 16 + n];
+        if (at.row == ~0u) continue;
+        const size_t to = static_cast<size_t>(at.row) * a.n_heads + (at.head & 0x7FFFFFFFu);
+        const bool bad = at.head >> 31;
+        float* out = a.out + to * HD + g * 8;
+        const float f = bad ? __builtin_nanf("") : l[c] == 0.0f ? 0.0f : 1.0f / l[c];
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 8; i++) out[32 * b + i] = o[c][b][i & 1][i >> 1] * ldexpf(f, vexp[b]);
-        if (a.lse && g == 0)
-            a.lse[static_cast<size_t>(col[c].row) * a.n_heads + col[c].head] =
-                col[c].bad ? __builtin_nanf("") : (base[c] + log2f(l[c])) * kLn2;
+        if (a.lse && g == 0) a.lse[to] = bad ? __builtin_nanf("") : (base[c] + log2f(l[c])) * kLn2;
     }
 }
 
