@@ -610,8 +610,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     Sums<HD> z;
     clear<HD>(z);
     const int t_lo = lo < hi ? lo / 32 : 0, tiles = lo < hi ? (hi + 31) / 32 - t_lo : 0;
-    const int t0 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-    const int t1 = t_lo + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    // (at most 2^20 tiles and 2^10 splits)
+    const uint32_t each = static_cast<uint32_t>(tiles), of = static_cast<uint32_t>(a.splits);
+    const int t0 = t_lo + static_cast<int>(each * split / of), t1 = t_lo + static_cast<int>(each * (split + 1) / of);
     __shared__ __align__(16) float so[4][16][LD];
     __shared__ float sb[4][16], sl[4][16];
     // (a wave's room for scales is in its own part of the sums')
@@ -1796,6 +1797,35 @@ Cache device_cache(const fh_kv4_cache& c) {
 constexpr size_t kUnits = 1024;
 constexpr size_t kPartBytes = kUnits * 16 * (128 + 2) * sizeof(float);
 
+// Over how many workgroups the keys of a unit (16 columns) are dealt: that power of two
+// of which least time is expected.  A wave's tile takes `step` us alone on its SIMD and
+// 0.85 of it with each further wave there, a workgroup two tiles' time besides, and
+// joining the splits 2.8 us and 1.2 for every pass of the last workgroup but the first.
+// us measured, by splits of 1 / 2 / 4 / 8 / 16 / 32 (the one taken in brackets):
+//   14 and 2 heads of width 64, 1 x 511      (6.3)  7.5  7.1  6.9  6.9  6.9
+//   14 and 2 heads of width 64, 1 x 4000     24.8  16.8  11.6  9.0  (7.7)  8.5
+//   14 and 2 heads of width 64, 64 x <= 1023 (9.2)  9.5  10.9  12.8
+//   14 and 2 heads of width 64, 64 x <= 4000 25.3  18.0  (15.8)  16.7
+//   12 and 12 heads of width 64, 16 x <= 2999 20.6  18.0  (15.6)
+//   32 and 8 heads of width 128, 8 x <= 2000 20.8  16.0  (12.9)  15.0
+//   32 and 8 heads of width 128, 8 x <= 32767 269  139  74  (59)  62
+size_t attention_splits(size_t units, size_t tiles, size_t cols, size_t width, size_t cus) {
+    const double step = width == 32 ? 0.48 : width == 64 ? 0.66 : 1.03;
+    const size_t pass = 8 * (cols > 8 ? 1 : cols > 4 ? 2 : cols > 2 ? 4 : 16 / cols);  // splits that are joined at once
+    size_t best = 1;
+    double least = 0;
+    for (size_t n = 1; n == 1 || (n <= tiles && n * units <= kUnits); n *= 2) {
+        const double there = static_cast<double>((units * n + cus - 1) / cus), walk = static_cast<double>((tiles + 4 * n - 1) / (4 * n));
+        const double t = step * (walk + 2) * std::max(1.0, 0.85 * there) +
+                         (n > 1 ? 2.8 + 1.2 * static_cast<double>((n - 1) / pass) : 0.0);
+        if (n == 1 || t < least) {
+            best = n;
+            least = t;
+        }
+    }
+    return best;
+}
+
 template <int HD, bool MODS>
 void launch_attention(fh_ctx* ctx, const AttnArgs& a, bool prompt, size_t grid) {
     const dim3 g(static_cast<unsigned>(grid));
@@ -1897,13 +1927,8 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     } else {
         a.col_tiles = static_cast<int>(tiles16);
         const size_t units = c.seqs * c.n_kv * tiles16;
-        // Keys of few columns are dealt over workgroups until the GPU has two each, but to no more
-        // than the root of their tiles (the last workgroup joins them all: at 1 x 32767 keys of 14 and 2
-        // heads of width 64, 32 take 12.9 us, 128 16.2; at 1 x 4000, 12 8.5 us and 8 9.4).
-        size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(ctx->num_cus) / units);
-        splits = std::min(splits, std::max<size_t>(1, key_tiles / 4));
-        splits = std::min(splits, static_cast<size_t>(std::ceil(std::sqrt(static_cast<double>(key_tiles)))));
-        if (units * splits > kUnits) splits = 1;
+        const size_t splits = attention_splits(units, key_tiles, std::min<size_t>(cols, 16), c.head_dim,
+                                               static_cast<size_t>(ctx->num_cus));
         a.splits = static_cast<int>(splits);
         grid = units * splits;
         if (splits > 1) {
