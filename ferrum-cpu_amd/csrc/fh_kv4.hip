@@ -1290,7 +1290,8 @@ struct AppendArgs {
     int n_heads, octets, heads;  // heads: kv heads of a workgroup, with their query heads
     const uint32_t *off, *len, *pos;
     int rope_dim, neox;
-    float base, linear;
+    double log2_base;
+    float linear;
     const float* ff;
     float* q;
 };
@@ -1298,7 +1299,7 @@ struct AppendArgs {
 // The frequency of pair i and the angle at a position: apply_rope's (llm.rs:146-175, RopeScaling::angle,
 // llm.rs:118-121), in 32 bits as there.
 __device__ __forceinline__ float rope_frequency(int i, const AppendArgs& a) {
-    return static_cast<float>(pow(static_cast<double>(a.base), -2.0 * i / static_cast<double>(a.rope_dim)));
+    return static_cast<float>(exp2(static_cast<double>(-2 * i) / a.rope_dim * a.log2_base));
 }
 __device__ __forceinline__ float rope_angle(uint32_t pos, int i, float freq, const AppendArgs& a) {
 #pragma clang fp contract(off)
@@ -1433,37 +1434,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
         }
         __syncthreads();
     }
-    if (a.q) {
-        // four quads a thread on their way at once
-        constexpr int PER = HD / 4, R = 4;
-        const int wide = heads * group * PER, all = (j1 - j0) * wide;
-        for (int u0 = threadIdx.x; u0 < all; u0 += R * kThreads) {
-            Quad q[R];
-            int jj[R], u[R];
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int v = min(u0 + i * kThreads, all - 1);
-                jj[i] = v / wide;
-                u[i] = v - jj[i] * wide;
-                q[i] = load_quad<QUADS>(a.qkv + (row0 + jj[i]) * a.ld + static_cast<size_t>(h0) * group * HD + u[i] / PER * HD,
-                                 u[i] % PER * 4, true, a);
-            }
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-                if (u0 + i * kThreads >= all) continue;
-                const f32x4 v = rotate_quad<QUADS>(q[i], u[i] % PER * 4, a, turn + (j0 + jj[i]) * half);
-                float* y = a.q + ((row0 + jj[i]) * static_cast<size_t>(a.n_heads) + static_cast<size_t>(h0) * group) * HD + u[i] * 4;
-                if constexpr (QUADS) *reinterpret_cast<f32x4*>(y) = v;
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) y[k] = v[k];
-            }
-        }
-    }
-    if (!store) return;
+    // Keys and values from the first wave on, queries from the wave after them on: of a
+    // single token each wave has one or the other.
     const int l = threadIdx.x & 7, blocks = heads * NB;
     constexpr int R = 4;
-    const int per = 2 * blocks, all = (j1 - j0) * per;
+    const int per = 2 * blocks, all = store ? (j1 - j0) * per : 0;
+    const bool one = j1 - j0 == 1;
+    const size_t plane = static_cast<size_t>(s) * a.c.n_kv + h0;
     for (int u0 = threadIdx.x >> 3; u0 < all; u0 += R * (kThreads / 8)) {
         Quad q[R];
 #pragma unroll
@@ -1485,22 +1462,65 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
             uint16_t scale;
             uint32_t lev;
             quantise4(y, scale, lev);
-            if (v) {
+            const auto lay_down = [&](uint8_t* to, uint16_t* to_d) {
+                if (v) {
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int n = 2 * l + k;
-                    const int at8 = HD >= 64 ? (n * BP + b / 2) * 16 + b % 2 : n % VN * 16 + n / VN;
-                    vl[h * 4 * HD + at8 + j * 2] = static_cast<uint8_t>(lev >> (8 * k));
+                    for (int k = 0; k < 2; k++) {
+                        const int n = 2 * l + k;
+                        to[(HD >= 64 ? (n * BP + b / 2) * 16 + b % 2 : n % VN * 16 + n / VN) + j * 2] =
+                            static_cast<uint8_t>(lev >> (8 * k));
+                    }
+                } else {
+                    *reinterpret_cast<uint16_t*>(to + j * (HD / 2) + ((l >> 1) * NB + b) * 4 + (l & 1) * 2) =
+                        static_cast<uint16_t>(lev);
                 }
+                if (l == 0) to_d[b * 8 + j] = scale;
+            };
+            if (one) {
+                const size_t o = (plane + h) * (a.c.cap / 8) + oct;
+                lay_down((v ? a.c.v : a.c.k) + o * (4 * HD), (v ? a.c.vd : a.c.kd) + o * (NB * 8));
             } else {
-                *reinterpret_cast<uint16_t*>(kl + (h * 8 + j) * (HD / 2) + ((l >> 1) * NB + b) * 4 + (l & 1) * 2) =
-                    static_cast<uint16_t>(lev);
+                lay_down((v ? vl : kl) + h * 4 * HD, (v ? vdl : kdl) + h * NB * 8);
             }
-            if (l == 0) (v ? vdl : kdl)[(h * NB + b) * 8 + j] = scale;
         }
     }
+    if (a.q) {
+        // four quads a thread on their way at once
+        constexpr int PER = HD / 4;
+        const int wide = heads * group * PER, all_q = (j1 - j0) * wide, ahead = (all * 8 + 63) / 64 * 64 % kThreads;
+        for (int u0 = (threadIdx.x + kThreads - ahead) % kThreads; u0 < all_q; u0 += R * kThreads) {
+            Quad q[R];
+            int jj[R], u[R];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int v = min(u0 + i * kThreads, all_q - 1);
+                jj[i] = v / wide;
+                u[i] = v - jj[i] * wide;
+                q[i] = load_quad<QUADS>(a.qkv + (row0 + jj[i]) * a.ld + static_cast<size_t>(h0) * group * HD + u[i] / PER * HD,
+                                 u[i] % PER * 4, true, a);
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (u0 + i * kThreads >= all_q) continue;
+                const f32x4 v = rotate_quad<QUADS>(q[i], u[i] % PER * 4, a, turn + (j0 + jj[i]) * half);
+                float* y = a.q + ((row0 + jj[i]) * static_cast<size_t>(a.n_heads) + static_cast<size_t>(h0) * group) * HD + u[i] * 4;
+                if constexpr (QUADS) *reinterpret_cast<f32x4*>(y) = v;
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; k++) y[k] = v[k];
+            }
+        }
+    }
+    if (!store) return;
+    for (int u = threadIdx.x; u < heads * 8; u += kThreads) {
+        const int h = u / 8, j = u % 8;
+        if (j < j0 || j >= j1) continue;
+        const size_t to = (plane + h) * a.c.cap + oct * 8 + j;
+        if (a.c.pos) a.c.pos[to] = a.pos ? a.pos[row0 + (j - j0)] : static_cast<uint32_t>(oct * 8 + j);
+        if (a.c.weight) a.c.weight[to] = 0.0f;
+    }
+    if (one) return;
     __syncthreads();
-    const size_t plane = static_cast<size_t>(s) * a.c.n_kv + h0;
     // keys: words of whole rows
     for (int u = threadIdx.x; u < heads * 8 * KW; u += kThreads) {
         const int h = u / (8 * KW), j = u / KW % 8, w = u % KW;
@@ -1528,13 +1548,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
         }
         if (whole) *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(from);
         else if (j >= j0 && j < j1) to[j] = from[j];
-    }
-    for (int u = threadIdx.x; u < heads * 8; u += kThreads) {
-        const int h = u / 8, j = u % 8;
-        if (j < j0 || j >= j1) continue;
-        const size_t to = (plane + h) * a.c.cap + oct * 8 + j;
-        if (a.c.pos) a.c.pos[to] = a.pos ? a.pos[row0 + (j - j0)] : static_cast<uint32_t>(oct * 8 + j);
-        if (a.c.weight) a.c.weight[to] = 0.0f;
     }
 }
 
@@ -1879,11 +1892,13 @@ int fh_launch_kv4_append(fh_ctx* ctx, const fh_kv4_cache& c, const float* qkv, s
     a.pos = pos;
     a.rope_dim = static_cast<int>(rope_dim);
     a.neox = rope_type == FH_ROPE_NEOX;
-    a.base = base;
+    a.log2_base = std::log2(static_cast<double>(base));
     a.linear = linear;
     a.ff = ff;
     a.q = q;
-    a.heads = static_cast<int>(std::min<size_t>(c.n_kv, 2));  // (8 x 1000 rows of 32 and 8 heads: 67 us, by eights 78)
+    // Two kv heads a workgroup (8 x 1000 rows of 32 and 8 heads of width 128: 63 us, by ones 80, by
+    // eights 78), single tokens one (64 of 14 and 2 heads of width 64: 5.8 us, by twos 7.0).
+    a.heads = static_cast<int>(std::min<size_t>(c.n_kv, max_rows == 1 ? 1 : 2));
     // 16-byte accesses: every four channels from a multiple of 4 are aligned, and so are their partners
     const bool quads = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q)) % 16 == 0 &&
               (rope_type != FH_ROPE_NEOX || rope_dim % 8 == 0) && rope_dim % 4 == 0;
