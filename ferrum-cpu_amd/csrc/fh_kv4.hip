@@ -65,6 +65,7 @@ struct AttnArgs {
     float* out;
     float* lse;
     const float* lse_in;
+    int weigh_cols;  // tiles of columns a batch
     float* part;
     unsigned* counters;
     int col_tiles, splits;
@@ -1107,7 +1108,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
 // split once for all the keys that a wave walks, and k_kv4_weigh_prompt.
 
 // The score of 32 keys and 16 columns as weights, added to acc.
-template <int HD, bool MODS, typename Scales>
+template <int HD, bool MODS, bool MASKED, typename Scales>
 __device__ __forceinline__ void add_weights(const AttnArgs& a, const half8 (&lv)[2][Shape<HD>::NB], const Scales& scales,
                                             const Column<HD>& col, float lse, const uint32_t* kpos, int key0,
                                             float (&acc)[8]) {
@@ -1127,7 +1128,7 @@ __device__ __forceinline__ void add_weights(const AttnArgs& a, const half8 (&lv)
     const float f = MODS ? 1.0f : col.factor * kLog2e;
 #pragma unroll
     for (int j = 0; j < 8; j++)
-        acc[j] += static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide)
+        acc[j] += !MASKED || static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide)
                       ? __builtin_amdgcn_exp2f(fmaf(x[j], f, -lse)) : 0.0f;
 }
 
@@ -1145,8 +1146,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
     column_range(col.on, col.first, col.wide, lo, hi, flo, fhi);
     if (lo >= hi) return;
     const int first = lo / 32, tiles = (hi + 31) / 32 - first;
-    const int t1 = first + static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-    int t = first + static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits) + wave;
+    // (at most 2^20 tiles and 2^10 splits)
+    const uint32_t each = static_cast<uint32_t>(tiles), of = static_cast<uint32_t>(a.splits);
+    const int t1 = first + static_cast<int>(each * (split + 1) / of);
+    int t = first + static_cast<int>(each * split / of) + wave;
     if (t >= t1) return;
     const Planes p = planes_of<HD>(a.c, s, kv);
     const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + static_cast<size_t>(id) * a.c.cap : nullptr;
@@ -1173,7 +1176,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
         const bool mine = n < 8 && key >= lo && key < hi;
         const float old = mine ? weight[key] : 0.0f;
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        add_weights<HD, MODS>(a, lv, [&](int b) { return sc[b]; }, col, lse, kpos, t * 32 + 8 * g, acc);
+        add_weights<HD, MODS, true>(a, lv, [&](int b) { return sc[b]; }, col, lse, kpos, t * 32 + 8 * g, acc);
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -1184,39 +1187,50 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
     }
 }
 
-// A workgroup has 32 KT keys, in every one of its eight waves, which take every eighth
-// tile of 16 columns of the workgroup's share (of `splits`; their sums then go to a.part
-// and k_kv4_add_weights adds them up in order).
+// A workgroup has 8 KT tiles of keys, KT to a wave (every eighth of them, so that a causal
+// prompt's diagonal is shared out), and takes 4 or 8 tiles of 16 columns at a time of its share
+// (of `splits`; their sums then go to a.part and k_kv4_add_weights adds them up in
+// order): each wave splits the queries of one into LDS for all of them, while the
+// next batch is on its way.  (Split by every wave for itself, 1 x 1000 rows of 32 and 8
+// heads of width 128 took 54 us; they take 31, 132 TFLOP/s of products of two terms.)
+// Bound by what follows the products, a scale a block and an exponential a score.
 constexpr int kWeighTiles = 2;  // KT
+
+template <int HD>
+struct WeighRoom {
+    half8 q[8][Shape<HD>::NB][2][64];
+    f32x4 unit[8][16];  // factor, slope, log-sum-exp (log2), position
+    int first[8][16], wide[8][16];
+    int range[4][8];  // of a tile's columns: keys that one sees, keys that all see
+    u32x4 kd[8][kWeighTiles][Shape<HD>::NB][4];  // (in registers they would crowd the queries on their way out)
+};
 
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
-    constexpr int NB = Shape<HD>::NB, WAVES = 8, KT = kWeighTiles;
-    __shared__ float red[WAVES][KT * 32];
+    constexpr int NB = Shape<HD>::NB, KT = kWeighTiles;
+    extern __shared__ __align__(16) char smem[];
+    WeighRoom<HD>& room = *reinterpret_cast<WeighRoom<HD>*>(smem);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int limit = static_cast<int>(a.max_keys), heads = a.c.seqs * a.c.n_kv;
     int id = static_cast<int>(blockIdx.x);
     const int split = id % a.splits;
     id /= a.splits;
-    const int tile = id / heads * KT;  // (the most seen keys first)
+    const int tile0 = id / heads * (8 * KT);  // (the most seen keys first)
     id %= heads;
     const int kv = id % a.c.n_kv, s = id / a.c.n_kv;
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     const Planes p = planes_of<HD>(a.c, s, kv);
     const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + static_cast<size_t>(id) * a.c.cap : nullptr;
-    __shared__ u32x4 kd[KT][NB][4];  // (in registers they would crowd the queries on their way out)
     half8 lv[KT][2][NB];
     float acc[KT][8];
-    if (threadIdx.x < KT * NB * 4) {
-        const int i = threadIdx.x / (NB * 4), b = threadIdx.x / 4 % NB, o = threadIdx.x % 4;
-        kd[i][b][o] = *reinterpret_cast<const u32x4*>(
-            p.kd + (static_cast<uint32_t>(min((tile + i) * 4 + o, a.c.cap / 8 - 1)) * (NB * 8) + b * 8));
-    }
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < KT; i++) {
+        const int tile = tile0 + i * 8 + wave;
+        if (lane < NB * 4)
+            room.kd[wave][i][lane / 4][lane % 4] = *reinterpret_cast<const u32x4*>(
+                p.kd + (static_cast<uint32_t>(min(tile * 4 + lane % 4, a.c.cap / 8 - 1)) * (NB * 8) + lane / 4 * 8));
         uint32_t k[2][NB];
-        load_k<HD>(p, a.c.cap, tile + i, lane, k);
+        load_k<HD>(p, a.c.cap, tile, lane, k);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -1224,48 +1238,95 @@ __global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) acc[i][j] = 0.0f;
     }
-    const uint32_t cols = r.count * a.group, tiles = (cols + 15) / 16;  // (below 2^31: total * n_heads is)
-    const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits) * 16;
-    const uint32_t c1 = min(cols, static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits) * 16);
-    // The next tile of columns that sees some of these keys, its queries on their way.
-    Column<HD> col;
+    const uint32_t tiles = (r.count * a.group + 15) / 16;  // (below 2^31: total * n_heads is)
+    const uint32_t per = static_cast<uint32_t>(a.weigh_cols), batches = (tiles + per - 1) / per;
+    const uint32_t b0 = static_cast<uint32_t>(static_cast<uint64_t>(batches) * split / a.splits);
+    const uint32_t b1 = static_cast<uint32_t>(static_cast<uint64_t>(batches) * (split + 1) / a.splits);
+    Column<HD> col;  // of the tile that this wave splits next
     float raw[NB][8], lse = 0.0f;
-    const auto seek = [&](uint32_t c) {
-        for (; c < c1; c += WAVES * 16) {
-            column_place<HD, MODS>(a, r, kv, c + n, col);
-            if (__any(col.wide && col.first < (tile + KT) * 32 && col.first + col.wide > tile * 32)) {
-                load_query<HD>(a, lane, col, raw);
-                lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
-                break;
+    int lo = 0, hi = 0, flo = 0, fhi = 0;
+    const auto load = [&](uint32_t batch) {
+        hi = 0;
+        if (wave >= a.weigh_cols) return;
+        column_place<HD, MODS>(a, r, kv, (batch * per + wave) * 16 + n, col);
+        column_range(true, col.first, col.wide, lo, hi, flo, fhi);  // (one that is not the call's sees nothing)
+        if (lo < (tile0 + 8 * KT) * 32 && hi > tile0 * 32) {
+            load_query<HD>(a, lane, col, raw);
+            lse = col.on ? a.lse_in[static_cast<size_t>(col.row) * a.n_heads + col.head] * kLog2e : 0.0f;
+        } else {
+            hi = 0;
+        }
+    };
+    if (b0 < b1) load(b0);
+    for (uint32_t batch = b0; batch < b1; batch++) {
+        if (hi) {
+            split_query<HD>(a, raw, col);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                room.q[wave][b][0][lane] = col.hi[b];
+                room.q[wave][b][1][lane] = col.lo[b];
+            }
+            if (g == 0) {
+                room.unit[wave][n] = f32x4{col.factor, MODS ? col.slope : 0.0f, lse, MODS ? __int_as_float(col.qpos) : 0.0f};
+                room.first[wave][n] = col.first;
+                room.wide[wave][n] = col.wide;
             }
         }
-        return c;
-    };
-    uint32_t c = seek(c0 + wave * 16);
-    while (c < c1) {
-        Column<HD> now = col;
-        const float lse_now = lse;
-        split_query<HD>(a, raw, now);
-        c = seek(c + WAVES * 16);
+        if (lane == 0) {
+            room.range[0][wave] = lo;
+            room.range[1][wave] = hi;
+            room.range[2][wave] = flo;
+            room.range[3][wave] = fhi;
+        }
+        __syncthreads();
+        if (batch + 1 < b1) load(batch + 1);
+        const int ranges = room.range[lane / 8 & 3][lane % 8];
+        for (int c = 0; c < a.weigh_cols; c++) {
+            const int from = __builtin_amdgcn_readlane(ranges, c), to = __builtin_amdgcn_readlane(ranges, 8 + c);
+            const int all_from = __builtin_amdgcn_readlane(ranges, 16 + c), all_to = __builtin_amdgcn_readlane(ranges, 24 + c);
+            const auto seen = [&](int i) {
+                const int key = (tile0 + i * 8 + wave) * 32;
+                return from < key + 32 && to > key;
+            };
+            bool any = false;
 #pragma unroll
-        for (int i = 0; i < KT; i++)
-            add_weights<HD, MODS>(a, lv[i], [&](int b) { return kd[i][b][g]; }, now, lse_now, kpos, (tile + i) * 32 + 8 * g,
-                                  acc[i]);
+            for (int i = 0; i < KT; i++) any = any || seen(i);
+            if (!any) continue;
+            Column<HD> now;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                now.hi[b] = room.q[c][b][0][lane];
+                now.lo[b] = room.q[c][b][1][lane];
+            }
+            const f32x4 unit = room.unit[c][n];
+            now.factor = unit[0];
+            now.slope = unit[1];
+            now.qpos = __float_as_int(unit[3]);
+            now.first = room.first[c][n];
+            now.wide = room.wide[c][n];
+#pragma unroll
+            for (int i = 0; i < KT; i++) {
+                if (!seen(i)) continue;
+                const int key = (tile0 + i * 8 + wave) * 32;
+                const auto scales = [&](int b) { return room.kd[wave][i][b][g]; };
+                if (key >= all_from && key + 32 <= all_to)
+                    add_weights<HD, MODS, false>(a, lv[i], scales, now, unit[2], kpos, key + 8 * g, acc[i]);
+                else
+                    add_weights<HD, MODS, true>(a, lv[i], scales, now, unit[2], kpos, key + 8 * g, acc[i]);
+            }
+        }
+        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < KT; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float v = fh::group_sum<16>(acc[i][j]);
-            if (n == 0) red[wave][i * 32 + 8 * g + j] = v;
+            const float sum = fh::group_sum<16>(acc[i][j]);
+            const int key = (tile0 + i * 8 + wave) * 32 + 8 * g + j;
+            if (n != j || key >= limit || static_cast<uint64_t>(key) >= r.at + r.count) continue;
+            if (a.splits > 1) a.part[(static_cast<size_t>(split) * heads + id) * limit + key] = sum;
+            else a.c.weight[static_cast<size_t>(id) * a.c.cap + key] += sum;
         }
-    __syncthreads();
-    const int t = threadIdx.x, key = tile * 32 + t;
-    if (t >= KT * 32 || key >= limit || static_cast<uint64_t>(key) >= r.at + r.count) return;
-    const float sum =
-        ((red[0][t] + red[1][t]) + (red[2][t] + red[3][t])) + ((red[4][t] + red[5][t]) + (red[6][t] + red[7][t]));
-    if (a.splits > 1) a.part[(static_cast<size_t>(split) * heads + id) * limit + key] = sum;
-    else a.c.weight[static_cast<size_t>(id) * a.c.cap + key] += sum;
 }
 
 __global__ void __launch_bounds__(kThreads) k_kv4_add_weights(AttnArgs a) {
@@ -1276,7 +1337,13 @@ __global__ void __launch_bounds__(kThreads) k_kv4_add_weights(AttnArgs a) {
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, static_cast<int>(id) / a.c.n_kv);
     if (key >= r.at + r.count) return;
     float sum = 0.0f;
-    for (int s = 0; s < a.splits; s++) sum += a.part[s * all + i];
+    for (int s = 0; s < a.splits; s += 8) {  // (eight on their way at once)
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = a.part[min(s + j, a.splits - 1) * all + i];
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum += s + j < a.splits ? x[j] : 0.0f;
+    }
     a.c.weight[static_cast<size_t>(id) * a.c.cap + key] += sum;
 }
 
@@ -1968,21 +2035,25 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
 template <int HD, bool MODS>
 static int launch_weigh(fh_ctx* ctx, AttnArgs& a, size_t tiles16) {
     const size_t heads = static_cast<size_t>(a.c.seqs) * a.c.n_kv, tiles = (a.max_keys + 31) / 32;
-    const size_t room = 4 * static_cast<size_t>(ctx->num_cus);
     if (tiles16 == 1) {
         // workgroups of at least four tiles, and no more than four to a CU
-        const size_t splits = std::max<size_t>(1, std::min(room / heads, tiles / 4));
+        const size_t splits = std::max<size_t>(1, std::min(4 * static_cast<size_t>(ctx->num_cus) / heads, tiles / 4));
         a.splits = static_cast<int>(splits);
         hipLaunchKernelGGL((k_kv4_weigh_step<HD, MODS>), dim3(static_cast<unsigned>(heads * splits)), dim3(kThreads), 0,
                            ctx->stream, a);
         FH_HIP(ctx, hipGetLastError());
         return FH_OK;
     }
-    // Few workgroups share out the columns too, until there are four for each CU (the first
-    // keys are seen by the most rows, so that many even out) or no more than two tiles a wave.
-    constexpr size_t KT = kWeighTiles;
-    const size_t groups = (tiles + KT - 1) / KT;
-    const size_t splits = std::max<size_t>(1, std::min(room / (heads * groups), tiles16 / 16));
+    // The columns are shared out too, over as many workgroups as the GPU holds at once, or, where
+    // that is not four times as many, over four times that (us, 1 x 1000 rows of 32 and 8 heads of
+    // width 128: 16 parts 34, 31 38; 4 x 2000: two parts 360, eight 345).  Eight tiles of
+    // columns a batch, four where that leaves the GPU half empty (8 x 16 rows behind 2000 of
+    // 14 and 2 heads of width 64: 14.0 and 12.1; 16 x 100, 192 workgroups by eights: 12.7 and 16.5).
+    const size_t cus = static_cast<size_t>(ctx->num_cus), groups = (tiles + 8 * kWeighTiles - 1) / (8 * kWeighTiles);
+    const size_t batch = heads * groups * ((tiles16 + 7) / 8) < cus / 2 ? 4 : 8, batches = (tiles16 + batch - 1) / batch;
+    const size_t room = cus / (heads * groups);
+    const size_t splits = std::max<size_t>(1, std::min(room >= 4 ? room : 4 * cus / (heads * groups), batches));
+    a.weigh_cols = static_cast<int>(batch);
     const size_t grid = heads * groups * splits;
     if (grid > 0x7FFFFFFF) return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_weigh: more than 2^31 - 1 workgroups");
     a.splits = static_cast<int>(splits);
@@ -1992,7 +2063,8 @@ static int launch_weigh(fh_ctx* ctx, AttnArgs& a, size_t tiles16) {
         if (rc) return rc;
         a.part = static_cast<float*>(ws);
     }
-    hipLaunchKernelGGL((k_kv4_weigh_prompt<HD, MODS>), dim3(static_cast<unsigned>(grid)), dim3(512), 0, ctx->stream, a);
+    hipLaunchKernelGGL((k_kv4_weigh_prompt<HD, MODS>), dim3(static_cast<unsigned>(grid)), dim3(512),
+                       sizeof(WeighRoom<HD>), ctx->stream, a);
     FH_HIP(ctx, hipGetLastError());
     if (splits > 1) {
         const size_t n = heads * a.max_keys;
