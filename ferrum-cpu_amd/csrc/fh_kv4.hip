@@ -436,6 +436,29 @@ __device__ __forceinline__ void clear(Sums<HD>& z) {
     z.base = -FLT_MAX;
 }
 
+// 1024 + the exponent field, as f16, of the largest scale of each key: a word of two
+// keys of one block in, the same keys' of all blocks out.  Of the eight lanes of an
+// octet, lanes j and j ^ 4 (two blocks) or j, j ^ 2, j ^ 4 and j ^ 6 (four) have one
+// key's blocks.
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t lanes(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+template <int NB>
+__device__ __forceinline__ uint32_t key_exponents(uint32_t scales) {
+    uint32_t x = scales & 0x7C007C00u;
+    if constexpr (NB == 4) {
+        x = larger(x, lanes<0x4E>(x));                // j ^ 2
+        x = larger(x, lanes<0x141>(lanes<0xB1>(x)));  // (j ^ 7) ^ 1, which has what j ^ 4 has
+    } else if constexpr (NB == 2) {
+        x = larger(x, lanes<0x141>(lanes<0x1B>(x)));  // (j ^ 7) ^ 3
+    }
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, x) >> 10) | 0x64006400u;
+}
+
 // One tile of 32 keys into the sums.  The weights times their block's value
 // scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that as
 // their last place, which is 2^-35 of the row's largest.  swap: the wave's LDS
@@ -446,9 +469,18 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
     constexpr int NB = Shape<HD>::NB;
     const int g = lane >> 4, n = lane & 15, key0 = tile * 32 + 8 * g;
     // (a wave's LDS instructions run in order: only the compiler has to be held)
-    if constexpr (NB == 4) *reinterpret_cast<u32x2*>(swap + lane * 4) = u32x2{t.sc[0], t.sc[1]};
-    else if constexpr (NB == 2) *reinterpret_cast<uint32_t*>(swap + lane * 2) = t.sc[0];
-    else swap[lane] = static_cast<uint16_t>(t.sc[0]);
+    // and their largest exponents behind them (those of the keys' own scales go unread)
+    uint16_t* large = swap + 64 * NB + (lane >> 3) * 8;
+    if constexpr (NB == 4) {
+        *reinterpret_cast<u32x2*>(swap + lane * 4) = u32x2{t.sc[0], t.sc[1]};
+        *reinterpret_cast<u32x2*>(large + lane % 2 * 4) = u32x2{key_exponents<NB>(t.sc[0]), key_exponents<NB>(t.sc[1])};
+    } else if constexpr (NB == 2) {
+        *reinterpret_cast<uint32_t*>(swap + lane * 2) = t.sc[0];
+        *reinterpret_cast<uint32_t*>(large + lane % 4 * 2) = key_exponents<NB>(t.sc[0]);
+    } else {
+        swap[lane] = static_cast<uint16_t>(t.sc[0]);
+        large[lane % 8] = static_cast<uint16_t>(key_exponents<NB>(t.sc[0]));
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -458,6 +490,7 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
         kd[b] = *reinterpret_cast<const u32x4*>(swap + (g * NB + b) * 8);
         vd[b] = *reinterpret_cast<const u32x4*>(swap + ((4 + g) * NB + b) * 8);
     }
+    const u32x4 e = *reinterpret_cast<const u32x4*>(swap + 64 * NB + (4 + g) * 8);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -473,15 +506,6 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
         }
     }
     const float f = MODS ? 1.0f : col.factor * kLog2e;
-    // 1024 + the exponent field of each key's largest scale, as f16
-    u32x4 e;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        u16x2 m = __builtin_bit_cast(u16x2, vd[0][i] & 0x7C007C00u);
-#pragma unroll
-        for (int b = 1; b < NB; b++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, vd[b][i] & 0x7C007C00u));
-        e[i] = __builtin_bit_cast(uint32_t, m >> 10) | 0x64006400u;
-    }
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; j++) top = fmaxf(top, fmaf(s[j], f, half_at(e, j)));
