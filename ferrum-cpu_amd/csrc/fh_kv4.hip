@@ -1264,8 +1264,13 @@ __global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
     }
     const uint32_t tiles = (r.count * a.group + 15) / 16;  // (below 2^31: total * n_heads is)
     const uint32_t per = static_cast<uint32_t>(a.weigh_cols), batches = (tiles + per - 1) / per;
-    const uint32_t b0 = static_cast<uint32_t>(static_cast<uint64_t>(batches) * split / a.splits);
-    const uint32_t b1 = static_cast<uint32_t>(static_cast<uint64_t>(batches) * (split + 1) / a.splits);
+    // (rows above the first key do not see it, unless the call says where their keys end)
+    const uint64_t key0 = static_cast<uint64_t>(tile0) * 32;
+    const uint32_t none = a.end || key0 <= r.at ? 0 : static_cast<uint32_t>(min(
+        (key0 - r.at) * static_cast<uint32_t>(a.group) / (16 * per), static_cast<uint64_t>(batches)));
+    const uint32_t some = batches - none;
+    const uint32_t b0 = none + static_cast<uint32_t>(static_cast<uint64_t>(some) * split / a.splits);
+    const uint32_t b1 = none + static_cast<uint32_t>(static_cast<uint64_t>(some) * (split + 1) / a.splits);
     Column<HD> col;  // of the tile that this wave splits next
     float raw[NB][8], lse = 0.0f;
     int lo = 0, hi = 0, flo = 0, fhi = 0;
@@ -1328,15 +1333,18 @@ __global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
             now.qpos = __float_as_int(unit[3]);
             now.first = room.first[c][n];
             now.wide = room.wide[c][n];
-#pragma unroll
-            for (int i = 0; i < KT; i++) {
-                if (!seen(i)) continue;
-                const int key = (tile0 + i * 8 + wave) * 32;
+            const auto add = [&](int i, auto masked) {
                 const auto scales = [&](int b) { return room.kd[wave][i][b][g]; };
-                if (key >= all_from && key + 32 <= all_to)
-                    add_weights<HD, MODS, false>(a, lv[i], scales, now, unit[2], kpos, key + 8 * g, acc[i]);
-                else
-                    add_weights<HD, MODS, true>(a, lv[i], scales, now, unit[2], kpos, key + 8 * g, acc[i]);
+                add_weights<HD, MODS, masked.value>(a, lv[i], scales, now, unit[2], kpos, (tile0 + i * 8 + wave) * 32 + 8 * g, acc[i]);
+            };
+            if ((tile0 + wave) * 32 >= all_from && (tile0 + (KT - 1) * 8 + wave) * 32 + 32 <= all_to) {
+                // (side by side: one's products hide behind what follows the other's)
+#pragma unroll
+                for (int i = 0; i < KT; i++) add(i, std::false_type{});
+            } else {
+#pragma unroll
+                for (int i = 0; i < KT; i++)
+                    if (seen(i)) add(i, std::true_type{});
             }
         }
         __syncthreads();
