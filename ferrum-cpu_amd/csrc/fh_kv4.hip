@@ -365,16 +365,44 @@ __device__ __forceinline__ void column_query(const AttnArgs& a, int lane, Column
     split_query<HD>(a, x, col);
 }
 
-// The scores of 32 keys and 16 columns: lane (g, n) gets keys 8 g + j of column n.
-template <int HD>
-__device__ __forceinline__ void scores(const uint32_t (&k)[2][Shape<HD>::NB], const u32x4 (&kd)[Shape<HD>::NB],
-                                       const Column<HD>& col, float (&s)[8]) {
+// A wave's queries: of 16 columns, or (T = 2) of at most eight, twice: lanes n < 8 have
+// them for the first tile of a pair of tiles, zeros for the second, lanes n >= 8 the other
+// way around.  The products of both tiles then add up to each lane's own, and what
+// follows them is done once for both tiles.
+template <int HD, int T>
+struct Queries {
+    half8 hi[T][Shape<HD>::NB], lo[T][Shape<HD>::NB];
+};
+template <int HD, int T>
+__device__ __forceinline__ Queries<HD, T> queries_of(const Column<HD>& col, int n) {
+    Queries<HD, T> q;
+    const half8 none = as_half8(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < T; i++)
+#pragma unroll
+        for (int b = 0; b < Shape<HD>::NB; b++) {
+            const bool mine = T == 1 || n >> 3 == i;
+            q.hi[i][b] = mine ? col.hi[b] : none;
+            q.lo[i][b] = mine ? col.lo[b] : none;
+        }
+    return q;
+}
+
+// The scores of 32 keys and 16 columns (of two tiles' and eight): lane (g, n) gets keys
+// 8 g + j of its tile and column.
+template <int HD, int T>
+__device__ __forceinline__ void scores(const Tile<HD> (&t)[T], const u32x4 (&kd)[Shape<HD>::NB],
+                                       const Queries<HD, T>& q, float (&s)[8]) {
 #pragma unroll
     for (int b = 0; b < Shape<HD>::NB; b++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const half8 lv = k_levels(k[h][b]);
-            const f32x4 d = mfma(lv, col.hi[b], mfma(lv, col.lo[b], f32x4{0, 0, 0, 0}));
+            f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < T; i++) {
+                const half8 lv = k_levels(t[i].k[h][b]);
+                d = mfma(lv, q.hi[i][b], mfma(lv, q.lo[i][b], d));
+            }
 #pragma unroll
             for (int r = 0; r < 4; r++)
                 s[4 * h + r] = b == 0 ? half_at(kd[b], 4 * h + r) * d[r] : fmaf(half_at(kd[b], 4 * h + r), d[r], s[4 * h + r]);
@@ -422,16 +450,18 @@ __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD
 // far, 2^E being above the key's value scales: what counts is not how large a weight
 // is but how large its product, so that a row whose keys have small values is as
 // exact beside a row, or a key of no weight, with large ones.
-template <int HD>
+template <int HD, int T>
 struct Sums {
-    f32x4 o[Shape<HD>::NB][2];
+    f32x4 o[T][Shape<HD>::NB][2];  // (of each tile of a pair: the other tile's columns mean nothing)
     float l, base;
 };
 
-template <int HD>
-__device__ __forceinline__ void clear(Sums<HD>& z) {
+template <int HD, int T>
+__device__ __forceinline__ void clear(Sums<HD, T>& z) {
 #pragma unroll
-    for (int b = 0; b < Shape<HD>::NB; b++) z.o[b][0] = z.o[b][1] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < T; i++)
+#pragma unroll
+        for (int b = 0; b < Shape<HD>::NB; b++) z.o[i][b][0] = z.o[i][b][1] = f32x4{0, 0, 0, 0};
     z.l = 0.0f;
     z.base = -FLT_MAX;
 }
@@ -459,27 +489,34 @@ __device__ __forceinline__ uint32_t key_exponents(uint32_t scales) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, x) >> 10) | 0x64006400u;
 }
 
-// One tile of 32 keys into the sums.  The weights times their block's value
-// scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that as
-// their last place, which is 2^-35 of the row's largest.  swap: the wave's LDS
-// room for a tile's scales.
-template <int HD, bool MODS, bool MASKED>
-__device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int tile, int lane, const Column<HD>& col,
-                                     const uint32_t* kpos, uint16_t* swap, Sums<HD>& z) {
-    constexpr int NB = Shape<HD>::NB;
-    const int g = lane >> 4, n = lane & 15, key0 = tile * 32 + 8 * g;
+// T tiles of 32 keys, at `tile` and behind, into the sums.  The weights times their
+// block's value scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that
+// as their last place, which is 2^-35 of the row's largest.  swap: the wave's LDS
+// room for the tiles' scales.
+constexpr int kSwap = 64;  // 2-byte words of it: 64 scales a block, 64 exponents
+template <int HD, bool MODS, bool MASKED, int T>
+__device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD> (&t)[T], int tile, int t1, int lane,
+                                     const Column<HD>& col, const Queries<HD, T>& q, const uint32_t* kpos,
+                                     uint16_t* swap, Sums<HD, T>& z) {
+    constexpr int NB = Shape<HD>::NB, SW = kSwap * (NB + 1);
+    const int g = lane >> 4, n = lane & 15, mine = T == 2 ? n >> 3 : 0, key0 = (tile + mine) * 32 + 8 * g;
     // (a wave's LDS instructions run in order: only the compiler has to be held)
-    // and their largest exponents behind them (those of the keys' own scales go unread)
-    uint16_t* large = swap + 64 * NB + (lane >> 3) * 8;
-    if constexpr (NB == 4) {
-        *reinterpret_cast<u32x2*>(swap + lane * 4) = u32x2{t.sc[0], t.sc[1]};
-        *reinterpret_cast<u32x2*>(large + lane % 2 * 4) = u32x2{key_exponents<NB>(t.sc[0]), key_exponents<NB>(t.sc[1])};
-    } else if constexpr (NB == 2) {
-        *reinterpret_cast<uint32_t*>(swap + lane * 2) = t.sc[0];
-        *reinterpret_cast<uint32_t*>(large + lane % 4 * 2) = key_exponents<NB>(t.sc[0]);
-    } else {
-        swap[lane] = static_cast<uint16_t>(t.sc[0]);
-        large[lane % 8] = static_cast<uint16_t>(key_exponents<NB>(t.sc[0]));
+#pragma unroll
+    for (int i = 0; i < T; i++) {
+        uint16_t* to = swap + i * SW;
+        // the scales, and their keys' largest exponents behind them (those of the keys' own go unread)
+        uint16_t* large = to + 64 * NB + (lane >> 3) * 8;
+        const auto& sc = t[i].sc;
+        if constexpr (NB == 4) {
+            *reinterpret_cast<u32x2*>(to + lane * 4) = u32x2{sc[0], sc[1]};
+            *reinterpret_cast<u32x2*>(large + lane % 2 * 4) = u32x2{key_exponents<NB>(sc[0]), key_exponents<NB>(sc[1])};
+        } else if constexpr (NB == 2) {
+            *reinterpret_cast<uint32_t*>(to + lane * 2) = sc[0];
+            *reinterpret_cast<uint32_t*>(large + lane % 4 * 2) = key_exponents<NB>(sc[0]);
+        } else {
+            to[lane] = static_cast<uint16_t>(sc[0]);
+            large[lane % 8] = static_cast<uint16_t>(key_exponents<NB>(sc[0]));
+        }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -487,21 +524,22 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
     u32x4 kd[NB], vd[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        kd[b] = *reinterpret_cast<const u32x4*>(swap + (g * NB + b) * 8);
-        vd[b] = *reinterpret_cast<const u32x4*>(swap + ((4 + g) * NB + b) * 8);
+        kd[b] = *reinterpret_cast<const u32x4*>(swap + mine * SW + (g * NB + b) * 8);
+        vd[b] = *reinterpret_cast<const u32x4*>(swap + mine * SW + ((4 + g) * NB + b) * 8);
     }
-    const u32x4 e = *reinterpret_cast<const u32x4*>(swap + 64 * NB + (4 + g) * 8);
+    const u32x4 e = *reinterpret_cast<const u32x4*>(swap + mine * SW + 64 * NB + (4 + g) * 8);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     float s[8];
-    scores<HD>(t.k, kd, col, s);
+    scores<HD, T>(t, kd, q, s);
     finish_scores<HD, MODS>(a, col, kpos, key0, s);
     bool seen[8];
     if constexpr (MASKED) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            seen[j] = static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide);
+            seen[j] = static_cast<uint32_t>(key0 + j - col.first) < static_cast<uint32_t>(col.wide) &&
+                      (T == 1 || tile + mine < t1);
             s[j] = seen[j] ? s[j] : -INFINITY;
         }
     }
@@ -516,10 +554,12 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
         const float k = __builtin_amdgcn_exp2f(z.base - base);
         z.l *= k;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            z.o[b][0] *= k;
-            z.o[b][1] *= k;
-        }
+        for (int i = 0; i < T; i++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                z.o[i][b][0] *= k;
+                z.o[i][b][1] *= k;
+            }
         z.base = base;
     }
     float p[8];
@@ -540,41 +580,49 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD>& t, int t
             split2(x, y, hi[i], lo[i]);
         }
         const half8 ph = as_half8(hi[0], hi[1], hi[2], hi[3]), pl = as_half8(lo[0], lo[1], lo[2], lo[3]);
-        u32x4 w = t.v[HD >= 64 ? b / 2 : 0];
-        if constexpr (HD == 32) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] >>= n & 8;
+        for (int i = 0; i < T; i++) {
+            u32x4 w = t[i].v[HD >= 64 ? b / 2 : 0];
+            if constexpr (HD == 32) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] >>= n & 8;
+            }
+            const half8 v0 = b & 1 ? v_levels<2>(w) : v_levels<0>(w), v1 = b & 1 ? v_levels<3>(w) : v_levels<1>(w);
+            z.o[i][b][0] = mfma(v0, ph, mfma(v0, pl, z.o[i][b][0]));
+            z.o[i][b][1] = mfma(v1, ph, mfma(v1, pl, z.o[i][b][1]));
         }
-        const half8 v0 = b & 1 ? v_levels<2>(w) : v_levels<0>(w), v1 = b & 1 ? v_levels<3>(w) : v_levels<1>(w);
-        z.o[b][0] = mfma(v0, ph, mfma(v0, pl, z.o[b][0]));
-        z.o[b][1] = mfma(v1, ph, mfma(v1, pl, z.o[b][1]));
     }
 }
 
-// The columns' queries against tiles t0, t0 + stride, .. below t1, the next two on their way
-// while one is worked on.
-template <int HD, bool MODS>
+// The columns' queries against T tiles at t0, t0 + stride, .. below t1, the next two such on
+// their way while one is worked on.
+template <int HD, bool MODS, int T>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lane, Column<HD>& col,
                                      const uint32_t* kpos, int t0, int t1, int stride, int full_lo, int full_hi,
-                                     uint16_t* swap, Sums<HD>& z) {
+                                     uint16_t* swap, Sums<HD, T>& z) {
     if (t0 >= t1) return;
     const uint16_t* scales = lane < 32 ? p.kd : p.vd;
-    Tile<HD> even, odd;
-    load_tile<HD>(p, scales, a.c.cap, t0, lane, even);
-    load_tile<HD>(p, scales, a.c.cap, min(t0 + stride, t1 - 1), lane, odd);
+    Tile<HD> even[T], odd[T];
+    const auto load = [&](Tile<HD> (&tiles)[T], int t) {
+#pragma unroll
+        for (int i = 0; i < T; i++) load_tile<HD>(p, scales, a.c.cap, min(t + i, t1 - 1), lane, tiles[i]);
+    };
+    load(even, t0);
+    load(odd, t0 + stride);
     column_query<HD>(a, lane, col);  // (its loads wait beside the tiles')
-    const auto work = [&](const Tile<HD>& tile, int t) {
-        if (t * 32 >= full_lo && t * 32 + 32 <= full_hi)
-            step<HD, MODS, false>(a, tile, t, lane, col, kpos, swap, z);
+    const Queries<HD, T> q = queries_of<HD, T>(col, lane & 15);
+    const auto work = [&](const Tile<HD> (&tiles)[T], int t) {
+        if (t * 32 >= full_lo && (t + T) * 32 <= full_hi && t + T <= t1)
+            step<HD, MODS, false, T>(a, tiles, t, t1, lane, col, q, kpos, swap, z);
         else
-            step<HD, MODS, true>(a, tile, t, lane, col, kpos, swap, z);
+            step<HD, MODS, true, T>(a, tiles, t, t1, lane, col, q, kpos, swap, z);
     };
     for (int t = t0; t < t1; t += 2 * stride) {
         work(even, t);
         if (t + stride >= t1) break;
-        load_tile<HD>(p, scales, a.c.cap, min(t + 2 * stride, t1 - 1), lane, even);
+        load(even, t + 2 * stride);
         work(odd, t + stride);
-        load_tile<HD>(p, scales, a.c.cap, min(t + 3 * stride, t1 - 1), lane, odd);
+        load(odd, t + 3 * stride);
     }
 }
 
@@ -592,12 +640,12 @@ __device__ __forceinline__ void column_range(bool on, int first, int wide, int& 
 }
 
 // Channels 32 b + 8 g .. + 7 of a column, from its sums.
-template <int HD>
-__device__ __forceinline__ void channels(const Sums<HD>& z, int b, float factor, float (&x)[8]) {
+template <int HD, int T>
+__device__ __forceinline__ void channels(const Sums<HD, T>& z, int b, int n, float (&x)[8]) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        x[2 * r] = z.o[b][0][r] * factor;
-        x[2 * r + 1] = z.o[b][1][r] * factor;
+        x[2 * r] = T == 2 && n >= 8 ? z.o[T - 1][b][0][r] : z.o[0][b][0][r];
+        x[2 * r + 1] = T == 2 && n >= 8 ? z.o[T - 1][b][1][r] : z.o[0][b][1][r];
     }
 }
 
@@ -611,9 +659,9 @@ __device__ __forceinline__ float2 load2(const float* from) {
                                                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// Attention of 16 columns by one workgroup: the four waves take every fourth tile
-// of the workgroup's share of the keys.
-template <int HD, bool MODS>
+// Attention of 16 columns (T = 2: of at most eight, two tiles at a time) by one workgroup: the
+// four waves take every fourth tile, or pair, of the workgroup's share of the keys.
+template <int HD, bool MODS, int T>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, LD = HD + 4;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -627,13 +675,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.c.seqs, s);
     if (static_cast<uint64_t>(ct) * 16 >= static_cast<uint64_t>(r.count) * a.group) return;
     Column<HD> col;
-    column_place<HD, MODS>(a, r, kv, static_cast<uint32_t>(ct) * 16 + n, col);
+    column_place<HD, MODS>(a, r, kv, static_cast<uint32_t>(ct) * 16 + (T == 2 ? n & 7 : n), col);
     int lo, hi, flo, fhi;
     column_range(col.on, col.first, col.wide, lo, hi, flo, fhi);
     const Planes p = planes_of<HD>(a.c, s, kv);
     const uint32_t* kpos = MODS && a.c.pos ? a.c.pos + (static_cast<size_t>(s) * a.c.n_kv + kv) * a.c.cap : nullptr;
-    Sums<HD> z;
-    clear<HD>(z);
+    Sums<HD, T> z;
+    clear<HD, T>(z);
     const int t_lo = lo < hi ? lo / 32 : 0, tiles = lo < hi ? (hi + 31) / 32 - t_lo : 0;
     // (at most 2^20 tiles and 2^10 splits)
     const uint32_t each = static_cast<uint32_t>(tiles), of = static_cast<uint32_t>(a.splits);
@@ -641,14 +689,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     __shared__ __align__(16) float so[4][16][LD];
     __shared__ float sb[4][16], sl[4][16];
     // (a wave's room for scales is in its own part of the sums')
-    walk<HD, MODS>(a, p, lane, col, kpos, t0 + wave, t1, 4, flo, fhi, reinterpret_cast<uint16_t*>(so[wave]), z);
+    walk<HD, MODS, T>(a, p, lane, col, kpos, t0 + T * wave, t1, 4 * T, flo, fhi, reinterpret_cast<uint16_t*>(so[wave]), z);
     // join the waves
     __shared__ int last;
     const float l = across_groups_sum(z.l);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         float x[8];
-        channels<HD>(z, b, 1.0f, x);
+        channels<HD, T>(z, b, n, x);
         *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g]) = f32x4{x[0], x[1], x[2], x[3]};
         *reinterpret_cast<f32x4*>(&so[wave][n][32 * b + 8 * g + 4]) = f32x4{x[4], x[5], x[6], x[7]};
     }
@@ -659,16 +707,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     __syncthreads();
     constexpr int PER = HD / 16;  // channels of a column that a thread joins
     const int cj = threadIdx.x >> 4, ch = (threadIdx.x & 15) * PER;
-    float base = fmaxf(fmaxf(sb[0][cj], sb[1][cj]), fmaxf(sb[2][cj], sb[3][cj]));
-    float sum = 0.0f, x[PER];
+    float base = -FLT_MAX, sum = 0.0f, x[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) x[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float f = __builtin_amdgcn_exp2f(sb[w][cj] - base);
-        sum = fmaf(sl[w][cj], f, sum);
+    for (int w = 0; w < 4 * T; w++) base = fmaxf(base, sb[w / T][(cj + w % T * 8) & 15]);
 #pragma unroll
-        for (int i = 0; i < PER; i++) x[i] = fmaf(so[w][cj][ch + i], f, x[i]);
+    for (int w = 0; w < 4 * T; w++) {
+        const int from = (cj + w % T * 8) & 15;
+        const float f = __builtin_amdgcn_exp2f(sb[w / T][from] - base);
+        sum = fmaf(sl[w / T][from], f, sum);
+#pragma unroll
+        for (int i = 0; i < PER; i++) x[i] = fmaf(so[w / T][from][ch + i], f, x[i]);
     }
     const uint32_t c = static_cast<uint32_t>(ct) * 16 + cj;
     Column<HD> mine;  // (its place only)
@@ -1909,27 +1959,31 @@ Cache device_cache(const fh_kv4_cache& c) {
 constexpr size_t kUnits = 1024;
 constexpr size_t kPartBytes = kUnits * 16 * (128 + 2) * sizeof(float);
 
-// Over how many workgroups the keys of a unit (16 columns) are dealt: that power of two
-// of which least time is expected.  A wave's tile takes `step` us alone on its SIMD and
-// 0.85 of it with each further wave there, a workgroup two tiles' time besides, and
-// joining the splits 2.8 us and 1.2 for every pass of the last workgroup but the first.
-// us measured, by splits of 1 / 2 / 4 / 8 / 16 / 32 (the one taken in brackets):
-//   14 and 2 heads of width 64, 1 x 511      (6.3)  7.5  7.1  6.9  6.9  6.9
-//   14 and 2 heads of width 64, 1 x 4000     24.8  16.8  11.6  9.0  (7.7)  8.5
-//   14 and 2 heads of width 64, 64 x <= 1023 (9.2)  9.5  10.9  12.8
-//   14 and 2 heads of width 64, 64 x <= 4000 25.3  18.0  (15.8)  16.7
-//   12 and 12 heads of width 64, 16 x <= 2999 20.6  18.0  (15.6)
+// Over how many workgroups the keys of a unit (16 columns, or eight) are dealt: that power
+// of two of which least time is expected.  A wave's tile, or pair of them, takes `step` us
+// alone on its SIMD and `crowd` of it with each further wave there, a workgroup two
+// steps' time besides, and joining the splits 2.8 us and 2 for every pass of the last
+// workgroup but the first.  us measured, by splits of 1 / 2 / 4 / 8 / 16 / 32 (the one
+// taken in brackets):
+//   14 and 2 heads of width 64, 1 x 511      (6.2)  7.4  7.8  7.5  7.6  8.8
+//   14 and 2 heads of width 64, 1 x 4000     19.2  14.2  10.6  8.8  (7.7)  9.0
+//   14 and 2 heads of width 64, 64 x <= 1023 (8.1)  9.2  10.2  18.1
+//   14 and 2 heads of width 64, 64 x <= 4000 20.0  15.8  (14.4)  21.3
+//   12 and 12 heads of width 64, 16 x <= 2999 (16.4)  16.5  19.4
 //   32 and 8 heads of width 128, 8 x <= 2000 20.8  16.0  (12.9)  15.0
 //   32 and 8 heads of width 128, 8 x <= 32767 269  139  74  (59)  62
-size_t attention_splits(size_t units, size_t tiles, size_t cols, size_t width, size_t cus) {
-    const double step = width == 32 ? 0.48 : width == 64 ? 0.66 : 1.03;
+size_t attention_splits(size_t units, size_t tiles, size_t cols, size_t width, bool pairs, size_t cus) {
+    const double step = pairs ? (width == 32 ? 0.63 : 0.95) : width == 32 ? 0.48 : width == 64 ? 0.66 : 1.03;
+    const double crowd = pairs ? 0.75 : 0.85;
     const size_t pass = 8 * (cols > 8 ? 1 : cols > 4 ? 2 : cols > 2 ? 4 : 16 / cols);  // splits that are joined at once
+    const size_t round = pairs ? 8 : 4;                                               // tiles that four waves take at once
     size_t best = 1;
     double least = 0;
     for (size_t n = 1; n == 1 || (n <= tiles && n * units <= kUnits); n *= 2) {
-        const double there = static_cast<double>((units * n + cus - 1) / cus), walk = static_cast<double>((tiles + 4 * n - 1) / (4 * n));
-        const double t = step * (walk + 2) * std::max(1.0, 0.85 * there) +
-                         (n > 1 ? 2.8 + 1.2 * static_cast<double>((n - 1) / pass) : 0.0);
+        const double there = static_cast<double>((units * n + cus - 1) / cus);
+        const double walk = static_cast<double>((tiles + round * n - 1) / (round * n));
+        const double t = step * (walk + 2) * std::max(1.0, crowd * there) +
+                         (n > 1 ? 2.8 + 2.0 * static_cast<double>((n - 1) / pass) : 0.0);
         if (n == 1 || t < least) {
             best = n;
             least = t;
@@ -1939,13 +1993,18 @@ size_t attention_splits(size_t units, size_t tiles, size_t cols, size_t width, s
 }
 
 template <int HD, bool MODS>
-void launch_attention(fh_ctx* ctx, const AttnArgs& a, bool prompt, size_t grid) {
+void launch_attention(fh_ctx* ctx, const AttnArgs& a, bool prompt, bool pairs, size_t grid) {
     const dim3 g(static_cast<unsigned>(grid));
     if (prompt) {
         if constexpr (HD >= 64)
             hipLaunchKernelGGL((k_kv4_prompt<HD, MODS>), g, dim3(kThreads), sizeof(Room<HD>), ctx->stream, a);
     } else {
-        hipLaunchKernelGGL((k_kv4_attention<HD, MODS>), g, dim3(kThreads), 0, ctx->stream, a);
+        if constexpr (HD <= 64)
+            if (pairs) {
+                hipLaunchKernelGGL((k_kv4_attention<HD, MODS, 2>), g, dim3(kThreads), 0, ctx->stream, a);
+                return;
+            }
+        hipLaunchKernelGGL((k_kv4_attention<HD, MODS, 1>), g, dim3(kThreads), 0, ctx->stream, a);
     }
 }
 
@@ -2034,6 +2093,10 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     // (and only with three quarters of those columns in use: its cost is a workgroup's.)
     const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus) &&
                         4 * tiles16 * c.seqs * c.n_kv >= 3 * 4 * kPromptTiles * shared;
+    // At most eight columns take the keys two tiles at a time.  us, 64 x <= 8000 keys of 12 heads of
+    // width 64: 81, and 97 by single tiles; 64 x <= 1023 of 14 and 2 heads 8.1 and 9.4.  At width 128
+    // a pair's registers would be spilled: 8 x <= 32767 of 32 and 8 heads 125 and 60.
+    const bool pairs = cols <= 8 && c.head_dim <= 64;
     size_t grid = shared;
     if (prompt) {
         a.col_tiles = static_cast<int>((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
@@ -2041,7 +2104,7 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     } else {
         a.col_tiles = static_cast<int>(tiles16);
         const size_t units = c.seqs * c.n_kv * tiles16;
-        const size_t splits = attention_splits(units, key_tiles, std::min<size_t>(cols, 16), c.head_dim,
+        const size_t splits = attention_splits(units, key_tiles, std::min<size_t>(cols, 16), c.head_dim, pairs,
                                                static_cast<size_t>(ctx->num_cus));
         a.splits = static_cast<int>(splits);
         grid = units * splits;
@@ -2056,9 +2119,9 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     if (grid > 0x7FFFFFFF) return fh_fail(ctx, FH_ERR_LIMIT, "fh_kv4_attention: more than 2^31 - 1 workgroups");
     const bool mods = a.softcap > 0.0f || a.slopes;
     switch (c.head_dim) {
-        case 32: mods ? launch_attention<32, true>(ctx, a, prompt, grid) : launch_attention<32, false>(ctx, a, prompt, grid); break;
-        case 64: mods ? launch_attention<64, true>(ctx, a, prompt, grid) : launch_attention<64, false>(ctx, a, prompt, grid); break;
-        default: mods ? launch_attention<128, true>(ctx, a, prompt, grid) : launch_attention<128, false>(ctx, a, prompt, grid); break;
+        case 32: mods ? launch_attention<32, true>(ctx, a, prompt, pairs, grid) : launch_attention<32, false>(ctx, a, prompt, pairs, grid); break;
+        case 64: mods ? launch_attention<64, true>(ctx, a, prompt, pairs, grid) : launch_attention<64, false>(ctx, a, prompt, pairs, grid); break;
+        default: mods ? launch_attention<128, true>(ctx, a, prompt, pairs, grid) : launch_attention<128, false>(ctx, a, prompt, pairs, grid); break;
     }
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
