@@ -263,7 +263,7 @@ __device__ __forceinline__ int group_min(int v) {
 // 2.4e-9), past it, where a wave has such scores, 1 - 2 / (1 + e^2y), whose rounding
 // is then no larger than the result's own.
 __device__ __forceinline__ void cap_scores(float (&x)[8], float cap, float unit) {
-    const float in = unit / cap;
+    const float in = fminf(unit / cap, FLT_MAX);  // (0 times it stays 0)
     float y[8], top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -322,7 +322,8 @@ __device__ __forceinline__ void column_place(const AttnArgs& a, const Rows& r, i
 // The column's query: lane group g holds channels 8 g .. 8 g + 7 of every block,
 // (a column that is not the call's: row 0's, whose result goes nowhere)
 // scaled so that the largest of the row is in [2^13, 2^14) (f16 then has 2^-39
-// of it as its last place).
+// of it as its last place; below 2^-96 by 2^110 only, so that factor stays normal:
+// such a row's scores are nothing beside 1).
 template <int HD>
 __device__ __forceinline__ void load_query(const AttnArgs& a, int lane, const Column<HD>& col,
                                            float (&x)[Shape<HD>::NB][8]) {
@@ -347,7 +348,7 @@ __device__ __forceinline__ void split_query(const AttnArgs& a, const float (&x)[
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[b][i]));
     top = across_groups_max(top);
-    const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+    const int e = top > 0.0f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -96) : 0;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         uint32_t h[4], l[4];
@@ -857,27 +858,24 @@ struct Load {
 // the 2-byte units of lane n in block vb.
 template <int HD>
 struct Part {
-    static constexpr int NB = Shape<HD>::NB, BP = Shape<HD>::BP, W = Load<HD>::W;
+    static constexpr int BP = Shape<HD>::BP, W = Load<HD>::W;
     int n, g, h, kb, vb, ve;
-    bool on;
     __device__ __forceinline__ explicit Part(int tid) {
         n = tid & 15;
         g = tid >> 4 & 3;
         h = tid >> 6 & 1;
         kb = (tid >> 7) * W;
-        vb = HD == 128 ? tid >> 6 : HD == 64 ? tid >> 6 & 1 : 0;
-        ve = HD == 128 ? 0 : HD == 64 ? tid >> 7 : tid >> 6 & 1;
-        on = HD >= 64 || tid < 128;
+        vb = HD == 128 ? tid >> 6 : tid >> 6 & 1;
+        ve = HD == 128 ? 0 : tid >> 7;
     }
     __device__ __forceinline__ int key() const { return 8 * (n >> 2) + (n & 3) + 4 * h; }
-    __device__ __forceinline__ int unit() const { return HD >= 64 ? n * BP + vb / 2 : n & 7; }
-    __device__ __forceinline__ int shift() const { return HD >= 64 ? vb % 2 * 8 : (n >> 3) * 8; }
+    __device__ __forceinline__ int unit() const { return n * BP + vb / 2; }
+    __device__ __forceinline__ int shift() const { return vb % 2 * 8; }
 };
 
 template <int HD>
 __device__ __forceinline__ void load_part(const Planes& p, int cap, int tile, const Part<HD>& w, Load<HD>& t) {
     constexpr int NB = Shape<HD>::NB, VU = HD / 4;
-    if (!w.on) return;
     // (a tile's end past the capacity reads the last rows again; they weigh nothing)
     const uint32_t key = min(tile * 32 + w.key(), cap - 1), o = min(tile * 4 + w.g, cap / 8 - 1);
     const uint8_t* a = p.k + static_cast<size_t>(key * (HD / 2) + (w.g * NB + w.kb) * 4);
@@ -912,7 +910,6 @@ __device__ __forceinline__ void store_values(const Part<HD>& w, const u32x4& v, 
 
 template <int HD>
 __device__ __forceinline__ void store_part(int tile, const Part<HD>& w, const Load<HD>& t, Room<HD>& room) {
-    if (!w.on) return;
     const int lane = w.g * 16 + w.n, f = tile & 3;
     Stage<HD>& st = room.stage[tile & 1];
 #pragma unroll
@@ -1448,7 +1445,7 @@ struct AppendArgs {
 // The frequency of pair i and the angle at a position: apply_rope's (llm.rs:146-175, RopeScaling::angle,
 // llm.rs:118-121), in 32 bits as there.
 __device__ __forceinline__ float rope_frequency(int i, const AppendArgs& a) {
-    return static_cast<float>(exp2(static_cast<double>(-2 * i) / a.rope_dim * a.log2_base));
+    return i == 0 ? 1.0f : static_cast<float>(exp2(static_cast<double>(-2 * i) / a.rope_dim * a.log2_base));
 }
 __device__ __forceinline__ float rope_angle(uint32_t pos, int i, float freq, const AppendArgs& a) {
 #pragma clang fp contract(off)

@@ -1506,8 +1506,9 @@ class LlamaDevice:
         """Feeds lens[r] >= 1 tokens of every row r at once (a 4-bit cache only):
         tokens holds the rows' ids one after the other, on the device; row r's go
         to positions self.pos[r] .. and cache rows self.used[r] .. .  The scores
-        of each row's last token land in self.z; positions are not advanced.
-        Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
+        of each row's last token land in self.z; positions are not advanced
+        (self.pos and self.used are the caller's, next_pos and next_used
+        forward_one's).  Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
         read on the host, so the call waits for the stream."""
         import torch
 

@@ -499,7 +499,7 @@ typedef struct {
  * rounding of it) at position d_pos[r] (NULL: the cache row).  q goes to d_q [total,
  * n_heads * head_dim] (NULL: nowhere); d_qkv is left as it is.  The cache's pos
  * and weight rows are set to the position and 0.  Rows that would lie past the
- * capacity are not stored.  Errors as fh_rope_async's and
+ * capacity are not stored.  Positions are below 2^31.  Errors as fh_rope_async's and
  * fh_gqa_attention_decode_async's. */
 int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_qkv, size_t ld, size_t total,
                         size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
@@ -512,7 +512,9 @@ int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q
  * exp(score).  A row that sees nothing gets 0 and -inf.  max_keys bounds the cache
  * rows in use after the call's rows (it sizes the launch); a row whose cache row is at or past
  * max_keys or the capacity gets NaN.  Within 1e-5 of float64 over the cache's
- * values.  A block that holds a NaN makes NaN of the rows that see it, of its own
+ * values, against the weighted sum of their blocks' largest magnitudes (scores and sums
+ * in 32 bits; a weight times its block's scale counts down to 2^-34 of the row's
+ * largest).  A block that holds a NaN makes NaN of the rows that see it, of its own
  * channels at least.  The context's workspace for these calls is never freed before the
  * context ends, so captured graphs stay valid; calls of one context must not
  * overlap, replayed graphs included. */

@@ -367,6 +367,22 @@ def test_values_far_apart(fh, repeat, hd):
     attend(fh, box, 8, lens, news, 81, True, (first, end))
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,rows", [(2, 2, 64, 1), (8, 1, 64, 1), (9, 1, 64, 1), (4, 2, 64, 4), (6, 2, 32, 2),
+                                                  (2, 2, 32, 8), (4, 1, 128, 2), (3, 1, 128, 3)])
+@pytest.mark.parametrize("kind", ["causal", "window", "holes"])
+def test_few_columns_around_tiles(fh, n_heads, n_kv, hd, rows, kind):
+    """Lengths around one tile of keys, two, the tiles that a workgroup's waves have, and its parts."""
+    lens = [0, 30, 31, 32, 33, 62, 63, 64, 65, 127, 255, 256, 257, 511, 513, 1000, 1023, 2040]
+    news = [rows] * len(lens)
+    box = Box(len(lens), n_kv, hd, 2048, [a + rows for a in lens], 84, tracked=True)
+    masks = None
+    if kind == "window":
+        masks = [max(0, a + t - 40) for a in lens for t in range(rows)], [a + t + 1 for a in lens for t in range(rows)]
+    elif kind == "holes":
+        masks = masks_of(kind, lens, news, np.random.default_rng(3))
+    attend(fh, box, n_heads, lens, news, 85, rows > 1, masks, weigh=True)
+
+
 def masks_of(kind, lens, news, rng):
     first, end = [], []
     for at, new in zip(lens, news):
@@ -405,6 +421,31 @@ def test_caps_and_biases(fh, n_heads, n_kv, hd, softcap, biased, rows):
     box = Box(2, n_kv, hd, 176, [a + b for a, b in zip(lens, news)], 12, tracked=True)
     slopes = 2.0 ** (-8.0 * np.arange(1, n_heads + 1) / n_heads) if biased else None
     attend(fh, box, n_heads, lens, news, 13, rows == "many", softcap=softcap, slopes=slopes, weigh=True)
+
+
+@pytest.mark.parametrize("repeat", [1, 64])  # (few columns, and many)
+@pytest.mark.parametrize("softcap", [0.0, 1e-44, 3e38])
+def test_scores_of_no_size_and_caps_of_any(fh, repeat, softcap):
+    """Rows of zero, of subnormal and of ordinary queries under a mask: with scores or a cap next to
+    nothing the weights are all alike, with a cap beyond every score it changes nothing."""
+    import ferrum_hip
+    import torch
+
+    seqs, rows, n_kv, hd = 2 * repeat, 48, 2, 64
+    box = Box(2, n_kv, hd, 48, [48, 48], 82, repeat=repeat)
+    q = np.random.default_rng(83).standard_normal((seqs, rows, 8, hd)).astype(np.float32)
+    size = np.where(np.arange(rows) % 3 == 0, 0.0, np.where(np.arange(rows) % 3 == 1, 1e-41, 1.0))
+    q = (q * size[None, :, None, None]).astype(np.float32)
+    first = np.tile(np.arange(rows) // 11 * 11, seqs)
+    out, lse = torch.zeros((seqs * rows, 8 * hd), device="cuda"), torch.zeros((seqs * rows, 8), device="cuda")
+    sc = ferrum_hip.AttnScore(softcap, None, None, ints(first), None)
+    args = (fh, box.c, gpu(q.reshape(seqs * rows, -1)), 8 * hd, seqs * rows, 8, None, rows, ints([0] * seqs), rows, sc)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_attention_async(*args, out, lse)
+    fh.sync()
+    # (a cap of 1e-44 leaves scores that no rounding of exp tells from 0)
+    check_attention(box, q.reshape(-1, 8, hd) * np.float32(softcap != 1e-44), [0] * seqs, [rows] * seqs,
+                    out.cpu().numpy().reshape(-1, 8, hd), lse.cpu().numpy(), first.tolist())
 
 
 def test_bias_goes_by_positions_not_rows(fh):
