@@ -437,12 +437,11 @@ template <int HD, bool MODS>
 __device__ __forceinline__ void finish_scores(const AttnArgs& a, const Column<HD>& col, const uint32_t* kpos, int key0,
                                               float (&s)[8]) {
     if constexpr (MODS) {
+        if (a.softcap > 0.0f) cap_scores(s, a.softcap, col.factor);
+        const float unit = col.factor * kLog2e;
 #pragma unroll
-        for (int j = 0; j < 8; j++) s[j] *= col.factor;
-        if (a.softcap > 0.0f) cap_scores(s, a.softcap, 1.0f);
-        if (a.slopes) less_distance(a, col.slope, col.qpos, kpos, key0, s);
-#pragma unroll
-        for (int j = 0; j < 8; j++) s[j] *= kLog2e;
+        for (int j = 0; j < 8; j++) s[j] *= unit;
+        if (a.slopes) less_distance(a, col.slope * kLog2e, col.qpos, kpos, key0, s);
     }
 }
 
@@ -1492,7 +1491,7 @@ __device__ __forceinline__ f32x4 rotate_quad(const Quad& q, int ch, const Append
             const bool hi = a.neox ? c >= half : c & 1;
             const double2 t = turn[a.neox ? (hi ? c - half : c) : c >> 1];  // (cosine, sine)
             const double u = q.own[k], v = q.other[k];
-            y[k] = static_cast<float>(hi ? v * t.y + u * t.x : u * t.x - v * t.y);
+            y[k] = static_cast<float>(fma(u, t.x, v * (hi ? t.y : -t.y)));
         }
     }
     return y;
