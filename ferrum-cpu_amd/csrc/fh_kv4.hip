@@ -661,6 +661,12 @@ __device__ __forceinline__ float2 load2(const float* from) {
 
 // Attention of 16 columns (T = 2: of at most eight, two tiles at a time) by one workgroup: the
 // four waves take every fourth tile, or pair, of the workgroup's share of the keys.
+// Waves share no keys, so none waits for another before the join; each wave's next two
+// tiles are on their way, which is what registers allow at two waves a SIMD.  Bound by
+// VALU issue (a tile of width 64 is 200 instructions beside 16 MFMAs, most of them per
+// column, in use or not): 8 x <= 32767 keys of 32 and 8 heads of width 128 65 us, 3.6 TB/s
+// of cache, VALU busy 76 %; 64 x <= 8000 keys of 12 heads of width 64 82 us, 3.1 TB/s.
+// Short calls are latency: 1 x 511 keys of 14 and 2 heads 6 us.
 template <int HD, bool MODS, int T>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_attention(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, LD = HD + 4;
@@ -944,6 +950,10 @@ constexpr int kPromptTiles = 2;  // tiles of 16 columns of a wave
 // weight, values under their block's largest exponent over all the keys.  The
 // running maximum is that of score + e, so that a row of keys with small values
 // has all the bits that it has where no other row sees larger ones.
+// At two waves a SIMD every register counts: what a column or a tile keeps is in LDS
+// (spilled, 4 x 2048 rows of documents, 32 and 8 heads of width 128, take 265 us; 220 so).
+// 16 columns a wave instead of 32: 312.  4 x 2000 causal rows of the same heads 382 us, 343
+// TFLOP/s or 1,030 of f16 products: the matrix cores; short documents, VALU (59 %).
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, CT = kPromptTiles;
@@ -1203,6 +1213,8 @@ __device__ __forceinline__ void add_weights(const AttnArgs& a, const half8 (&lv)
 }
 
 // A workgroup: every fourth tile of its share of the keys to a wave, the next on its way.
+// 8 x 16000 keys of 32 and 8 heads of width 128 26 us (68 with the queries split again for
+// every two tiles), 64 x <= 1023 of 14 and 2 heads of width 64 7: load latency.
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB;
@@ -1407,6 +1419,7 @@ __global__ void __launch_bounds__(512, 2) k_kv4_weigh_prompt(AttnArgs a) {
         }
 }
 
+// (2 x 1000 weights of 55 parts, a load at a time: 15.6 us; 8 x 1000 of 16, eight at once: 4.8.)
 __global__ void __launch_bounds__(kThreads) k_kv4_add_weights(AttnArgs a) {
     const uint32_t heads = static_cast<uint32_t>(a.c.seqs) * a.c.n_kv;
     const size_t i = blockIdx.x * static_cast<size_t>(kThreads) + threadIdx.x, all = static_cast<size_t>(heads) * a.max_keys;
@@ -1543,7 +1556,11 @@ __device__ __forceinline__ void quantise4(const f32x4& x, uint16_t& scale, uint3
 }
 
 // The eight cache rows of one octet: rotate and store their queries, quantise
-// their keys and values, eight lanes a block.
+// their keys and values, eight lanes a block.  Whole octets leave as they lie in the
+// planes, through LDS; four quads a thread are on their way at once (213 us at 8 x <= 1000
+// rows of 32 and 8 heads of width 128 with one channel a thread and one load, 62 so).  Bound by VALU
+// issue: the rotation in 64 bits and the quantiser.  A token's row is a chain of
+// latencies, 5.5 us: loads before the angles spill and gain nothing.
 template <int HD, bool QUADS>
 __global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
     constexpr int NB = Shape<HD>::NB, VN = Shape<HD>::N, BP = Shape<HD>::BP, KW = HD / 8, VU = HD / 4;
@@ -1700,7 +1717,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_kv4_append(AppendArgs a) {
 
 // Rows first[s] .. + rows - 1 of every head as f32 rows of n_kv * HD, the f32
 // cache's layout.  One thread: four channels of a key and of its value, so that
-// a wave's stores are whole lines.
+// a wave's stores are whole lines, and past the caches (what is written is larger than
+// they are): 8 x 8192 rows of 8 heads of width 128 130 us, 4.7 TB/s, 210 with neither.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_kv4_read(Cache c, const uint32_t* __restrict__ first, uint32_t rows,
                                                       float* __restrict__ ko, float* __restrict__ vo) {
@@ -1766,8 +1784,8 @@ constexpr int kSelect = 1024, kHeld = 16;  // threads, and weights that each kee
 // of the others up to `keep`, in order; idx gets their cache rows, *count how
 // many.  The lightest weight that stays is found by a radix select of 8-bit digits,
 // from registers up to 16384 rows (a bit at a time by counting, without atomics, the
-// 32 rounds of barriers cost more: 21 us, and 30 at 16384 rows).  Row k * 1024 + t is thread t's k-th, so places follow from
-// counts per (k, wave).
+// 32 rounds of barriers cost more: 21 us, and 30 at 16384 rows).  Row k * 1024 + t is
+// thread t's k-th, so places follow from counts per (k, wave).
 __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t* __restrict__ len, uint32_t max_len,
                                                        uint32_t keep, uint32_t recent, uint32_t* __restrict__ idx,
                                                        uint32_t* __restrict__ counts) {
@@ -1885,7 +1903,8 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
 }
 
 // Moves the rows that stay.  A workgroup: 64 rows of one (sequence, kv head),
-// keys in 16-byte pieces of a row, values and scales eight rows' units at once.
+// keys in 16-byte pieces of a row, values and scales eight rows' units at once (2-byte
+// reads, 16-byte writes): 64 x 8192 rows of width 128 34 us, 4.4 TB/s.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_kv4_move(Cache c, Cache d, uint32_t keep, int chunks,
                                                       const uint32_t* __restrict__ idx,
