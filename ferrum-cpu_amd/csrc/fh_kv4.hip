@@ -1783,14 +1783,15 @@ constexpr int kSelect = 1024, kHeld = 16;  // threads, and weights that each kee
 // Which rows of a (sequence, kv head) stay: the last `recent` and the heaviest
 // of the others up to `keep`, in order; idx gets their cache rows, *count how
 // many.  The lightest weight that stays is found by a radix select of 8-bit digits,
-// from registers up to 16384 rows (a bit at a time by counting, without atomics, the
-// 32 rounds of barriers cost more: 21 us, and 30 at 16384 rows).  Row k * 1024 + t is
-// thread t's k-th, so places follow from counts per (k, wave).
+// until what is left of a digit all stays, from registers up to 16384 rows (a bit at a
+// time by counting, without atomics, the 32 rounds of barriers cost more: 19 us, and 30
+// at 16384 rows).  Row k * 1024 + t is thread t's k-th, so places follow from counts per
+// (k, wave).
 __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t* __restrict__ len, uint32_t max_len,
                                                        uint32_t keep, uint32_t recent, uint32_t* __restrict__ idx,
                                                        uint32_t* __restrict__ counts) {
     constexpr int W = kSelect / 64;
-    __shared__ uint32_t hist[256], pick[2], slot[kHeld * W], base;
+    __shared__ uint32_t hist[256], pick[3], slot[kHeld * W], base;
     const int s = static_cast<int>(blockIdx.x) / c.n_kv;
     const uint32_t n = min(min(len[s], max_len), static_cast<uint32_t>(c.cap));
     uint32_t* to = idx + static_cast<size_t>(blockIdx.x) * keep;
@@ -1812,7 +1813,8 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
     }
     // the largest `cut` that at least `want` rows reach, 8 bits at a time
     uint32_t cut = 0, mask = 0, left = want;  // `left` of the rows that agree with `cut` so far
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    bool whole = false;                       // all of them: then every row from `cut` up stays
+    for (int shift = 24; shift >= 0 && !whole; shift -= 8) {
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
 #pragma unroll
@@ -1837,6 +1839,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
                 if (before < left && before + h[i] >= left) {
                     pick[0] = 255 - (lane * 4 + i);
                     pick[1] = left - before;
+                    pick[2] = before + h[i] == left;
                 }
                 before += h[i];
             }
@@ -1844,6 +1847,7 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
         __syncthreads();
         cut |= pick[0] << shift;
         left = pick[1];
+        whole = pick[2] != 0;
         mask |= 255u << shift;
     }
     // rows above `cut` all stay, and the first `left` of those at it
@@ -1857,10 +1861,16 @@ __global__ void __launch_bounds__(kSelect) k_kv4_select(Cache c, const uint32_t*
                 held[k] = i < free ? ordered(w[i]) : 0;
             }
         }
-        // twice: places among the equals, then among the rows that stay
+        // twice: places among the equals (if some go), then among the rows that stay
         uint32_t stay = 0;
 #pragma unroll
         for (int pass = 0; pass < 2; pass++) {
+            if (pass == 0 && whole) {
+#pragma unroll
+                for (int k = 0; k < kHeld; k++)
+                    if (c0 + k * kSelect + tid < free && held[k] >= cut) stay |= 1u << k;
+                continue;
+            }
             uint64_t votes[kHeld];
 #pragma unroll
             for (int k = 0; k < kHeld; k++) {

@@ -621,6 +621,30 @@ def test_evict(fh, n_heads, n_kv, hd, lens, keep, recent):
 # ---- together -------------------------------------------------------------------
 
 
+@pytest.mark.parametrize("keep,recent", [(16000, 100), (20000, 20000), (39999, 1), (1, 0)])
+@pytest.mark.parametrize("values", ["distinct", "few", "one"])
+def test_evict_from_long_caches(fh, keep, recent, values):
+    """More rows than are held in registers; cuts between weights and within ties."""
+    import ferrum_hip
+    import torch
+
+    lens, cap, rng = [40000, 16385, 16384, 30011], 40000, np.random.default_rng(86)
+    src, dst = (ferrum_hip.KV4Cache.alloc(4, 1, 32, c, True) for c in (cap, -(-keep // 8) * 8))
+    w = rng.random((4, 1, cap)).astype(np.float32) ** 4
+    w = w if values == "distinct" else np.floor(w * 7).astype(np.float32) if values == "few" else np.ones_like(w)
+    src.planes["weight"].copy_(gpu(w))
+    src.planes["pos"].copy_(torch.arange(cap, dtype=torch.int32, device="cuda"))
+    new = ints([0] * 4)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_evict_async(fh, src, dst, ints(lens), cap, keep, recent, new)
+    fh.sync()
+    assert list(new.cpu().numpy()) == [min(n, keep) for n in lens]
+    pos, got = dst.planes["pos"].cpu().numpy(), dst.planes["weight"].cpu().numpy()
+    for s, n in enumerate(lens):
+        kept = ref.evict(w[s, 0], n, keep, recent)
+        assert np.array_equal(pos[s, 0, :len(kept)], kept) and np.array_equal(got[s, 0, :len(kept)], w[s, 0, kept])
+
+
 def test_a_run_of_them_together(fh):
     """A prompt, its weights, an eviction and decode steps over what is left: the
     attention of every step is that of the rows that a float64 account keeps."""
