@@ -149,15 +149,18 @@ __device__ __forceinline__ void load_kd(const Planes& p, int cap, int tile, int 
 }
 
 template <int HD>
-__device__ __forceinline__ void load_tile(const Planes& p, const uint16_t* scales, int cap, int tile, int lane, Tile<HD>& t) {
-    constexpr int NB = Shape<HD>::NB, N = Shape<HD>::N, BP = Shape<HD>::BP;
-    load_k<HD>(p, cap, tile, lane, t.k);
-    const int g = lane >> 4, n = lane & 15, last = cap / 8 - 1;
-    const uint32_t vo = min(tile * 4 + g, last) * (N * BP * 16) + n % N * (BP * 16);
+__device__ __forceinline__ void load_v(const Planes& p, int cap, int tile, int lane, Tile<HD>& t) {
+    constexpr int N = Shape<HD>::N, BP = Shape<HD>::BP;
+    const int g = lane >> 4, n = lane & 15;
+    const uint32_t vo = min(tile * 4 + g, cap / 8 - 1) * (N * BP * 16) + n % N * (BP * 16);
 #pragma unroll
     for (int i = 0; i < BP; i++) t.v[i] = *reinterpret_cast<const u32x4*>(p.v + vo + i * 16);
-    // eight lanes an octet, NB scales each, as they lie
-    const uint16_t* a = scales + (min(tile * 4 + (lane >> 3 & 3), last) * (8 * NB) + (lane & 7) * NB);
+}
+// (scales: of keys for lanes 0 .. 31, of values for the others; eight lanes an octet, NB each, as they lie)
+template <int HD>
+__device__ __forceinline__ void load_scales(const uint16_t* scales, int cap, int tile, int lane, Tile<HD>& t) {
+    constexpr int NB = Shape<HD>::NB;
+    const uint16_t* a = scales + (min(tile * 4 + (lane >> 3 & 3), cap / 8 - 1) * (8 * NB) + (lane & 7) * NB);
     if constexpr (NB == 4) {
         const u32x2 w = *reinterpret_cast<const u32x2*>(a);
         t.sc[0] = w[0];
@@ -489,15 +492,16 @@ __device__ __forceinline__ uint32_t key_exponents(uint32_t scales) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, x) >> 10) | 0x64006400u;
 }
 
-// T tiles of 32 keys, at `tile` and behind, into the sums.  The weights times their
+// T tiles of 32 keys, at `tile` and behind, into the sums.  next(0), (1) and (2): the tiles'
+// scales, keys and values are used up.  The weights times their
 // block's value scale are the f16 operand (two terms): at most 2^14, with 2^-39 of that
 // as their last place, which is 2^-35 of the row's largest.  swap: the wave's LDS
 // room for the tiles' scales.
 constexpr int kSwap = 64;  // 2-byte words of it: 64 scales a block, 64 exponents
-template <int HD, bool MODS, bool MASKED, int T>
+template <int HD, bool MODS, bool MASKED, int T, typename Next>
 __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD> (&t)[T], int tile, int t1, int lane,
                                      const Column<HD>& col, const Queries<HD, T>& q, const uint32_t* kpos,
-                                     uint16_t* swap, Sums<HD, T>& z) {
+                                     uint16_t* swap, Sums<HD, T>& z, Next next) {
     constexpr int NB = Shape<HD>::NB, SW = kSwap * (NB + 1);
     const int g = lane >> 4, n = lane & 15, mine = T == 2 ? n >> 3 : 0, key0 = (tile + mine) * 32 + 8 * g;
     // (a wave's LDS instructions run in order: only the compiler has to be held)
@@ -532,7 +536,9 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD> (&t)[T], 
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     float s[8];
+    next(0);
     scores<HD, T>(t, kd, q, s);
+    next(1);
     finish_scores<HD, MODS>(a, col, kpos, key0, s);
     bool seen[8];
     if constexpr (MASKED) {
@@ -592,37 +598,47 @@ __device__ __forceinline__ void step(const AttnArgs& a, const Tile<HD> (&t)[T], 
             z.o[i][b][1] = mfma(v1, ph, mfma(v1, pl, z.o[i][b][1]));
         }
     }
+    next(2);
 }
 
-// The columns' queries against T tiles at t0, t0 + stride, .. below t1, the next two such on
-// their way while one is worked on.
+// The columns' queries against T tiles at t0, t0 + stride, .. below t1.  Two steps' tiles are
+// at hand; what comes after them is loaded part by part as soon as a step has used
+// up what lies in its place (8 x <= 32767 keys of 32 and 8 heads of width 128 63.6 us, with the
+// loads behind the step 65.4, with one place 66).
 template <int HD, bool MODS, int T>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Planes& p, int lane, Column<HD>& col,
                                      const uint32_t* kpos, int t0, int t1, int stride, int full_lo, int full_hi,
                                      uint16_t* swap, Sums<HD, T>& z) {
     if (t0 >= t1) return;
     const uint16_t* scales = lane < 32 ? p.kd : p.vd;
-    Tile<HD> even[T], odd[T];
-    const auto load = [&](Tile<HD> (&tiles)[T], int t) {
+    Tile<HD> tiles[2][T];
+    const auto load = [&](int d, int t, int part) {
 #pragma unroll
-        for (int i = 0; i < T; i++) load_tile<HD>(p, scales, a.c.cap, min(t + i, t1 - 1), lane, tiles[i]);
+        for (int i = 0; i < T; i++) {
+            const int at = min(t + i, t1 - 1);
+            if (part == 0) load_scales<HD>(scales, a.c.cap, at, lane, tiles[d][i]);
+            if (part == 1) load_k<HD>(p, a.c.cap, at, lane, tiles[d][i].k);
+            if (part == 2) load_v<HD>(p, a.c.cap, at, lane, tiles[d][i]);
+        }
     };
-    load(even, t0);
-    load(odd, t0 + stride);
+#pragma unroll
+    for (int d = 0; d < 2; d++)
+#pragma unroll
+        for (int part = 0; part < 3; part++) load(d, t0 + d * stride, part);
     column_query<HD>(a, lane, col);  // (its loads wait beside the tiles')
     const Queries<HD, T> q = queries_of<HD, T>(col, lane & 15);
-    const auto work = [&](const Tile<HD> (&tiles)[T], int t) {
+    const auto work = [&](auto place, int t) {
+        constexpr int d = decltype(place)::value;
+        const auto next = [&](int part) { load(d, t + 2 * stride, part); };
         if (t * 32 >= full_lo && (t + T) * 32 <= full_hi && t + T <= t1)
-            step<HD, MODS, false, T>(a, tiles, t, t1, lane, col, q, kpos, swap, z);
+            step<HD, MODS, false, T>(a, tiles[d], t, t1, lane, col, q, kpos, swap, z, next);
         else
-            step<HD, MODS, true, T>(a, tiles, t, t1, lane, col, q, kpos, swap, z);
+            step<HD, MODS, true, T>(a, tiles[d], t, t1, lane, col, q, kpos, swap, z, next);
     };
     for (int t = t0; t < t1; t += 2 * stride) {
-        work(even, t);
+        work(std::integral_constant<int, 0>{}, t);
         if (t + stride >= t1) break;
-        load(even, t + 2 * stride);
-        work(odd, t + stride);
-        load(odd, t + 3 * stride);
+        work(std::integral_constant<int, 1>{}, t + stride);
     }
 }
 
@@ -661,8 +677,7 @@ __device__ __forceinline__ float2 load2(const float* from) {
 
 // Attention of 16 columns (T = 2: of at most eight, two tiles at a time) by one workgroup: the
 // four waves take every fourth tile, or pair, of the workgroup's share of the keys.
-// Waves share no keys, so none waits for another before the join; each wave's next two
-// tiles are on their way, which is what registers allow at two waves a SIMD.  Bound by
+// Waves share no keys, so none waits for another before the join.  Bound by
 // VALU issue (a tile of width 64 is 200 instructions beside 16 MFMAs, most of them per
 // column, in use or not): 8 x <= 32767 keys of 32 and 8 heads of width 128 65 us, 3.6 TB/s
 // of cache, VALU busy 76 %; 64 x <= 8000 keys of 12 heads of width 64 82 us, 3.1 TB/s.
