@@ -448,6 +448,19 @@ def test_scores_of_no_size_and_caps_of_any(fh, repeat, softcap):
                     out.cpu().numpy().reshape(-1, 8, hd), lse.cpu().numpy(), first.tolist())
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,lens,news", [(8, 2, 128, [0], [700]), (4, 4, 64, [600, 0, 37], [530, 1, 300]),
+                                                       (6, 1, 32, [1100, 513], [70, 129]), (2, 2, 64, [0] * 40, [33] * 40)])
+@pytest.mark.parametrize("kind", ["causal", "window", "documents", "prefix", "beyond"])
+@pytest.mark.parametrize("options", [False, True])
+def test_weights_of_long_prompts(fh, n_heads, n_kv, hd, lens, news, kind, options):
+    """Several groups of keys, parts of the rows and batches of columns; rows that see none of a group."""
+    top = max(a + b for a, b in zip(lens, news))
+    box = Box(len(lens), n_kv, hd, -(-top // 8) * 8, [a + b for a, b in zip(lens, news)], 87, tracked=True)
+    masks = None if kind == "causal" else masks_of(kind, lens, news, np.random.default_rng(4))
+    slopes = 2.0 ** (-8.0 * np.arange(1, n_heads + 1) / n_heads) if options else None
+    attend(fh, box, n_heads, lens, news, 88, True, masks, softcap=4.0 if options else 0.0, slopes=slopes, weigh=True, tail=3)
+
+
 def test_bias_goes_by_positions_not_rows(fh):
     """A cache whose rows are no longer their positions (as after an eviction)."""
     box = Box(2, 2, 64, 104, [100, 61], 14, tracked=True)
