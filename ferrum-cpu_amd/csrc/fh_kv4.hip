@@ -417,22 +417,23 @@ __device__ __forceinline__ void scores(const Tile<HD> (&t)[T], const u32x4 (&kd)
 // Less slope * distance, of the octet of keys at key0.
 __device__ __forceinline__ void less_distance(const AttnArgs& a, float slope, int qpos, const uint32_t* kpos, int key0,
                                               float (&x)[8]) {
-    int kp[8];
+    float d[8];
     if (kpos) {
         typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
         const u32x4u* from = reinterpret_cast<const u32x4u*>(kpos + min(key0, a.c.cap - 8));
         const u32x4u u = from[0], v = from[1];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            kp[j] = static_cast<int>(u[j]);
-            kp[4 + j] = static_cast<int>(v[j]);
+            d[j] = static_cast<float>(qpos - static_cast<int>(u[j]));
+            d[4 + j] = static_cast<float>(qpos - static_cast<int>(v[j]));
         }
     } else {
+        const float d0 = static_cast<float>(qpos - key0);
 #pragma unroll
-        for (int j = 0; j < 8; j++) kp[j] = key0 + j;
+        for (int j = 0; j < 8; j++) d[j] = d0 - static_cast<float>(j);
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = fmaf(-slope, static_cast<float>(abs(qpos - kp[j])), x[j]);
+    for (int j = 0; j < 8; j++) x[j] = fmaf(-slope, fabsf(d[j]), x[j]);
 }
 
 // Options applied: scores then in the exponent's unit (log2), as they were without any.
