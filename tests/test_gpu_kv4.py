@@ -634,6 +634,69 @@ def test_evict(fh, n_heads, n_kv, hd, lens, keep, recent):
 # ---- together -------------------------------------------------------------------
 
 
+@pytest.mark.parametrize("src_pos,dst_pos,dst_weight", [(True, False, False), (False, True, True), (True, True, False)])
+def test_evict_with_fewer_planes_and_lengths_cut(fh, src_pos, dst_pos, dst_weight):
+    """Planes that one side lacks, lengths above max_len and the capacity, the lengths' own place kept."""
+    import ferrum_hip
+    import torch
+
+    lens, cap, max_len, keep, recent = [90, 64, 300, 20, 0], 96, 80, 33, 5
+    box = Box(5, 2, 64, cap, [min(n, cap) for n in lens], 89, tracked=True)
+    p = box.c.planes
+    src = ferrum_hip.KV4Cache(5, 2, 64, cap, p["k"], p["k_d"], p["v"], p["v_d"], p["pos"] if src_pos else None, p["weight"])
+    to = Box(5, 2, 64, 40, [0] * 5, 90, tracked=True)
+    t = to.c.planes
+    dst = ferrum_hip.KV4Cache(5, 2, 64, 40, t["k"], t["k_d"], t["v"], t["v_d"], t["pos"] if dst_pos else None,
+                              t["weight"] if dst_weight else None)
+    untouched = {n: to.plane(n).copy() for n, own in (("pos", dst_pos), ("weight", dst_weight)) if not own}
+    ln, new = ints(lens), ints([7] * 5)
+    torch.cuda.synchronize()
+    ferrum_hip.kv4_evict_async(fh, src, dst, ln, max_len, keep, recent, new)
+    fh.sync()
+    assert list(ln.cpu().numpy()) == lens and list(new.cpu().numpy()) == [33, 33, 33, 20, 0]
+    for n, old in untouched.items():
+        assert np.array_equal(to.plane(n).view(np.uint8), old.view(np.uint8))
+    k, v = (torch.zeros((5, keep, 2 * 64), device="cuda") for _ in range(2))
+    ferrum_hip.kv4_read_async(fh, dst, None, keep, k, v)
+    fh.sync()
+    k, v = (x.cpu().numpy().reshape(5, keep, 2, 64) for x in (k, v))
+    for s, n in enumerate(min(n, max_len) for n in lens):
+        for h in range(2):
+            kept = ref.evict(box.weight[s, h], n, keep, recent)
+            assert np.array_equal(k[s, :len(kept), h], box.k[s, h, kept].astype(np.float32))
+            assert np.array_equal(v[s, :len(kept), h], box.v[s, h, kept].astype(np.float32))
+            if dst_pos:
+                assert np.array_equal(to.plane("pos")[s, h, :len(kept)], box.pos[s, h, kept] if src_pos else kept)
+            if dst_weight:
+                assert np.array_equal(to.plane("weight")[s, h, :len(kept)], box.weight[s, h, kept])
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,rows", [(14, 2, 64, 1), (64, 1, 64, 1), (8, 2, 128, 1), (6, 3, 32, 50)])
+def test_the_same_call_gives_the_same_bits(fh, n_heads, n_kv, hd, rows):
+    """Keys dealt over workgroups are joined in order; no length array: caches that begin with the call."""
+    import ferrum_hip
+    import torch
+
+    lens = [3000, 17] if rows == 1 else None
+    news = [rows, rows]
+    box = Box(2, n_kv, hd, 3008, [a + rows for a in lens] if lens else news, 91, tracked=True)
+    q = gpu(np.random.default_rng(92).standard_normal((2 * rows, n_heads * hd)).astype(np.float32))
+    results = []
+    for _ in range(3):
+        out, lse = torch.zeros_like(q), torch.zeros((2 * rows, n_heads), device="cuda")
+        box.c.planes["weight"].copy_(gpu(box.weight))
+        torch.cuda.synchronize()
+        args = (fh, box.c, q, n_heads * hd, 2 * rows, n_heads, None, rows, ints(lens) if lens else None, 3008, None)
+        ferrum_hip.kv4_attention_async(*args, out, lse)
+        ferrum_hip.kv4_weigh_async(*args, lse)
+        fh.sync()
+        results.append((out.cpu().numpy(), lse.cpu().numpy(), box.plane("weight").copy()))
+    for r in results[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(r, results[0]))
+    o, z, w = results[0]
+    check_attention(box, q.cpu().numpy().reshape(-1, n_heads, hd), lens or [0, 0], news, o.reshape(-1, n_heads, hd), z, weight=w)
+
+
 @pytest.mark.parametrize("keep,recent", [(16000, 100), (20000, 20000), (39999, 1), (1, 0)])
 @pytest.mark.parametrize("values", ["distinct", "few", "one"])
 def test_evict_from_long_caches(fh, keep, recent, values):
