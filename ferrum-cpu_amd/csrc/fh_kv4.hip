@@ -1114,7 +1114,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
             const float *kup = room.kup[t & 3] + 8 * g, *ve = room.ve[t & 3] + 8 * g, *vdown = room.vdown[t & 3] + 8 * g;
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                if (c) asm volatile("" ::: "memory");  // (the factors are read again: registers for them would be spilled)
                 const Place& at = room.place[(wave * CT + c) * 16 + n];
                 float x[8];
 #pragma unroll
