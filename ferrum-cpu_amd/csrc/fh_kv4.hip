@@ -2126,10 +2126,11 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     a.lse = lse;
     const size_t cols = max_rows * a.group, tiles16 = (cols + 15) / 16, key_tiles = (a.max_keys + 31) / 32;
     // Many columns share each key's expansion (128 to a workgroup) where that still fills the
-    // GPU twice over, so that one workgroup's barriers hide behind another's work.  us, at 8
-    // x 500 rows of 32 and 8 heads of width 128 (1024 such workgroups): 77, and 129 by 16
-    // columns; at 1 x 1000 (256): 80 and 59; 8 x 1001 rows of 14 and 2 heads of width 64 (880):
-    // 80 and 99.  At width 32 a key's expansion costs less than its sharing.
+    // GPU twice over, so that one workgroup's barriers hide behind another's work.  us, and by 16
+    // columns: 8 x 500 rows of 32 and 8 heads of width 128 (1024 such workgroups) 75, 122; 3 x
+    // 1000 (768) 87, 119; 2 x 1000 (512) 80, 81; 1 x 1000 (256) 73, 43; 8 x 1001 rows of 14 and 2
+    // heads of width 64 (880) 73, 83; 4 x 1000 (440) 58, 40.  At width 32 a key's expansion
+    // costs less than its sharing.
     const size_t shared = c.seqs * c.n_kv * ((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
     // (and only with three quarters of those columns in use: its cost is a workgroup's.)
     const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus) &&
