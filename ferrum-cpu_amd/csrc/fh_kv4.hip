@@ -1228,8 +1228,8 @@ __device__ __forceinline__ void add_weights(const AttnArgs& a, const half8 (&lv)
 }
 
 // A workgroup: every fourth tile of its share of the keys to a wave, the next on its way.
-// 8 x 16000 keys of 32 and 8 heads of width 128 26 us (68 with the queries split again for
-// every two tiles), 64 x <= 1023 of 14 and 2 heads of width 64 7: load latency.
+// 8 x 16000 keys of 32 and 8 heads of width 128 24 us (68 with the queries split again for
+// every two tiles), 64 x <= 1023 of 14 and 2 heads of width 64 6: load latency.
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB;
@@ -2173,8 +2173,12 @@ template <int HD, bool MODS>
 static int launch_weigh(fh_ctx* ctx, AttnArgs& a, size_t tiles16) {
     const size_t heads = static_cast<size_t>(a.c.seqs) * a.c.n_kv, tiles = (a.max_keys + 31) / 32;
     if (tiles16 == 1) {
-        // workgroups of at least four tiles, and no more than four to a CU
-        const size_t splits = std::max<size_t>(1, std::min(4 * static_cast<size_t>(ctx->num_cus) / heads, tiles / 4));
+        // One workgroup for each CU, of four tiles of keys at least, or four, of eight.  us, by this
+        // rule and by four of four: 64 x <= 1023 keys of 14 and 2 heads of width 64 5.7, 6.3; 8 x <=
+        // 2000 of 32 and 8 heads of width 128 7.3, 8.6; by it and by four of eight: 1 x 8000 4.7,
+        // 5.2; 4 x <= 700 of 12 heads of width 64 5.1, 5.5; and by one only: 8 x 16000 23.6, 31.1.
+        const size_t cus = static_cast<size_t>(ctx->num_cus);
+        const size_t splits = std::max<size_t>(1, std::max(std::min(cus / heads, tiles / 4), std::min(4 * cus / heads, tiles / 8)));
         a.splits = static_cast<int>(splits);
         hipLaunchKernelGGL((k_kv4_weigh_step<HD, MODS>), dim3(static_cast<unsigned>(heads * splits)), dim3(kThreads), 0,
                            ctx->stream, a);
