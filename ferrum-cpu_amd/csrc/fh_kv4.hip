@@ -852,9 +852,15 @@ struct Place {
     uint32_t head;  // the top bit: its row has no place in the cache
 };
 
-// Of four tiles' keys: the block scales under 2^e (0 of a key that nobody sees or that
-// holds a NaN), e being the largest exponent of a key's own; as 2^e of keys (NaN
-// where they hold one), as e and 2^-e of values (under their blocks' exponents).
+// Staged scales are 2^kLift above their key's exponent: a level times a scale is below 2^15
+// then, and a block's scale exact in f16 as far as 2^25 below the key's largest (below 1 it
+// would be to 2^13 only), or at any distance where that is under 2^12: an f16 scale's last
+// place is 2^-24 at least.
+constexpr int kLift = 12;
+
+// Of four tiles' keys: the block scales under 2^(e - kLift) (0 of a key that nobody sees or
+// that holds a NaN), e being the largest exponent of a key's own; as 2^(e - kLift) of keys
+// (NaN where they hold one), as e and 2^-e of values.
 template <int HD>
 struct Room {
     Stage<HD> stage[2];
@@ -862,7 +868,7 @@ struct Room {
     float kup[4][32], ve[4][32], vdown[4][32];
     uint16_t d[2][4][Shape<HD>::NB][32];  // of values, of keys
     uint32_t nan[4];                      // a bit a key whose values hold one
-    int range[2], vbits[4];
+    int range[2];
 };
 
 // One thread's share of a tile on its way to LDS.
@@ -963,9 +969,10 @@ constexpr int kPromptTiles = 2;  // tiles of 16 columns of a wave
 // neither a score nor a weight takes its scale block by block, and every product
 // of an f32 operand (two terms as well) is three matrix products, the lowest left
 // out (2^-22).  The range of f16 is each key's own: 2^-e here, 2^e on its score or
-// weight, values under their block's largest exponent over all the keys.  The
-// running maximum is that of score + e, so that a row of keys with small values
-// has all the bits that it has where no other row sees larger ones.
+// weight, e being the key's largest block's exponent and nothing of any other key's, so that
+// a row has the bits of what it sees whatever the other 127 columns see.  The running maximum
+// is that of score + e.  A block of values counts, as in k_kv4_attention, down to 2^-34 of the
+// row's largest weight times scale; one of keys down to 2^-36 of its key's largest.
 // At two waves a SIMD every register counts: what a column or a tile keeps is in LDS
 // (spilled, 4 x 2048 rows of documents, 32 and 8 heads of width 128, take 265 us; 220 so).
 // 16 columns a wave instead of 32: 312.  4 x 2000 causal rows of the same heads 382 us, 343
@@ -998,7 +1005,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         room.range[0] = 0x7FFFFFFF;
         room.range[1] = 0;
     }
-    if (tid < 4) room.vbits[tid] = 0;
     __syncthreads();
     if (lane == 0) {
         atomicMin(&room.range[0], lo);
@@ -1017,21 +1023,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; b++) ld.d[b] = from[b * 8];
     };
-    if (t0 < t1) {
-        load_part<HD>(p, a.c.cap, t0, part, ld);
-        // the largest exponent of each block's value scales
-        uint32_t m = 0;
-        for (int i = t0 * 4 * NB + tid; i < min(t1 * 4, a.c.cap / 8) * NB; i += kThreads) {  // (NB divides kThreads: one block a thread)
-            const u32x4 w = *reinterpret_cast<const u32x4*>(p.vd + static_cast<size_t>(i) * 8);
-            const int k0 = i / NB * 8;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t x = w[j >> 1] >> (16 * (j & 1)) & 0x7FFFu;
-                m = k0 + j >= glo && k0 + j < ghi && x < 0x7C00u ? max(m, x) : m;
-            }
-        }
-        atomicMax(&room.vbits[tid % NB], static_cast<int>(m));
-    }
+    if (t0 < t1) load_part<HD>(p, a.c.cap, t0, part, ld);
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         column_query<HD>(a, lane, col[c]);
@@ -1043,25 +1035,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         }
     }
     __syncthreads();
-    int vexp[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) vexp[b] = min(__builtin_amdgcn_readfirstlane(room.vbits[b]) >> 10, 30) - 14;
     const auto key_factors = [&](int tile) {  // of key lane % 32, from ld.d
         const int i = tile & 3, j = lane & 31, key = tile * 32 + j;
-        int e = -64;
+        int e = -14;
         bool fine = true;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const int x = ld.d[b] >> 10 & 31;
             fine = fine && x < 31;
-            e = max(e, x - 14 - (lane < 32 ? vexp[b] : 0));
+            e = max(e, x - 14);
         }
         const bool seen = key >= glo && key < ghi, use = fine && seen;
         e = use ? e : 0;
         const uint64_t nans = __ballot(seen && !fine);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const float x = ldexpf(fh_h2f(ld.d[b]), -e - (lane < 32 ? vexp[b] : 0));
+            const float x = ldexpf(fh_h2f(ld.d[b]), kLift - e);
             room.d[lane >> 5][i][b][j] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(use ? x : 0.0f));
         }
         if (lane < 32) {
@@ -1069,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
             room.vdown[i][j] = ldexpf(1.0f, -e);
             if (lane == 0) room.nan[i] = static_cast<uint32_t>(nans);
         } else {
-            room.kup[i][j] = fine || !seen ? ldexpf(1.0f, e) : __builtin_nanf("");
+            room.kup[i][j] = fine || !seen ? ldexpf(1.0f, e - kLift) : __builtin_nanf("");
         }
     };
     f32x4 o[CT][NB][2];
@@ -1179,7 +1168,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         if (t + 1 < t1) store_part<HD>(t + 1, part, ld, room);
         if (wave == (t & 3)) key_factors(t + 2);
     }
-    // Each lane has 8 channels of every block of its columns: 32 b + 8 g + i at o[b][i & 1][i >> 1] * 2^vexp[b].
+    // Each lane has 8 channels of every block of its columns: 32 b + 8 g + i at o[b][i & 1][i >> 1] * 2^-kLift.
 #pragma unroll
     for (int c = 0; c < CT; c++) l[c] = across_groups_sum(l[c]);
 #pragma unroll
@@ -1189,11 +1178,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
         const size_t to = static_cast<size_t>(at.row) * a.n_heads + (at.head & 0x7FFFFFFFu);
         const bool bad = at.head >> 31;
         float* out = a.out + to * HD + g * 8;
-        const float f = bad ? __builtin_nanf("") : l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+        const float f = bad ? __builtin_nanf("") : l[c] == 0.0f ? 0.0f : 1.0f / (static_cast<float>(1 << kLift) * l[c]);
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) out[32 * b + i] = o[c][b][i & 1][i >> 1] * ldexpf(f, vexp[b]);
+            for (int i = 0; i < 8; i++) out[32 * b + i] = o[c][b][i & 1][i >> 1] * f;
         if (a.lse && g == 0) a.lse[to] = bad ? __builtin_nanf("") : (base[c] + log2f(l[c])) * kLn2;
     }
 }

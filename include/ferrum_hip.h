@@ -514,7 +514,8 @@ int fh_kv4_append_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q
  * max_keys or the capacity gets NaN.  Within 1e-5 of float64 over the cache's
  * values, against the weighted sum of their blocks' largest magnitudes (scores and sums
  * in 32 bits; a weight times its block's scale counts down to 2^-34 of the row's
- * largest).  A block that holds a NaN makes NaN of the rows that see it, of its own
+ * largest, a query's channel to 2^-38 of its head's largest, a key's block to 2^-36 of
+ * its key's largest).  A block that holds a NaN makes NaN of the rows that see it, of its own
  * channels at least.  The context's workspace for these calls is never freed before the
  * context ends, so captured graphs stay valid; calls of one context must not
  * overlap, replayed graphs included. */
