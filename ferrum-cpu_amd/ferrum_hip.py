@@ -1495,6 +1495,9 @@ class LlamaDevice:
         self.feed_async(nxt)
         self.next_pos = nxt + 1
         self.ctx.sync()
+        if self.kv == "q4":  # the place of what comes next: an eviction's rows, a prompt's first
+            self.pos.fill_(nxt + 1)
+            self.used.fill_(used + 1)
         return self.z[0].cpu().numpy()
 
     def _attend4_async(self, b, qkv, total: int, off, max_rows: int, pos, max_keys: int, q, att, lse):
