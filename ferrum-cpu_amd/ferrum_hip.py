@@ -1278,6 +1278,8 @@ class LlamaDevice:
             self.lse = torch.empty((B, self.nh), device=dev) if self.tracked else None
             self.used = torch.zeros(B, dtype=torch.int32, device=dev)  # cache rows in use, as pos until rows are evicted
             self.spare = None
+        self._next_pos = self._next_used = 0
+        self._used_given = False  # next_used was set since forward_one last went on
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
         self.fused = 3 <= B <= 64 and self.d % 32 == 0
@@ -1473,16 +1475,70 @@ class LlamaDevice:
         per = 4 if g >= 5 else 2
         return self.hd == 64 and g >= 2 and self.rows * self.nkv * -(-g // per) >= 128
 
+    @property
+    def next_pos(self) -> int:
+        """The position that forward_one feeds next.  0 starts another text.  Over a
+        4-bit cache a move takes next_used with it (forwards by the rows that
+        prefill_async fed, backwards to feed them again: that only while no rows have
+        been evicted, since then next_used has to say which row it is), and a
+        single row's self.pos and self.used."""
+        return self._next_pos
+
+    @next_pos.setter
+    def next_pos(self, pos: int):
+        pos, used = int(pos), self._next_used
+        if self.kv == "q4" and not self._used_given:
+            if pos < self._next_pos and pos and used != self._next_pos:
+                raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.next_pos: rows below position {self._next_pos} were "
+                                                     f"evicted: set next_used to the cache row of position {pos} first")
+            used = used + pos - self._next_pos if pos else 0
+        self._place(pos, used)
+
+    @property
+    def next_used(self) -> int:
+        """The cache row (of a 4-bit cache) that forward_one writes next: next_pos less
+        the rows evicted so far."""
+        return self._next_used
+
+    @next_used.setter
+    def next_used(self, used: int):
+        self._place(self._next_pos, int(used))
+        self._used_given = True
+
+    def reset(self):
+        """The next token of every row starts another text, in an empty cache."""
+        import torch
+
+        self._used_given = False
+        self.next_pos = 0
+        self.ctx.sync()
+        self.pos.zero_()
+        if self.kv == "q4":
+            self.used.zero_()
+        torch.cuda.current_stream().synchronize()
+
+    def _place(self, pos: int, used: int):
+        """forward_one's place, on the device too where prefill_async and evict_async read it."""
+        import torch
+
+        self._next_pos, self._next_used = pos, used
+        if self.kv == "q4" and self.rows == 1:
+            self.ctx.sync()
+            self.pos.fill_(pos)
+            self.used.fill_(used)
+            torch.cuda.current_stream().synchronize()
+
     def forward_one(self, token: int):
         """LlamaModel::forward_one (llm.rs:606-616) for a single sequence (rows
-        == 1): feed `token` at the next position and return the logits (host)
-        — the callback llama_decode drives.  A full cache is FH_ERR_DIM."""
+        == 1): feed `token` at the next position (next_pos) and return the logits
+        (host) — the callback llama_decode drives.  A full cache is FH_ERR_DIM;
+        reset (or next_pos = 0) clears it."""
         import torch
 
         if self.rows != 1:
             raise FerrumHipError(FH_ERR_INVALID, "forward_one drives a single-row LlamaDevice")
-        nxt = getattr(self, "next_pos", 0)
-        used = getattr(self, "next_used", 0) if self.kv == "q4" else nxt
+        nxt = self._next_pos
+        used = self._next_used if self.kv == "q4" else nxt
         if used >= self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
         self.ctx.sync()
@@ -1490,10 +1546,9 @@ class LlamaDevice:
         self.pos.fill_(nxt)
         if self.kv == "q4":
             self.used.fill_(used)
-            self.next_used = used + 1
         torch.cuda.current_stream().synchronize()
         self.feed_async(nxt)
-        self.next_pos = nxt + 1
+        self._next_pos, self._next_used, self._used_given = nxt + 1, used + 1, False
         self.ctx.sync()
         if self.kv == "q4":  # the place of what comes next: an eviction's rows, a prompt's first
             self.pos.fill_(nxt + 1)
@@ -1516,8 +1571,8 @@ class LlamaDevice:
         tokens holds the rows' ids one after the other, on the device; row r's go
         to positions self.pos[r] .. and cache rows self.used[r] .. .  The scores
         of each row's last token land in self.z; positions are not advanced
-        (self.pos and self.used are the caller's, next_pos and next_used
-        forward_one's).  Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
+        (self.pos and self.used are the caller's; before forward_one goes on from
+        there, next_pos, which moves them all).  Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
         read on the host, so the call waits for the stream."""
         import torch
 
@@ -1590,8 +1645,7 @@ class LlamaDevice:
             kv4_evict_async(self.ctx, b["k"], self.spare, self.used, self.cap, keep, recent,
                             self.used if last else self._cut)
             b["k"], self.spare = self.spare, b["k"]
-        if hasattr(self, "next_used"):
-            self.next_used = min(self.next_used, keep)
+        self._next_used, self._used_given = min(self._next_used, keep), False
 
     def feed_async(self, max_pos: int):
         """One decode step of every row: token self.tokens[r] at position

@@ -34,3 +34,89 @@ def test_eviction_after_forward_one_keeps_the_newest_rows(fh, orc):
             assert (np.diff(kept, axis=2) > 0).all()
             assert (kept[:, :, -3:] == np.arange(pos - 2, pos + 1)).all(), pos
     m.free()
+
+
+def run(m, ids):
+    return [m.forward_one(int(t)) for t in ids]
+
+
+@pytest.mark.parametrize("how", ["next_pos", "reset"])
+@pytest.mark.parametrize("first", [5, 16, 30])  # (a few tokens, a full cache, one that has been cut)
+def test_a_second_text_is_as_on_a_fresh_device(fh, orc, how, first):
+    import ferrum_hip
+
+    cfg, w = dict(QWEN, context=16, kv="q4", kv_tracked=True), make_weights(orc, QWEN, 4, True, True)
+    rng = np.random.default_rng(2)
+    one, two = rng.integers(0, QWEN["vocab"], first), rng.integers(0, QWEN["vocab"], 12)
+    m = ferrum_hip.LlamaDevice.from_weights(fh, w, cfg, 1)
+    for t in one:
+        if m.next_used == 16:
+            m.evict_async(9, 2)
+        m.forward_one(int(t))
+    if how == "reset":
+        m.reset()
+    else:
+        m.next_pos = 0
+    assert (m.next_pos, m.next_used) == (0, 0) and m.used.cpu().tolist() == m.pos.cpu().tolist() == [0]
+    got = run(m, two)
+    fresh = ferrum_hip.LlamaDevice.from_weights(fh, w, cfg, 1)
+    assert np.array_equal(got, run(fresh, two)) and np.isfinite(got).all()
+    m.free()
+    fresh.free()
+
+
+def test_going_back_feeds_the_same_rows_again(fh, orc):
+    """next_pos moved back takes next_used with it, until rows have been evicted: then only with next_used."""
+    import ferrum_hip
+
+    cfg, w = dict(QWEN, context=16, kv="q4", kv_tracked=True), make_weights(orc, QWEN, 4, True, True)
+    ids = np.random.default_rng(3).integers(0, QWEN["vocab"], 16)
+    m = ferrum_hip.LlamaDevice.from_weights(fh, w, cfg, 1)
+    z = run(m, ids)
+    m.next_pos = 9
+    assert m.next_used == 9
+    assert np.array_equal(run(m, ids[9:]), z[9:])
+    m.evict_async(10, 5)
+    assert (m.next_pos, m.next_used) == (16, 10)
+    with pytest.raises(ferrum_hip.FerrumHipError, match="set next_used"):
+        m.next_pos = 14
+    want = m.forward_one(7)
+    m.next_used = 10
+    m.next_pos = 16
+    assert (m.next_pos, m.next_used) == (16, 10)
+    assert np.array_equal(m.forward_one(7), want)
+    m.free()
+
+
+def test_forward_one_goes_on_behind_a_prompt_and_an_eviction(fh, orc):
+    """A prompt at once, its place handed on by next_pos alone, tokens, an eviction, a second prompt:
+    each result against a float64 walk over the device's own caches."""
+    import ferrum_hip
+    import torch
+
+    cfg, w = dict(QWEN, context=24, kv="q4", kv_tracked=True), make_weights(orc, QWEN, 4, True, True)
+    walk = Walk(orc, w, QWEN)
+    m = ferrum_hip.LlamaDevice.from_weights(fh, w, cfg, 1)
+    ids = np.random.default_rng(5).integers(0, QWEN["vocab"], 60).astype(np.int32)
+    pos = used = 0
+
+    def check(z):
+        seen = [tuple(a[0, :, :used] for a in read(m, i)) for i in range(m.layers)]
+        assert close(z, walk.step(ids[pos - 1], pos - 1, seen)[0]), pos
+
+    for prompt, tokens in ((11, 6), (5, 4)):
+        m.prefill_async(torch.from_numpy(ids[pos:pos + prompt]).cuda(), [prompt])
+        pos, used = pos + prompt, used + prompt
+        m.next_pos = pos
+        assert m.next_used == used
+        fh.sync()
+        check(m.z[0].cpu().numpy())
+        for _ in range(tokens):
+            z = m.forward_one(int(ids[pos]))
+            pos, used = pos + 1, used + 1
+            check(z)
+        m.evict_async(12, 4)
+        fh.sync()
+        used = min(used, 12)
+        assert m.next_used == used and (positions(m, used)[:, :, -4:] == np.arange(pos - 4, pos)).all()
+    m.free()
