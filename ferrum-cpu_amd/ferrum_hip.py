@@ -1547,7 +1547,7 @@ class LlamaDevice:
         if self.kv == "q4":
             self.used.fill_(used)
         torch.cuda.current_stream().synchronize()
-        self.feed_async(nxt)
+        self.feed_async(nxt, used)
         self._next_pos, self._next_used, self._used_given = nxt + 1, used + 1, False
         self.ctx.sync()
         if self.kv == "q4":  # the place of what comes next: an eviction's rows, a prompt's first
@@ -1647,13 +1647,16 @@ class LlamaDevice:
             b["k"], self.spare = self.spare, b["k"]
         self._next_used, self._used_given = min(self._next_used, keep), False
 
-    def feed_async(self, max_pos: int):
+    def feed_async(self, max_pos: int, max_used=None):
         """One decode step of every row: token self.tokens[r] at position
         self.pos[r] (both on the device; max_pos bounds the positions).  The
         head's scores land in self.z; positions are not advanced.  (A 4-bit cache:
-        at cache row self.used[r], which is not advanced either.)"""
+        at cache row self.used[r], which is not advanced either; max_used bounds
+        these, None: max_pos does.  A row beyond gets NaN; a bound far above them, as
+        max_pos is once rows have been evicted, plans the step for keys that are not
+        there.)"""
         ctx, d, B = self.ctx, self.d, self.rows
-        max_keys = min(max_pos + 1, self.cap)
+        max_keys = min((max_pos if max_used is None else max_used) + 1, self.cap)
         embed_rows_async(ctx, self.tok_w, self.vocab, d, self.tokens, B, self.x)
         if self.fused:
             # x is updated in place by the o and down projections, which leave

@@ -120,3 +120,29 @@ def test_forward_one_goes_on_behind_a_prompt_and_an_eviction(fh, orc):
         used = min(used, 12)
         assert m.next_used == used and (positions(m, used)[:, :, -4:] == np.arange(pos - 4, pos)).all()
     m.free()
+
+
+def test_cache_rows_beyond_the_position(fh, orc):
+    """Rows whose texts' positions start again behind other rows: feed_async is told how many there are."""
+    import ferrum_hip
+    import torch
+
+    w = make_weights(orc, QWEN, 4, True, True)
+    walk = Walk(orc, w, QWEN)
+    m = ferrum_hip.LlamaDevice.from_weights(fh, w, dict(QWEN, kv="q4"), 3)
+    lens, pos = np.array([20, 1, 37]), np.array([3, 0, 2])
+    ids = np.random.default_rng(6).integers(0, QWEN["vocab"], lens.sum() + 3).astype(np.int32)
+    m.prefill_async(torch.from_numpy(ids[:-3]).cuda(), lens)
+    fh.sync()
+    m.pos.copy_(torch.from_numpy(pos.astype(np.int32)))
+    m.used.copy_(torch.from_numpy(lens.astype(np.int32)))
+    m.tokens.copy_(torch.from_numpy(ids[-3:]))
+    torch.cuda.synchronize()
+    m.feed_async(int(pos.max()), int(lens.max()))
+    fh.sync()
+    z = m.z.cpu().numpy()
+    caches = [read(m, i) for i in range(m.layers)]
+    for r in range(3):
+        seen = [(k[r, :, :lens[r] + 1], v[r, :, :lens[r] + 1]) for k, v in caches]
+        assert close(z[r], walk.step(ids[-3 + r], pos[r], seen)[0]), r
+    m.free()
