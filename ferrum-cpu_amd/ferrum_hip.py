@@ -1568,7 +1568,7 @@ class LlamaDevice:
 
     def prefill_async(self, tokens, lens):
         """Feeds lens[r] >= 1 tokens of every row r at once (a 4-bit cache only):
-        tokens holds the rows' ids one after the other, on the device; row r's go
+        tokens (int32) holds the rows' ids one after the other, on the device; row r's go
         to positions self.pos[r] .. and cache rows self.used[r] .. .  The scores
         of each row's last token land in self.z; positions are not advanced
         (self.pos and self.used are the caller's; before forward_one goes on from
@@ -1583,6 +1583,11 @@ class LlamaDevice:
         if n.shape != (B,) or (n < 1).any():
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {B} lengths of at least 1")
         total, most = int(n.sum()), int(n.max())
+        if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int32, torch.uint32):
+            kind = getattr(tokens, "dtype", type(tokens).__name__)
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: tokens are an int32 tensor, not {kind}")
+        if not tokens.is_cuda or not tokens.is_contiguous():
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async: tokens lie on the device, side by side")
         if tokens.numel() != total:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {tokens.numel()} tokens for {total} places")
         ctx.sync()

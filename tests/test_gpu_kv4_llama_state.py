@@ -146,3 +146,16 @@ def test_cache_rows_beyond_the_position(fh, orc):
         seen = [(k[r, :, :lens[r] + 1], v[r, :, :lens[r] + 1]) for k, v in caches]
         assert close(z[r], walk.step(ids[-3 + r], pos[r], seen)[0]), r
     m.free()
+
+
+def test_prefill_takes_32_bit_ids_only(fh):
+    """torch's own ids are 64-bit: read as pairs of 32 they would be others."""
+    import ferrum_hip
+    import torch
+
+    m = ferrum_hip.LlamaDevice(fh, dict(QWEN, kv="q4"), 2)
+    ids = torch.randint(0, QWEN["vocab"], (5,), device="cuda")
+    for tokens, what in ((ids, "int32 tensor, not torch.int64"), (ids.int().cpu(), "on the device"),
+                         (ids.int().repeat(2)[::2], "side by side")):
+        with pytest.raises(ferrum_hip.FerrumHipError, match=what):
+            m.prefill_async(tokens, [3, 2])
