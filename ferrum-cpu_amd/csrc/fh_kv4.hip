@@ -310,7 +310,7 @@ __device__ __forceinline__ void column_place(const AttnArgs& a, const Rows& r, i
                                                 r.at + r.count);
     col.bad = col.on && place >= keys;
     uint64_t lo = 0, hi = place + 1;
-    if (col.on && a.first) lo = a.first[col.row];
+    if (col.on && a.first) lo = static_cast<uint32_t>(max(static_cast<int>(a.first[col.row]), 0));  // (a window's may be below 0)
     if (col.on && a.end) hi = a.end[col.row];
     hi = min(hi, keys);
     if (!col.on || col.bad || lo >= hi) lo = hi = 0;

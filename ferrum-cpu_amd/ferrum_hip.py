@@ -162,7 +162,8 @@ class AttnScore(C.Structure):
     """fh_attn_score: score options of the 4-bit cache's attention.  softcap > 0
     caps scores with a tanh; slopes [n_heads] subtracts slope * distance (the rows'
     positions: pos [total], None = their cache rows); row r sees cache rows
-    first[r] <= j < end[r] (None: 0 and its own + 1).  Tensors are kept alive here."""
+    first[r] <= j < end[r] (None: 0 and its own + 1; a first below 0 is 0).  All three
+    are 32-bit.  Tensors are kept alive here."""
 
     _fields_ = [("softcap", C.c_float)] + [(n, C.c_void_p) for n in ("slopes", "pos", "first", "end")]
 

@@ -477,7 +477,8 @@ typedef struct {
  *     the row's from d_pos [total] (NULL: its cache row), the key's from the
  *     cache's pos;
  *   d_first, d_end [total]: the row sees cache rows first <= j < end, cut to the
- *     rows that are there (NULL: 0, and the row's own cache row + 1).  A document
+ *     rows that are there (NULL: 0, and the row's own cache row + 1; a first of 2^31
+ *     or more is one below 0, wrapped, and counts as 0).  A document
  *     mask is first = its document's start; a sliding window of w, first = row + 1 -
  *     w; a prefix whose rows see each other, end = max(row + 1, the prefix's end). */
 typedef struct {

@@ -113,3 +113,12 @@ def test_key_blocks_far_apart_under_queries_of_the_small_one(fh, repeat, hd, dow
     q = np.random.default_rng(106).standard_normal((box.seqs * 96, 8, hd)).astype(np.float32) * np.float32(2.0 ** 11)
     q[..., :hd - 32] = 0
     attend(fh, box, q, 96)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("repeat", FORMS)
+def test_a_sliding_window_by_its_formula(fh, repeat, hd):
+    """first = row + 1 - w, below 0 for the first rows: they see all that is before them."""
+    box = Box(2, 2, hd, 96, [96, 96], 107, repeat=repeat)
+    q = np.random.default_rng(108).standard_normal((box.seqs * 96, 8, hd)).astype(np.float32)
+    attend(fh, box, q, 96, np.arange(96) + 1 - 9)
