@@ -122,3 +122,13 @@ def test_a_sliding_window_by_its_formula(fh, repeat, hd):
     box = Box(2, 2, hd, 96, [96, 96], 107, repeat=repeat)
     q = np.random.default_rng(108).standard_normal((box.seqs * 96, 8, hd)).astype(np.float32)
     attend(fh, box, q, 96, np.arange(96) + 1 - 9)
+
+
+@pytest.mark.parametrize("n_heads,hd,keys", [(1, 128, 32760), (5, 128, 32760), (16, 64, 65536), (8, 32, 262144)])
+def test_a_long_row_over_many_workgroups(fh, n_heads, hd, keys):
+    """The keys of one unit of columns are dealt over 128, 64, 32 and 64 workgroups, whose parts the
+    last to arrive joins in several passes."""
+    from test_gpu_kv4 import attend as attend_box
+
+    box = Box(1, 1, hd, keys, [keys], 109, tracked=True)
+    attend_box(fh, box, n_heads, [keys - 1], [1], 110, False, weigh=True)
