@@ -132,3 +132,53 @@ def test_a_long_row_over_many_workgroups(fh, n_heads, hd, keys):
 
     box = Box(1, 1, hd, keys, [keys], 109, tracked=True)
     attend_box(fh, box, n_heads, [keys - 1], [1], 110, False, weigh=True)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd", [(8, 2, 32), (8, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("repeat", [1, 90])
+def test_bias_by_positions_that_are_not_rows_in_prompts(fh, n_heads, n_kv, hd, repeat):
+    """Distances from the cache's own positions (gaps, as after an eviction) under a cap, and the weights."""
+    from test_gpu_kv4 import attend as attend_box
+
+    lens, news = [0, 41, 7, 130] * repeat, [70, 61, 57, 68] * repeat
+    top = max(a + b for a, b in zip(lens, news))
+    box = Box(4, n_kv, hd, -(-top // 8) * 8, [a + b for a, b in zip(lens, news)][:4], 111, tracked=True, repeat=repeat)
+    rng = np.random.default_rng(112)
+    box.pos = np.sort(rng.integers(0, 3000, box.pos.shape), axis=2).astype(np.int32)
+    box.c.planes["pos"].copy_(gpu(box.pos))
+    slopes = 2.0 ** (-8.0 * np.arange(1, n_heads + 1) / n_heads)
+    qpos = rng.integers(0, 3000, sum(news))  # (in front of some keys, behind others)
+    attend_box(fh, box, n_heads, lens, news, 113, True, softcap=6.0, slopes=slopes, qpos=qpos, weigh=True)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("repeat", [1, 90])
+def test_rows_of_prompts_beyond_the_bound(fh, repeat, hd):
+    """Rows at or past max_keys are NaN, the others as without that bound; the NaN rows weigh nothing."""
+    import ferrum_hip
+    import torch
+
+    rows, most, n_heads = 96, 70, 8
+    box = Box(4, 2, hd, 96, [96] * 4, 114, tracked=True, repeat=repeat)
+    total = box.seqs * rows
+    q = torch.randn((total, n_heads * hd), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    got = []
+    for keys in (rows, most):
+        out, lse = torch.zeros_like(q), torch.zeros((total, n_heads), device="cuda")
+        weight = box.c.planes["weight"]
+        weight.zero_()
+        torch.cuda.synchronize()
+        args = (fh, box.c, q, n_heads * hd, total, n_heads, None, rows, None, keys, None)
+        ferrum_hip.kv4_attention_async(*args, out, lse)
+        ferrum_hip.kv4_weigh_async(*args, lse)
+        fh.sync()
+        got.append((out.cpu().numpy().reshape(box.seqs, rows, -1), lse.cpu().numpy().reshape(box.seqs, rows, -1),
+                    weight.cpu().numpy()))
+    (o, z, _), (ob, zb, wb) = got
+    assert np.isnan(ob[:, most:]).all() and np.isnan(zb[:, most:]).all()
+    # (the same products and sums; how the keys are dealt may differ: 1e-5 of the values' size)
+    assert np.abs(ob[:, :most] - o[:, :most]).max() <= 1e-5 * np.abs(box.v).max()
+    assert np.abs(zb[:, :most] - z[:, :most]).max() <= 1e-5
+    assert (wb[:, :, most:] == 0).all() and np.isfinite(wb).all()
+    # each row's heads give 1 each; 2^-18 of a weight (its score's and its lse's roundings) and of the sums
+    assert np.allclose(wb.sum(axis=2), most * n_heads / 2, rtol=2.0 ** -17)
