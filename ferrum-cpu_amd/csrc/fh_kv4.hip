@@ -214,7 +214,9 @@ __device__ __forceinline__ half8 v_levels(const u32x4& w) {
 __device__ __forceinline__ float half_at(const u32x4& w, int i) {
     return fh_h2f(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
 }
-// Two f32 as a pair of f16 and what that leaves, each rounded to nearest: 22 bits in all.
+// Two f32 as a pair of f16 and what that leaves, each rounded to nearest: 22 bits in all, for
+// queries and weights alike.  A third term would make every product half as long again for
+// less than the roundings of the sums behind it (check_attention's count of a score: 2^-21).
 // (The values and the pair are kept from the compiler's view: it would form a product's
 // hi in one mixed-precision instruction, with one rounding, and lo from the twice rounded
 // one, or the pair twice over.)
@@ -975,8 +977,9 @@ constexpr int kPromptTiles = 2;  // tiles of 16 columns of a wave
 // row's largest weight times scale; one of keys down to 2^-36 of its key's largest.
 // At two waves a SIMD every register counts: what a column or a tile keeps is in LDS
 // (spilled, 4 x 2048 rows of documents, 32 and 8 heads of width 128, take 265 us; 220 so).
-// 16 columns a wave instead of 32: 312.  4 x 2000 causal rows of the same heads 382 us, 343
-// TFLOP/s or 1,030 of f16 products: the matrix cores; short documents, VALU (59 %).
+// 16 columns a wave instead of 32: 312.  4 x 2000 causal rows of the same heads 366 us, 358
+// TFLOP/s or 1,075 of f16 products, near a large f16 product's rate (MFMA 46 % busy, VALU 52 %);
+// short documents: VALU 58 %, MFMA 33 %.
 template <int HD, bool MODS>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     constexpr int NB = Shape<HD>::NB, CT = kPromptTiles;
@@ -1187,7 +1190,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_prompt(AttnArgs a) {
     }
 }
 
-// Adds to each key's weight what every (query row, head of its group) gave it.
+// Adds to each key's weight what every (query row, head of its group) gave it: exp(score - lse), the
+// lse rounded to f32 between the two calls, so that a row's weights share an error of 2^-24 |lse|
+// of themselves beside the scores' own.  (A sum over the keys again would cost the attention's first
+// half once more.)
 // Two forms: k_kv4_weigh_step for a single tile of 16 columns, whose queries are
 // split once for all the keys that a wave walks, and k_kv4_weigh_prompt.
 
@@ -1279,7 +1285,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_weigh_step(AttnArgs a) {
 // order): each wave splits the queries of one into LDS for all of them, while the
 // next batch is on its way.  (Split by every wave for itself, 1 x 1000 rows of 32 and 8
 // heads of width 128 took 54 us; they take 31, 132 TFLOP/s of products of two terms.)
-// Bound by what follows the products, a scale a block and an exponential a score.
+// Bound by its waits (49 % of the waves' cycles; VALU 45 % busy, MFMA 17 %): a workgroup has two
+// batches there, each with two barriers, and nothing of the next one's split behind the products.
 constexpr int kWeighTiles = 2;  // KT
 
 template <int HD>
@@ -2002,6 +2009,11 @@ constexpr size_t kPartBytes = kUnits * 16 * (128 + 2) * sizeof(float);
 //   12 and 12 heads of width 64, 16 x <= 2999 (16.4)  16.5  19.4
 //   32 and 8 heads of width 128, 8 x <= 2000 20.8  16.0  (12.9)  15.0
 //   32 and 8 heads of width 128, 8 x <= 32767 269  139  74  (59)  62
+// and of single units, by splits of 16 / 32 / 64 / 128 / 256:
+//   1 head of width 128, 1 x 32760            23.7  16.1  12.9  (12.4)  15.9
+//   5 and 1 heads of width 128, 1 x 32760     24.0  18.4  (18.0)  23.5  37.5
+//   8 and 1 heads of width 32, 1 x 262144     47.5  28.0  (19.3)  17.3  21.2
+//   16 and 1 heads of width 64, 1 x 65536     27.3  (19.2)  17.8  22.5
 size_t attention_splits(size_t units, size_t tiles, size_t cols, size_t width, bool pairs, size_t cus) {
     const double step = pairs ? (width == 32 ? 0.63 : 0.95) : width == 32 ? 0.48 : width == 64 ? 0.66 : 1.03;
     const double crowd = pairs ? 0.75 : 0.85;
@@ -2118,10 +2130,14 @@ int fh_launch_kv4_attention(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, 
     // GPU twice over, so that one workgroup's barriers hide behind another's work.  us, and by 16
     // columns: 8 x 500 rows of 32 and 8 heads of width 128 (1024 such workgroups) 75, 122; 3 x
     // 1000 (768) 87, 119; 2 x 1000 (512) 80, 81; 1 x 1000 (256) 73, 43; 8 x 1001 rows of 14 and 2
-    // heads of width 64 (880) 73, 83; 4 x 1000 (440) 58, 40.  At width 32 a key's expansion
-    // costs less than its sharing.
+    // heads of width 64 (880) 73, 83; 4 x 1000 (440) 58, 40.  (Width 32 has one form only: a tile of
+    // it is half a workgroup's parts.  8 x 500 rows of 32 and 8 heads of it take 45, of width 64 60
+    // by 16 columns and 51 shared.)
     const size_t shared = c.seqs * c.n_kv * ((tiles16 + 4 * kPromptTiles - 1) / (4 * kPromptTiles));
-    // (and only with three quarters of those columns in use: its cost is a workgroup's.)
+    // (and only with three quarters of those columns in use: its cost is a workgroup's.  us, and by
+    // 16 columns, 32 sequences of 32 and 8 heads of width 128 behind 1000 keys: 36 rows, 56 % in use,
+    // 100, 82; 40, 62 %, 103, 92; 44, 69 %, 104, 99; 48, 75 %, 104, 109; 56, 88 %, 107, 124.  The
+    // fewer the keys, the sooner it wins: 40 rows behind none 17, 25.)
     const bool prompt = c.head_dim >= 64 && shared >= 2 * static_cast<size_t>(ctx->num_cus) &&
                         4 * tiles16 * c.seqs * c.n_kv >= 3 * 4 * kPromptTiles * shared;
     // At most eight columns take the keys two tiles at a time.  us, 64 x <= 8000 keys of 12 heads of

@@ -1459,7 +1459,8 @@ class LlamaDevice:
         of its own (nine).  The head counts as one call (a wide head at more
         than 32 rows takes one launch per 32 rows).  A 4-bit cache takes two
         launches per block where the f32 one takes RoPE and attention, three
-        when it keeps the keys' weights."""
+        when it keeps the keys' weights (with more than 64 query heads to a kv
+        head possibly four: their weights may be added up by a launch of their own)."""
         per = (6 if all(b.get("glu") for b in self.blocks) else 7) if self.fused else 9
         if self.kv == "q4":
             per += self.tracked

@@ -525,7 +525,8 @@ int fh_kv4_attention_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* 
                            size_t max_keys, const fh_attn_score* score, float* d_out, float* d_lse);
 /* Adds to the cache's weight of every key what the rows' query heads gave it:
  * exp(score - lse) over rows and heads of its kv head, d_lse as
- * fh_kv4_attention_async wrote it for the same arguments. */
+ * fh_kv4_attention_async wrote it for the same arguments (in f32: a row's weights carry
+ * 2^-24 |lse| of themselves, and their scores' roundings). */
 int fh_kv4_weigh_async(fh_ctx* ctx, const fh_kv4_cache* cache, const float* d_q, size_t ld, size_t total,
                        size_t n_heads, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len, size_t max_keys,
                        const fh_attn_score* score, const float* d_lse);
