@@ -1588,8 +1588,8 @@ class LlamaDevice:
         if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int32, torch.uint32):
             kind = getattr(tokens, "dtype", type(tokens).__name__)
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: tokens are an int32 tensor, not {kind}")
-        if not tokens.is_cuda or not tokens.is_contiguous():
-            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async: tokens lie on the device, side by side")
+        if not tokens.is_cuda or tokens.device != self.used.device or not tokens.is_contiguous():
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async: tokens lie on the model's device, side by side")
         if tokens.numel() != total:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {tokens.numel()} tokens for {total} places")
         ctx.sync()

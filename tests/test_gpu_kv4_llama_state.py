@@ -155,7 +155,7 @@ def test_prefill_takes_32_bit_ids_only(fh):
 
     m = ferrum_hip.LlamaDevice(fh, dict(QWEN, kv="q4"), 2)
     ids = torch.randint(0, QWEN["vocab"], (5,), device="cuda")
-    for tokens, what in ((ids, "int32 tensor, not torch.int64"), (ids.int().cpu(), "on the device"),
+    for tokens, what in ((ids, "int32 tensor, not torch.int64"), (ids.int().cpu(), "on the model's device"),
                          (ids.int().repeat(2)[::2], "side by side")):
         with pytest.raises(ferrum_hip.FerrumHipError, match=what):
             m.prefill_async(tokens, [3, 2])
