@@ -1523,6 +1523,8 @@ class LlamaDevice:
         """forward_one's place, on the device too where prefill_async and evict_async read it."""
         import torch
 
+        if pos < 0 or used < 0:
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice: no position {pos} or cache row {used}")
         self._next_pos, self._next_used = pos, used
         if self.kv == "q4" and self.rows == 1:
             self.ctx.sync()

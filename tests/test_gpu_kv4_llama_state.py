@@ -159,3 +159,22 @@ def test_prefill_takes_32_bit_ids_only(fh):
                          (ids.int().repeat(2)[::2], "side by side")):
         with pytest.raises(ferrum_hip.FerrumHipError, match=what):
             m.prefill_async(tokens, [3, 2])
+
+
+@pytest.mark.parametrize("kv", ["f32", "q4"])
+def test_reset_clears_every_row(fh, kv):
+    import ferrum_hip
+
+    m = ferrum_hip.LlamaDevice(fh, dict(QWEN, kv=kv), 3)
+    for t in [m.pos] + ([m.used] if kv == "q4" else []):
+        t.fill_(7)
+    m.next_pos = 5
+    assert m.pos.cpu().tolist() == [7, 7, 7]  # (several rows' counters are the caller's)
+    m.reset()
+    assert m.next_pos == 0 and m.pos.cpu().tolist() == [0, 0, 0]
+    if kv == "q4":
+        assert m.next_used == 0 and m.used.cpu().tolist() == [0, 0, 0]
+    for name in ("next_pos", "next_used"):
+        with pytest.raises(ferrum_hip.FerrumHipError, match="no position"):
+            setattr(m, name, -1)
+    assert (m.next_pos, m.next_used) == (0, 0)
