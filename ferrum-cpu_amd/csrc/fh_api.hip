@@ -138,6 +138,10 @@ int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out) {
     return zeroed_area(ctx, &ctx->kv4, &ctx->kv4_bytes, bytes, "the 4-bit cache's workspace", out);
 }
 
+int fh_gqa_counters(fh_ctx* ctx, size_t bytes, void** out) {
+    return zeroed_area(ctx, &ctx->gqa, &ctx->gqa_bytes, bytes, "the attention's counters", out);
+}
+
 int fh_kv4_room(fh_ctx* ctx, size_t bytes, void** out) {
     if (ctx->kv4_room_bytes < bytes) {
         hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -258,6 +262,7 @@ void fh_ctx_destroy(fh_ctx* ctx) {
     if (ctx->sync) (void)hipFree(ctx->sync);
     if (ctx->counters) (void)hipFree(ctx->counters);
     if (ctx->kv4) (void)hipFree(ctx->kv4);
+    if (ctx->gqa) (void)hipFree(ctx->gqa);
     if (ctx->kv4_room) (void)hipFree(ctx->kv4_room);
     for (void* p : ctx->kv4_old) (void)hipFree(p);
     if (ctx->act) (void)hipFree(ctx->act);
@@ -1040,6 +1045,129 @@ int fh_gqa_attention_rope_decode_async(fh_ctx* ctx, float* d_qkv, size_t ld, siz
     return fh_launch_gqa_attention_rope_decode(ctx, d_qkv, ld, rows, n_heads, n_kv, head_dim, d_k_cache, d_v_cache,
                                                capacity, d_pos, max_pos, rope_dim, base, rope_type, d_freq_factors,
                                                linear_factor, d_out);
+}
+
+// ---- many rows of a sequence over its f32 cache -------------------------------------
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+static int gqa_rows(fh_ctx* ctx, const std::string& who, fh_gqa_call& g, size_t max_keys, bool tree) {
+    if (g.n_kv == 0 || g.n_heads == 0 || g.n_heads % g.n_kv != 0)
+        return fh_fail(ctx, FH_ERR_DIM, "n_heads " + std::to_string(g.n_heads) + " must be a multiple of n_kv_heads " +
+                                            std::to_string(g.n_kv));
+    if (g.rope_dim > g.hd || g.rope_dim % 2 != 0)
+        return fh_fail(ctx, FH_ERR_DIM, "rope_dim " + std::to_string(g.rope_dim) + " must be even and \u2264 head_dim " +
+                                            std::to_string(g.hd));
+    if (g.rope_dim && (!(g.linear_factor > 0.0f) || !std::isfinite(g.linear_factor)))
+        return fh_fail(ctx, FH_ERR_DIM, "RoPE scaling factors must be finite and > 0");
+    if (g.rope_dim && g.rope_type != FH_ROPE_NORM && g.rope_type != FH_ROPE_NEOX)
+        return fh_fail(ctx, FH_ERR_INVALID, who + ": unknown rope_type " + std::to_string(g.rope_type));
+    if (g.hd != 8 && g.hd != 16 && g.hd != 32 && g.hd != 64 && g.hd != 128)
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": head width " + std::to_string(g.hd) + " is not 8, 16, 32, 64 or 128");
+    if (g.seqs == 0 || g.capacity == 0) return fh_fail(ctx, FH_ERR_INVALID, who + ": no sequences or no capacity");
+    if (g.seqs > 65535 || g.n_heads > 65535 || g.total > 0x7FFFFFFFu / g.n_heads || g.capacity > 0x7FFFFFFFu ||
+        g.seqs * g.n_kv > 0x7FFFFFu || g.seqs * g.capacity > (size_t(1) << 40) / (g.n_kv * g.hd))
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": a dimension is too large");
+    if (g.ld < (g.n_heads + 2 * g.n_kv) * g.hd)
+        return fh_fail(ctx, FH_ERR_DIM, who + ": ld is below (n_heads + 2 n_kv) * head_dim");
+    if (!g.off) {
+        if (g.total % g.seqs != 0)
+            return fh_fail(ctx, FH_ERR_DIM, who + ": " + std::to_string(g.total) + " rows do not divide over " +
+                                                std::to_string(g.seqs) + " sequences");
+        g.max_rows = g.total / g.seqs;
+    } else {
+        g.max_rows = std::min(g.max_rows, g.total);
+    }
+    if (tree && g.max_rows > 1024)
+        return fh_fail(ctx, FH_ERR_LIMIT, who + ": more than 1024 rows of a sequence");
+    if (g.total == 0 || g.max_rows == 0) return FH_OK;
+    if (!g.qkv || !g.k_cache || !g.v_cache || !g.out || (tree && !g.parent))
+        return fh_fail(ctx, FH_ERR_INVALID, who + ": a pointer is NULL");
+    if (!aligned16(g.k_cache) || !aligned16(g.v_cache) || !aligned16(g.out))
+        return fh_fail(ctx, FH_ERR_INVALID, who + ": a cache or out is not 16-byte aligned");
+    if (g.out == g.qkv) return fh_fail(ctx, FH_ERR_INVALID, who + ": out must not be qkv");
+    g.limit = std::min(g.capacity, max_keys);
+    FH_ON_DEVICE(ctx);
+    return fh_launch_gqa_rows(ctx, g);
+}
+
+int fh_gqa_attention_rope_prefill_async(fh_ctx* ctx, const float* d_qkv, size_t ld, size_t total, size_t n_heads,
+                                        size_t n_kv, size_t head_dim, float* d_k_cache, float* d_v_cache, size_t seqs,
+                                        size_t capacity, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                                        size_t max_keys, const uint32_t* d_pos, size_t rope_dim, float base,
+                                        int rope_type, const float* d_freq_factors, float linear_factor, float* d_out) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    fh_gqa_call g{d_qkv, ld, total, n_heads, n_kv, head_dim, d_k_cache, d_v_cache, seqs, capacity, 0, max_rows, d_off, d_len,
+                  nullptr, d_pos, rope_dim, base, rope_type, d_freq_factors, linear_factor, d_out};
+    return gqa_rows(ctx, "fh_gqa_attention_rope_prefill", g, max_keys, false);
+}
+
+int fh_gqa_attention_rope_tree_async(fh_ctx* ctx, const float* d_qkv, size_t ld, size_t total, size_t n_heads,
+                                     size_t n_kv, size_t head_dim, float* d_k_cache, float* d_v_cache, size_t seqs,
+                                     size_t capacity, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                                     size_t max_keys, const uint32_t* d_parent, const uint32_t* d_pos, size_t rope_dim,
+                                     float base, int rope_type, const float* d_freq_factors, float linear_factor,
+                                     float* d_out) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    fh_gqa_call g{d_qkv, ld, total, n_heads, n_kv, head_dim, d_k_cache, d_v_cache, seqs, capacity, 0, max_rows, d_off, d_len,
+                  d_parent, d_pos, rope_dim, base, rope_type, d_freq_factors, linear_factor, d_out};
+    return gqa_rows(ctx, "fh_gqa_attention_rope_tree", g, max_keys, true);
+}
+
+int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
+                         size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
+                         const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
+                         uint32_t* d_count, uint32_t* d_next, uint32_t* d_new_len) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    if (seqs == 0) return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: no sequences");
+    if (seqs > 65535 || n_planes > 65535 || total > 0x7FFFFFFFu || capacity > 0x7FFFFFFFu || kv_dim > 0x7FFFFFFFu)
+        return fh_fail(ctx, FH_ERR_LIMIT, "fh_tree_accept: a dimension is too large");
+    if (!d_off) {
+        if (total % seqs != 0)
+            return fh_fail(ctx, FH_ERR_DIM, "fh_tree_accept: " + std::to_string(total) + " rows do not divide over " +
+                                                std::to_string(seqs) + " sequences");
+        max_rows = total / seqs;
+    } else {
+        max_rows = std::min(max_rows, total);
+    }
+    if (max_rows > 1024) return fh_fail(ctx, FH_ERR_LIMIT, "fh_tree_accept: more than 1024 rows of a sequence");
+    if (!d_count || !d_next || !d_new_len) return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: a pointer is NULL");
+    if (total && (!d_parent || !d_tokens || !d_chosen || !d_path))
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: a pointer is NULL");
+    if (n_planes && (!d_planes || kv_dim == 0 || capacity == 0))
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: caches without addresses, width or capacity");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_tree_accept(ctx, d_parent, d_tokens, d_chosen, total, d_off, seqs, max_rows, d_len, d_planes, n_planes,
+                                 kv_dim, capacity, d_path, d_count, d_next, d_new_len);
+}
+
+int fh_logits_edit_async(fh_ctx* ctx, const float* d_logits, size_t rows, size_t vocab, const fh_logits_edit* edit,
+                         float* d_out) {
+    if (!ctx) return FH_ERR_INVALID;
+    ctx->err.clear();
+    if (!edit) return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: edit is NULL");
+    if (vocab == 0) return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: vocab is 0");
+    if (rows > 0x7FFFFFFFu || vocab > 0x7FFFFFFFu || edit->seqs > 0x7FFFFFFFu)
+        return fh_fail(ctx, FH_ERR_LIMIT, "fh_logits_edit: a dimension is too large");
+    if (rows == 0) return FH_OK;
+    if (!d_logits || !d_out) return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: logits or out is NULL");
+    const fh_logits_edit& e = *edit;
+    if (e.d_ranges && !e.d_recent) return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: ranges without recent");
+    if (e.d_tokens) {
+        if (e.seqs == 0) return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: tokens of no sequences");
+        if (!e.d_off && rows % e.seqs != 0)
+            return fh_fail(ctx, FH_ERR_DIM, "fh_logits_edit: " + std::to_string(rows) + " rows do not divide over " +
+                                                std::to_string(e.seqs) + " sequences");
+        if (!e.d_off && rows / e.seqs > 1024)
+            return fh_fail(ctx, FH_ERR_LIMIT, "fh_logits_edit: more than 1024 rows of a sequence");
+    }
+    if (e.d_bias_off && (!e.d_bias_id || !e.d_bias))
+        return fh_fail(ctx, FH_ERR_INVALID, "fh_logits_edit: bias_off without bias_id or bias");
+    FH_ON_DEVICE(ctx);
+    return fh_launch_logits_edit(ctx, d_logits, rows, vocab, e, d_out);
 }
 
 // ---- the 4-bit cache -----------------------------------------------------------

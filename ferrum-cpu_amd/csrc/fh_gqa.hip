@@ -1,0 +1,845 @@
+// fh_gqa.hip — many rows of a sequence at once over its f32 key/value cache: prompts
+// of different lengths packed one after the other, and trees of drafted tokens
+// (Attention::forward_one, llm.rs:285-358, for rows that it feeds one by one; the trees,
+// what is accepted of them and the cache made compact again have no reference
+// counterpart).
+//
+// With K, V the cache rows of a sequence after its new rows went there, s(r, j) =
+// q_r . k_j / sqrt(hd) and
+//   prompt: row t at cache row c = len + t sees j <= c;
+//   tree:   node t sees j < len, and len + a for itself and its ancestors a,
+// out_r = sum over seen j of exp(s - max) v_j / sum of exp(s - max).
+// Two launches: k_gqa_append (rotate q and k, store k and v, and of a tree the depths
+// and ancestors), k_gqa_rows (the rest).
+#include "fh_internal.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#pragma clang fp contract(off)
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef _Float16 h8f __attribute__((ext_vector_type(8)));
+typedef _Float16 h2f __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Rows [begin, begin + count) of the call belong to sequence s, row t of them is cache
+// row at + t.  What the device arrays say is cut to the call's own bounds, so no value of
+// theirs leads outside its buffers.
+struct Rows {
+    uint32_t begin, count;
+    uint64_t at;
+};
+__device__ __forceinline__ Rows rows_of(const uint32_t* off, const uint32_t* len, uint32_t total, uint32_t max_rows,
+                                        uint32_t seqs, uint32_t s) {
+    Rows r;
+    if (off) {
+        r.begin = min(off[s], total);
+        const uint32_t fin = min(off[s + 1], total);
+        r.count = fin > r.begin ? min(fin - r.begin, max_rows) : 0;
+    } else {
+        r.count = total / seqs;
+        r.begin = r.count * s;
+    }
+    r.at = len ? len[s] : 0;
+    return r;
+}
+
+// ---- rotation and storing ------------------------------------------------------------
+
+constexpr int kMaxTree = 1024;  // nodes of a sequence's tree
+
+struct AppendArgs {
+    const float* qkv;
+    size_t ld;
+    float *kc, *vc;
+    size_t seq_stride;  // of the caches (floats)
+    int n_heads, n_kv, hd;
+    uint32_t seqs, total, max_rows, limit;
+    const uint32_t *off, *len, *pos, *parent;
+    float* q;           // [total, n_heads * hd]
+    uint32_t* seen;     // [total, words]: a node's path, bit a for node a
+    int words;
+    int rope_dim, neox;
+    float linear;
+    const float* ff;
+    int heads_each, chunks;
+    float freq[64];
+};
+
+// A workgroup takes some rows of a sequence and `heads_each` of their heads: a thread
+// keeps one pair of channels' sine and cosine for all of them.
+template <bool TREE>
+__global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
+    const uint32_t s = blockIdx.y;
+    const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
+    const int slots = a.hd / 2, each = kThreads / slots;  // rows of a workgroup
+    const uint32_t t0 = blockIdx.x / a.chunks * static_cast<uint32_t>(each);
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    if (t0 >= r.count) return;
+    __shared__ uint32_t up[TREE ? kMaxTree : 1];
+    if constexpr (TREE) {
+        // (a parent that is not one of the nodes before it: none)
+        for (uint32_t t = threadIdx.x; t < min(r.count, t0 + each); t += kThreads) {
+            const uint32_t p = a.parent[r.begin + t];
+            up[t] = p < t ? p : ~0u;
+        }
+        __syncthreads();
+    }
+    const int slot = static_cast<int>(threadIdx.x) % slots;
+    const uint32_t t = t0 + threadIdx.x / slots, row = r.begin + t;
+    if (t >= r.count) return;
+    uint32_t depth = t;
+    if constexpr (TREE) {
+        depth = 0;
+        for (uint32_t x = up[t]; x != ~0u; x = up[x]) depth++;
+        if (chunk == 0)
+            for (int w = slot; w < a.words; w += slots) {
+                uint32_t bits = 0;
+                for (uint32_t x = t; x != ~0u; x = up[x])
+                    if (static_cast<int>(x >> 5) == w) bits |= 1u << (x & 31);
+                a.seen[static_cast<size_t>(row) * a.words + w] = bits;
+            }
+    }
+    const int half = a.rope_dim / 2;
+    const bool turns = slot < half;
+    // the pair's two channels (past rope_dim: two that stay as they are)
+    const int ia = turns ? (a.neox ? slot : 2 * slot) : 2 * slot;
+    const int ib = turns ? (a.neox ? slot + half : 2 * slot + 1) : 2 * slot + 1;
+    float sn = 0.0f, cs = 1.0f;
+    if (turns) {
+        const uint32_t p = a.pos ? a.pos[row] : static_cast<uint32_t>(r.at) + depth;
+        const float f = a.ff ? a.ff[slot] : 1.0f;
+        const float theta = static_cast<float>(static_cast<int>(p)) * a.freq[slot] / f * (1.0f / a.linear);
+        sn = sinf(theta);
+        cs = cosf(theta);
+    }
+    const float* x = a.qkv + row * a.ld;
+    const uint64_t c = r.at + t;
+    const bool fits = c < a.limit;
+    const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
+    const size_t to = s * a.seq_stride + (fits ? c : 0) * kv_dim;
+    const int h1 = min(a.n_heads + 2 * a.n_kv, (chunk + 1) * a.heads_each);
+    for (int h = chunk * a.heads_each; h < h1; h++) {
+        const float* xh = x + static_cast<size_t>(h) * a.hd;
+        const float u = xh[ia], w = xh[ib];
+        float y = u, z = w;
+        if (turns && h < a.n_heads + a.n_kv) {
+            y = u * cs - w * sn;
+            z = u * sn + w * cs;
+        }
+        float* dst;
+        if (h < a.n_heads) {
+            dst = a.q + (static_cast<size_t>(row) * a.n_heads + h) * a.hd;
+        } else {
+            if (!fits) continue;
+            dst = h < a.n_heads + a.n_kv ? a.kc + to + static_cast<size_t>(h - a.n_heads) * a.hd
+                                         : a.vc + to + static_cast<size_t>(h - a.n_heads - a.n_kv) * a.hd;
+        }
+        dst[ia] = y;
+        dst[ib] = z;
+    }
+}
+
+// ---- attention -------------------------------------------------------------------------
+
+constexpr int kKeys = 32;  // keys of a tile
+
+struct RowsArgs {
+    const float* q;  // [total, n_heads * hd], rotated
+    const float *kc, *vc;
+    size_t seq_stride;
+    int n_heads, n_kv, group, hd;
+    uint32_t seqs, total, max_rows, limit;
+    const uint32_t *off, *len, *seen;
+    int words;
+    float scale;  // log2(e) / sqrt(hd)
+    float* out;
+    int col_blocks, splits;
+    float2* part;
+    unsigned* counters;
+};
+
+__device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
+__device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+constexpr uint32_t kInf = 0x7F800000u;  // magnitudes from here on: infinity, NaN
+
+// The largest of G consecutive lanes' values (G a power of two up to 64), in all of them.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_of(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF, 0xF, true));
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    if constexpr (G >= 2) v = max(v, dpp_of<0xB1>(v));
+    if constexpr (G >= 4) v = max(v, dpp_of<0x4E>(v));
+    if constexpr (G >= 8) v = max(v, dpp_of<0x141>(v));
+    if constexpr (G >= 16) v = max(v, dpp_of<0x140>(v));
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    return v;
+}
+__device__ __forceinline__ float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
+// Two f32 values as two f16 terms each: h = f16(x), l = f16(x - h), 22 bits.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const h2f h = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    const h2f l = {static_cast<_Float16>(x - static_cast<float>(h.x)), static_cast<_Float16>(y - static_cast<float>(h.y))};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+// The same where a value may be infinite (its lower term is 0 then).
+__device__ __forceinline__ void split2_any(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const h2f h = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    const float rx = mag(x) == kInf ? 0.0f : x - static_cast<float>(h.x);
+    const float ry = mag(y) == kInf ? 0.0f : y - static_cast<float>(h.y);
+    const h2f l = {static_cast<_Float16>(rx), static_cast<_Float16>(ry)};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// e with x 2^e in [2^14, 2^15) for a magnitude's bits, as far as it is in range.
+__device__ __forceinline__ int lift(uint32_t bits, int most) { return min(max(141 - static_cast<int>(bits >> 23), -113), most); }
+
+__device__ __forceinline__ f32x16 mfma(h8f a, h8f b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// Row of accumulator v in a lane of half `half` of a 32 x 32 product.
+__device__ __forceinline__ constexpr int acc_row(int v, int half) { return (v >> 2) * 8 + half * 4 + (v & 3); }
+
+__device__ __forceinline__ void store_part(float2* to, float2 x) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_part(const float2* from) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float2*>(from)), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Columns are (row, query head of the kv head), heads fastest; a wave has 32 of them, a
+// workgroup CW waves of columns times KW waves that deal tiles of 32 keys among them.
+// A tile is read from the cache once for the workgroup and kept in LDS as MFMA
+// operands: every f32 value in two f16 terms (22 bits; three products of a product's four,
+// the lowest left out at 2^-22).  Each key's channels are brought to [2^14, 2^15) by a power of
+// two of that key's own, undone exactly on its score; each value row's power of two goes into
+// the weights (the running maximum is that of score - exponent), so that a row's accuracy
+// does not hang on keys beside it that it does not see, nor on how large the values are.
+// S^T = K Q^T leaves a lane 16 keys of one column, which is where O^T += V^T P^T wants them.
+// W: the head width brought to 32, 64 or 128.
+template <int W, int CW, int KW>
+struct Stage {
+    static constexpr int KI = W / 16, OT = W / 32;
+    _Float16 k[2][KW][KI][2][64][8];
+    _Float16 v[2][KW][OT][2][2][64][8];
+    float kdown[2][KW][kKeys];  // 2^-e of a key
+    float vexp[2][KW][kKeys];   // -e of a value row
+    float vup[2][KW][kKeys];    // 2^e of it
+    int unsafe[3][KW];          // a value that is not finite (step st: st % 3)
+};
+
+template <int W, int CW, int KW, bool TREE>
+__global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
+    constexpr int NW = CW * KW, KI = W / 16, OT = W / 32;
+    constexpr int WK = KW * W / 16;                        // a stage's keys: pieces of 64 threads; its values as many
+    constexpr int PER = (2 * WK + NW - 1) / NW;            // pieces of a wave
+    extern __shared__ __align__(16) char smem[];
+    Stage<W, CW, KW>& st = *reinterpret_cast<Stage<W, CW, KW>*>(smem);
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), cw = wave % CW, kw = wave / CW;
+    const uint32_t heads = a.seqs * static_cast<uint32_t>(a.n_kv);
+    uint32_t id = blockIdx.x;
+    const uint32_t pair = id % heads;  // (the blocks of a sequence and kv head on as few XCDs as can be)
+    id /= heads;
+    const int split = static_cast<int>(id % a.splits);
+    const uint32_t cb = a.col_blocks - 1 - id / a.splits;  // (the longest rows first)
+    const uint32_t s = pair / a.n_kv;
+    const int kv = static_cast<int>(pair % a.n_kv);
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    const uint32_t ncols = r.count * static_cast<uint32_t>(a.group), c0 = cb * (32 * CW);
+    if (c0 >= ncols) return;
+
+    // this lane's column
+    const uint32_t c = c0 + cw * 32 + col, cc = min(c, ncols - 1);
+    const uint32_t t = cc / a.group, row = r.begin + t;
+    const int head = kv * a.group + static_cast<int>(cc % a.group);
+    const bool on = c < ncols, bad = r.at + t >= a.limit;
+    const uint32_t at = static_cast<uint32_t>(min(r.at, static_cast<uint64_t>(a.limit)));  // keys before the call's rows
+    const uint32_t own = on && !bad ? at + t + 1 : 0;           // (prompt) the keys this column sees
+    // the workgroup's keys, and the wave's
+    const uint32_t t_last = (min(ncols, c0 + 32 * CW) - 1) / a.group;
+    const uint32_t keys = static_cast<uint32_t>(min(r.at + (TREE ? r.count : t_last + 1), static_cast<uint64_t>(a.limit)));
+    const uint32_t wc = c0 + cw * 32;
+    const uint32_t w_last = (min(ncols, wc + 32) - 1) / a.group;
+    const uint32_t wkeys = wc >= ncols ? 0 : min(keys, static_cast<uint32_t>(min(r.at + (TREE ? r.count : w_last + 1), static_cast<uint64_t>(a.limit))));
+    const uint32_t wfull = TREE ? at : wc >= ncols ? 0 : min(keys, at + wc / a.group + 1);  // keys that all its columns see
+    const uint32_t tiles = (keys + kKeys - 1) / kKeys;
+    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits);
+    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits);
+
+    // its query, scaled by its own power of two, dims 16 i + 8 half + (0..7)
+    h8f qh[KI], ql[KI];
+    float qscale;
+    {
+        const float* qp = a.q + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 8;
+        float x[8 * KI];
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            const bool in = W > 32 || 16 * i + half * 8 < a.hd;
+            const float4 u = in ? *reinterpret_cast<const float4*>(qp + 16 * i) : make_float4(0, 0, 0, 0);
+            const float4 w = in ? *reinterpret_cast<const float4*>(qp + 16 * i + 4) : make_float4(0, 0, 0, 0);
+            x[8 * i] = u.x; x[8 * i + 1] = u.y; x[8 * i + 2] = u.z; x[8 * i + 3] = u.w;
+            x[8 * i + 4] = w.x; x[8 * i + 5] = w.y; x[8 * i + 6] = w.z; x[8 * i + 7] = w.w;
+        }
+        uint32_t top = 0;  // (of the finite ones)
+#pragma unroll
+        for (int i = 0; i < 8 * KI; i++) top = mag(x[i]) < kInf ? max(top, mag(x[i])) : top;
+        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        const int e = lift(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])), 126);
+        const float up = pow2f(e);
+        qscale = pow2f(-e) * a.scale;
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t h, l;
+                split2_any(x[8 * i + 2 * j] * up, x[8 * i + 2 * j + 1] * up, h, l);
+                hi[j] = h;
+                lo[j] = l;
+            }
+            qh[i] = __builtin_bit_cast(h8f, hi);
+            ql[i] = __builtin_bit_cast(h8f, lo);
+        }
+    }
+
+    // Staging.  Piece i < WK: 512 / W keys, eight channels a thread; the others: values
+    // of 128 / W quads of keys, two channels a thread.
+    const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
+    const float* kp = a.kc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    const float* vp = a.vc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    float x[PER][8];
+    const auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {  // (the stage's first tile; past the end: its last key)
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int p = wave + i * NW;
+            if (p < WK) {
+                const int k = p * (512 / W) + lane / (W / 8), d = lane % (W / 8) * 8;
+                const float* from = kp + static_cast<size_t>(min(tile * kKeys + k, keys - 1)) * kv_dim + d;
+                const bool in = W > 32 || d < a.hd;
+                const float4 u = in ? *reinterpret_cast<const float4*>(from) : make_float4(0, 0, 0, 0);
+                const float4 w = in ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0, 0, 0, 0);
+                x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
+                x[i][4] = w.x; x[i][5] = w.y; x[i][6] = w.z; x[i][7] = w.w;
+            } else if (p < 2 * WK) {
+                const int q = (p - WK) * (128 / W) + lane / (W / 2), d = lane % (W / 2) * 2;
+                const bool in = W > 32 || d < a.hd;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float* from = vp + static_cast<size_t>(min(tile * kKeys + 4 * q + j, keys - 1)) * kv_dim + d;
+                    const float2 u = in ? *reinterpret_cast<const float2*>(from) : make_float2(0, 0);
+                    x[i][j] = u.x;
+                    x[i][4 + j] = u.y;
+                }
+            }
+        }
+    };
+    const auto stash = [&](int step) __attribute__((always_inline)) {
+        const int buf = step & 1;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int p = wave + i * NW;
+            if (p < WK) {
+                const int k = p * (512 / W) + lane / (W / 8), ch = lane % (W / 8);
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = max(top, mag(x[i][j]));
+                top = group_max<W / 8>(top);
+                u32x4 hi, lo;
+                int e;
+                if (__builtin_expect(__ballot(top >= kInf) != 0, 0)) {
+                    uint32_t fin = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) fin = mag(x[i][j]) < kInf ? max(fin, mag(x[i][j])) : fin;
+                    e = lift(group_max<W / 8>(fin), 126);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t h, l;
+                        split2_any(x[i][2 * j] * pow2f(e), x[i][2 * j + 1] * pow2f(e), h, l);
+                        hi[j] = h;
+                        lo[j] = l;
+                    }
+                } else {
+                    e = lift(top, 126);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t h, l;
+                        split2(x[i][2 * j] * pow2f(e), x[i][2 * j + 1] * pow2f(e), h, l);
+                        hi[j] = h;
+                        lo[j] = l;
+                    }
+                }
+                const int kt = k / kKeys, kk = k % kKeys;
+                *reinterpret_cast<u32x4*>(st.k[buf][kt][ch >> 1][0][(ch & 1) * 32 + kk]) = hi;
+                *reinterpret_cast<u32x4*>(st.k[buf][kt][ch >> 1][1][(ch & 1) * 32 + kk]) = lo;
+                if (ch == 0) st.kdown[buf][kt][kk] = pow2f(-e);
+            } else if (p < 2 * WK) {
+                const int q = (p - WK) * (128 / W) + lane / (W / 2), d = lane % (W / 2) * 2;
+                const int kt = q >> 3, qq = q & 7;
+                float y[8], ex[4], up[4];
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t top = group_max<W / 2>(max(mag(x[i][j]), mag(x[i][4 + j])));
+                    most = max(most, top);
+                    const int e = lift(top, 100);
+                    up[j] = pow2f(e);
+                    ex[j] = static_cast<float>(-e);
+                    y[j] = x[i][j] * up[j];
+                    y[4 + j] = x[i][4 + j] * up[j];
+                }
+                // keys 4 qq .. + 3 are steps 4 jq .. + 3 of lane half hq in product s2
+                const int s2 = qq >> 2, jq = qq >> 1 & 1, hq = qq & 1;
+#pragma unroll
+                for (int ch = 0; ch < 2; ch++) {
+                    u32x2 hi, lo;
+                    uint32_t h, l;
+                    split2(y[4 * ch], y[4 * ch + 1], h, l);
+                    hi[0] = h;
+                    lo[0] = l;
+                    split2(y[4 * ch + 2], y[4 * ch + 3], h, l);
+                    hi[1] = h;
+                    lo[1] = l;
+                    const int dd = d + ch;
+                    *reinterpret_cast<u32x2*>(&st.v[buf][kt][dd >> 5][s2][0][hq * 32 + (dd & 31)][4 * jq]) = hi;
+                    *reinterpret_cast<u32x2*>(&st.v[buf][kt][dd >> 5][s2][1][hq * 32 + (dd & 31)][4 * jq]) = lo;
+                }
+                if (d == 0) {
+                    *reinterpret_cast<float4*>(&st.vexp[buf][kt][4 * qq]) = make_float4(ex[0], ex[1], ex[2], ex[3]);
+                    *reinterpret_cast<float4*>(&st.vup[buf][kt][4 * qq]) = make_float4(up[0], up[1], up[2], up[3]);
+                }
+                if (__builtin_expect(most >= kInf, 0)) st.unsafe[step % 3][kt] = 1;
+            }
+        }
+    };
+
+    float base = -FLT_MAX, l = 0.0f;
+    f32x16 o[OT];
+#pragma unroll
+    for (int d = 0; d < OT; d++) o[d] = f32x16{};
+    const int steps = static_cast<int>((tile1 - tile0 + KW - 1) / KW);
+    if (threadIdx.x < 3 * KW) st.unsafe[threadIdx.x / KW][threadIdx.x % KW] = 0;
+    if (steps > 0) fetch(tile0);
+    __syncthreads();
+    if (steps > 0) stash(0);
+    __syncthreads();
+    for (int step = 0; step < steps; step++) {
+        const uint32_t first = tile0 + step * KW, tile = first + kw, k0 = tile * kKeys;
+        const int buf = step & 1;
+        if (step + 1 < steps) fetch(first + KW);
+        const bool vbad = st.unsafe[step % 3][kw] != 0;
+        if (threadIdx.x < KW) st.unsafe[(step + 2) % 3][threadIdx.x] = 0;  // (read at step - 1, written next at step + 1)
+        if (tile < tile1 && k0 < wkeys) {
+            f32x16 sacc = f32x16{};
+#pragma unroll
+            for (int i = 0; i < KI; i++) {
+                const h8f kh = *reinterpret_cast<const h8f*>(st.k[buf][kw][i][0][lane]);
+                const h8f kl = *reinterpret_cast<const h8f*>(st.k[buf][kw][i][1][lane]);
+                sacc = mfma(kl, qh[i], sacc);
+                sacc = mfma(kh, ql[i], sacc);
+                sacc = mfma(kh, qh[i], sacc);
+            }
+            float u[16], up[16];
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const float4 kd = *reinterpret_cast<const float4*>(&st.kdown[buf][kw][8 * b + 4 * half]);
+                const float4 ve = *reinterpret_cast<const float4*>(&st.vexp[buf][kw][8 * b + 4 * half]);
+                const float4 vu = *reinterpret_cast<const float4*>(&st.vup[buf][kw][8 * b + 4 * half]);
+                u[4 * b] = fmaf(sacc[4 * b] * kd.x, qscale, ve.x);
+                u[4 * b + 1] = fmaf(sacc[4 * b + 1] * kd.y, qscale, ve.y);
+                u[4 * b + 2] = fmaf(sacc[4 * b + 2] * kd.z, qscale, ve.z);
+                u[4 * b + 3] = fmaf(sacc[4 * b + 3] * kd.w, qscale, ve.w);
+                up[4 * b] = vu.x; up[4 * b + 1] = vu.y; up[4 * b + 2] = vu.z; up[4 * b + 3] = vu.w;
+            }
+            uint32_t seen = ~0u;  // the tile's keys that this column sees
+            if (k0 + kKeys > wfull) {
+                if constexpr (TREE) {
+                    const uint32_t* path = a.seen + static_cast<size_t>(row) * a.words;
+                    const auto word = [&](uint32_t w) { return w < static_cast<uint32_t>(a.words) ? path[w] : 0u; };
+                    if (k0 >= at) {
+                        const uint32_t n = k0 - at, sh = n & 31;
+                        seen = word(n >> 5) >> sh | (sh ? word((n >> 5) + 1) << (32 - sh) : 0u);
+                    } else {
+                        seen = at - k0 >= 32 ? ~0u : word(0) << (at - k0) | ((1u << (at - k0)) - 1);
+                    }
+                    seen = on && !bad ? seen : 0u;
+                    if (keys - k0 < 32) seen &= (1u << (keys - k0)) - 1;
+                } else {
+                    seen = own > k0 ? (own - k0 >= 32 ? ~0u : (1u << (own - k0)) - 1) : 0u;
+                }
+#pragma unroll
+                for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = fmaxf(top, u[v]);
+            // Weights lie at 2^10 of the largest so far, and up to 2^14 before the sums are
+            // brought to a new one: their lower terms stay normal numbers of f16 far below it.
+            if (__any(top > base + 14.0f)) {
+                const float m = fmaxf(base == -FLT_MAX ? -FLT_MAX : base + 10.0f, max_halves(top));
+                const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, f = __builtin_amdgcn_exp2f(base - nb);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < OT; d++) o[d] *= f;
+                base = nb;
+            }
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                u[v] = __builtin_amdgcn_exp2f(u[v] - base);
+                up[v] *= u[v];
+                l += up[v];
+            }
+            if (!vbad) {
+#pragma unroll
+                for (int s2 = 0; s2 < 2; s2++) {
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t h, lw;
+                        split2(u[8 * s2 + 2 * j], u[8 * s2 + 2 * j + 1], h, lw);
+                        hi[j] = h;
+                        lo[j] = lw;
+                    }
+                    const h8f ph = __builtin_bit_cast(h8f, hi), pl = __builtin_bit_cast(h8f, lo);
+#pragma unroll
+                    for (int d = 0; d < OT; d++) {
+                        const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][lane]);
+                        const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][lane]);
+                        o[d] = mfma(vl, ph, o[d]);
+                        o[d] = mfma(vh, pl, o[d]);
+                        o[d] = mfma(vh, ph, o[d]);
+                    }
+                }
+            } else {
+                // (a value that is not finite reaches the rows that see it and no others: on the vector units)
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, up[v]),
+                                                                     __builtin_bit_cast(uint32_t, up[v]), false, false);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {  // (lanes 0 .. 31's in sw[0], of both halves; 32 .. 63's in sw[1])
+                        const int j = acc_row(v, e);
+                        const float p = __builtin_bit_cast(float, static_cast<uint32_t>(sw[e]));
+                        if (k0 + j < keys && (seen >> j & 1)) {
+                            const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim;
+#pragma unroll
+                            for (int d = 0; d < OT; d++)
+#pragma unroll
+                                for (int w = 0; w < 16; w++) {
+                                    const int dim = 32 * d + acc_row(w, half);
+                                    if (W > 32 || dim < a.hd) o[d][w] += p * from[dim];
+                                }
+                        }
+                    }
+                }
+            }
+        }
+        if (step + 1 < steps) stash(step + 1);
+        __syncthreads();
+    }
+    l = sum_halves(l);
+
+    constexpr int PL = 1 + 8 * OT;  // float2s of a lane's sums
+    if constexpr (KW > 1) {
+        // the waves' sums, in order, through the stage's LDS (every wave is past its last read of it)
+        static_assert(sizeof(Stage<W, CW, KW>) >= (KW - 1) * CW * PL * 64 * sizeof(float2), "the sums fit");
+        float2* mine = reinterpret_cast<float2*>(smem) + lane;
+        if (kw > 0) {
+            float2* to = mine + ((kw - 1) * CW + cw) * (PL * 64);
+            to[0] = make_float2(base, l);
+#pragma unroll
+            for (int d = 0; d < OT; d++)
+#pragma unroll
+                for (int w = 0; w < 8; w++) to[(1 + 8 * d + w) * 64] = make_float2(o[d][2 * w], o[d][2 * w + 1]);
+        }
+        __syncthreads();
+        if (kw == 0)
+#pragma unroll
+            for (int k = 1; k < KW; k++) {
+                const float2* from = mine + ((k - 1) * CW + cw) * (PL * 64);
+                const float2 b = from[0];
+                const float nb = fmaxf(base, b.x), f0 = __builtin_amdgcn_exp2f(base - nb), f1 = __builtin_amdgcn_exp2f(b.x - nb);
+                l = l * f0 + b.y * f1;
+#pragma unroll
+                for (int d = 0; d < OT; d++)
+#pragma unroll
+                    for (int w = 0; w < 8; w++) {
+                        const float2 y = from[(1 + 8 * d + w) * 64];
+                        o[d][2 * w] = o[d][2 * w] * f0 + y.x * f1;
+                        o[d][2 * w + 1] = o[d][2 * w + 1] * f0 + y.y * f1;
+                    }
+                base = nb;
+            }
+    }
+    if (a.splits > 1) {
+        // the last of a block's workgroups joins all shares, in order
+        const uint32_t unit = pair + heads * cb;
+        float2* part = a.part + (static_cast<size_t>(unit) * a.splits * CW + cw) * (PL * 64) + lane;
+        if (kw == 0) {
+            float2* to = part + static_cast<size_t>(split) * CW * (PL * 64);
+            store_part(to, make_float2(base, l));
+#pragma unroll
+            for (int d = 0; d < OT; d++)
+#pragma unroll
+                for (int w = 0; w < 8; w++) store_part(to + (1 + 8 * d + w) * 64, make_float2(o[d][2 * w], o[d][2 * w + 1]));
+        }
+        // Every thread's coherent stores complete before the arrival count moves.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __shared__ int last;
+        __syncthreads();
+        if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (kw == 0) {
+            base = -FLT_MAX;
+            l = 0.0f;
+#pragma unroll
+            for (int d = 0; d < OT; d++) o[d] = f32x16{};
+            for (int k = 0; k < a.splits; k++) {
+                const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
+                float2 y[PL];
+#pragma unroll
+                for (int i = 0; i < PL; i++) y[i] = load_part(from + i * 64);
+                const float nb = fmaxf(base, y[0].x), f0 = __builtin_amdgcn_exp2f(base - nb), f1 = __builtin_amdgcn_exp2f(y[0].x - nb);
+                l = l * f0 + y[0].y * f1;
+#pragma unroll
+                for (int d = 0; d < OT; d++)
+#pragma unroll
+                    for (int w = 0; w < 8; w++) {
+                        o[d][2 * w] = o[d][2 * w] * f0 + y[1 + 8 * d + w].x * f1;
+                        o[d][2 * w + 1] = o[d][2 * w + 1] * f0 + y[1 + 8 * d + w].y * f1;
+                    }
+                base = nb;
+            }
+        }
+    }
+    if (kw != 0 || !on) return;
+    float* out = a.out + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 4;
+    const float f = bad ? __builtin_nanf("") : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < OT; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            if (W == 32 && 8 * b + half * 4 >= a.hd) continue;
+            *reinterpret_cast<float4*>(out + 32 * d + 8 * b) =
+                make_float4(o[d][4 * b] * f, o[d][4 * b + 1] * f, o[d][4 * b + 2] * f, o[d][4 * b + 3] * f);
+        }
+}
+
+constexpr size_t kUnits = 8192;  // column blocks whose keys may be split
+
+template <int W, int CW, int KW, bool TREE>
+int launch_rows(fh_ctx* ctx, const RowsArgs& a) {
+    constexpr size_t lds = sizeof(Stage<W, CW, KW>);
+    static_assert(lds <= 160 * 1024, "a stage fits the LDS");
+    const auto kern = k_gqa_rows<W, CW, KW, TREE>;
+    if (lds > 64 * 1024)
+        FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.splits * a.col_blocks)), dim3(64 * CW * KW), lds,
+                       ctx->stream, a);
+    FH_HIP(ctx, hipGetLastError());
+    return FH_OK;
+}
+
+template <int W, bool TREE>
+int launch_width(fh_ctx* ctx, const RowsArgs& a, int cw) {
+    if (cw == 8) return launch_rows<W, 8, 1, TREE>(ctx, a);
+    if (cw == 4) return launch_rows<W, 4, 1, TREE>(ctx, a);
+    if constexpr (W == 128) return launch_rows<W, 2, 1, TREE>(ctx, a);
+    else return launch_rows<W, 2, 2, TREE>(ctx, a);
+}
+
+}  // namespace
+
+int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
+    const size_t group = g.n_heads / g.n_kv, cols = g.max_rows * group, heads = g.seqs * g.n_kv;
+    const int words = g.parent ? static_cast<int>((g.max_rows + 31) / 32) : 0;
+    const int w = g.hd <= 32 ? 32 : static_cast<int>(g.hd);
+    const int cw = cols > 128 ? 8 : cols > 64 ? 4 : 2;
+    const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
+    if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
+    // Keys of few columns are dealt over several workgroups, four tiles of keys each at least.
+    const size_t cus = static_cast<size_t>(ctx->num_cus), tiles = (g.limit + kKeys - 1) / kKeys;
+    size_t splits = 1;
+    while (splits < 64 && heads * blocks * splits * 2 <= cus && splits * 2 * 4 <= tiles) splits *= 2;
+    if (heads * blocks > kUnits) splits = 1;
+    unsigned* counters = nullptr;
+    if (splits > 1) {
+        void* area = nullptr;
+        const int rc = fh_gqa_counters(ctx, kUnits * sizeof(unsigned), &area);
+        if (rc) return rc;
+        counters = static_cast<unsigned*>(area);
+    }
+    const size_t q_bytes = fh_align256(g.total * g.n_heads * g.hd * sizeof(float));
+    const size_t seen_bytes = fh_align256(g.total * words * sizeof(uint32_t));
+    const size_t part = splits > 1 ? heads * blocks * splits * cw * (1 + w / 4) * 64 * sizeof(float2) : 0;
+    void* room = nullptr;
+    const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + part, &room);
+    if (rc) return rc;
+
+    AppendArgs p{};
+    p.qkv = g.qkv;
+    p.ld = g.ld;
+    p.kc = g.k_cache;
+    p.vc = g.v_cache;
+    p.seq_stride = g.capacity * g.n_kv * g.hd;
+    p.n_heads = static_cast<int>(g.n_heads);
+    p.n_kv = static_cast<int>(g.n_kv);
+    p.hd = static_cast<int>(g.hd);
+    p.seqs = static_cast<uint32_t>(g.seqs);
+    p.total = static_cast<uint32_t>(g.total);
+    p.max_rows = static_cast<uint32_t>(g.max_rows);
+    p.limit = static_cast<uint32_t>(g.limit);
+    p.off = g.off;
+    p.len = g.len;
+    p.pos = g.pos;
+    p.parent = g.parent;
+    p.q = static_cast<float*>(room);
+    p.seen = reinterpret_cast<uint32_t*>(static_cast<char*>(room) + q_bytes);
+    p.words = words;
+    p.rope_dim = static_cast<int>(g.rope_dim);
+    p.neox = g.rope_type == FH_ROPE_NEOX;
+    p.linear = g.linear_factor;
+    p.ff = g.freq_factors;
+    // (the frequencies as fh_rope_async forms them: in 64 bits, then rounded)
+    for (size_t i = 0; i < g.rope_dim / 2; i++)
+        p.freq[i] = static_cast<float>(std::pow(static_cast<double>(g.base), -2.0 * static_cast<double>(i) / static_cast<double>(g.rope_dim)));
+    const size_t each = 2 * kThreads / g.hd, row_blocks = (g.max_rows + each - 1) / each, all = g.n_heads + 2 * g.n_kv;
+    size_t chunks = 1;
+    while (chunks < all && row_blocks * g.seqs * chunks < 4 * cus) chunks *= 2;
+    p.heads_each = static_cast<int>((all + chunks - 1) / chunks);
+    p.chunks = static_cast<int>((all + p.heads_each - 1) / p.heads_each);
+    const dim3 grid(static_cast<unsigned>(row_blocks * p.chunks), static_cast<unsigned>(g.seqs));
+    if (g.parent) hipLaunchKernelGGL(k_gqa_append<true>, grid, dim3(kThreads), 0, ctx->stream, p);
+    else hipLaunchKernelGGL(k_gqa_append<false>, grid, dim3(kThreads), 0, ctx->stream, p);
+    FH_HIP(ctx, hipGetLastError());
+
+    RowsArgs a{};
+    a.q = p.q;
+    a.kc = g.k_cache;
+    a.vc = g.v_cache;
+    a.seq_stride = p.seq_stride;
+    a.n_heads = p.n_heads;
+    a.n_kv = p.n_kv;
+    a.group = static_cast<int>(group);
+    a.hd = p.hd;
+    a.seqs = p.seqs;
+    a.total = p.total;
+    a.max_rows = p.max_rows;
+    a.limit = p.limit;
+    a.off = g.off;
+    a.len = g.len;
+    a.seen = p.seen;
+    a.words = words;
+    a.scale = kLog2e / sqrtf(static_cast<float>(g.hd));
+    a.out = g.out;
+    a.col_blocks = static_cast<int>(blocks);
+    a.splits = static_cast<int>(splits);
+    a.part = reinterpret_cast<float2*>(static_cast<char*>(room) + q_bytes + seen_bytes);
+    a.counters = counters;
+    if (g.parent) return w == 32 ? launch_width<32, true>(ctx, a, cw) : w == 64 ? launch_width<64, true>(ctx, a, cw) : launch_width<128, true>(ctx, a, cw);
+    return w == 32 ? launch_width<32, false>(ctx, a, cw) : w == 64 ? launch_width<64, false>(ctx, a, cw) : launch_width<128, false>(ctx, a, cw);
+}
+
+// ---- what is accepted of a tree ------------------------------------------------------------
+
+namespace {
+
+struct AcceptArgs {
+    const uint32_t *parent, *tokens, *chosen, *off, *len;
+    uint32_t seqs, total, max_rows;
+    uint32_t *path, *count, *next, *new_len;
+    const uint64_t* planes;
+    size_t kv_dim, capacity;
+};
+
+// A workgroup a sequence: every row finds out whether it is the first that continues its parent
+// with the token chosen there, then one thread follows them from row 0.
+__global__ void __launch_bounds__(kThreads) k_tree_walk(AcceptArgs a) {
+    __shared__ uint32_t up[kMaxTree], child[kMaxTree], way[kMaxTree];
+    __shared__ uint32_t steps;
+    const uint32_t s = blockIdx.x;
+    const Rows r = rows_of(a.off, nullptr, a.total, a.max_rows, a.seqs, s);
+    const uint32_t len = a.len ? a.len[s] : 0;
+    for (uint32_t t = threadIdx.x; t < r.count; t += kThreads) {
+        const uint32_t p = a.parent[r.begin + t];
+        up[t] = p < t && a.tokens[r.begin + t] == a.chosen[r.begin + p] ? p : ~0u;
+        child[t] = ~0u;
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < r.count; t += kThreads)
+        if (up[t] != ~0u) atomicMin(&child[up[t]], t);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t n = 0;
+        for (uint32_t t = 0; t < r.count; t = child[t]) way[n++] = t;  // (rows of a path rise; ~0 ends it)
+        steps = n;
+    }
+    __syncthreads();
+    const uint32_t n = steps;
+    for (uint32_t t = threadIdx.x; t < r.count; t += kThreads) a.path[r.begin + t] = t < n ? way[t] : ~0u;
+    if (threadIdx.x == 0) {
+        a.count[s] = n;
+        if (n) a.next[s] = a.chosen[r.begin + way[n - 1]];
+        a.new_len[s] = len + n;
+    }
+}
+
+// A workgroup a sequence and plane: its accepted rows, each to its place, in order (a row
+// moves down only, so what it overwrites has moved before or is left behind).
+__global__ void __launch_bounds__(kThreads) k_tree_move(AcceptArgs a) {
+    const uint32_t s = blockIdx.x;
+    const Rows r = rows_of(a.off, nullptr, a.total, a.max_rows, a.seqs, s);
+    const uint32_t n = min(a.count[s], r.count);
+    const uint64_t at = a.new_len[s] - a.count[s];
+    float* plane = reinterpret_cast<float*>(a.planes[blockIdx.y]) + static_cast<size_t>(s) * a.capacity * a.kv_dim;
+    for (size_t c = threadIdx.x; c < a.kv_dim; c += kThreads)
+        for (uint32_t i = 1; i < n; i++) {
+            const uint32_t p = a.path[r.begin + i];
+            if (p != i && at + p < a.capacity) plane[(at + i) * a.kv_dim + c] = plane[(at + p) * a.kv_dim + c];
+        }
+}
+
+}  // namespace
+
+int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* tokens, const uint32_t* chosen, size_t total,
+                          const uint32_t* off, size_t seqs, size_t max_rows, const uint32_t* len, const uint64_t* planes,
+                          size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
+                          uint32_t* new_len) {
+    AcceptArgs a{parent, tokens, chosen, off, len, static_cast<uint32_t>(seqs), static_cast<uint32_t>(total),
+                 static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, kv_dim, capacity};
+    hipLaunchKernelGGL(k_tree_walk, dim3(a.seqs), dim3(kThreads), 0, ctx->stream, a);
+    FH_HIP(ctx, hipGetLastError());
+    if (n_planes == 0 || max_rows < 2) return FH_OK;
+    hipLaunchKernelGGL(k_tree_move, dim3(a.seqs, static_cast<unsigned>(n_planes)), dim3(kThreads), 0, ctx->stream, a);
+    FH_HIP(ctx, hipGetLastError());
+    return FH_OK;
+}

@@ -42,12 +42,17 @@ struct fh_ctx {
     // sums of keys split over workgroups.  Allocated once, at its only size.
     void* kv4 = nullptr;
     size_t kv4_bytes = 0;
-    // Room for its other calls (evicted rows' indices, a prompt's partial weights).
+    // Room for its other calls (evicted rows' indices, a prompt's partial weights) and for
+    // fh_gqa.hip's (rotated queries, paths of a tree's nodes, partial sums).
     // Grows to at least twice its size, and what it grows out of is kept until the
     // context ends: a graph that was captured with it may still be replayed.
     void* kv4_room = nullptr;
     size_t kv4_room_bytes = 0;
     std::vector<void*> kv4_old;
+    // Arrival counters (left at zero) of fh_gqa.hip's keys split over workgroups.
+    // Allocated once, at their only size; its other room is kv4_room.
+    void* gqa = nullptr;
+    size_t gqa_bytes = 0;
     // Grow-on-demand activation staging (a LayerNorm output feeding a
     // linear), separate from ws, which the linear itself may use.
     void* act = nullptr;
@@ -128,6 +133,8 @@ int fh_counter_area(fh_ctx* ctx, size_t bytes, void** out);
 int fh_kv4_area(fh_ctx* ctx, size_t bytes, void** out);
 // Make sure ctx->kv4_room holds at least `bytes`; refused under capture where it must grow.
 int fh_kv4_room(fh_ctx* ctx, size_t bytes, void** out);
+// The same for ctx->gqa.
+int fh_gqa_counters(fh_ctx* ctx, size_t bytes, void** out);
 // Round up to a multiple of 256 bytes.
 static inline size_t fh_align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -261,6 +268,27 @@ int fh_launch_kv4_weigh(fh_ctx* ctx, const fh_kv4_cache& c, const float* q, size
 int fh_launch_kv4_read(fh_ctx* ctx, const fh_kv4_cache& c, const uint32_t* first, size_t rows, float* k, float* v);
 int fh_launch_kv4_evict(fh_ctx* ctx, const fh_kv4_cache& src, const fh_kv4_cache& dst, const uint32_t* len,
                         size_t max_len, size_t keep, size_t recent, uint32_t* new_len);
+// Many rows of a sequence over its f32 cache (fh_gqa.hip), arguments as the entry points'
+// and checked there; limit: the capacity, cut to max_keys; parent: NULL for a prompt.
+struct fh_gqa_call {
+    const float* qkv;
+    size_t ld, total, n_heads, n_kv, hd;
+    float *k_cache, *v_cache;
+    size_t seqs, capacity, limit, max_rows;
+    const uint32_t *off, *len, *parent, *pos;
+    size_t rope_dim;
+    float base;
+    int rope_type;
+    const float* freq_factors;
+    float linear_factor;
+    float* out;
+};
+int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g);
+int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* tokens, const uint32_t* chosen, size_t total,
+                          const uint32_t* off, size_t seqs, size_t max_rows, const uint32_t* len, const uint64_t* planes,
+                          size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
+                          uint32_t* new_len);
+int fh_launch_logits_edit(fh_ctx* ctx, const float* logits, size_t rows, size_t vocab, const fh_logits_edit& e, float* out);
 int fh_launch_dequant(fh_ctx* ctx, const uint8_t* raw, size_t n, float* out);
 int fh_launch_block_dots(fh_ctx* ctx, const fh_q8_0* w, const int8_t* qx, size_t m,
                          int32_t* dots);

@@ -51,6 +51,8 @@ EXPORTS = (
     "fh_q8_0_linear_residual_async", "fh_q8_0_linear_normed_async",
     "fh_gpt2_stack_create", "fh_gpt2_stack_free", "fh_gpt2_stack_forward_async",
     "fh_rmsnorm_async", "fh_rope_async", "fh_gqa_attention_decode_async", "fh_gqa_attention_rope_decode_async",
+    "fh_gqa_attention_rope_prefill_async", "fh_gqa_attention_rope_tree_async", "fh_tree_accept_async",
+    "fh_logits_edit_async",
     "fh_swiglu_async", "fh_embed_rows_async",
     "fh_embed_rows_pos_async",
     "fh_gguf_open", "fh_gguf_close", "fh_gguf_error", "fh_gguf_version", "fh_gguf_tensor_count", "fh_gguf_find_tensor",
@@ -172,6 +174,27 @@ class AttnScore(C.Structure):
         self.tensors = (slopes, pos, first, end)
 
 
+class LogitsEdit(C.Structure):
+    """fh_logits_edit: what logits_edit_async does to each row's logits, every part
+    nullable (include/ferrum_hip.h has the order and the formulas).  recent, ranges
+    [rows, 2]: each row's list of ids; repetition, frequency, presence [rows]; tokens,
+    parent [rows] of drafted trees, `seqs` sequences with rows off[s] .. off[s + 1] - 1 (off
+    None: equal parts); bias_off [rows + 1], bias_id, bias; mask [masks, ceil(vocab / 32)]
+    bits of the ids that stay, mask_of [rows] (None: row r's is mask r).  Integers are
+    32-bit.  Tensors are kept alive here."""
+
+    _FIELDS = ("recent", "ranges", "repetition", "frequency", "presence", "parent", "tokens", "off", "seqs", "bias_off",
+               "bias_id", "bias", "mask", "mask_of", "masks")
+    _fields_ = [(n, C.c_size_t if n in ("seqs", "masks") else C.c_void_p) for n in _FIELDS]
+
+    def __init__(self, recent=None, ranges=None, repetition=None, frequency=None, presence=None, parent=None, tokens=None,
+                 off=None, seqs: int = 0, bias_off=None, bias_id=None, bias=None, mask=None, mask_of=None, masks: int = 0):
+        values = (recent, ranges, repetition, frequency, presence, parent, tokens, off, int(seqs), bias_off, bias_id, bias,
+                  mask, mask_of, int(masks))
+        super().__init__(*(v if n in ("seqs", "masks") else _ptr(v) for n, v in zip(self._FIELDS, values)))
+        self.tensors = values
+
+
 _lib = None
 _Tensor = None  # torch.Tensor, once torch is there
 
@@ -287,6 +310,12 @@ def lib():
         L.fh_kv4_weigh_async.argtypes = [vp, kv, vp, sz, sz, sz, vp, sz, vp, sz, sc, vp]
         L.fh_kv4_evict_async.argtypes = [vp, kv, kv, vp, sz, sz, sz, vp]
         L.fh_kv4_read_async.argtypes = [vp, kv, vp, sz, vp, vp]
+        rows = [vp, vp, sz, sz, sz, sz, sz, vp, vp, sz, sz, vp, sz, vp, sz]
+        turn = [sz, f32, i32, vp, f32, vp]
+        L.fh_gqa_attention_rope_prefill_async.argtypes = rows + [vp] + turn
+        L.fh_gqa_attention_rope_tree_async.argtypes = rows + [vp, vp] + turn
+        L.fh_tree_accept_async.argtypes = [vp, vp, vp, vp, sz, vp, sz, sz, vp, vp, sz, sz, sz, vp, vp, vp, vp]
+        L.fh_logits_edit_async.argtypes = [vp, vp, sz, sz, C.POINTER(LogitsEdit), vp]
         _lib = L
     return _lib
 
@@ -1159,6 +1188,52 @@ def gqa_attention_rope_decode_async(ctx: Context, qkv, ld: int, rows: int, n_hea
                                                        _ptr(k_cache), _ptr(v_cache), capacity, _ptr(pos), max_pos,
                                                        rope_dim, base, rope_type, _ptr(freq_factors), linear_factor,
                                                        _ptr(out)))
+
+
+def gqa_attention_rope_prefill_async(ctx: Context, qkv, ld: int, total: int, n_heads: int, n_kv: int, head_dim: int,
+                                     k_cache, v_cache, seqs: int, capacity: int, off, max_rows: int, len_,
+                                     max_keys: int, pos, rope_dim: int, base: float, rope_type: int, freq_factors,
+                                     linear_factor: float, out):
+    """Prompts at once over f32 caches: `total` rows of q|k|v, sequence s's at off[s] ..
+    off[s + 1] - 1 (off None: total / seqs each), rotated (rope_dim > 0) at pos (None:
+    the cache row), k and v stored at cache rows len_[s] + t, each row attending over
+    its sequence's rows up to its own.  max_keys bounds the cache rows in use, the
+    call's own included."""
+    ctx.check(lib().fh_gqa_attention_rope_prefill_async(ctx.h, _ptr(qkv), ld, total, n_heads, n_kv, head_dim,
+                                                        _ptr(k_cache), _ptr(v_cache), seqs, capacity, _ptr(off),
+                                                        max_rows, _ptr(len_), max_keys, _ptr(pos), rope_dim, base,
+                                                        rope_type, _ptr(freq_factors), linear_factor, _ptr(out)))
+
+
+def gqa_attention_rope_tree_async(ctx: Context, qkv, ld: int, total: int, n_heads: int, n_kv: int, head_dim: int,
+                                  k_cache, v_cache, seqs: int, capacity: int, off, max_rows: int, len_, max_keys: int,
+                                  parent, pos, rope_dim: int, base: float, rope_type: int, freq_factors,
+                                  linear_factor: float, out):
+    """The same for a tree of drafted tokens over each sequence's cache: parent[r] is
+    the row of its sequence that row r continues (-1: none), and a row sees the cache
+    before the call's rows, the rows on its path and itself; pos None: len_ + the rows
+    on its path."""
+    ctx.check(lib().fh_gqa_attention_rope_tree_async(ctx.h, _ptr(qkv), ld, total, n_heads, n_kv, head_dim,
+                                                     _ptr(k_cache), _ptr(v_cache), seqs, capacity, _ptr(off), max_rows,
+                                                     _ptr(len_), max_keys, _ptr(parent), _ptr(pos), rope_dim, base,
+                                                     rope_type, _ptr(freq_factors), linear_factor, _ptr(out)))
+
+
+def tree_accept_async(ctx: Context, parent, tokens, chosen, total: int, off, seqs: int, max_rows: int, len_, planes,
+                      n_planes: int, kv_dim: int, capacity: int, path, count, next_, new_len):
+    """Follows each sequence's tree from its row 0 along the drafted tokens that the model
+    chose itself (chosen [total]): path [total] (-1 behind the last), count, next_ (the id
+    chosen behind it) and new_len [seqs]; the accepted rows move together in the caches
+    whose device addresses planes (int64) holds."""
+    ctx.check(lib().fh_tree_accept_async(ctx.h, _ptr(parent), _ptr(tokens), _ptr(chosen), total, _ptr(off), seqs, max_rows,
+                                         _ptr(len_), _ptr(planes), n_planes, kv_dim, capacity, _ptr(path), _ptr(count),
+                                         _ptr(next_), _ptr(new_len)))
+
+
+def logits_edit_async(ctx: Context, logits, rows: int, vocab: int, edit: LogitsEdit, out):
+    """Penalties, biases and masks on rows of logits before they are sampled; out may be
+    logits."""
+    ctx.check(lib().fh_logits_edit_async(ctx.h, _ptr(logits), rows, vocab, edit, _ptr(out)))
 
 
 def kv4_append_async(ctx: Context, cache: KV4Cache, qkv, ld: int, total: int, n_heads: int, off, max_rows: int, len_,

@@ -61,6 +61,26 @@ pub mod sys {
         pub head_dim: usize,
         pub capacity: usize,
     }
+    /// What `fh_logits_edit_async` does to each row's logits (every pointer may be null).
+    #[repr(C)]
+    #[derive(Clone, Copy)]
+    pub struct fh_logits_edit {
+        pub d_recent: *const u32,
+        pub d_ranges: *const u32,
+        pub d_repetition: *const f32,
+        pub d_frequency: *const f32,
+        pub d_presence: *const f32,
+        pub d_parent: *const u32,
+        pub d_tokens: *const u32,
+        pub d_off: *const u32,
+        pub seqs: usize,
+        pub d_bias_off: *const u32,
+        pub d_bias_id: *const u32,
+        pub d_bias: *const f32,
+        pub d_mask: *const u32,
+        pub d_mask_of: *const u32,
+        pub masks: usize,
+    }
     /// Score options of `fh_kv4_attention_async`.
     #[repr(C)]
     #[derive(Clone, Copy)]
@@ -170,6 +190,10 @@ pub mod sys {
         pub fn fh_rope_async(ctx: *mut fh_ctx, d_x: *mut f32, rows: usize, ld: usize, n_heads: usize, head_dim: usize, rope_dim: usize, d_pos: *const u32, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32) -> c_int;
         pub fn fh_gqa_attention_decode_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, rows: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, capacity: usize, d_pos: *const u32, max_pos: usize, d_out: *mut f32) -> c_int;
         pub fn fh_gqa_attention_rope_decode_async(ctx: *mut fh_ctx, d_qkv: *mut f32, ld: usize, rows: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, capacity: usize, d_pos: *const u32, max_pos: usize, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
+        pub fn fh_gqa_attention_rope_prefill_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, seqs: usize, capacity: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
+        pub fn fh_gqa_attention_rope_tree_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, seqs: usize, capacity: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, d_parent: *const u32, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
+        pub fn fh_tree_accept_async(ctx: *mut fh_ctx, d_parent: *const u32, d_tokens: *const u32, d_chosen: *const u32, total: usize, d_off: *const u32, seqs: usize, max_rows: usize, d_len: *const u32, d_planes: *const u64, n_planes: usize, kv_dim: usize, capacity: usize, d_path: *mut u32, d_count: *mut u32, d_next: *mut u32, d_new_len: *mut u32) -> c_int;
+        pub fn fh_logits_edit_async(ctx: *mut fh_ctx, d_logits: *const f32, rows: usize, vocab: usize, edit: *const fh_logits_edit, d_out: *mut f32) -> c_int;
         pub fn fh_kv4_append_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_q: *mut f32) -> c_int;
         pub fn fh_kv4_attention_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_q: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, score: *const fh_attn_score, d_out: *mut f32, d_lse: *mut f32) -> c_int;
         pub fn fh_kv4_weigh_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_q: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, score: *const fh_attn_score, d_lse: *const f32) -> c_int;

@@ -546,6 +546,104 @@ int fh_kv4_evict_async(fh_ctx* ctx, const fh_kv4_cache* src, const fh_kv4_cache*
 int fh_kv4_read_async(fh_ctx* ctx, const fh_kv4_cache* cache, const uint32_t* d_first, size_t rows, float* d_k,
                       float* d_v);
 
+/* ---- many rows of a sequence at once over its f32 cache ----------------------------
+ * Attention::forward_one (llm.rs:285-358) feeds a prompt's positions one by one, as
+ * fh_gqa_attention_rope_decode_async does for many sequences.  Here a call has any
+ * number of rows of each sequence: prompts of different lengths, or a tree of drafted
+ * tokens over each sequence's cache, with what is accepted of it (no reference
+ * counterpart for the trees).
+ *
+ * `total` rows of d_qkv ([q (n_heads heads) | k (n_kv) | v (n_kv)] at r * ld, left as they
+ * are) belong to `seqs` sequences: rows d_off[s] .. d_off[s + 1] - 1 to sequence s (d_off
+ * [seqs + 1], at most max_rows rows each; rows past that and rows outside all sequences
+ * are left as they are), or with d_off NULL total / seqs to each, in order.  d_len [seqs]
+ * (NULL: 0) is the number of cache rows in use before them: row t of sequence s is
+ * cache row d_len[s] + t of its caches at d_k_cache / d_v_cache + s * capacity * n_kv *
+ * head_dim ([capacity, n_kv * head_dim] each).  The calls rotate q and k as
+ * fh_rope_async does (rope_dim 0: not at all) at position d_pos[r], store k and v, and
+ * attend: query head h with kv head h / (n_heads / n_kv), scale 1 / sqrt(head_dim).
+ * d_out is [total, n_heads * head_dim].  max_keys bounds the cache rows in use after the
+ * call's (it sizes the launch); a row whose cache row is at or past max_keys or the capacity
+ * gets NaN and is not stored.  Positions are below 2^31.
+ *
+ * head_dim 8, 16, 32, 64 or 128, else FH_ERR_LIMIT; caches and d_out 16-byte aligned.
+ * Within 1e-5 of float64 over the same rotated rows, against each output's sum of
+ * weight * the value row's largest magnitude (operands as two f16 terms under a power of
+ * two of each row's own: value rows from 2^-86 to 2^27 may be mixed freely).  A key or
+ * value that is not finite reaches the rows that see it and no others.  Errors otherwise
+ * as fh_gqa_attention_rope_decode_async's.  The context's workspace for these calls grows
+ * outside graph capture only and is never freed before the context ends, so captured
+ * graphs stay valid; calls of one context must not overlap, replayed graphs included. */
+/* Prompts: row t sees cache rows 0 .. d_len[s] + t.  d_pos NULL: the cache row. */
+int fh_gqa_attention_rope_prefill_async(fh_ctx* ctx, const float* d_qkv, size_t ld, size_t total, size_t n_heads,
+                                        size_t n_kv, size_t head_dim, float* d_k_cache, float* d_v_cache, size_t seqs,
+                                        size_t capacity, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                                        size_t max_keys, const uint32_t* d_pos, size_t rope_dim, float base,
+                                        int rope_type, const float* d_freq_factors, float linear_factor, float* d_out);
+/* Trees: d_parent[r] is the row within its sequence that row r continues, one before it
+ * (anything else: none, such as 0xFFFFFFFF); a row sees cache rows 0 .. d_len[s] - 1, the
+ * rows on its path (its parent, that one's, ..) and itself.  d_pos NULL: d_len[s] + the
+ * number of rows on its path.  At most 1024 rows a sequence, else FH_ERR_LIMIT. */
+int fh_gqa_attention_rope_tree_async(fh_ctx* ctx, const float* d_qkv, size_t ld, size_t total, size_t n_heads,
+                                     size_t n_kv, size_t head_dim, float* d_k_cache, float* d_v_cache, size_t seqs,
+                                     size_t capacity, const uint32_t* d_off, size_t max_rows, const uint32_t* d_len,
+                                     size_t max_keys, const uint32_t* d_parent, const uint32_t* d_pos, size_t rope_dim,
+                                     float base, int rope_type, const float* d_freq_factors, float linear_factor,
+                                     float* d_out);
+/* What is accepted of each sequence's tree (rows, d_off, d_len and d_parent as above; row 0 is
+ * the token that the model chose last, accepted as it is): from row 0 on, the first row that
+ * continues it and whose d_tokens [total] is the d_chosen [total] of the row before, until
+ * there is none.  d_path [total]: the accepted rows in order, at the sequence's rows, then
+ * 0xFFFFFFFF; d_count [seqs] their number; d_next [seqs] the last one's d_chosen;
+ * d_new_len [seqs] (it may be d_len) d_len + the number.  In each of the n_planes caches
+ * whose device addresses d_planes holds ([seqs, capacity, kv_dim] floats each; every layer's
+ * keys and values), cache row d_len[s] + path[i] goes to d_len[s] + i; rows past the
+ * capacity are not touched.  A sequence without rows: d_count 0, d_next left as it is.  At
+ * most 1024 rows a sequence, 65535 sequences, else FH_ERR_LIMIT. */
+int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
+                         size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
+                         const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
+                         uint32_t* d_count, uint32_t* d_next, uint32_t* d_new_len);
+
+/* ---- logits before they are sampled --------------------------------------------------
+ * sample_with_params (slm/sampling.rs:124-210) knows one penalty, once per occurrence;
+ * these edits come before it (its own penalty then off).  No reference counterpart.
+ * Of row r with logits l[v], v < vocab, in this order, each nullable:
+ *   c(v): how often v is in d_recent[d_ranges[2r] .. d_ranges[2r + 1]], and (d_tokens) in the
+ *     tokens of the row and of its path in its sequence's tree: rows d_off[s] .. d_off[s + 1]
+ *     - 1 are sequence s's (NULL: rows / seqs to each), d_parent as for
+ *     fh_gqa_attention_rope_tree_async, at most 1024 rows a sequence.  Ids at or past vocab
+ *     do not count.
+ *   d_repetition [rows]: l / p where l > 0, else l * p, if c > 0 (p <= 0: off);
+ *   d_frequency  [rows]: l - p * c;
+ *   d_presence   [rows]: l - p if c > 0;
+ *   d_bias_off [rows + 1], d_bias_id, d_bias: l + d_bias[i] for v = d_bias_id[i], d_bias_off[r]
+ *     <= i < d_bias_off[r + 1] (an id more than once: its last; ids at or past vocab do not
+ *     count);
+ *   d_mask [masks, ceil(vocab / 32)]: -inf where bit v % 32 of word v / 32 of the row's mask is
+ *     0; its mask is d_mask_of[r] (NULL: r), none if that is masks or more.
+ * Decreasing ranges or offsets are empty. */
+typedef struct {
+    const uint32_t* d_recent;
+    const uint32_t* d_ranges;
+    const float* d_repetition;
+    const float* d_frequency;
+    const float* d_presence;
+    const uint32_t* d_parent;
+    const uint32_t* d_tokens;
+    const uint32_t* d_off;
+    size_t seqs;
+    const uint32_t* d_bias_off;
+    const uint32_t* d_bias_id;
+    const float* d_bias;
+    const uint32_t* d_mask;
+    const uint32_t* d_mask_of;
+    size_t masks;
+} fh_logits_edit;
+/* d_out [rows, vocab] gets the edited logits; it may be d_logits. */
+int fh_logits_edit_async(fh_ctx* ctx, const float* d_logits, size_t rows, size_t vocab, const fh_logits_edit* edit,
+                         float* d_out);
+
 /* ---- a batched decode step's residual adds and norms, fused into the linears ---
  * The block of forward_with_cache (layer/transformer.rs:221-294; Llama:
  * LlamaBlock::forward_one, llm.rs:445-456) adds each projection to the
