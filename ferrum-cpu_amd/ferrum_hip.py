@@ -1307,9 +1307,13 @@ class LlamaDevice:
     output.weight).  Each row's token and position live on the device
     (self.tokens, self.pos), so a step can be captured in one graph.
 
+    Prompts go in at once with prompt_async.  Over f32 caches verify_async scores a
+    tree of drafted tokens for every row, and accept_async keeps what the model agreed
+    with.
+
     cfg["kv"] = "q4" holds the caches in 4 bits (KV4Cache; head_dim 32, 64 or
-    128): prompts can then be fed at once (prefill_async), self.used counts each
-    row's cache rows beside its position, and with cfg["kv_tracked"] every step
+    128): self.used counts each row's cache rows beside its position (prefill_async
+    is prompt_async for these caches alone), and with cfg["kv_tracked"] every step
     adds up the weight each cached key draws, for evict_async to make room by.
 
     from_weights takes numpy arrays keyed as a GGUF file names them
@@ -1356,6 +1360,7 @@ class LlamaDevice:
             self.spare = None
         self._next_pos = self._next_used = 0
         self._used_given = False  # next_used was set since forward_one last went on
+        self._trees, self._tree, self._planes = {}, None, None  # verify_async's buffers by size; the last call's
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
         self.fused = 3 <= B <= 64 and self.d % 32 == 0
@@ -1554,11 +1559,10 @@ class LlamaDevice:
 
     @property
     def next_pos(self) -> int:
-        """The position that forward_one feeds next.  0 starts another text.  Over a
-        4-bit cache a move takes next_used with it (forwards by the rows that
-        prefill_async fed, backwards to feed them again: that only while no rows have
-        been evicted, since then next_used has to say which row it is), and a
-        single row's self.pos and self.used."""
+        """The position that forward_one feeds next.  0 starts another text.  A move takes
+        a single row's self.pos with it; over a 4-bit cache also next_used (forwards by the
+        rows that prefill_async fed, backwards to feed them again: that only while no rows
+        have been evicted, since then next_used has to say which row it is) and self.used."""
         return self._next_pos
 
     @next_pos.setter
@@ -1601,10 +1605,11 @@ class LlamaDevice:
         if pos < 0 or used < 0:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice: no position {pos} or cache row {used}")
         self._next_pos, self._next_used = pos, used
-        if self.kv == "q4" and self.rows == 1:
+        if self.rows == 1:
             self.ctx.sync()
             self.pos.fill_(pos)
-            self.used.fill_(used)
+            if self.kv == "q4":
+                self.used.fill_(used)
             torch.cuda.current_stream().synchronize()
 
     def forward_one(self, token: int):
@@ -1629,8 +1634,8 @@ class LlamaDevice:
         self.feed_async(nxt, used)
         self._next_pos, self._next_used, self._used_given = nxt + 1, used + 1, False
         self.ctx.sync()
-        if self.kv == "q4":  # the place of what comes next: an eviction's rows, a prompt's first
-            self.pos.fill_(nxt + 1)
+        self.pos.fill_(nxt + 1)  # the place of what comes next: an eviction's rows, a prompt's first
+        if self.kv == "q4":
             self.used.fill_(used + 1)
         return self.z[0].cpu().numpy()
 
@@ -1653,39 +1658,88 @@ class LlamaDevice:
         (self.pos and self.used are the caller's; before forward_one goes on from
         there, next_pos, which moves them all).  Rows that would outgrow the cache are FH_ERR_DIM; the rows in use are
         read on the host, so the call waits for the stream."""
-        import torch
-
         if self.kv != "q4":
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async needs the 4-bit cache (cfg['kv'] = 'q4')")
-        ctx, d, B = self.ctx, self.d, self.rows
+        self._prompt_async("prefill_async", tokens, lens)
+
+    def prompt_async(self, tokens, lens):
+        """Feeds lens[r] >= 1 tokens of every row r at once, over either cache:
+        tokens (int32) holds the rows' ids one after the other, on the device; row r's go to
+        positions self.pos[r] .. (and over a 4-bit cache to its rows self.used[r] ..).  The scores
+        of each row's last token land in self.z; positions are not advanced (before forward_one
+        goes on from there, next_pos, which moves them).  Rows that would outgrow the
+        cache are FH_ERR_DIM; the rows in use are read on the host, so the call waits for the
+        stream."""
+        self._prompt_async("prompt_async", tokens, lens)
+
+    def _ids(self, who: str, what: str, ids, count: int, places: str):
+        """Refuses ids that the kernels cannot read."""
+        import torch
+
+        if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.uint32):
+            kind = getattr(ids, "dtype", type(ids).__name__)
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {what} are an int32 tensor, not {kind}")
+        place = self.used if self.kv == "q4" else self.pos
+        if not ids.is_cuda or ids.device != place.device or not ids.is_contiguous():
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {what} lie on the model's device, side by side")
+        if ids.numel() != count:
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {ids.numel()} {what} for {places}")
+
+    def _prompt_async(self, who: str, tokens, lens):
+        import torch
+
+        ctx, B = self.ctx, self.rows
         n = np.asarray(lens, np.int64)
         if n.shape != (B,) or (n < 1).any():
-            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {B} lengths of at least 1")
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {B} lengths of at least 1")
         total, most = int(n.sum()), int(n.max())
-        if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int32, torch.uint32):
-            kind = getattr(tokens, "dtype", type(tokens).__name__)
-            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: tokens are an int32 tensor, not {kind}")
-        if not tokens.is_cuda or tokens.device != self.used.device or not tokens.is_contiguous():
-            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.prefill_async: tokens lie on the model's device, side by side")
-        if tokens.numel() != total:
-            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.prefill_async: {tokens.numel()} tokens for {total} places")
+        self._ids(who, "tokens", tokens, total, f"{total} places")
         ctx.sync()
         torch.cuda.synchronize()
-        max_keys = int((self.used.cpu().numpy().astype(np.int64) + n).max())
+        place = self.used if self.kv == "q4" else self.pos
+        max_keys = int((place.cpu().numpy().astype(np.int64) + n).max())
         if max_keys > self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
         dev, ends = "cuda", np.cumsum(n)
         off = torch.from_numpy(np.concatenate([[0], ends]).astype(np.int32)).to(dev)
-        rep = torch.from_numpy(n).to(dev)
-        first = torch.repeat_interleave(off[:-1].long(), rep)
-        pos = (torch.repeat_interleave(self.pos, rep) + torch.arange(total, device=dev) - first).to(torch.int32)
-        x, x2, h, proj = (torch.empty((total, d), device=dev) for _ in range(4))
-        qkv, q, att = (torch.empty((total, w), device=dev) for w in (self.qkv_dim, self.q_dim, self.q_dim))
-        gu, mid = torch.empty((total, 2 * self.ffn), device=dev), torch.empty((total, self.ffn), device=dev)
-        lse = torch.empty((total, self.nh), device=dev) if self.tracked else None
+        w = self._row_buffers(total)
+        if self.kv == "q4":
+            rep = torch.from_numpy(n).to(dev)
+            first = torch.repeat_interleave(off[:-1].long(), rep)
+            pos = (torch.repeat_interleave(self.pos, rep) + torch.arange(total, device=dev) - first).to(torch.int32)
+            q = torch.empty((total, self.q_dim), device=dev)
+            lse = torch.empty((total, self.nh), device=dev) if self.tracked else None
+
+            def attend(b):
+                self._attend4_async(b, w["qkv"], total, off, most, pos, max_keys, q, w["att"], lse)
+        else:
+            def attend(b):
+                gqa_attention_rope_prefill_async(ctx, w["qkv"], self.qkv_dim, total, self.nh, self.nkv, self.hd, b["k"],
+                                                 b["v"], B, self.cap, off, most, self.pos, max_keys, None, self.rope_dim,
+                                                 self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear, w["att"])
         torch.cuda.synchronize()
-        embed_rows_async(ctx, self.tok_w, self.vocab, d, tokens, total, x)
-        cur, other = x, x2
+        self._blocks_async(tokens, total, w, attend)
+        ctx.sync()
+        last = w["h"][torch.from_numpy(ends - 1).to(dev)].contiguous()
+        torch.cuda.synchronize()
+        linear_forward_async(ctx, self.head, last, B, self.d, None, 0, self.z)
+        self._keep = last  # alive until the stream has used it
+
+    def _row_buffers(self, total: int) -> dict:
+        """Activations of `total` rows that _blocks_async feeds at once."""
+        import torch
+
+        widths = {"x": self.d, "x2": self.d, "h": self.d, "proj": self.d, "qkv": self.qkv_dim, "att": self.q_dim,
+                  "gu": 2 * self.ffn, "mid": self.ffn}
+        return {name: torch.empty((total, wide), device="cuda") for name, wide in widths.items()}
+
+    def _blocks_async(self, tokens, total: int, w: dict, attend):
+        """The blocks over `total` rows of any sequences (attend: a block's attention, from
+        w["qkv"] to w["att"]); w["h"] gets the rows as the head takes them."""
+        ctx, d = self.ctx, self.d
+        h, qkv, att, gu, mid, proj = (w[name] for name in ("h", "qkv", "att", "gu", "mid", "proj"))
+        embed_rows_async(ctx, self.tok_w, self.vocab, d, tokens, total, w["x"])
+        cur, other = w["x"], w["x2"]
         for i, b in enumerate(self.blocks):
             if i == 0:
                 rmsnorm_async(ctx, cur, None, None, total, d, b["attn_norm"], self.eps, h)
@@ -1694,7 +1748,7 @@ class LlamaDevice:
                 cur, other = other, cur
             qkv_b = b.get("qkv_b")
             linear_forward_async(ctx, b["qkv"], h, total, d, qkv_b, 0 if qkv_b is None else self.qkv_dim, qkv)
-            self._attend4_async(b, qkv, total, off, most, pos, max_keys, q, att, lse)
+            attend(b)
             linear_forward_async(ctx, b["o"], att, total, self.q_dim, None, 0, proj)
             rmsnorm_async(ctx, cur, proj, other, total, d, b["ffn_norm"], self.eps, h)
             cur, other = other, cur
@@ -1705,11 +1759,59 @@ class LlamaDevice:
                 swiglu_async(ctx, gu, gu[:, self.ffn:], total, self.ffn, 2 * self.ffn, mid)
             linear_forward_async(ctx, b["down"], mid, total, self.ffn, None, 0, proj)
         rmsnorm_async(ctx, cur, proj, other, total, d, self.out_norm, self.eps, h)
-        ctx.sync()
-        last = h[torch.from_numpy(ends - 1).to(dev)].contiguous()
-        torch.cuda.synchronize()
-        linear_forward_async(ctx, self.head, last, B, d, None, 0, self.z)
-        self._keep = last  # alive until the stream has used it
+
+    def verify_async(self, tokens, parents, n: int, max_pos: int):
+        """Scores a tree of n drafted tokens for every row over its f32 cache: tokens and
+        parents (int32, [rows, n], on the device) hold the rows' trees one after the other.  Node 0
+        is the token that the row goes on with (self.tokens of a plain step), node t > 0 a
+        draft to follow node parents[t] < t of its tree.  Node t lies at cache row self.pos[r] + t
+        and is seen by the nodes behind it; max_pos bounds self.pos.  The nodes' scores land in
+        self.zt [rows * n, vocab]; nothing is advanced (accept_async).  Nodes past the cache get
+        NaN scores."""
+        import torch
+
+        if self.kv != "f32":
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.verify_async needs the f32 cache")
+        if not 1 <= n <= 1024:
+            raise FerrumHipError(FH_ERR_LIMIT, f"LlamaDevice.verify_async: trees of 1 to 1024 tokens, not {n}")
+        ctx, B, total = self.ctx, self.rows, self.rows * n
+        for what, ids in (("tokens", tokens), ("parents", parents)):
+            self._ids("verify_async", what, ids, total, f"{B} trees of {n}")
+        if n not in self._trees:
+            ints = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+            self._trees[n] = dict(self._row_buffers(total), z=torch.empty((total, self.vocab), device="cuda"),
+                                  path=ints(total), count=ints(B))
+            if self._planes is None:
+                self._planes = torch.tensor([b[c].data_ptr() for b in self.blocks for c in "kv"], dtype=torch.int64,
+                                            device="cuda")
+            torch.cuda.synchronize()
+        w = self._trees[n]
+        max_keys = min(max_pos + n, self.cap)
+
+        def attend(b):
+            gqa_attention_rope_tree_async(ctx, w["qkv"], self.qkv_dim, total, self.nh, self.nkv, self.hd, b["k"], b["v"], B,
+                                          self.cap, None, n, self.pos, max_keys, parents, None, self.rope_dim, self.rope_base,
+                                          self.rope_type, self.rope_freqs, self.rope_linear, w["att"])
+
+        self._blocks_async(tokens, total, w, attend)
+        linear_forward_async(ctx, self.head, w["h"], total, self.d, None, 0, w["z"])
+        self._tree, self.zt = (n, tokens, parents), w["z"]
+
+    def accept_async(self, chosen):
+        """After verify_async: follows each row's tree from node 0 along the drafts that equal
+        what was chosen (chosen, int32 [rows, n] on the device: an id for every node, sampled
+        from self.zt) at the node before.  The accepted nodes' cache rows move together in every
+        layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
+        last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
+        many they were."""
+        if self._tree is None:
+            raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
+        n, tokens, parents = self._tree
+        total, w = self.rows * n, self._trees[n]
+        self._ids("accept_async", "ids", chosen, total, f"{self.rows} trees of {n}")
+        tree_accept_async(self.ctx, parents, tokens, chosen, total, None, self.rows, n, self.pos, self._planes,
+                          2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos)
+        self.path, self.count, self._tree = w["path"].view(self.rows, n), w["count"], None
 
     def evict_async(self, keep: int, recent: int):
         """Cuts every row's caches that hold more than `keep` keys to the last
