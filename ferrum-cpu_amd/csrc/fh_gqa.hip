@@ -218,6 +218,9 @@ __device__ __forceinline__ void split2_any(float x, float y, uint32_t& hi, uint3
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// How far queries and keys are brought up, and values: 2^-e of a query times 2^-e of a key stays a
+// normal number (its product with a masked score is -inf, not NaN).
+constexpr int kLiftMost = 60, kValueLift = 100;
 // e with x 2^e in [2^14, 2^15) for a magnitude's bits, as far as it is in range.
 __device__ __forceinline__ int lift(uint32_t bits, int most) { return min(max(141 - static_cast<int>(bits >> 23), -113), most); }
 
@@ -232,6 +235,194 @@ __device__ __forceinline__ void store_part(float2* to, float2 x) {
 __device__ __forceinline__ float2 load_part(const float2* from) {
     return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float2*>(from)), __ATOMIC_RELAXED,
                                                         __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// What a lane has summed for its column over the keys so far: weights are 2^(score - base).
+template <int OT>
+struct Sums {
+    static constexpr int kParts = 1 + 8 * OT;  // float2s
+    float base, l;
+    f32x16 o[OT];
+};
+template <int OT>
+__device__ __forceinline__ void clear(Sums<OT>& z) {
+    z.base = -FLT_MAX;
+    z.l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < OT; d++) z.o[d] = f32x16{};
+}
+// Weights lie at 2^10 of the largest so far, and up to 2^14 before the sums are brought to a
+// new one: their lower terms stay normal numbers of f16 far below it.
+template <int OT>
+__device__ __forceinline__ void raise_base(Sums<OT>& z, float top) {
+    if (__any(top > z.base + 14.0f)) {
+        const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + 10.0f, max_halves(top));
+        const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, f = __builtin_amdgcn_exp2f(z.base - nb);
+        z.l *= f;
+#pragma unroll
+        for (int d = 0; d < OT; d++) z.o[d] *= f;
+        z.base = nb;
+    }
+}
+// Eight weights in two f16 terms.
+__device__ __forceinline__ void split8(const float* p, h8f& hi, h8f& lo) {
+    u32x4 h, l;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t x, y;
+        split2(p[2 * j], p[2 * j + 1], x, y);
+        h[j] = x;
+        l[j] = y;
+    }
+    hi = __builtin_bit_cast(h8f, h);
+    lo = __builtin_bit_cast(h8f, l);
+}
+// A tile with a value that is not finite: it reaches the rows that see it and no others, on
+// the vector units; w: the lane's weights of the values themselves.
+template <int W>
+__device__ __forceinline__ void add_seen(Sums<W / 32>& z, const float (&w)[16], const float* vp, size_t kv_dim, int hd, uint32_t k0,
+                                         uint32_t keys, uint32_t seen, int half) {
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        const uint32_t mine = __builtin_bit_cast(uint32_t, w[v]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(mine, mine, false, false);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {  // (lanes 0 .. 31's in sw[0], of both halves; 32 .. 63's in sw[1])
+            const int j = acc_row(v, e);
+            const float p = __builtin_bit_cast(float, static_cast<uint32_t>(sw[e]));
+            if (k0 + j < keys && (seen >> j & 1)) {
+                const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim;
+#pragma unroll
+                for (int d = 0; d < W / 32; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int dim = 32 * d + acc_row(i, half);
+                        if (W > 32 || dim < hd) z.o[d][i] += p * from[dim];
+                    }
+            }
+        }
+    }
+}
+template <int OT>
+__device__ __forceinline__ void add_sums(Sums<OT>& z, const float2 (&y)[Sums<OT>::kParts]) {
+    const float nb = fmaxf(z.base, y[0].x), f0 = __builtin_amdgcn_exp2f(z.base - nb), f1 = __builtin_amdgcn_exp2f(y[0].x - nb);
+    z.l = z.l * f0 + y[0].y * f1;
+#pragma unroll
+    for (int d = 0; d < OT; d++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            z.o[d][2 * i] = z.o[d][2 * i] * f0 + y[1 + 8 * d + i].x * f1;
+            z.o[d][2 * i + 1] = z.o[d][2 * i + 1] * f0 + y[1 + 8 * d + i].y * f1;
+        }
+    z.base = nb;
+}
+// The sums of the waves that shared the keys, in order, to those of kw = 0, through LDS that every wave
+// is past its last read of.
+template <int OT, int CW, int KW>
+__device__ __forceinline__ void join_waves(Sums<OT>& z, float2* room, int cw, int kw, int lane) {
+    constexpr int PL = Sums<OT>::kParts;
+    if (kw > 0) {
+        float2* to = room + ((kw - 1) * CW + cw) * (PL * 64) + lane;
+        to[0] = make_float2(z.base, z.l);
+#pragma unroll
+        for (int d = 0; d < OT; d++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) to[(1 + 8 * d + i) * 64] = make_float2(z.o[d][2 * i], z.o[d][2 * i + 1]);
+    }
+    __syncthreads();
+    if (kw == 0)
+#pragma unroll
+        for (int k = 1; k < KW; k++) {
+            const float2* from = room + ((k - 1) * CW + cw) * (PL * 64) + lane;
+            float2 y[PL];
+#pragma unroll
+            for (int i = 0; i < PL; i++) y[i] = from[i * 64];
+            add_sums(z, y);
+        }
+}
+
+// A column's query, scaled by its own power of two, dims 16 i + 8 half + (0..7) in two f16 terms;
+// returns what undoes the power and brings scores to base 2.
+template <int W>
+__device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, int head, int half, h8f (&qh)[W / 16], h8f (&ql)[W / 16]) {
+    constexpr int KI = W / 16;
+    const float* qp = a.q + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 8;
+    float x[8 * KI];
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+        const bool in = W > 32 || 16 * i + half * 8 < a.hd;
+        const float4 u = in ? *reinterpret_cast<const float4*>(qp + 16 * i) : make_float4(0, 0, 0, 0);
+        const float4 w = in ? *reinterpret_cast<const float4*>(qp + 16 * i + 4) : make_float4(0, 0, 0, 0);
+        x[8 * i] = u.x; x[8 * i + 1] = u.y; x[8 * i + 2] = u.z; x[8 * i + 3] = u.w;
+        x[8 * i + 4] = w.x; x[8 * i + 5] = w.y; x[8 * i + 6] = w.z; x[8 * i + 7] = w.w;
+    }
+    uint32_t top = 0;  // (of the finite ones)
+#pragma unroll
+    for (int i = 0; i < 8 * KI; i++) top = mag(x[i]) < kInf ? max(top, mag(x[i])) : top;
+    const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    const int e = lift(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])), kLiftMost);
+    const float up = pow2f(e);
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t h, l;
+            split2_any(x[8 * i + 2 * j] * up, x[8 * i + 2 * j + 1] * up, h, l);
+            hi[j] = h;
+            lo[j] = l;
+        }
+        qh[i] = __builtin_bit_cast(h8f, hi);
+        ql[i] = __builtin_bit_cast(h8f, lo);
+    }
+    return pow2f(-e) * a.scale;
+}
+// A workgroup's sums to memory; the last of a block's workgroups joins all shares of the keys, in
+// order (true: it is this one).
+template <int OT, int CW>
+__device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint32_t unit, int split, int cw, bool mine, int lane) {
+    constexpr int PL = Sums<OT>::kParts;
+    float2* part = a.part + (static_cast<size_t>(unit) * a.splits * CW + cw) * (PL * 64) + lane;
+    if (mine) {
+        float2* to = part + static_cast<size_t>(split) * CW * (PL * 64);
+        store_part(to, make_float2(z.base, z.l));
+#pragma unroll
+        for (int d = 0; d < OT; d++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) store_part(to + (1 + 8 * d + i) * 64, make_float2(z.o[d][2 * i], z.o[d][2 * i + 1]));
+    }
+    // Every thread's coherent stores complete before the arrival count moves.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __shared__ int last;
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
+    __syncthreads();
+    if (!last) return false;
+    if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (mine) {
+        clear(z);
+        for (int k = 0; k < a.splits; k++) {
+            const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
+            float2 y[PL];
+#pragma unroll
+            for (int i = 0; i < PL; i++) y[i] = load_part(from + i * 64);
+            add_sums(z, y);
+        }
+    }
+    return true;
+}
+template <int W>
+__device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs& a, uint32_t row, int head, int half, bool bad) {
+    float* out = a.out + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 4;
+    const float f = bad ? __builtin_nanf("") : 1.0f / z.l;
+#pragma unroll
+    for (int d = 0; d < W / 32; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            if (W == 32 && 8 * b + half * 4 >= a.hd) continue;
+            *reinterpret_cast<float4*>(out + 32 * d + 8 * b) =
+                make_float4(z.o[d][4 * b] * f, z.o[d][4 * b + 1] * f, z.o[d][4 * b + 2] * f, z.o[d][4 * b + 3] * f);
+        }
 }
 
 // Columns are (row, query head of the kv head), heads fastest; a wave has 32 of them, a
@@ -294,41 +485,8 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
     const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits);
     const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits);
 
-    // its query, scaled by its own power of two, dims 16 i + 8 half + (0..7)
     h8f qh[KI], ql[KI];
-    float qscale;
-    {
-        const float* qp = a.q + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 8;
-        float x[8 * KI];
-#pragma unroll
-        for (int i = 0; i < KI; i++) {
-            const bool in = W > 32 || 16 * i + half * 8 < a.hd;
-            const float4 u = in ? *reinterpret_cast<const float4*>(qp + 16 * i) : make_float4(0, 0, 0, 0);
-            const float4 w = in ? *reinterpret_cast<const float4*>(qp + 16 * i + 4) : make_float4(0, 0, 0, 0);
-            x[8 * i] = u.x; x[8 * i + 1] = u.y; x[8 * i + 2] = u.z; x[8 * i + 3] = u.w;
-            x[8 * i + 4] = w.x; x[8 * i + 5] = w.y; x[8 * i + 6] = w.z; x[8 * i + 7] = w.w;
-        }
-        uint32_t top = 0;  // (of the finite ones)
-#pragma unroll
-        for (int i = 0; i < 8 * KI; i++) top = mag(x[i]) < kInf ? max(top, mag(x[i])) : top;
-        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        const int e = lift(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])), 126);
-        const float up = pow2f(e);
-        qscale = pow2f(-e) * a.scale;
-#pragma unroll
-        for (int i = 0; i < KI; i++) {
-            u32x4 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t h, l;
-                split2_any(x[8 * i + 2 * j] * up, x[8 * i + 2 * j + 1] * up, h, l);
-                hi[j] = h;
-                lo[j] = l;
-            }
-            qh[i] = __builtin_bit_cast(h8f, hi);
-            ql[i] = __builtin_bit_cast(h8f, lo);
-        }
-    }
+    const float qscale = load_query<W>(a, row, head, half, qh, ql);
 
     // Staging.  Piece i < WK: 512 / W keys, eight channels a thread; the others: values
     // of 128 / W quads of keys, two channels a thread.
@@ -378,7 +536,7 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
                     uint32_t fin = 0;
 #pragma unroll
                     for (int j = 0; j < 8; j++) fin = mag(x[i][j]) < kInf ? max(fin, mag(x[i][j])) : fin;
-                    e = lift(group_max<W / 8>(fin), 126);
+                    e = lift(group_max<W / 8>(fin), kLiftMost);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         uint32_t h, l;
@@ -387,7 +545,7 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
                         lo[j] = l;
                     }
                 } else {
-                    e = lift(top, 126);
+                    e = lift(top, kLiftMost);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         uint32_t h, l;
@@ -409,7 +567,7 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
                 for (int j = 0; j < 4; j++) {
                     const uint32_t top = group_max<W / 2>(max(mag(x[i][j]), mag(x[i][4 + j])));
                     most = max(most, top);
-                    const int e = lift(top, 100);
+                    const int e = lift(top, kValueLift);
                     up[j] = pow2f(e);
                     ex[j] = static_cast<float>(-e);
                     y[j] = x[i][j] * up[j];
@@ -440,10 +598,8 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
         }
     };
 
-    float base = -FLT_MAX, l = 0.0f;
-    f32x16 o[OT];
-#pragma unroll
-    for (int d = 0; d < OT; d++) o[d] = f32x16{};
+    Sums<OT> z;
+    clear(z);
     const int steps = static_cast<int>((tile1 - tile0 + KW - 1) / KW);
     if (threadIdx.x < 3 * KW) st.unsafe[threadIdx.x / KW][threadIdx.x % KW] = 0;
     if (steps > 0) fetch(tile0);
@@ -500,158 +656,375 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
             float top = -INFINITY;
 #pragma unroll
             for (int v = 0; v < 16; v++) top = fmaxf(top, u[v]);
-            // Weights lie at 2^10 of the largest so far, and up to 2^14 before the sums are
-            // brought to a new one: their lower terms stay normal numbers of f16 far below it.
-            if (__any(top > base + 14.0f)) {
-                const float m = fmaxf(base == -FLT_MAX ? -FLT_MAX : base + 10.0f, max_halves(top));
-                const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, f = __builtin_amdgcn_exp2f(base - nb);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < OT; d++) o[d] *= f;
-                base = nb;
-            }
+            raise_base(z, top);
 #pragma unroll
             for (int v = 0; v < 16; v++) {
-                u[v] = __builtin_amdgcn_exp2f(u[v] - base);
+                u[v] = __builtin_amdgcn_exp2f(u[v] - z.base);
                 up[v] *= u[v];
-                l += up[v];
+                z.l += up[v];
             }
             if (!vbad) {
 #pragma unroll
                 for (int s2 = 0; s2 < 2; s2++) {
-                    u32x4 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t h, lw;
-                        split2(u[8 * s2 + 2 * j], u[8 * s2 + 2 * j + 1], h, lw);
-                        hi[j] = h;
-                        lo[j] = lw;
-                    }
-                    const h8f ph = __builtin_bit_cast(h8f, hi), pl = __builtin_bit_cast(h8f, lo);
+                    h8f ph, pl;
+                    split8(u + 8 * s2, ph, pl);
 #pragma unroll
                     for (int d = 0; d < OT; d++) {
                         const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][lane]);
                         const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][lane]);
-                        o[d] = mfma(vl, ph, o[d]);
-                        o[d] = mfma(vh, pl, o[d]);
-                        o[d] = mfma(vh, ph, o[d]);
+                        z.o[d] = mfma(vl, ph, z.o[d]);
+                        z.o[d] = mfma(vh, pl, z.o[d]);
+                        z.o[d] = mfma(vh, ph, z.o[d]);
                     }
                 }
             } else {
-                // (a value that is not finite reaches the rows that see it and no others: on the vector units)
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, up[v]),
-                                                                     __builtin_bit_cast(uint32_t, up[v]), false, false);
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {  // (lanes 0 .. 31's in sw[0], of both halves; 32 .. 63's in sw[1])
-                        const int j = acc_row(v, e);
-                        const float p = __builtin_bit_cast(float, static_cast<uint32_t>(sw[e]));
-                        if (k0 + j < keys && (seen >> j & 1)) {
-                            const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim;
-#pragma unroll
-                            for (int d = 0; d < OT; d++)
-#pragma unroll
-                                for (int w = 0; w < 16; w++) {
-                                    const int dim = 32 * d + acc_row(w, half);
-                                    if (W > 32 || dim < a.hd) o[d][w] += p * from[dim];
-                                }
-                        }
-                    }
-                }
+                add_seen<W>(z, up, vp, kv_dim, a.hd, k0, keys, seen, half);
             }
         }
         if (step + 1 < steps) stash(step + 1);
         __syncthreads();
     }
-    l = sum_halves(l);
-
-    constexpr int PL = 1 + 8 * OT;  // float2s of a lane's sums
+    z.l = sum_halves(z.l);
     if constexpr (KW > 1) {
-        // the waves' sums, in order, through the stage's LDS (every wave is past its last read of it)
-        static_assert(sizeof(Stage<W, CW, KW>) >= (KW - 1) * CW * PL * 64 * sizeof(float2), "the sums fit");
-        float2* mine = reinterpret_cast<float2*>(smem) + lane;
-        if (kw > 0) {
-            float2* to = mine + ((kw - 1) * CW + cw) * (PL * 64);
-            to[0] = make_float2(base, l);
-#pragma unroll
-            for (int d = 0; d < OT; d++)
-#pragma unroll
-                for (int w = 0; w < 8; w++) to[(1 + 8 * d + w) * 64] = make_float2(o[d][2 * w], o[d][2 * w + 1]);
-        }
-        __syncthreads();
-        if (kw == 0)
-#pragma unroll
-            for (int k = 1; k < KW; k++) {
-                const float2* from = mine + ((k - 1) * CW + cw) * (PL * 64);
-                const float2 b = from[0];
-                const float nb = fmaxf(base, b.x), f0 = __builtin_amdgcn_exp2f(base - nb), f1 = __builtin_amdgcn_exp2f(b.x - nb);
-                l = l * f0 + b.y * f1;
-#pragma unroll
-                for (int d = 0; d < OT; d++)
-#pragma unroll
-                    for (int w = 0; w < 8; w++) {
-                        const float2 y = from[(1 + 8 * d + w) * 64];
-                        o[d][2 * w] = o[d][2 * w] * f0 + y.x * f1;
-                        o[d][2 * w + 1] = o[d][2 * w + 1] * f0 + y.y * f1;
-                    }
-                base = nb;
-            }
+        static_assert(sizeof(Stage<W, CW, KW>) >= (KW - 1) * CW * Sums<OT>::kParts * 64 * sizeof(float2), "the sums fit");
+        join_waves<OT, CW, KW>(z, reinterpret_cast<float2*>(smem), cw, kw, lane);
     }
-    if (a.splits > 1) {
-        // the last of a block's workgroups joins all shares, in order
-        const uint32_t unit = pair + heads * cb;
-        float2* part = a.part + (static_cast<size_t>(unit) * a.splits * CW + cw) * (PL * 64) + lane;
-        if (kw == 0) {
-            float2* to = part + static_cast<size_t>(split) * CW * (PL * 64);
-            store_part(to, make_float2(base, l));
+    if (a.splits > 1 && !join_shares<OT, CW>(z, a, pair + heads * cb, split, cw, kw == 0, lane)) return;
+    if (kw == 0 && on) store_out<W>(z, a, row, head, half, bad);
+}
+
+// ---- prompts ---------------------------------------------------------------------------------
+//
+// Many columns read the same keys, so what a key costs beside its products is done once, in
+// a launch of its own: k_gqa_pack writes each tile of 32 keys as the MFMA operands that
+// k_gqa_prompt loads, f16 terms under one power of two for the tile's keys and one for its
+// values.  A tile whose rows' largest magnitudes lie more than 2^4 apart has one of each row's
+// own instead (a row's lower terms would fall below f16's normal numbers, its accuracy hang on
+// the rows beside it), which the weights then take key by key.
+template <int W>
+struct Packed {
+    _Float16 k[W / 16][2][64][8];
+    _Float16 v[W / 32][2][2][64][8];
+};
+struct TileInfo {
+    float kdown[kKeys], vexp[kKeys], vup[kKeys];  // of each key: 2^-e; of each value row: -e, 2^e
+    float one[4];                                 // of all of them, where they are alike: kdown, vexp, vup
+    uint32_t flags, pad[27];
+};
+enum { kKeysApart = 1, kValuesApart = 2, kNotFinite = 4 };
+constexpr int kApart = 4;
+
+struct PackArgs {
+    const float *kc, *vc;
+    size_t seq_stride;
+    int n_kv, hd, tiles;  // tiles of a (sequence, kv head)'s room
+    uint32_t seqs, total, max_rows, limit;
+    const uint32_t *off, *len;
+    char* packed;
+    TileInfo* info;
+};
+
+template <int W>
+__global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
+    constexpr int PER = W / 64 > 0 ? W / 64 : 1;  // pieces of 256 threads, of keys and of values each
+    const uint32_t tile = blockIdx.x, kv = blockIdx.y, s = blockIdx.z;
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    const uint32_t keys = r.count ? static_cast<uint32_t>(min(r.at + r.count, static_cast<uint64_t>(a.limit))) : 0;
+    if (tile * kKeys >= keys) return;
+    __shared__ uint32_t top[2][kKeys];
+    const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
+    const float* kp = a.kc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    const float* vp = a.vc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    float x[PER][8], y[PER][8];
+    const auto key_of = [&](int i) { return (i * kThreads + static_cast<int>(threadIdx.x)) / (W / 8); };
+    const auto quad_of = [&](int i) { return (i * kThreads + static_cast<int>(threadIdx.x)) / (W / 2); };
+    const int ch = threadIdx.x % (W / 8), dv = threadIdx.x % (W / 2) * 2;
 #pragma unroll
-            for (int d = 0; d < OT; d++)
+    for (int i = 0; i < PER; i++) {
+        const int k = key_of(i), q = quad_of(i);
+        // (rows past the last key: zeros)
+        const float* from = kp + static_cast<size_t>(tile * kKeys + k) * kv_dim + ch * 8;
+        const bool in = k < kKeys && tile * kKeys + k < keys && (W > 32 || ch * 8 < a.hd);
+        const float4 u = in ? *reinterpret_cast<const float4*>(from) : make_float4(0, 0, 0, 0);
+        const float4 w = in ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0, 0, 0, 0);
+        x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
+        x[i][4] = w.x; x[i][5] = w.y; x[i][6] = w.z; x[i][7] = w.w;
 #pragma unroll
-                for (int w = 0; w < 8; w++) store_part(to + (1 + 8 * d + w) * 64, make_float2(o[d][2 * w], o[d][2 * w + 1]));
+        for (int j = 0; j < 4; j++) {
+            const uint32_t key = tile * kKeys + 4 * q + j;
+            const bool vin = q < 8 && key < keys && (W > 32 || dv < a.hd);
+            const float2 t = vin ? *reinterpret_cast<const float2*>(vp + key * kv_dim + dv) : make_float2(0, 0);
+            y[i][j] = t.x;
+            y[i][4 + j] = t.y;
         }
-        // Every thread's coherent stores complete before the arrival count moves.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __shared__ int last;
-        __syncthreads();
-        if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
-        __syncthreads();
-        if (!last) return;
-        if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (kw == 0) {
-            base = -FLT_MAX;
-            l = 0.0f;
+    }
 #pragma unroll
-            for (int d = 0; d < OT; d++) o[d] = f32x16{};
-            for (int k = 0; k < a.splits; k++) {
-                const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
-                float2 y[PL];
+    for (int i = 0; i < PER; i++) {
+        uint32_t m = 0, inf = 0;  // (the largest finite one; of keys the others keep their upper term alone)
 #pragma unroll
-                for (int i = 0; i < PL; i++) y[i] = load_part(from + i * 64);
-                const float nb = fmaxf(base, y[0].x), f0 = __builtin_amdgcn_exp2f(base - nb), f1 = __builtin_amdgcn_exp2f(y[0].x - nb);
-                l = l * f0 + y[0].y * f1;
+        for (int j = 0; j < 8; j++) {
+            m = mag(x[i][j]) < kInf ? max(m, mag(x[i][j])) : m;
+            inf = max(inf, mag(x[i][j]));
+        }
+        (void)inf;
+        m = group_max<W / 8>(m);
+        if (ch == 0 && key_of(i) < kKeys) top[0][key_of(i)] = m;
 #pragma unroll
-                for (int d = 0; d < OT; d++)
-#pragma unroll
-                    for (int w = 0; w < 8; w++) {
-                        o[d][2 * w] = o[d][2 * w] * f0 + y[1 + 8 * d + w].x * f1;
-                        o[d][2 * w + 1] = o[d][2 * w + 1] * f0 + y[1 + 8 * d + w].y * f1;
-                    }
-                base = nb;
+        for (int j = 0; j < 4; j++) {
+            const uint32_t t = group_max<W / 2>(max(mag(y[i][j]), mag(y[i][4 + j])));
+            if (dv == 0 && quad_of(i) < 8) top[1][4 * quad_of(i) + j] = t;
+        }
+    }
+    __syncthreads();
+    // what lane l of every wave holds of row l % 32: keys' in the lower half, values' in the upper one
+    const int lane = threadIdx.x & 63, of = lane >> 5;
+    const uint32_t mine = top[of][lane & 31];
+    const bool used = tile * kKeys + (lane & 31) < keys && mine > 0;
+    int hi = used ? static_cast<int>(mine >> 23) : 0, lo = used ? static_cast<int>(mine >> 23) : 255;
+    hi = static_cast<int>(group_max<32>(static_cast<uint32_t>(hi)));
+    lo = 255 - static_cast<int>(group_max<32>(static_cast<uint32_t>(255 - lo)));
+    const bool apart = hi - lo > kApart;
+    const int alike = lift(static_cast<uint32_t>(hi) << 23, of ? kValueLift : kLiftMost);
+    const int e = apart ? lift(mine, of ? kValueLift : kLiftMost) : alike;
+    TileInfo& info = a.info[(static_cast<size_t>(s) * a.n_kv + kv) * a.tiles + tile];
+    if (threadIdx.x < 64) {
+        const uint64_t bad = __ballot(of == 1 && mine >= kInf), far = __ballot(apart);
+        if (of == 0) {
+            info.kdown[lane] = pow2f(-e);
+            if (lane == 0) info.one[0] = pow2f(-alike);
+        } else {
+            info.vexp[lane - 32] = static_cast<float>(-e);
+            info.vup[lane - 32] = pow2f(e);
+            if (lane == 32) {
+                info.one[1] = static_cast<float>(-alike);
+                info.one[2] = pow2f(alike);
+                info.flags = (far & 1 ? kKeysApart : 0) | (far >> 32 ? kValuesApart : 0) | (bad ? kNotFinite : 0);
             }
         }
     }
-    if (kw != 0 || !on) return;
-    float* out = a.out + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 4;
-    const float f = bad ? __builtin_nanf("") : 1.0f / l;
+    Packed<W>& to = reinterpret_cast<Packed<W>*>(a.packed)[(static_cast<size_t>(s) * a.n_kv + kv) * a.tiles + tile];
 #pragma unroll
-    for (int d = 0; d < OT; d++)
+    for (int i = 0; i < PER; i++) {
+        const int k = key_of(i), q = quad_of(i);
+        const float up = pow2f(__shfl(e, k & 31, 64));
+        if (k < kKeys) {
+            u32x4 h, l;
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            if (W == 32 && 8 * b + half * 4 >= a.hd) continue;
-            *reinterpret_cast<float4*>(out + 32 * d + 8 * b) =
-                make_float4(o[d][4 * b] * f, o[d][4 * b + 1] * f, o[d][4 * b + 2] * f, o[d][4 * b + 3] * f);
+            for (int j = 0; j < 4; j++) {
+                uint32_t b, c;
+                split2_any(x[i][2 * j] * up, x[i][2 * j + 1] * up, b, c);
+                h[j] = b;
+                l[j] = c;
+            }
+            *reinterpret_cast<u32x4*>(to.k[ch >> 1][0][(ch & 1) * 32 + k]) = h;
+            *reinterpret_cast<u32x4*>(to.k[ch >> 1][1][(ch & 1) * 32 + k]) = l;
         }
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float vu = pow2f(__shfl(e, 32 + ((4 * q + j) & 31), 64));
+            z[j] = y[i][j] * vu;
+            z[4 + j] = y[i][4 + j] * vu;
+        }
+        if (q < 8) {
+            // keys 4 q .. + 3 are steps 4 (q / 2 % 2) .. + 3 of lane half q % 2 in product q / 4
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                u32x2 h, l;
+                uint32_t b, d;
+                split2(z[4 * c], z[4 * c + 1], b, d);
+                h[0] = b;
+                l[0] = d;
+                split2(z[4 * c + 2], z[4 * c + 3], b, d);
+                h[1] = b;
+                l[1] = d;
+                const int dd = dv + c;
+                *reinterpret_cast<u32x2*>(&to.v[dd >> 5][q >> 2][0][(q & 1) * 32 + (dd & 31)][4 * (q >> 1 & 1)]) = h;
+                *reinterpret_cast<u32x2*>(&to.v[dd >> 5][q >> 2][1][(q & 1) * 32 + (dd & 31)][4 * (q >> 1 & 1)]) = l;
+            }
+        }
+    }
+}
+
+// 128 columns a workgroup of four waves.  Step t multiplies tile t + 1's scores while tile t's
+// become weights, and stages tile t + 2's keys and t + 1's values: the matrix and the vector
+// units have work of their own side by side.
+template <int W>
+__global__ void __launch_bounds__(kThreads, 2) k_gqa_prompt(RowsArgs a, const char* packed, const TileInfo* infos, int room) {
+    constexpr int CW = 4, KI = W / 16, OT = W / 32, PIECE = W * 128 / 16 / kThreads;  // 16-byte loads a thread, of K and of V
+    extern __shared__ __align__(16) char smem[];
+    struct Ring {
+        u32x4 k[2][W * 8], v[2][W * 8];
+        TileInfo info[2];
+    };
+    Ring& ring = *reinterpret_cast<Ring*>(smem);
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const uint32_t heads = a.seqs * static_cast<uint32_t>(a.n_kv);
+    uint32_t id = blockIdx.x;
+    const uint32_t pair = id % heads;  // (the blocks of a sequence and kv head on as few XCDs as can be)
+    id /= heads;
+    const int split = static_cast<int>(id % a.splits);
+    const uint32_t cb = a.col_blocks - 1 - id / a.splits;  // (the longest rows first)
+    const uint32_t s = pair / a.n_kv;
+    const int kv = static_cast<int>(pair % a.n_kv);
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    const uint32_t ncols = r.count * static_cast<uint32_t>(a.group), c0 = cb * (32 * CW);
+    if (c0 >= ncols) return;
+    const uint32_t wc = c0 + wave * 32, c = wc + col, cc = min(c, ncols - 1);
+    const uint32_t t = cc / a.group, row = r.begin + t;
+    const int head = kv * a.group + static_cast<int>(cc % a.group);
+    const bool on = c < ncols, bad = r.at + t >= a.limit;
+    const uint32_t at = static_cast<uint32_t>(min(r.at, static_cast<uint64_t>(a.limit)));
+    const uint32_t own = on && !bad ? at + t + 1 : 0;  // the keys this column sees
+    const auto upto = [&](uint32_t cols) {
+        return static_cast<uint32_t>(min(r.at + (min(ncols, cols) - 1) / a.group + 1, static_cast<uint64_t>(a.limit)));
+    };
+    const uint32_t keys = upto(c0 + 32 * CW), wkeys = wc >= ncols ? 0 : upto(wc + 32);
+    const uint32_t wfull = wc >= ncols ? 0 : min(keys, at + wc / a.group + 1);  // keys that all its columns see
+    const uint32_t tiles = (keys + kKeys - 1) / kKeys, wtiles = (wkeys + kKeys - 1) / kKeys;
+    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits);
+    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits);
+    const uint32_t mine1 = min(tile1, wtiles);  // past the wave's last tile
+    const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
+    const float* vp = a.vc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+
+    h8f qh[KI], ql[KI];
+    const float qscale = load_query<W>(a, row, head, half, qh, ql);
+
+    const u32x4* from = reinterpret_cast<const u32x4*>(packed) + static_cast<size_t>(pair) * room * (W * 16) + threadIdx.x;
+    const u32x4* from_info = reinterpret_cast<const u32x4*>(infos + static_cast<size_t>(pair) * room) + threadIdx.x;
+    constexpr int kInfo = sizeof(TileInfo) / 16;
+    u32x4 piece[PIECE], info_piece{};
+    const auto fetch_k = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) piece[i] = from[static_cast<size_t>(tile) * (W * 16) + i * kThreads];
+    };
+    const auto fetch_v = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) piece[i] = from[static_cast<size_t>(tile) * (W * 16) + W * 8 + i * kThreads];
+        if (threadIdx.x < kInfo) info_piece = from_info[static_cast<size_t>(tile) * kInfo];
+    };
+    const auto put_k = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) ring.k[tile & 1][i * kThreads + threadIdx.x] = piece[i];
+    };
+    const auto put_v = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) ring.v[tile & 1][i * kThreads + threadIdx.x] = piece[i];
+        if (threadIdx.x < kInfo) reinterpret_cast<u32x4*>(&ring.info[tile & 1])[threadIdx.x] = info_piece;
+    };
+    const auto scores = [&](uint32_t tile) __attribute__((always_inline)) {
+        f32x16 x = f32x16{};
+        const u32x4* k = ring.k[tile & 1] + lane;
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            const h8f kh = __builtin_bit_cast(h8f, k[(2 * i) * 64]), kl = __builtin_bit_cast(h8f, k[(2 * i + 1) * 64]);
+            x = mfma(kl, qh[i], x);
+            x = mfma(kh, ql[i], x);
+            x = mfma(kh, qh[i], x);
+        }
+        return x;
+    };
+
+    Sums<OT> z;
+    clear(z);
+    f32x16 next = f32x16{};
+    if (tile0 < tile1) {
+        fetch_k(tile0);
+        put_k(tile0);
+        fetch_v(tile0);
+        put_v(tile0);
+        if (tile0 + 1 < tile1) {
+            fetch_k(tile0 + 1);
+            put_k(tile0 + 1);
+        }
+        __syncthreads();
+        if (tile0 < mine1) next = scores(tile0);
+        __syncthreads();
+    }
+    for (uint32_t tile = tile0; tile < tile1; tile++) {
+        const uint32_t k0 = tile * kKeys;
+        if (tile + 2 < tile1) fetch_k(tile + 2);
+        float u[16];
+        uint32_t flags = 0, seen = ~0u;
+        const TileInfo& info = ring.info[tile & 1];
+        const bool work = tile < mine1;
+        if (work) {
+            flags = __builtin_amdgcn_readfirstlane(info.flags);
+            float sc = info.one[0] * qscale, ex = info.one[1];
+#pragma unroll
+            for (int v = 0; v < 16; v++) u[v] = next[v];
+            if (__builtin_expect(flags != 0, 0)) {
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const float4 kd = *reinterpret_cast<const float4*>(&info.kdown[8 * b + 4 * half]);
+                    const float4 ve = *reinterpret_cast<const float4*>(&info.vexp[8 * b + 4 * half]);
+                    u[4 * b] = fmaf(u[4 * b] * kd.x, qscale, ve.x);
+                    u[4 * b + 1] = fmaf(u[4 * b + 1] * kd.y, qscale, ve.y);
+                    u[4 * b + 2] = fmaf(u[4 * b + 2] * kd.z, qscale, ve.z);
+                    u[4 * b + 3] = fmaf(u[4 * b + 3] * kd.w, qscale, ve.w);
+                }
+                sc = 1.0f;
+                ex = 0.0f;
+            }
+            if (k0 + kKeys > wfull) {
+                seen = own > k0 ? (own - k0 >= 32 ? ~0u : (1u << (own - k0)) - 1) : 0u;
+#pragma unroll
+                for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
+            }
+            float top = u[0];
+#pragma unroll
+            for (int v = 1; v < 16; v++) top = fmaxf(top, u[v]);
+            raise_base(z, fmaf(top, sc, ex));
+            const float less = ex - z.base;
+            if (tile + 1 < mine1) next = scores(tile + 1);
+#pragma unroll
+            for (int v = 0; v < 16; v++) u[v] = __builtin_amdgcn_exp2f(fmaf(u[v], sc, less));
+            if (__builtin_expect(flags != 0, 0)) {
+                float w[16];
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const float4 vu = *reinterpret_cast<const float4*>(&info.vup[8 * b + 4 * half]);
+                    w[4 * b] = u[4 * b] * vu.x;
+                    w[4 * b + 1] = u[4 * b + 1] * vu.y;
+                    w[4 * b + 2] = u[4 * b + 2] * vu.z;
+                    w[4 * b + 3] = u[4 * b + 3] * vu.w;
+                }
+#pragma unroll
+                for (int v = 0; v < 16; v++) z.l += w[v];
+                if (flags & kNotFinite) add_seen<W>(z, w, vp, kv_dim, a.hd, k0, keys, seen, half);
+            } else {
+                float sum[4] = {};
+#pragma unroll
+                for (int v = 0; v < 16; v++) sum[v & 3] += u[v];
+                z.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), info.one[2], z.l);
+            }
+        }
+        if (tile + 2 < tile1) put_k(tile + 2);
+        if (tile + 1 < tile1) fetch_v(tile + 1);
+        if (work && !(flags & kNotFinite)) {
+            const u32x4* v = ring.v[tile & 1] + lane;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++) {
+                h8f ph, pl;
+                split8(u + 8 * s2, ph, pl);
+#pragma unroll
+                for (int d = 0; d < OT; d++) {
+                    const h8f vh = __builtin_bit_cast(h8f, v[((d * 2 + s2) * 2) * 64]);
+                    const h8f vl = __builtin_bit_cast(h8f, v[((d * 2 + s2) * 2 + 1) * 64]);
+                    z.o[d] = mfma(vl, ph, z.o[d]);
+                    z.o[d] = mfma(vh, pl, z.o[d]);
+                    z.o[d] = mfma(vh, ph, z.o[d]);
+                }
+            }
+        }
+        if (tile + 1 < tile1) put_v(tile + 1);
+        __syncthreads();
+    }
+    z.l = sum_halves(z.l);
+    if (a.splits > 1 && !join_shares<OT, CW>(z, a, pair + heads * cb, split, wave, true, lane)) return;
+    if (on) store_out<W>(z, a, row, head, half, bad);
 }
 
 constexpr size_t kUnits = 8192;  // column blocks whose keys may be split
@@ -665,6 +1038,20 @@ int launch_rows(fh_ctx* ctx, const RowsArgs& a) {
         FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
     hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.splits * a.col_blocks)), dim3(64 * CW * KW), lds,
                        ctx->stream, a);
+    FH_HIP(ctx, hipGetLastError());
+    return FH_OK;
+}
+
+template <int W>
+int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p) {
+    hipLaunchKernelGGL(k_gqa_pack<W>, dim3(p.tiles, a.n_kv, a.seqs), dim3(kThreads), 0, ctx->stream, p);
+    FH_HIP(ctx, hipGetLastError());
+    constexpr size_t lds = 2 * W * 256 + 2 * sizeof(TileInfo);
+    const auto kern = k_gqa_prompt<W>;
+    if (lds > 64 * 1024)
+        FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.splits * a.col_blocks)), dim3(kThreads), lds,
+                       ctx->stream, a, p.packed, p.info, p.tiles);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
@@ -683,13 +1070,15 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const size_t group = g.n_heads / g.n_kv, cols = g.max_rows * group, heads = g.seqs * g.n_kv;
     const int words = g.parent ? static_cast<int>((g.max_rows + 31) / 32) : 0;
     const int w = g.hd <= 32 ? 32 : static_cast<int>(g.hd);
-    const int cw = cols > 128 ? 8 : cols > 64 ? 4 : 2;
+    const size_t tiles = (g.limit + kKeys - 1) / kKeys, pack = heads * tiles * (static_cast<size_t>(w) * 256);
+    const bool prompt = !g.parent && cols > 512 && pack < (size_t(1) << 31);
+    const int cw = prompt ? 4 : cols > 128 ? 8 : cols > 64 ? 4 : 2;
     const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
     // Keys of few columns are dealt over several workgroups, four tiles of keys each at least.
-    const size_t cus = static_cast<size_t>(ctx->num_cus), tiles = (g.limit + kKeys - 1) / kKeys;
+    const size_t cus = static_cast<size_t>(ctx->num_cus), places = prompt ? 2 * cus : cus;
     size_t splits = 1;
-    while (splits < 64 && heads * blocks * splits * 2 <= cus && splits * 2 * 4 <= tiles) splits *= 2;
+    while (splits < 64 && heads * blocks * splits * 2 <= places && splits * 2 * 4 <= tiles) splits *= 2;
     if (heads * blocks > kUnits) splits = 1;
     unsigned* counters = nullptr;
     if (splits > 1) {
@@ -701,8 +1090,9 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const size_t q_bytes = fh_align256(g.total * g.n_heads * g.hd * sizeof(float));
     const size_t seen_bytes = fh_align256(g.total * words * sizeof(uint32_t));
     const size_t part = splits > 1 ? heads * blocks * splits * cw * (1 + w / 4) * 64 * sizeof(float2) : 0;
+    const size_t info_bytes = prompt ? heads * tiles * sizeof(TileInfo) : 0;
     void* room = nullptr;
-    const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + part, &room);
+    const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + fh_align256(part) + (prompt ? pack + info_bytes : 0), &room);
     if (rc) return rc;
 
     AppendArgs p{};
@@ -765,6 +1155,24 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     a.splits = static_cast<int>(splits);
     a.part = reinterpret_cast<float2*>(static_cast<char*>(room) + q_bytes + seen_bytes);
     a.counters = counters;
+    if (prompt) {
+        PackArgs k{};
+        k.kc = g.k_cache;
+        k.vc = g.v_cache;
+        k.seq_stride = p.seq_stride;
+        k.n_kv = p.n_kv;
+        k.hd = p.hd;
+        k.tiles = static_cast<int>(tiles);
+        k.seqs = p.seqs;
+        k.total = p.total;
+        k.max_rows = p.max_rows;
+        k.limit = p.limit;
+        k.off = g.off;
+        k.len = g.len;
+        k.packed = static_cast<char*>(room) + q_bytes + seen_bytes + fh_align256(part);
+        k.info = reinterpret_cast<TileInfo*>(k.packed + pack);
+        return w == 32 ? launch_prompt<32>(ctx, a, k) : w == 64 ? launch_prompt<64>(ctx, a, k) : launch_prompt<128>(ctx, a, k);
+    }
     if (g.parent) return w == 32 ? launch_width<32, true>(ctx, a, cw) : w == 64 ? launch_width<64, true>(ctx, a, cw) : launch_width<128, true>(ctx, a, cw);
     return w == 32 ? launch_width<32, false>(ctx, a, cw) : w == 64 ? launch_width<64, false>(ctx, a, cw) : launch_width<128, false>(ctx, a, cw);
 }
