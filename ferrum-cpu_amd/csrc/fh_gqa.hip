@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
@@ -52,6 +53,12 @@ __device__ __forceinline__ Rows rows_of(const uint32_t* off, const uint32_t* len
     return r;
 }
 
+__device__ __forceinline__ void turn_pair(float& a, float& b, float cs, float sn) {
+    const float x = a, y = b;
+    a = x * cs - y * sn;
+    b = x * sn + y * cs;
+}
+
 // ---- rotation and storing ------------------------------------------------------------
 
 constexpr int kMaxTree = 1024;  // nodes of a sequence's tree
@@ -64,13 +71,16 @@ struct AppendArgs {
     int n_heads, n_kv, hd;
     uint32_t seqs, total, max_rows, limit;
     const uint32_t *off, *len, *pos, *parent;
-    float* q;           // [total, n_heads * hd]
+    float* q;           // [total, n_heads * hd], or NULL and
+    float2* cs;         // (nullable) [total, rope_dim / 2]: cosine and sine of a row's pairs
+    int first;          // the first head taken: 0, or without q n_heads
     uint32_t* seen;     // [total, words]: a node's path, bit a for node a
     int words;
     int rope_dim, neox;
     float linear;
     const float* ff;
     int heads_each, chunks;
+    uint32_t* clear;  // [seqs, n_kv], 1 (NULL: nowhere): set to 0
     float freq[64];
 };
 
@@ -83,6 +93,8 @@ __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
     const int slots = a.hd / 2, each = kThreads / slots;  // rows of a workgroup
     const uint32_t t0 = blockIdx.x / a.chunks * static_cast<uint32_t>(each);
     const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    if (a.clear && blockIdx.x == 0)
+        for (int h = threadIdx.x; h < a.n_kv + (s + 1 == a.seqs); h += kThreads) a.clear[s * static_cast<uint32_t>(a.n_kv) + h] = 0;
     if (t0 >= r.count) return;
     __shared__ uint32_t up[TREE ? kMaxTree : 1];
     if constexpr (TREE) {
@@ -126,15 +138,13 @@ __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
     const bool fits = c < a.limit;
     const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
     const size_t to = s * a.seq_stride + (fits ? c : 0) * kv_dim;
-    const int h1 = min(a.n_heads + 2 * a.n_kv, (chunk + 1) * a.heads_each);
-    for (int h = chunk * a.heads_each; h < h1; h++) {
+    if (a.cs && chunk == 0 && turns) a.cs[static_cast<size_t>(row) * half + slot] = make_float2(cs, sn);
+    const int h0 = a.first + chunk * a.heads_each, h1 = min(a.n_heads + 2 * a.n_kv, h0 + a.heads_each);
+    for (int h = h0; h < h1; h++) {
         const float* xh = x + static_cast<size_t>(h) * a.hd;
         const float u = xh[ia], w = xh[ib];
         float y = u, z = w;
-        if (turns && h < a.n_heads + a.n_kv) {
-            y = u * cs - w * sn;
-            z = u * sn + w * cs;
-        }
+        if (turns && h < a.n_heads + a.n_kv) turn_pair(y, z, cs, sn);
         float* dst;
         if (h < a.n_heads) {
             dst = a.q + (static_cast<size_t>(row) * a.n_heads + h) * a.hd;
@@ -152,19 +162,32 @@ __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
 
 constexpr int kKeys = 32;  // keys of a tile
 
+// Division by a number of the host's: n / d = the upper half of n * (2^64 / d + 1), exact for n < 2^32.
+struct Div {
+    uint64_t m;
+    uint32_t d;
+    Div(uint32_t by = 1) : m(by > 1 ? ~uint64_t(0) / by + 1 : 0), d(by) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return m ? static_cast<uint32_t>(__umul64hi(n, m)) : n; }
+};
+
 struct RowsArgs {
-    const float* q;  // [total, n_heads * hd], rotated
+    const float* q;  // row r's heads at r * q_ld: rotated, or with cs to be rotated
+    size_t q_ld;
+    const float2* cs;  // [total, half]: cosine and sine of a row's pairs of channels
+    int half, neox;
     const float *kc, *vc;
     size_t seq_stride;
-    int n_heads, n_kv, group, hd;
+    int n_heads, n_kv, hd;
+    Div group, pairs, kvs;  // query heads of a kv head; (sequence, kv head) pairs; kv heads
     uint32_t seqs, total, max_rows, limit;
     const uint32_t *off, *len, *seen;
     int words;
     float scale;  // log2(e) / sqrt(hd)
     float* out;
-    int col_blocks, splits;
+    int col_blocks, splits_log2;
     float2* part;
     unsigned* counters;
+    const uint32_t* apart;  // [seqs, n_kv], 1: (prompt) not 0 where the blocks are k_gqa_rest's; where any are
 };
 
 __device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
@@ -201,11 +224,17 @@ __device__ __forceinline__ float sum_halves(float v) {
     return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
 }
 
-// Two f32 values as two f16 terms each: h = f16(x), l = f16(x - h), 22 bits.
+// Two f32 values as two f16 terms each: h = f16(x), l = f16(x - h), 22 bits; x - h is one instruction of
+// mixed precision.  (The pair and the factor are kept from the compiler's view: it would
+// convert each half there and back.)
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     const h2f h = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
-    const h2f l = {static_cast<_Float16>(x - static_cast<float>(h.x)), static_cast<_Float16>(y - static_cast<float>(h.y))};
     hi = __builtin_bit_cast(uint32_t, h);
+    float minus = -1.0f;
+    asm("" : "+v"(hi), "+s"(minus));
+    const h2f k = __builtin_bit_cast(h2f, hi);
+    const h2f l = {static_cast<_Float16>(fmaf(static_cast<float>(k.x), minus, x)),
+                   static_cast<_Float16>(fmaf(static_cast<float>(k.y), minus, y))};
     lo = __builtin_bit_cast(uint32_t, l);
 }
 // The same where a value may be infinite (its lower term is 0 then).
@@ -253,9 +282,10 @@ __device__ __forceinline__ void clear(Sums<OT>& z) {
 }
 // Weights lie at 2^10 of the largest so far, and up to 2^14 before the sums are brought to a
 // new one: their lower terms stay normal numbers of f16 far below it.
+constexpr float kRaise = 14.0f;
 template <int OT>
 __device__ __forceinline__ void raise_base(Sums<OT>& z, float top) {
-    if (__any(top > z.base + 14.0f)) {
+    if (__any(top > z.base + kRaise)) {
         const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + 10.0f, max_halves(top));
         const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, f = __builtin_amdgcn_exp2f(z.base - nb);
         z.l *= f;
@@ -280,25 +310,32 @@ __device__ __forceinline__ void split8(const float* p, h8f& hi, h8f& lo) {
 // A tile with a value that is not finite: it reaches the rows that see it and no others, on
 // the vector units; w: the lane's weights of the values themselves.
 template <int W>
-__device__ __forceinline__ void add_seen(Sums<W / 32>& z, const float (&w)[16], const float* vp, size_t kv_dim, int hd, uint32_t k0,
+__device__ __forceinline__ void add_seen(Sums<W / 32>& z, float (&w)[16], const float* vp, size_t kv_dim, int hd, uint32_t k0,
                                          uint32_t keys, uint32_t seen, int half) {
-#pragma unroll
+#pragma clang loop unroll(disable)
     for (int v = 0; v < 16; v++) {
-        const uint32_t mine = __builtin_bit_cast(uint32_t, w[v]);
+        const uint32_t mine = __builtin_bit_cast(uint32_t, w[0]);
+#pragma unroll
+        for (int i = 0; i < 15; i++) w[i] = w[i + 1];
         const auto sw = __builtin_amdgcn_permlane32_swap(mine, mine, false, false);
 #pragma unroll
         for (int e = 0; e < 2; e++) {  // (lanes 0 .. 31's in sw[0], of both halves; 32 .. 63's in sw[1])
             const int j = acc_row(v, e);
             const float p = __builtin_bit_cast(float, static_cast<uint32_t>(sw[e]));
-            if (k0 + j < keys && (seen >> j & 1)) {
-                const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim;
+            if (k0 + j >= keys || !(seen >> j & 1)) continue;
+            const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim + half * 4;
 #pragma unroll
-                for (int d = 0; d < W / 32; d++)
+            for (int d = 0; d < W / 32; d++) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int dim = 32 * d + acc_row(i, half);
-                        if (W > 32 || dim < hd) z.o[d][i] += p * from[dim];
-                    }
+                for (int b = 0; b < 4; b++) {
+                    if (W == 32 && 8 * b + half * 4 >= hd) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(from + 32 * d + 8 * b);
+                    z.o[d][4 * b] += p * y.x;
+                    z.o[d][4 * b + 1] += p * y.y;
+                    z.o[d][4 * b + 2] += p * y.z;
+                    z.o[d][4 * b + 3] += p * y.w;
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (few registers for what comes seldom)
             }
         }
     }
@@ -341,12 +378,12 @@ __device__ __forceinline__ void join_waves(Sums<OT>& z, float2* room, int cw, in
         }
 }
 
-// A column's query, scaled by its own power of two, dims 16 i + 8 half + (0..7) in two f16 terms;
-// returns what undoes the power and brings scores to base 2.
+// A column's query, rotated, scaled by its own power of two, dims 16 i + 8 half + (0..7) in two f16
+// terms; returns what undoes the power and brings scores to base 2.
 template <int W>
-__device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, int head, int half, h8f (&qh)[W / 16], h8f (&ql)[W / 16]) {
+__device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, uint32_t head, int half, h8f (&qh)[W / 16], h8f (&ql)[W / 16]) {
     constexpr int KI = W / 16;
-    const float* qp = a.q + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 8;
+    const float* qp = a.q + row * a.q_ld + static_cast<size_t>(head) * a.hd + half * 8;
     float x[8 * KI];
 #pragma unroll
     for (int i = 0; i < KI; i++) {
@@ -355,6 +392,38 @@ __device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, int
         const float4 w = in ? *reinterpret_cast<const float4*>(qp + 16 * i + 4) : make_float4(0, 0, 0, 0);
         x[8 * i] = u.x; x[8 * i + 1] = u.y; x[8 * i + 2] = u.z; x[8 * i + 3] = u.w;
         x[8 * i + 4] = w.x; x[8 * i + 5] = w.y; x[8 * i + 6] = w.z; x[8 * i + 7] = w.w;
+    }
+    if (a.cs) {
+        const float2* cs = a.cs + static_cast<size_t>(row) * a.half;
+        if (a.neox) {  // (pairs of channels d, d + half; half a multiple of 16)
+            const auto turn = [&](auto steps) {
+                constexpr int S = decltype(steps)::value;
+#pragma unroll
+                for (int i = 0; i < S; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const float4 t = *reinterpret_cast<const float4*>(cs + 16 * i + half * 8 + j);
+                        turn_pair(x[8 * i + j], x[8 * (i + S) + j], t.x, t.y);
+                        turn_pair(x[8 * i + j + 1], x[8 * (i + S) + j + 1], t.z, t.w);
+                    }
+            };
+            if (W >= 128 && a.half == 64) turn(std::integral_constant<int, W >= 128 ? 4 : 1>{});
+            else if (W >= 128 && a.half == 48) turn(std::integral_constant<int, W >= 128 ? 3 : 1>{});
+            else if (W >= 64 && a.half == 32) turn(std::integral_constant<int, W >= 64 ? 2 : 1>{});
+            else turn(std::integral_constant<int, 1>{});
+        } else {
+#pragma unroll
+            for (int i = 0; i < KI; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                    const int p = (16 * i + half * 8 + j) / 2;
+                    if (p < a.half) {  // (half is even)
+                        const float4 t = *reinterpret_cast<const float4*>(cs + p);
+                        turn_pair(x[8 * i + j], x[8 * i + j + 1], t.x, t.y);
+                        turn_pair(x[8 * i + j + 2], x[8 * i + j + 3], t.z, t.w);
+                    }
+                }
+        }
     }
     uint32_t top = 0;  // (of the finite ones)
 #pragma unroll
@@ -380,9 +449,9 @@ __device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, int
 // A workgroup's sums to memory; the last of a block's workgroups joins all shares of the keys, in
 // order (true: it is this one).
 template <int OT, int CW>
-__device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint32_t unit, int split, int cw, bool mine, int lane) {
+__device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint32_t unit, uint32_t split, int cw, bool mine, int lane) {
     constexpr int PL = Sums<OT>::kParts;
-    float2* part = a.part + (static_cast<size_t>(unit) * a.splits * CW + cw) * (PL * 64) + lane;
+    float2* part = a.part + ((static_cast<size_t>(unit) << a.splits_log2) * CW + cw) * (PL * 64) + lane;
     if (mine) {
         float2* to = part + static_cast<size_t>(split) * CW * (PL * 64);
         store_part(to, make_float2(z.base, z.l));
@@ -395,13 +464,13 @@ __device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __shared__ int last;
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>(a.splits - 1);
+    if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>((1 << a.splits_log2) - 1);
     __syncthreads();
     if (!last) return false;
     if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (mine) {
         clear(z);
-        for (int k = 0; k < a.splits; k++) {
+        for (int k = 0; k < 1 << a.splits_log2; k++) {
             const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
             float2 y[PL];
 #pragma unroll
@@ -412,7 +481,7 @@ __device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint
     return true;
 }
 template <int W>
-__device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs& a, uint32_t row, int head, int half, bool bad) {
+__device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs& a, uint32_t row, uint32_t head, int half, bool bad) {
     float* out = a.out + (static_cast<size_t>(row) * a.n_heads + head) * a.hd + half * 4;
     const float f = bad ? __builtin_nanf("") : 1.0f / z.l;
 #pragma unroll
@@ -446,53 +515,84 @@ struct Stage {
     int unsafe[3][KW];          // a value that is not finite (step st: st % 3)
 };
 
+// What a workgroup is to do.  Workgroups of a sequence and kv head are dealt to as few XCDs as can be,
+// and the longest rows come first.  An XCD deals its workgroups to its four shader engines in turn and waits where
+// one is full, so the pairs of an XCD (every eighth) come in another order for each block: with one order a long
+// sequence's blocks, between others' that have none, filled one engine (16 prompts of up to 1000 rows: 228 of 512
+// workgroups ran for the first 40 us).
+template <int CW, bool TREE>
+struct Block {
+    uint32_t pair, cb, s, kv, split;
+    Rows r;
+    uint32_t ncols, c0;
+    // the wave's columns, and this lane's
+    uint32_t wc, t, row, head;
+    bool on, bad;
+    uint32_t at, own;            // keys before the call's rows; (prompt) the keys that this column sees
+    uint32_t keys, wkeys, wfull;  // of the workgroup; of the wave; those that all of its columns see
+    uint32_t tile0, tile1;
+
+    __device__ __forceinline__ bool place(const RowsArgs& a, uint32_t workgroup) {
+        const uint32_t id = a.pairs(workgroup);
+        pair = workgroup - id * a.pairs.d;
+        if (a.pairs.d % 8 == 0) {
+            const uint32_t turned = pair + 8 * id;
+            pair = turned - a.pairs(turned) * a.pairs.d;
+        }
+        split = id & ((1u << a.splits_log2) - 1);
+        cb = a.col_blocks - 1 - (id >> a.splits_log2);
+        s = a.kvs(pair);
+        kv = pair - s * a.kvs.d;
+        r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+        ncols = r.count * a.group.d;
+        c0 = cb * (32 * CW);
+        return c0 < ncols;
+    }
+    __device__ __forceinline__ uint32_t upto(const RowsArgs& a, uint32_t cols) const {
+        const uint32_t n = TREE ? r.count : a.group(min(ncols, cols) - 1) + 1;
+        return static_cast<uint32_t>(min(r.at + n, static_cast<uint64_t>(a.limit)));
+    }
+    __device__ __forceinline__ void share(const RowsArgs& a, int cw) {
+        at = static_cast<uint32_t>(min(r.at, static_cast<uint64_t>(a.limit)));
+        keys = upto(a, c0 + 32 * CW);
+        wc = c0 + cw * 32;
+        wkeys = wc >= ncols ? 0 : upto(a, wc + 32);
+        wfull = TREE ? at : wc >= ncols ? 0 : min(keys, at + a.group(wc) + 1);
+        const uint64_t tiles = (keys + kKeys - 1) / kKeys;
+        tile0 = static_cast<uint32_t>(tiles * split >> a.splits_log2);
+        tile1 = static_cast<uint32_t>(tiles * (split + 1) >> a.splits_log2);
+    }
+    __device__ __forceinline__ void column(const RowsArgs& a, int col) {
+        const uint32_t c = wc + col, cc = min(c, ncols - 1);
+        t = a.group(cc);
+        row = r.begin + t;
+        head = kv * a.group.d + (cc - t * a.group.d);
+        on = c < ncols;
+        bad = r.at + t >= a.limit;
+        own = on && !bad ? at + t + 1 : 0;
+    }
+};
+
 template <int W, int CW, int KW, bool TREE>
-__global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
+__device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<CW, TREE>& b) {
     constexpr int NW = CW * KW, KI = W / 16, OT = W / 32;
     constexpr int WK = KW * W / 16;                        // a stage's keys: pieces of 64 threads; its values as many
     constexpr int PER = (2 * WK + NW - 1) / NW;            // pieces of a wave
-    extern __shared__ __align__(16) char smem[];
     Stage<W, CW, KW>& st = *reinterpret_cast<Stage<W, CW, KW>*>(smem);
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), cw = wave % CW, kw = wave / CW;
-    const uint32_t heads = a.seqs * static_cast<uint32_t>(a.n_kv);
-    uint32_t id = blockIdx.x;
-    const uint32_t pair = id % heads;  // (the blocks of a sequence and kv head on as few XCDs as can be)
-    id /= heads;
-    const int split = static_cast<int>(id % a.splits);
-    const uint32_t cb = a.col_blocks - 1 - id / a.splits;  // (the longest rows first)
-    const uint32_t s = pair / a.n_kv;
-    const int kv = static_cast<int>(pair % a.n_kv);
-    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
-    const uint32_t ncols = r.count * static_cast<uint32_t>(a.group), c0 = cb * (32 * CW);
-    if (c0 >= ncols) return;
-
-    // this lane's column
-    const uint32_t c = c0 + cw * 32 + col, cc = min(c, ncols - 1);
-    const uint32_t t = cc / a.group, row = r.begin + t;
-    const int head = kv * a.group + static_cast<int>(cc % a.group);
-    const bool on = c < ncols, bad = r.at + t >= a.limit;
-    const uint32_t at = static_cast<uint32_t>(min(r.at, static_cast<uint64_t>(a.limit)));  // keys before the call's rows
-    const uint32_t own = on && !bad ? at + t + 1 : 0;           // (prompt) the keys this column sees
-    // the workgroup's keys, and the wave's
-    const uint32_t t_last = (min(ncols, c0 + 32 * CW) - 1) / a.group;
-    const uint32_t keys = static_cast<uint32_t>(min(r.at + (TREE ? r.count : t_last + 1), static_cast<uint64_t>(a.limit)));
-    const uint32_t wc = c0 + cw * 32;
-    const uint32_t w_last = (min(ncols, wc + 32) - 1) / a.group;
-    const uint32_t wkeys = wc >= ncols ? 0 : min(keys, static_cast<uint32_t>(min(r.at + (TREE ? r.count : w_last + 1), static_cast<uint64_t>(a.limit))));
-    const uint32_t wfull = TREE ? at : wc >= ncols ? 0 : min(keys, at + wc / a.group + 1);  // keys that all its columns see
-    const uint32_t tiles = (keys + kKeys - 1) / kKeys;
-    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits);
-    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits);
+    b.share(a, cw);
+    b.column(a, col);
+    const uint32_t keys = b.keys, at = b.at, row = b.row;
 
     h8f qh[KI], ql[KI];
-    const float qscale = load_query<W>(a, row, head, half, qh, ql);
+    const float qscale = load_query<W>(a, row, b.head, half, qh, ql);
 
     // Staging.  Piece i < WK: 512 / W keys, eight channels a thread; the others: values
     // of 128 / W quads of keys, two channels a thread.
     const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
-    const float* kp = a.kc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
-    const float* vp = a.vc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    const float* kp = a.kc + b.s * a.seq_stride + static_cast<size_t>(b.kv) * a.hd;
+    const float* vp = a.vc + b.s * a.seq_stride + static_cast<size_t>(b.kv) * a.hd;
     float x[PER][8];
     const auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {  // (the stage's first tile; past the end: its last key)
 #pragma unroll
@@ -600,19 +700,19 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
 
     Sums<OT> z;
     clear(z);
-    const int steps = static_cast<int>((tile1 - tile0 + KW - 1) / KW);
+    const int steps = static_cast<int>((b.tile1 - b.tile0 + KW - 1) / KW);
     if (threadIdx.x < 3 * KW) st.unsafe[threadIdx.x / KW][threadIdx.x % KW] = 0;
-    if (steps > 0) fetch(tile0);
+    if (steps > 0) fetch(b.tile0);
     __syncthreads();
     if (steps > 0) stash(0);
     __syncthreads();
     for (int step = 0; step < steps; step++) {
-        const uint32_t first = tile0 + step * KW, tile = first + kw, k0 = tile * kKeys;
+        const uint32_t first = b.tile0 + step * KW, tile = first + kw, k0 = tile * kKeys;
         const int buf = step & 1;
         if (step + 1 < steps) fetch(first + KW);
         const bool vbad = st.unsafe[step % 3][kw] != 0;
         if (threadIdx.x < KW) st.unsafe[(step + 2) % 3][threadIdx.x] = 0;  // (read at step - 1, written next at step + 1)
-        if (tile < tile1 && k0 < wkeys) {
+        if (tile < b.tile1 && k0 < b.wkeys) {
             f32x16 sacc = f32x16{};
 #pragma unroll
             for (int i = 0; i < KI; i++) {
@@ -624,18 +724,18 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
             }
             float u[16], up[16];
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const float4 kd = *reinterpret_cast<const float4*>(&st.kdown[buf][kw][8 * b + 4 * half]);
-                const float4 ve = *reinterpret_cast<const float4*>(&st.vexp[buf][kw][8 * b + 4 * half]);
-                const float4 vu = *reinterpret_cast<const float4*>(&st.vup[buf][kw][8 * b + 4 * half]);
-                u[4 * b] = fmaf(sacc[4 * b] * kd.x, qscale, ve.x);
-                u[4 * b + 1] = fmaf(sacc[4 * b + 1] * kd.y, qscale, ve.y);
-                u[4 * b + 2] = fmaf(sacc[4 * b + 2] * kd.z, qscale, ve.z);
-                u[4 * b + 3] = fmaf(sacc[4 * b + 3] * kd.w, qscale, ve.w);
-                up[4 * b] = vu.x; up[4 * b + 1] = vu.y; up[4 * b + 2] = vu.z; up[4 * b + 3] = vu.w;
+            for (int g = 0; g < 4; g++) {
+                const float4 kd = *reinterpret_cast<const float4*>(&st.kdown[buf][kw][8 * g + 4 * half]);
+                const float4 ve = *reinterpret_cast<const float4*>(&st.vexp[buf][kw][8 * g + 4 * half]);
+                const float4 vu = *reinterpret_cast<const float4*>(&st.vup[buf][kw][8 * g + 4 * half]);
+                u[4 * g] = fmaf(sacc[4 * g] * kd.x, qscale, ve.x);
+                u[4 * g + 1] = fmaf(sacc[4 * g + 1] * kd.y, qscale, ve.y);
+                u[4 * g + 2] = fmaf(sacc[4 * g + 2] * kd.z, qscale, ve.z);
+                u[4 * g + 3] = fmaf(sacc[4 * g + 3] * kd.w, qscale, ve.w);
+                up[4 * g] = vu.x; up[4 * g + 1] = vu.y; up[4 * g + 2] = vu.z; up[4 * g + 3] = vu.w;
             }
             uint32_t seen = ~0u;  // the tile's keys that this column sees
-            if (k0 + kKeys > wfull) {
+            if (k0 + kKeys > b.wfull) {
                 if constexpr (TREE) {
                     const uint32_t* path = a.seen + static_cast<size_t>(row) * a.words;
                     const auto word = [&](uint32_t w) { return w < static_cast<uint32_t>(a.words) ? path[w] : 0u; };
@@ -645,10 +745,10 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
                     } else {
                         seen = at - k0 >= 32 ? ~0u : word(0) << (at - k0) | ((1u << (at - k0)) - 1);
                     }
-                    seen = on && !bad ? seen : 0u;
+                    seen = b.on && !b.bad ? seen : 0u;
                     if (keys - k0 < 32) seen &= (1u << (keys - k0)) - 1;
                 } else {
-                    seen = own > k0 ? (own - k0 >= 32 ? ~0u : (1u << (own - k0)) - 1) : 0u;
+                    seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;
                 }
 #pragma unroll
                 for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
@@ -689,8 +789,27 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
         static_assert(sizeof(Stage<W, CW, KW>) >= (KW - 1) * CW * Sums<OT>::kParts * 64 * sizeof(float2), "the sums fit");
         join_waves<OT, CW, KW>(z, reinterpret_cast<float2*>(smem), cw, kw, lane);
     }
-    if (a.splits > 1 && !join_shares<OT, CW>(z, a, pair + heads * cb, split, cw, kw == 0, lane)) return;
-    if (kw == 0 && on) store_out<W>(z, a, row, head, half, bad);
+    if (a.splits_log2 && !join_shares<OT, CW>(z, a, b.pair + a.pairs.d * b.cb, b.split, cw, kw == 0, lane)) return;
+    if (kw == 0 && b.on) store_out<W>(z, a, row, b.head, half, b.bad);
+}
+
+template <int W, int CW, int KW, bool TREE>
+__global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    Block<CW, TREE> b;
+    if (b.place(a, blockIdx.x)) rows_block<W, CW, KW, TREE>(a, smem, b);
+}
+
+// The blocks that k_gqa_prompt leaves out, if there are any.
+template <int W, int CW>
+__global__ void __launch_bounds__(64 * CW, 2) k_gqa_rest(RowsArgs a, uint32_t blocks) {
+    extern __shared__ __align__(16) char smem[];
+    if (!a.apart[a.pairs.d]) return;
+    for (uint32_t id = blockIdx.x; id < blocks; id += gridDim.x) {
+        Block<CW, false> b;
+        if (b.place(a, id) && a.apart[b.pair]) rows_block<W, CW, 1, false>(a, smem, b);
+        __syncthreads();
+    }
 }
 
 // ---- prompts ---------------------------------------------------------------------------------
@@ -698,21 +817,21 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
 // Many columns read the same keys, so what a key costs beside its products is done once, in
 // a launch of its own: k_gqa_pack writes each tile of 32 keys as the MFMA operands that
 // k_gqa_prompt loads, f16 terms under one power of two for the tile's keys and one for its
-// values.  A tile whose rows' largest magnitudes lie more than 2^4 apart has one of each row's
-// own instead (a row's lower terms would fall below f16's normal numbers, its accuracy hang on
-// the rows beside it), which the weights then take key by key.
+// values.  Where a tile's rows differ by more than 2^8 in their largest magnitudes, the lower terms
+// of some would fall so far below f16's normal numbers that more than 2^-21 of a row were lost to
+// the rows beside it; and a value that is not finite has to be kept from rows that do not see it.
+// The blocks of such a (sequence, kv head) are k_gqa_rest's, in a launch behind k_gqa_prompt's (in the
+// same kernel, its registers were spilled from those of the hot loop: 16 prompts of up to 1000 rows 76 us
+// and 70 without).
 template <int W>
 struct Packed {
     _Float16 k[W / 16][2][64][8];
     _Float16 v[W / 32][2][2][64][8];
 };
 struct TileInfo {
-    float kdown[kKeys], vexp[kKeys], vup[kKeys];  // of each key: 2^-e; of each value row: -e, 2^e
-    float one[4];                                 // of all of them, where they are alike: kdown, vexp, vup
-    uint32_t flags, pad[27];
+    float kdown, vexp, vup, pad;  // 2^-e of the keys; -e and 2^e of the values
 };
-enum { kKeysApart = 1, kValuesApart = 2, kNotFinite = 4 };
-constexpr int kApart = 4;
+constexpr int kApart = 8;
 
 struct PackArgs {
     const float *kc, *vc;
@@ -722,6 +841,7 @@ struct PackArgs {
     const uint32_t *off, *len;
     char* packed;
     TileInfo* info;
+    uint32_t* apart;
 };
 
 template <int W>
@@ -760,13 +880,9 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        uint32_t m = 0, inf = 0;  // (the largest finite one; of keys the others keep their upper term alone)
+        uint32_t m = 0;  // (the largest finite one: of keys the others keep their upper term alone)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            m = mag(x[i][j]) < kInf ? max(m, mag(x[i][j])) : m;
-            inf = max(inf, mag(x[i][j]));
-        }
-        (void)inf;
+        for (int j = 0; j < 8; j++) m = mag(x[i][j]) < kInf ? max(m, mag(x[i][j])) : m;
         m = group_max<W / 8>(m);
         if (ch == 0 && key_of(i) < kKeys) top[0][key_of(i)] = m;
 #pragma unroll
@@ -783,36 +899,31 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
     int hi = used ? static_cast<int>(mine >> 23) : 0, lo = used ? static_cast<int>(mine >> 23) : 255;
     hi = static_cast<int>(group_max<32>(static_cast<uint32_t>(hi)));
     lo = 255 - static_cast<int>(group_max<32>(static_cast<uint32_t>(255 - lo)));
-    const bool apart = hi - lo > kApart;
-    const int alike = lift(static_cast<uint32_t>(hi) << 23, of ? kValueLift : kLiftMost);
-    const int e = apart ? lift(mine, of ? kValueLift : kLiftMost) : alike;
-    TileInfo& info = a.info[(static_cast<size_t>(s) * a.n_kv + kv) * a.tiles + tile];
+    const int e = lift(static_cast<uint32_t>(hi) << 23, of ? kValueLift : kLiftMost);
+    const uint32_t pair = s * static_cast<uint32_t>(a.n_kv) + kv;
     if (threadIdx.x < 64) {
-        const uint64_t bad = __ballot(of == 1 && mine >= kInf), far = __ballot(apart);
-        if (of == 0) {
-            info.kdown[lane] = pow2f(-e);
-            if (lane == 0) info.one[0] = pow2f(-alike);
-        } else {
-            info.vexp[lane - 32] = static_cast<float>(-e);
-            info.vup[lane - 32] = pow2f(e);
-            if (lane == 32) {
-                info.one[1] = static_cast<float>(-alike);
-                info.one[2] = pow2f(alike);
-                info.flags = (far & 1 ? kKeysApart : 0) | (far >> 32 ? kValuesApart : 0) | (bad ? kNotFinite : 0);
-            }
+        TileInfo& info = a.info[static_cast<size_t>(pair) * a.tiles + tile];
+        if (lane == 0) info.kdown = pow2f(-e);
+        if (lane == 32) {
+            info.vexp = static_cast<float>(-e);
+            info.vup = pow2f(e);
+        }
+        if (__any(hi - lo > kApart || (of == 1 && mine >= kInf)) && lane == 0) {
+            atomicOr(a.apart + pair, 1u);
+            atomicOr(a.apart + static_cast<uint32_t>(a.n_kv) * a.seqs, 1u);
         }
     }
-    Packed<W>& to = reinterpret_cast<Packed<W>*>(a.packed)[(static_cast<size_t>(s) * a.n_kv + kv) * a.tiles + tile];
+    const float kup = pow2f(__builtin_amdgcn_readlane(e, 0)), vup = pow2f(__builtin_amdgcn_readlane(e, 32));
+    Packed<W>& to = reinterpret_cast<Packed<W>*>(a.packed)[static_cast<size_t>(pair) * a.tiles + tile];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int k = key_of(i), q = quad_of(i);
-        const float up = pow2f(__shfl(e, k & 31, 64));
         if (k < kKeys) {
             u32x4 h, l;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 uint32_t b, c;
-                split2_any(x[i][2 * j] * up, x[i][2 * j + 1] * up, b, c);
+                split2_any(x[i][2 * j] * kup, x[i][2 * j + 1] * kup, b, c);
                 h[j] = b;
                 l[j] = c;
             }
@@ -821,11 +932,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
         }
         float z[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float vu = pow2f(__shfl(e, 32 + ((4 * q + j) & 31), 64));
-            z[j] = y[i][j] * vu;
-            z[4 + j] = y[i][4 + j] * vu;
-        }
+        for (int j = 0; j < 8; j++) z[j] = y[i][j] * vup;
         if (q < 8) {
             // keys 4 q .. + 3 are steps 4 (q / 2 % 2) .. + 3 of lane half q % 2 in product q / 4
 #pragma unroll
@@ -846,74 +953,63 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
     }
 }
 
-// 128 columns a workgroup of four waves.  Step t multiplies tile t + 1's scores while tile t's
-// become weights, and stages tile t + 2's keys and t + 1's values: the matrix and the vector
-// units have work of their own side by side.
-template <int W>
-__global__ void __launch_bounds__(kThreads, 2) k_gqa_prompt(RowsArgs a, const char* packed, const TileInfo* infos, int room) {
-    constexpr int CW = 4, KI = W / 16, OT = W / 32, PIECE = W * 128 / 16 / kThreads;  // 16-byte loads a thread, of K and of V
+// NWV waves of 32 columns a workgroup.  Step t multiplies tile t + 1's scores while tile t's become
+// weights, and stages tile t + 2's keys and t + 1's values, so that a wave has work for the matrix and
+// for the vector units side by side.  Width 128: eight waves, near the rate of a large f16 product (1 x 8192
+// rows of 32 and 8 heads 1460 us, 377 TFLOP/s or 1130 of f16 products; the clock falls as the matrix
+// units fill: 2.1 GHz where they were busy 40 % of the time, 1.7 at 60 %; four waves, each tile read
+// twice as often, 1557); 64: four, three to a SIMD (16 prompts of up to 1000 rows, 14 and 2 heads, 73
+// us; two to a SIMD 77, eight waves 90).  64 columns a wave with a SIMD to itself: 2000 and 125.
+template <int W, int NWV, int OCC>
+__global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const char* packed, const TileInfo* infos,
+                                                                     int room) {
+    constexpr int CW = NWV, KI = W / 16, OT = W / 32, NT = 64 * NWV;
+    constexpr int PIECE = W * 8 / NT;  // 16-byte loads a thread, of a tile's keys and of its values
     extern __shared__ __align__(16) char smem[];
+    Block<CW, false> b;
+    if (!b.place(a, blockIdx.x) || a.apart[b.pair]) return;
     struct Ring {
         u32x4 k[2][W * 8], v[2][W * 8];
-        TileInfo info[2];
     };
     Ring& ring = *reinterpret_cast<Ring*>(smem);
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const uint32_t heads = a.seqs * static_cast<uint32_t>(a.n_kv);
-    uint32_t id = blockIdx.x;
-    const uint32_t pair = id % heads;  // (the blocks of a sequence and kv head on as few XCDs as can be)
-    id /= heads;
-    const int split = static_cast<int>(id % a.splits);
-    const uint32_t cb = a.col_blocks - 1 - id / a.splits;  // (the longest rows first)
-    const uint32_t s = pair / a.n_kv;
-    const int kv = static_cast<int>(pair % a.n_kv);
-    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
-    const uint32_t ncols = r.count * static_cast<uint32_t>(a.group), c0 = cb * (32 * CW);
-    if (c0 >= ncols) return;
-    const uint32_t wc = c0 + wave * 32, c = wc + col, cc = min(c, ncols - 1);
-    const uint32_t t = cc / a.group, row = r.begin + t;
-    const int head = kv * a.group + static_cast<int>(cc % a.group);
-    const bool on = c < ncols, bad = r.at + t >= a.limit;
-    const uint32_t at = static_cast<uint32_t>(min(r.at, static_cast<uint64_t>(a.limit)));
-    const uint32_t own = on && !bad ? at + t + 1 : 0;  // the keys this column sees
-    const auto upto = [&](uint32_t cols) {
-        return static_cast<uint32_t>(min(r.at + (min(ncols, cols) - 1) / a.group + 1, static_cast<uint64_t>(a.limit)));
-    };
-    const uint32_t keys = upto(c0 + 32 * CW), wkeys = wc >= ncols ? 0 : upto(wc + 32);
-    const uint32_t wfull = wc >= ncols ? 0 : min(keys, at + wc / a.group + 1);  // keys that all its columns see
-    const uint32_t tiles = (keys + kKeys - 1) / kKeys, wtiles = (wkeys + kKeys - 1) / kKeys;
-    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / a.splits);
-    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / a.splits);
-    const uint32_t mine1 = min(tile1, wtiles);  // past the wave's last tile
-    const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
-    const float* vp = a.vc + s * a.seq_stride + static_cast<size_t>(kv) * a.hd;
+    b.share(a, wave);
+    const uint32_t tile0 = b.tile0, tile1 = b.tile1;
+    const uint32_t mine1 = min(tile1, (b.wkeys + kKeys - 1) / kKeys);  // past the wave's last tile
 
-    h8f qh[KI], ql[KI];
-    const float qscale = load_query<W>(a, row, head, half, qh, ql);
-
-    const u32x4* from = reinterpret_cast<const u32x4*>(packed) + static_cast<size_t>(pair) * room * (W * 16) + threadIdx.x;
-    const u32x4* from_info = reinterpret_cast<const u32x4*>(infos + static_cast<size_t>(pair) * room) + threadIdx.x;
-    constexpr int kInfo = sizeof(TileInfo) / 16;
-    u32x4 piece[PIECE], info_piece{};
+    const u32x4* from = reinterpret_cast<const u32x4*>(packed) + static_cast<size_t>(b.pair) * room * (W * 16) + threadIdx.x;
+    const TileInfo* info = infos + static_cast<size_t>(b.pair) * room;
+    u32x4 kpiece[PIECE], vpiece[PIECE];
     const auto fetch_k = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) piece[i] = from[static_cast<size_t>(tile) * (W * 16) + i * kThreads];
+        for (int i = 0; i < PIECE; i++) kpiece[i] = from[static_cast<size_t>(tile) * (W * 16) + i * NT];
     };
     const auto fetch_v = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) piece[i] = from[static_cast<size_t>(tile) * (W * 16) + W * 8 + i * kThreads];
-        if (threadIdx.x < kInfo) info_piece = from_info[static_cast<size_t>(tile) * kInfo];
+        for (int i = 0; i < PIECE; i++) vpiece[i] = from[static_cast<size_t>(tile) * (W * 16) + W * 8 + i * NT];
     };
     const auto put_k = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) ring.k[tile & 1][i * kThreads + threadIdx.x] = piece[i];
+        for (int i = 0; i < PIECE; i++) ring.k[tile & 1][i * NT + threadIdx.x] = kpiece[i];
     };
     const auto put_v = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) ring.v[tile & 1][i * kThreads + threadIdx.x] = piece[i];
-        if (threadIdx.x < kInfo) reinterpret_cast<u32x4*>(&ring.info[tile & 1])[threadIdx.x] = info_piece;
+        for (int i = 0; i < PIECE; i++) ring.v[tile & 1][i * NT + threadIdx.x] = vpiece[i];
     };
+    // (the first tiles are on their way while the queries are split)
+    const uint32_t second = min(tile0 + 1, max(tile1, 1u) - 1);
+    u32x4 ahead[PIECE];
+    if (tile0 < tile1) {
+        fetch_k(second);
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) ahead[i] = kpiece[i];
+        fetch_k(tile0);
+        fetch_v(tile0);
+    }
+    b.column(a, col);
+    h8f qh[KI], ql[KI];
+    const float qscale = load_query<W>(a, b.row, b.head, half, qh, ql);
     const auto scores = [&](uint32_t tile) __attribute__((always_inline)) {
         f32x16 x = f32x16{};
         const u32x4* k = ring.k[tile & 1] + lane;
@@ -926,84 +1022,45 @@ __global__ void __launch_bounds__(kThreads, 2) k_gqa_prompt(RowsArgs a, const ch
         }
         return x;
     };
-
     Sums<OT> z;
     clear(z);
-    f32x16 next = f32x16{};
+    f32x16 score[2] = {f32x16{}, f32x16{}};  // of even and odd steps' tiles
     if (tile0 < tile1) {
-        fetch_k(tile0);
         put_k(tile0);
-        fetch_v(tile0);
         put_v(tile0);
-        if (tile0 + 1 < tile1) {
-            fetch_k(tile0 + 1);
-            put_k(tile0 + 1);
-        }
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) kpiece[i] = ahead[i];
+        put_k(tile0 + 1);
         __syncthreads();
-        if (tile0 < mine1) next = scores(tile0);
+        score[0] = scores(tile0);
         __syncthreads();
     }
-    for (uint32_t tile = tile0; tile < tile1; tile++) {
-        const uint32_t k0 = tile * kKeys;
-        if (tile + 2 < tile1) fetch_k(tile + 2);
-        float u[16];
-        uint32_t flags = 0, seen = ~0u;
-        const TileInfo& info = ring.info[tile & 1];
-        const bool work = tile < mine1;
-        if (work) {
-            flags = __builtin_amdgcn_readfirstlane(info.flags);
-            float sc = info.one[0] * qscale, ex = info.one[1];
+    const auto step = [&](uint32_t tile, f32x16& now, f32x16& next) __attribute__((always_inline)) {
+        const uint32_t k0 = tile * kKeys, last = tile1 - 1;
+        // (past the last tile: it again, to where nothing reads it)
+        fetch_k(min(tile + 2, last));
+        fetch_v(min(tile + 1, last));
+        if (tile < mine1) {
+            const TileInfo of = info[tile];
+            if (k0 + kKeys > b.wfull) {
+                const uint32_t seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;
 #pragma unroll
-            for (int v = 0; v < 16; v++) u[v] = next[v];
-            if (__builtin_expect(flags != 0, 0)) {
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float4 kd = *reinterpret_cast<const float4*>(&info.kdown[8 * b + 4 * half]);
-                    const float4 ve = *reinterpret_cast<const float4*>(&info.vexp[8 * b + 4 * half]);
-                    u[4 * b] = fmaf(u[4 * b] * kd.x, qscale, ve.x);
-                    u[4 * b + 1] = fmaf(u[4 * b + 1] * kd.y, qscale, ve.y);
-                    u[4 * b + 2] = fmaf(u[4 * b + 2] * kd.z, qscale, ve.z);
-                    u[4 * b + 3] = fmaf(u[4 * b + 3] * kd.w, qscale, ve.w);
-                }
-                sc = 1.0f;
-                ex = 0.0f;
+                for (int v = 0; v < 16; v++) now[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? now[v] : -INFINITY;
             }
-            if (k0 + kKeys > wfull) {
-                seen = own > k0 ? (own - k0 >= 32 ? ~0u : (1u << (own - k0)) - 1) : 0u;
+            const float sc = of.kdown * qscale;
+            float top = now[0];
 #pragma unroll
-                for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
+            for (int v = 1; v < 16; v++) top = fmaxf(top, now[v]);
+            raise_base(z, fmaf(top, sc, of.vexp));
+            const float less = of.vexp - z.base;
+            float u[16], sum[4] = {};
+            next = scores(tile + 1);
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                u[v] = __builtin_amdgcn_exp2f(fmaf(now[v], sc, less));
+                sum[v & 3] += u[v];
             }
-            float top = u[0];
-#pragma unroll
-            for (int v = 1; v < 16; v++) top = fmaxf(top, u[v]);
-            raise_base(z, fmaf(top, sc, ex));
-            const float less = ex - z.base;
-            if (tile + 1 < mine1) next = scores(tile + 1);
-#pragma unroll
-            for (int v = 0; v < 16; v++) u[v] = __builtin_amdgcn_exp2f(fmaf(u[v], sc, less));
-            if (__builtin_expect(flags != 0, 0)) {
-                float w[16];
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float4 vu = *reinterpret_cast<const float4*>(&info.vup[8 * b + 4 * half]);
-                    w[4 * b] = u[4 * b] * vu.x;
-                    w[4 * b + 1] = u[4 * b + 1] * vu.y;
-                    w[4 * b + 2] = u[4 * b + 2] * vu.z;
-                    w[4 * b + 3] = u[4 * b + 3] * vu.w;
-                }
-#pragma unroll
-                for (int v = 0; v < 16; v++) z.l += w[v];
-                if (flags & kNotFinite) add_seen<W>(z, w, vp, kv_dim, a.hd, k0, keys, seen, half);
-            } else {
-                float sum[4] = {};
-#pragma unroll
-                for (int v = 0; v < 16; v++) sum[v & 3] += u[v];
-                z.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), info.one[2], z.l);
-            }
-        }
-        if (tile + 2 < tile1) put_k(tile + 2);
-        if (tile + 1 < tile1) fetch_v(tile + 1);
-        if (work && !(flags & kNotFinite)) {
+            z.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), of.vup, z.l);
             const u32x4* v = ring.v[tile & 1] + lane;
 #pragma unroll
             for (int s2 = 0; s2 < 2; s2++) {
@@ -1019,12 +1076,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_gqa_prompt(RowsArgs a, const ch
                 }
             }
         }
-        if (tile + 1 < tile1) put_v(tile + 1);
+        put_k(tile + 2);
+        put_v(tile + 1);
         __syncthreads();
+    };
+    for (uint32_t tile = tile0; tile < tile1; tile += 2) {
+        step(tile, score[0], score[1]);
+        if (tile + 1 == tile1) break;
+        step(tile + 1, score[1], score[0]);
     }
     z.l = sum_halves(z.l);
-    if (a.splits > 1 && !join_shares<OT, CW>(z, a, pair + heads * cb, split, wave, true, lane)) return;
-    if (on) store_out<W>(z, a, row, head, half, bad);
+    if (a.splits_log2 && !join_shares<OT, CW>(z, a, b.pair + a.pairs.d * b.cb, b.split, wave, true, lane)) return;
+    if (b.on) store_out<W>(z, a, b.row, b.head, half, b.bad);
 }
 
 constexpr size_t kUnits = 8192;  // column blocks whose keys may be split
@@ -1036,22 +1099,27 @@ int launch_rows(fh_ctx* ctx, const RowsArgs& a) {
     const auto kern = k_gqa_rows<W, CW, KW, TREE>;
     if (lds > 64 * 1024)
         FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.splits * a.col_blocks)), dim3(64 * CW * KW), lds,
+    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.col_blocks << a.splits_log2)), dim3(64 * CW * KW), lds,
                        ctx->stream, a);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
 
-template <int W>
+template <int W, int NWV, int OCC>
 int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p) {
-    hipLaunchKernelGGL(k_gqa_pack<W>, dim3(p.tiles, a.n_kv, a.seqs), dim3(kThreads), 0, ctx->stream, p);
+    hipLaunchKernelGGL(k_gqa_pack<W>, dim3(p.tiles, a.kvs.d, a.seqs), dim3(kThreads), 0, ctx->stream, p);
     FH_HIP(ctx, hipGetLastError());
-    constexpr size_t lds = 2 * W * 256 + 2 * sizeof(TileInfo);
-    const auto kern = k_gqa_prompt<W>;
-    if (lds > 64 * 1024)
-        FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.splits * a.col_blocks)), dim3(kThreads), lds,
-                       ctx->stream, a, p.packed, p.info, p.tiles);
+    constexpr size_t lds = 2 * W * 256;
+    static_assert(lds <= 64 * 1024, "without a larger limit");
+    hipLaunchKernelGGL((k_gqa_prompt<W, NWV, OCC>), dim3(a.pairs.d * static_cast<uint32_t>(a.col_blocks << a.splits_log2)),
+                       dim3(64 * NWV), lds, ctx->stream, a, p.packed, p.info, p.tiles);
+    FH_HIP(ctx, hipGetLastError());
+    constexpr size_t rest = sizeof(Stage<W, NWV, 1>);
+    const auto kern = k_gqa_rest<W, NWV>;
+    if (rest > 64 * 1024)
+        FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rest)));
+    const uint32_t blocks = a.pairs.d * static_cast<uint32_t>(a.col_blocks << a.splits_log2);
+    hipLaunchKernelGGL(kern, dim3(std::min(blocks, static_cast<uint32_t>(ctx->num_cus))), dim3(64 * NWV), rest, ctx->stream, a, blocks);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
@@ -1072,14 +1140,15 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const int w = g.hd <= 32 ? 32 : static_cast<int>(g.hd);
     const size_t tiles = (g.limit + kKeys - 1) / kKeys, pack = heads * tiles * (static_cast<size_t>(w) * 256);
     const bool prompt = !g.parent && cols > 512 && pack < (size_t(1) << 31);
-    const int cw = prompt ? 4 : cols > 128 ? 8 : cols > 64 ? 4 : 2;
+    const int cw = prompt ? (w == 128 ? 8 : 4) : cols > 128 ? 8 : cols > 64 ? 4 : 2;
     const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
     // Keys of few columns are dealt over several workgroups, four tiles of keys each at least.
-    const size_t cus = static_cast<size_t>(ctx->num_cus), places = prompt ? 2 * cus : cus;
-    size_t splits = 1;
-    while (splits < 64 && heads * blocks * splits * 2 <= places && splits * 2 * 4 <= tiles) splits *= 2;
-    if (heads * blocks > kUnits) splits = 1;
+    const size_t cus = static_cast<size_t>(ctx->num_cus), places = cus;
+    int splits_log2 = 0;
+    while (splits_log2 < 6 && heads * blocks << (splits_log2 + 1) <= places && size_t(8) << splits_log2 <= tiles) splits_log2++;
+    if (heads * blocks > kUnits) splits_log2 = 0;
+    const size_t splits = size_t(1) << splits_log2;
     unsigned* counters = nullptr;
     if (splits > 1) {
         void* area = nullptr;
@@ -1087,10 +1156,16 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
         if (rc) return rc;
         counters = static_cast<unsigned*>(area);
     }
-    const size_t q_bytes = fh_align256(g.total * g.n_heads * g.hd * sizeof(float));
+    // Queries are rotated where they are loaded, from a table of their rows' cosines and sines; where a load
+    // has not both channels of its pairs, or is not aligned, by the first launch (12700 rows of 14 and 2 heads of
+    // width 64: 9.5 us of it against 21).
+    const size_t half = g.rope_dim / 2;
+    const bool copy = (reinterpret_cast<uintptr_t>(g.qkv) | g.ld * sizeof(float)) % 16 != 0 ||
+                      (g.rope_dim && (g.rope_type == FH_ROPE_NEOX ? half % 16 != 0 : half % 2 != 0));
+    const size_t q_bytes = fh_align256(copy ? g.total * g.n_heads * g.hd * sizeof(float) : g.total * half * sizeof(float2));
     const size_t seen_bytes = fh_align256(g.total * words * sizeof(uint32_t));
     const size_t part = splits > 1 ? heads * blocks * splits * cw * (1 + w / 4) * 64 * sizeof(float2) : 0;
-    const size_t info_bytes = prompt ? heads * tiles * sizeof(TileInfo) : 0;
+    const size_t info_bytes = prompt ? heads * tiles * sizeof(TileInfo) + (heads + 1) * sizeof(uint32_t) : 0;
     void* room = nullptr;
     const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + fh_align256(part) + (prompt ? pack + info_bytes : 0), &room);
     if (rc) return rc;
@@ -1112,7 +1187,16 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     p.len = g.len;
     p.pos = g.pos;
     p.parent = g.parent;
-    p.q = static_cast<float*>(room);
+    PackArgs k{};
+    if (prompt) {
+        k.packed = static_cast<char*>(room) + q_bytes + seen_bytes + fh_align256(part);
+        k.info = reinterpret_cast<TileInfo*>(k.packed + pack);
+        k.apart = reinterpret_cast<uint32_t*>(k.info + heads * tiles);
+        p.clear = k.apart;
+    }
+    if (copy) p.q = static_cast<float*>(room);
+    else if (half) p.cs = static_cast<float2*>(room);
+    p.first = copy ? 0 : static_cast<int>(g.n_heads);
     p.seen = reinterpret_cast<uint32_t*>(static_cast<char*>(room) + q_bytes);
     p.words = words;
     p.rope_dim = static_cast<int>(g.rope_dim);
@@ -1122,7 +1206,7 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     // (the frequencies as fh_rope_async forms them: in 64 bits, then rounded)
     for (size_t i = 0; i < g.rope_dim / 2; i++)
         p.freq[i] = static_cast<float>(std::pow(static_cast<double>(g.base), -2.0 * static_cast<double>(i) / static_cast<double>(g.rope_dim)));
-    const size_t each = 2 * kThreads / g.hd, row_blocks = (g.max_rows + each - 1) / each, all = g.n_heads + 2 * g.n_kv;
+    const size_t each = 2 * kThreads / g.hd, row_blocks = (g.max_rows + each - 1) / each, all = (copy ? g.n_heads : 0) + 2 * g.n_kv;
     size_t chunks = 1;
     while (chunks < all && row_blocks * g.seqs * chunks < 4 * cus) chunks *= 2;
     p.heads_each = static_cast<int>((all + chunks - 1) / chunks);
@@ -1133,13 +1217,19 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     FH_HIP(ctx, hipGetLastError());
 
     RowsArgs a{};
-    a.q = p.q;
+    a.q = copy ? p.q : g.qkv;
+    a.q_ld = copy ? g.n_heads * g.hd : g.ld;
+    a.cs = p.cs;
+    a.half = static_cast<int>(half);
+    a.neox = p.neox;
     a.kc = g.k_cache;
     a.vc = g.v_cache;
     a.seq_stride = p.seq_stride;
     a.n_heads = p.n_heads;
     a.n_kv = p.n_kv;
-    a.group = static_cast<int>(group);
+    a.group = Div(static_cast<uint32_t>(group));
+    a.pairs = Div(static_cast<uint32_t>(heads));
+    a.kvs = Div(static_cast<uint32_t>(g.n_kv));
     a.hd = p.hd;
     a.seqs = p.seqs;
     a.total = p.total;
@@ -1152,11 +1242,11 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     a.scale = kLog2e / sqrtf(static_cast<float>(g.hd));
     a.out = g.out;
     a.col_blocks = static_cast<int>(blocks);
-    a.splits = static_cast<int>(splits);
+    a.splits_log2 = splits_log2;
     a.part = reinterpret_cast<float2*>(static_cast<char*>(room) + q_bytes + seen_bytes);
     a.counters = counters;
     if (prompt) {
-        PackArgs k{};
+        a.apart = k.apart;
         k.kc = g.k_cache;
         k.vc = g.v_cache;
         k.seq_stride = p.seq_stride;
@@ -1169,9 +1259,7 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
         k.limit = p.limit;
         k.off = g.off;
         k.len = g.len;
-        k.packed = static_cast<char*>(room) + q_bytes + seen_bytes + fh_align256(part);
-        k.info = reinterpret_cast<TileInfo*>(k.packed + pack);
-        return w == 32 ? launch_prompt<32>(ctx, a, k) : w == 64 ? launch_prompt<64>(ctx, a, k) : launch_prompt<128>(ctx, a, k);
+        return w == 32 ? launch_prompt<32, 4, 3>(ctx, a, k) : w == 64 ? launch_prompt<64, 4, 3>(ctx, a, k) : launch_prompt<128, 8, 2>(ctx, a, k);
     }
     if (g.parent) return w == 32 ? launch_width<32, true>(ctx, a, cw) : w == 64 ? launch_width<64, true>(ctx, a, cw) : launch_width<128, true>(ctx, a, cw);
     return w == 32 ? launch_width<32, false>(ctx, a, cw) : w == 64 ? launch_width<64, false>(ctx, a, cw) : launch_width<128, false>(ctx, a, cw);
