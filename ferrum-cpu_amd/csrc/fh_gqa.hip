@@ -307,38 +307,32 @@ __device__ __forceinline__ void split8(const float* p, h8f& hi, h8f& lo) {
     hi = __builtin_bit_cast(h8f, h);
     lo = __builtin_bit_cast(h8f, l);
 }
-// A tile with a value that is not finite: it reaches the rows that see it and no others, on
-// the vector units; w: the lane's weights of the values themselves.
-template <int W>
-__device__ __forceinline__ void add_seen(Sums<W / 32>& z, float (&w)[16], const float* vp, size_t kv_dim, int hd, uint32_t k0,
-                                         uint32_t keys, uint32_t seen, int half) {
-#pragma clang loop unroll(disable)
-    for (int v = 0; v < 16; v++) {
-        const uint32_t mine = __builtin_bit_cast(uint32_t, w[0]);
+// Eight channels times 2^e.
+__device__ __forceinline__ void split8(const float* x, float up, h8f& hi, h8f& lo) {
+    u32x4 h, l;
 #pragma unroll
-        for (int i = 0; i < 15; i++) w[i] = w[i + 1];
-        const auto sw = __builtin_amdgcn_permlane32_swap(mine, mine, false, false);
-#pragma unroll
-        for (int e = 0; e < 2; e++) {  // (lanes 0 .. 31's in sw[0], of both halves; 32 .. 63's in sw[1])
-            const int j = acc_row(v, e);
-            const float p = __builtin_bit_cast(float, static_cast<uint32_t>(sw[e]));
-            if (k0 + j >= keys || !(seen >> j & 1)) continue;
-            const float* from = vp + static_cast<size_t>(k0 + j) * kv_dim + half * 4;
-#pragma unroll
-            for (int d = 0; d < W / 32; d++) {
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    if (W == 32 && 8 * b + half * 4 >= hd) continue;
-                    const float4 y = *reinterpret_cast<const float4*>(from + 32 * d + 8 * b);
-                    z.o[d][4 * b] += p * y.x;
-                    z.o[d][4 * b + 1] += p * y.y;
-                    z.o[d][4 * b + 2] += p * y.z;
-                    z.o[d][4 * b + 3] += p * y.w;
-                }
-                __builtin_amdgcn_sched_barrier(0);  // (few registers for what comes seldom)
-            }
-        }
+    for (int j = 0; j < 4; j++) {
+        uint32_t a, b;
+        split2(x[2 * j] * up, x[2 * j + 1] * up, a, b);
+        h[j] = a;
+        l[j] = b;
     }
+    hi = __builtin_bit_cast(h8f, h);
+    lo = __builtin_bit_cast(h8f, l);
+}
+// The same where some may be infinite (any, the same in all lanes).
+__device__ __forceinline__ void split8(const float* x, float up, bool any, h8f& hi, h8f& lo) {
+    u32x4 h, l;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t a, b;
+        if (__builtin_expect(any, 0)) split2_any(x[2 * j] * up, x[2 * j + 1] * up, a, b);
+        else split2(x[2 * j] * up, x[2 * j + 1] * up, a, b);
+        h[j] = a;
+        l[j] = b;
+    }
+    hi = __builtin_bit_cast(h8f, h);
+    lo = __builtin_bit_cast(h8f, l);
 }
 template <int OT>
 __device__ __forceinline__ void add_sums(Sums<OT>& z, const float2 (&y)[Sums<OT>::kParts]) {
@@ -425,25 +419,21 @@ __device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, uin
                 }
         }
     }
-    uint32_t top = 0;  // (of the finite ones)
+    float top = 0.0f;  // (NaN aside)
 #pragma unroll
-    for (int i = 0; i < 8 * KI; i++) top = mag(x[i]) < kInf ? max(top, mag(x[i])) : top;
-    const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-    const int e = lift(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])), kLiftMost);
+    for (int i = 0; i < 8 * KI; i++) top = fmaxf(top, fabsf(x[i]));
+    top = max_halves(top);
+    const bool any = __any(mag(top) == kInf);
+    if (any) {
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8 * KI; i++) top = mag(x[i]) < kInf ? fmaxf(top, fabsf(x[i])) : top;
+        top = max_halves(top);
+    }
+    const int e = lift(mag(top), kLiftMost);
     const float up = pow2f(e);
 #pragma unroll
-    for (int i = 0; i < KI; i++) {
-        u32x4 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t h, l;
-            split2_any(x[8 * i + 2 * j] * up, x[8 * i + 2 * j + 1] * up, h, l);
-            hi[j] = h;
-            lo[j] = l;
-        }
-        qh[i] = __builtin_bit_cast(h8f, hi);
-        ql[i] = __builtin_bit_cast(h8f, lo);
-    }
+    for (int i = 0; i < KI; i++) split8(x + 8 * i, up, any, qh[i], ql[i]);
     return pow2f(-e) * a.scale;
 }
 // A workgroup's sums to memory; the last of a block's workgroups joins all shares of the keys, in
@@ -470,12 +460,15 @@ __device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint
     if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (mine) {
         clear(z);
-        for (int k = 0; k < 1 << a.splits_log2; k++) {
+        for (int k = 0; k < 1 << a.splits_log2; k += 2) {  // (two shares' loads at once)
             const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
-            float2 y[PL];
+            float2 y[2][PL];
 #pragma unroll
-            for (int i = 0; i < PL; i++) y[i] = load_part(from + i * 64);
-            add_sums(z, y);
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < PL; i++) y[j][i] = load_part(from + j * CW * (PL * 64) + i * 64);
+            add_sums(z, y[0]);
+            add_sums(z, y[1]);
         }
     }
     return true;
@@ -509,10 +502,10 @@ struct Stage {
     static constexpr int KI = W / 16, OT = W / 32;
     _Float16 k[2][KW][KI][2][64][8];
     _Float16 v[2][KW][OT][2][2][64][8];
-    float kdown[2][KW][kKeys];  // 2^-e of a key
+    float kdown[4][KW][kKeys];  // 2^-e of a key (step st: st % 4)
     float vexp[2][KW][kKeys];   // -e of a value row
     float vup[2][KW][kKeys];    // 2^e of it
-    int unsafe[3][KW];          // a value that is not finite (step st: st % 3)
+    uint32_t poison[3][KW];     // keys with a value that is not finite (step st: st % 3)
 };
 
 // What a workgroup is to do.  Workgroups of a sequence and kv head are dealt to as few XCDs as can be,
@@ -576,163 +569,175 @@ struct Block {
 template <int W, int CW, int KW, bool TREE>
 __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<CW, TREE>& b) {
     constexpr int NW = CW * KW, KI = W / 16, OT = W / 32;
-    constexpr int WK = KW * W / 16;                        // a stage's keys: pieces of 64 threads; its values as many
-    constexpr int PER = (2 * WK + NW - 1) / NW;            // pieces of a wave
+    constexpr int WK = KW * W / 16;            // a stage's keys in pieces of 64 threads; its values in as many
+    constexpr int PER = (WK + NW - 1) / NW;    // pieces of either that a wave has; where there are more waves than pieces,
+    constexpr int V0 = WK < NW ? NW - WK : 0;  // the first waves have the keys', the last the values'
     Stage<W, CW, KW>& st = *reinterpret_cast<Stage<W, CW, KW>*>(smem);
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), cw = wave % CW, kw = wave / CW;
     b.share(a, cw);
-    b.column(a, col);
-    const uint32_t keys = b.keys, at = b.at, row = b.row;
-
-    h8f qh[KI], ql[KI];
-    const float qscale = load_query<W>(a, row, b.head, half, qh, ql);
-
-    // Staging.  Piece i < WK: 512 / W keys, eight channels a thread; the others: values
-    // of 128 / W quads of keys, two channels a thread.
+    const uint32_t keys = b.keys, at = b.at;
+    // Staging.  A piece of keys: 512 / W of them, eight channels a thread; of values: 128 / W quads of keys,
+    // two channels a thread.
     const size_t kv_dim = static_cast<size_t>(a.n_kv) * a.hd;
     const float* kp = a.kc + b.s * a.seq_stride + static_cast<size_t>(b.kv) * a.hd;
     const float* vp = a.vc + b.s * a.seq_stride + static_cast<size_t>(b.kv) * a.hd;
-    float x[PER][8];
-    const auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {  // (the stage's first tile; past the end: its last key)
+    const int kd = lane % (W / 8) * 8, vd = lane % (W / 2) * 2;  // the thread's channels
+    const bool kin = W > 32 || kd < a.hd, vin = W > 32 || vd < a.hd;
+    typedef float Pieces[PER][8];
+    // (tile: the stage's first; past the end: its last key)
+    const auto fetch_k = [&](uint32_t tile, Pieces& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int p = wave + i * NW;
-            if (p < WK) {
-                const int k = p * (512 / W) + lane / (W / 8), d = lane % (W / 8) * 8;
-                const float* from = kp + static_cast<size_t>(min(tile * kKeys + k, keys - 1)) * kv_dim + d;
-                const bool in = W > 32 || d < a.hd;
-                const float4 u = in ? *reinterpret_cast<const float4*>(from) : make_float4(0, 0, 0, 0);
-                const float4 w = in ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0, 0, 0, 0);
-                x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
-                x[i][4] = w.x; x[i][5] = w.y; x[i][6] = w.z; x[i][7] = w.w;
-            } else if (p < 2 * WK) {
-                const int q = (p - WK) * (128 / W) + lane / (W / 2), d = lane % (W / 2) * 2;
-                const bool in = W > 32 || d < a.hd;
+            if (WK % NW != 0 && p >= WK) continue;
+            const int k = p * (512 / W) + lane / (W / 8);
+            const float* from = kp + static_cast<size_t>(min(tile * kKeys + k, keys - 1)) * kv_dim + kd;
+            const float4 u = kin ? *reinterpret_cast<const float4*>(from) : make_float4(0, 0, 0, 0);
+            const float4 w = kin ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0, 0, 0, 0);
+            x[i][0] = u.x; x[i][1] = u.y; x[i][2] = u.z; x[i][3] = u.w;
+            x[i][4] = w.x; x[i][5] = w.y; x[i][6] = w.z; x[i][7] = w.w;
+        }
+    };
+    const auto fetch_v = [&](uint32_t tile, Pieces& x) __attribute__((always_inline)) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float* from = vp + static_cast<size_t>(min(tile * kKeys + 4 * q + j, keys - 1)) * kv_dim + d;
-                    const float2 u = in ? *reinterpret_cast<const float2*>(from) : make_float2(0, 0);
-                    x[i][j] = u.x;
-                    x[i][4 + j] = u.y;
-                }
+        for (int i = 0; i < PER; i++) {
+            const int p = wave - V0 + i * NW;
+            if (V0 && p < 0) continue;
+            const int q = p * (128 / W) + lane / (W / 2);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float* from = vp + static_cast<size_t>(min(tile * kKeys + 4 * q + j, keys - 1)) * kv_dim + vd;
+                const float2 u = vin ? *reinterpret_cast<const float2*>(from) : make_float2(0, 0);
+                x[i][j] = u.x;
+                x[i][4 + j] = u.y;
             }
         }
     };
-    const auto stash = [&](int step) __attribute__((always_inline)) {
-        const int buf = step & 1;
+    // (A key with an infinity has a scale that leaves its other channels nothing, and an infinity less itself as a
+    // lower term: its score is NaN, as that of a key with a NaN is.)
+    const auto stash_k = [&](uint32_t step, Pieces& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int p = wave + i * NW;
-            if (p < WK) {
-                const int k = p * (512 / W) + lane / (W / 8), ch = lane % (W / 8);
-                uint32_t top = 0;
+            if (WK % NW != 0 && p >= WK) continue;
+            const int k = p * (512 / W) + lane / (W / 8), kt = k / kKeys, kk = k % kKeys;
+            float most = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) top = max(top, mag(x[i][j]));
-                top = group_max<W / 8>(top);
-                u32x4 hi, lo;
-                int e;
-                if (__builtin_expect(__ballot(top >= kInf) != 0, 0)) {
-                    uint32_t fin = 0;
+            for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[i][j]));
+            const int e = lift(group_max<W / 8>(mag(most)), kLiftMost);
+            h8f hi, lo;
+            split8(x[i], pow2f(e), hi, lo);
+            *reinterpret_cast<h8f*>(st.k[step & 1][kt][kd >> 4][0][(kd & 8) * 4 + kk]) = hi;
+            *reinterpret_cast<h8f*>(st.k[step & 1][kt][kd >> 4][1][(kd & 8) * 4 + kk]) = lo;
+            if (kd == 0) st.kdown[step & 3][kt][kk] = pow2f(-e);
+        }
+    };
+    const auto stash_v = [&](uint32_t step, Pieces& x) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) fin = mag(x[i][j]) < kInf ? max(fin, mag(x[i][j])) : fin;
-                    e = lift(group_max<W / 8>(fin), kLiftMost);
+        for (int i = 0; i < PER; i++) {
+            const int p = wave - V0 + i * NW;
+            if (V0 && p < 0) continue;
+            const int q = p * (128 / W) + lane / (W / 2), kt = q >> 3, qq = q & 7;
+            float y[8], ex[4], up[4];
+            uint32_t bad = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t h, l;
-                        split2_any(x[i][2 * j] * pow2f(e), x[i][2 * j + 1] * pow2f(e), h, l);
-                        hi[j] = h;
-                        lo[j] = l;
-                    }
-                } else {
-                    e = lift(top, kLiftMost);
+            for (int j = 0; j < 4; j++) {
+                const uint32_t top = group_max<W / 2>(max(mag(x[i][j]), mag(x[i][4 + j])));
+                const int e = lift(top, kValueLift);
+                up[j] = pow2f(e);
+                ex[j] = static_cast<float>(-e);
+                y[j] = x[i][j] * up[j];
+                y[4 + j] = x[i][4 + j] * up[j];
+                bad |= (top >= kInf ? 1u : 0u) << j;
+            }
+            if (__builtin_expect(__any(bad != 0), 0)) {  // (kept out of the sums; the rows that see it are told by its bit)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t h, l;
-                        split2(x[i][2 * j] * pow2f(e), x[i][2 * j + 1] * pow2f(e), h, l);
-                        hi[j] = h;
-                        lo[j] = l;
-                    }
-                }
-                const int kt = k / kKeys, kk = k % kKeys;
-                *reinterpret_cast<u32x4*>(st.k[buf][kt][ch >> 1][0][(ch & 1) * 32 + kk]) = hi;
-                *reinterpret_cast<u32x4*>(st.k[buf][kt][ch >> 1][1][(ch & 1) * 32 + kk]) = lo;
-                if (ch == 0) st.kdown[buf][kt][kk] = pow2f(-e);
-            } else if (p < 2 * WK) {
-                const int q = (p - WK) * (128 / W) + lane / (W / 2), d = lane % (W / 2) * 2;
-                const int kt = q >> 3, qq = q & 7;
-                float y[8], ex[4], up[4];
-                uint32_t most = 0;
+                for (int j = 0; j < 8; j++) y[j] = bad >> (j & 3) & 1 ? 0.0f : y[j];
+                if (vd == 0 && bad) atomicOr(&st.poison[step % 3][kt], bad << (4 * qq));
+            }
+            // keys 4 qq .. + 3 are steps 4 jq .. + 3 of lane half hq in product s2
+            const int s2 = qq >> 2, jq = qq >> 1 & 1, hq = qq & 1;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t top = group_max<W / 2>(max(mag(x[i][j]), mag(x[i][4 + j])));
-                    most = max(most, top);
-                    const int e = lift(top, kValueLift);
-                    up[j] = pow2f(e);
-                    ex[j] = static_cast<float>(-e);
-                    y[j] = x[i][j] * up[j];
-                    y[4 + j] = x[i][4 + j] * up[j];
-                }
-                // keys 4 qq .. + 3 are steps 4 jq .. + 3 of lane half hq in product s2
-                const int s2 = qq >> 2, jq = qq >> 1 & 1, hq = qq & 1;
-#pragma unroll
-                for (int ch = 0; ch < 2; ch++) {
-                    u32x2 hi, lo;
-                    uint32_t h, l;
-                    split2(y[4 * ch], y[4 * ch + 1], h, l);
-                    hi[0] = h;
-                    lo[0] = l;
-                    split2(y[4 * ch + 2], y[4 * ch + 3], h, l);
-                    hi[1] = h;
-                    lo[1] = l;
-                    const int dd = d + ch;
-                    *reinterpret_cast<u32x2*>(&st.v[buf][kt][dd >> 5][s2][0][hq * 32 + (dd & 31)][4 * jq]) = hi;
-                    *reinterpret_cast<u32x2*>(&st.v[buf][kt][dd >> 5][s2][1][hq * 32 + (dd & 31)][4 * jq]) = lo;
-                }
-                if (d == 0) {
-                    *reinterpret_cast<float4*>(&st.vexp[buf][kt][4 * qq]) = make_float4(ex[0], ex[1], ex[2], ex[3]);
-                    *reinterpret_cast<float4*>(&st.vup[buf][kt][4 * qq]) = make_float4(up[0], up[1], up[2], up[3]);
-                }
-                if (__builtin_expect(most >= kInf, 0)) st.unsafe[step % 3][kt] = 1;
+            for (int ch = 0; ch < 2; ch++) {
+                u32x2 hi, lo;
+                uint32_t h, l;
+                split2(y[4 * ch], y[4 * ch + 1], h, l);
+                hi[0] = h;
+                lo[0] = l;
+                split2(y[4 * ch + 2], y[4 * ch + 3], h, l);
+                hi[1] = h;
+                lo[1] = l;
+                const int dd = vd + ch;
+                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][0][hq * 32 + (dd & 31)][4 * jq]) = hi;
+                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][1][hq * 32 + (dd & 31)][4 * jq]) = lo;
+            }
+            if (vd == 0) {
+                *reinterpret_cast<float4*>(&st.vexp[step & 1][kt][4 * qq]) = make_float4(ex[0], ex[1], ex[2], ex[3]);
+                *reinterpret_cast<float4*>(&st.vup[step & 1][kt][4 * qq]) = make_float4(up[0], up[1], up[2], up[3]);
             }
         }
     };
 
     Sums<OT> z;
     clear(z);
-    const int steps = static_cast<int>((b.tile1 - b.tile0 + KW - 1) / KW);
-    if (threadIdx.x < 3 * KW) st.unsafe[threadIdx.x / KW][threadIdx.x % KW] = 0;
-    if (steps > 0) fetch(b.tile0);
-    __syncthreads();
-    if (steps > 0) stash(0);
-    __syncthreads();
-    for (int step = 0; step < steps; step++) {
+    const uint32_t steps = (b.tile1 - b.tile0 + KW - 1) / KW;
+    if (threadIdx.x < 3 * KW) st.poison[threadIdx.x / KW][threadIdx.x % KW] = 0;
+    Pieces kx, vx;
+    h8f qh[KI], ql[KI];
+    float qscale;
+    {
+        Pieces first;
+        if (steps) {
+            fetch_k(b.tile0, first);
+            fetch_v(b.tile0, vx);
+            fetch_k(b.tile0 + KW, kx);
+        }
+        b.column(a, col);
+        qscale = load_query<W>(a, b.row, b.head, half, qh, ql);
+        if (steps) {
+            __syncthreads();  // (the poison is clear)
+            stash_k(0, first);
+            stash_v(0, vx);
+            stash_k(1, kx);
+            fetch_k(b.tile0 + 2 * KW, kx);
+            fetch_v(b.tile0 + KW, vx);
+        }
+    }
+    const uint32_t row = b.row;
+    const auto scores = [&](uint32_t step) __attribute__((always_inline)) {
+        f32x16 x = f32x16{};
+#pragma unroll
+        for (int i = 0; i < KI; i++) {
+            const h8f kh = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][i][0][lane]);
+            const h8f kl = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][i][1][lane]);
+            x = mfma(kl, qh[i], x);
+            x = mfma(kh, ql[i], x);
+            x = mfma(kh, qh[i], x);
+        }
+        return x;
+    };
+    f32x16 score[2] = {f32x16{}, f32x16{}};  // of even and odd steps' tiles
+    if (steps) {
+        __syncthreads();
+        score[0] = scores(0);
+        __syncthreads();
+    }
+    // Step t multiplies the next tiles' scores while this one's become weights, and stages what comes after them.
+    const auto work = [&](uint32_t step, f32x16& u, f32x16& next) __attribute__((always_inline)) {
         const uint32_t first = b.tile0 + step * KW, tile = first + kw, k0 = tile * kKeys;
         const int buf = step & 1;
-        if (step + 1 < steps) fetch(first + KW);
-        const bool vbad = st.unsafe[step % 3][kw] != 0;
-        if (threadIdx.x < KW) st.unsafe[(step + 2) % 3][threadIdx.x] = 0;  // (read at step - 1, written next at step + 1)
+        const uint32_t poison = __builtin_amdgcn_readfirstlane(st.poison[step % 3][kw]);
+        if (threadIdx.x < KW) st.poison[(step + 2) % 3][threadIdx.x] = 0;  // (read at step - 1, written next at step + 1)
         if (tile < b.tile1 && k0 < b.wkeys) {
-            f32x16 sacc = f32x16{};
-#pragma unroll
-            for (int i = 0; i < KI; i++) {
-                const h8f kh = *reinterpret_cast<const h8f*>(st.k[buf][kw][i][0][lane]);
-                const h8f kl = *reinterpret_cast<const h8f*>(st.k[buf][kw][i][1][lane]);
-                sacc = mfma(kl, qh[i], sacc);
-                sacc = mfma(kh, ql[i], sacc);
-                sacc = mfma(kh, qh[i], sacc);
-            }
-            float u[16], up[16];
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const float4 kd = *reinterpret_cast<const float4*>(&st.kdown[buf][kw][8 * g + 4 * half]);
+                const float4 down = *reinterpret_cast<const float4*>(&st.kdown[step & 3][kw][8 * g + 4 * half]);
                 const float4 ve = *reinterpret_cast<const float4*>(&st.vexp[buf][kw][8 * g + 4 * half]);
-                const float4 vu = *reinterpret_cast<const float4*>(&st.vup[buf][kw][8 * g + 4 * half]);
-                u[4 * g] = fmaf(sacc[4 * g] * kd.x, qscale, ve.x);
-                u[4 * g + 1] = fmaf(sacc[4 * g + 1] * kd.y, qscale, ve.y);
-                u[4 * g + 2] = fmaf(sacc[4 * g + 2] * kd.z, qscale, ve.z);
-                u[4 * g + 3] = fmaf(sacc[4 * g + 3] * kd.w, qscale, ve.w);
-                up[4 * g] = vu.x; up[4 * g + 1] = vu.y; up[4 * g + 2] = vu.z; up[4 * g + 3] = vu.w;
+                u[4 * g] = fmaf(u[4 * g] * down.x, qscale, ve.x);
+                u[4 * g + 1] = fmaf(u[4 * g + 1] * down.y, qscale, ve.y);
+                u[4 * g + 2] = fmaf(u[4 * g + 2] * down.z, qscale, ve.z);
+                u[4 * g + 3] = fmaf(u[4 * g + 3] * down.w, qscale, ve.w);
             }
             uint32_t seen = ~0u;  // the tile's keys that this column sees
             if (k0 + kKeys > b.wfull) {
@@ -753,36 +758,50 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
 #pragma unroll
                 for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
             }
-            float top = -INFINITY;
+            if (__builtin_expect(poison != 0, 0)) z.l = seen & poison ? __builtin_nanf("") : z.l;
+            float top = u[0];
 #pragma unroll
-            for (int v = 0; v < 16; v++) top = fmaxf(top, u[v]);
+            for (int v = 1; v < 16; v++) top = fmaxf(top, u[v]);
             raise_base(z, top);
+            next = scores(step + 1);
+            float w[16];
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                u[v] = __builtin_amdgcn_exp2f(u[v] - z.base);
-                up[v] *= u[v];
-                z.l += up[v];
+            for (int g = 0; g < 4; g++) {
+                const float4 vu = *reinterpret_cast<const float4*>(&st.vup[buf][kw][8 * g + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[4 * g + j] = __builtin_amdgcn_exp2f(u[4 * g + j] - z.base);
+                z.l = fmaf(w[4 * g], vu.x, z.l);
+                z.l = fmaf(w[4 * g + 1], vu.y, z.l);
+                z.l = fmaf(w[4 * g + 2], vu.z, z.l);
+                z.l = fmaf(w[4 * g + 3], vu.w, z.l);
             }
-            if (!vbad) {
 #pragma unroll
-                for (int s2 = 0; s2 < 2; s2++) {
-                    h8f ph, pl;
-                    split8(u + 8 * s2, ph, pl);
+            for (int s2 = 0; s2 < 2; s2++) {
+                h8f ph, pl;
+                split8(w + 8 * s2, ph, pl);
 #pragma unroll
-                    for (int d = 0; d < OT; d++) {
-                        const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][lane]);
-                        const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][lane]);
-                        z.o[d] = mfma(vl, ph, z.o[d]);
-                        z.o[d] = mfma(vh, pl, z.o[d]);
-                        z.o[d] = mfma(vh, ph, z.o[d]);
-                    }
+                for (int d = 0; d < OT; d++) {
+                    const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][lane]);
+                    const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][lane]);
+                    z.o[d] = mfma(vl, ph, z.o[d]);
+                    z.o[d] = mfma(vh, pl, z.o[d]);
+                    z.o[d] = mfma(vh, ph, z.o[d]);
                 }
-            } else {
-                add_seen<W>(z, up, vp, kv_dim, a.hd, k0, keys, seen, half);
             }
         }
-        if (step + 1 < steps) stash(step + 1);
+        // (past the last step: its last key's, to where nothing reads it)
+        stash_k(step + 2, kx);
+        stash_v(step + 1, vx);
+        if (step + 2 < steps) {
+            fetch_k(first + 3 * KW, kx);
+            fetch_v(first + 2 * KW, vx);
+        }
         __syncthreads();
+    };
+    for (uint32_t step = 0; step < steps; step += 2) {
+        work(step, score[0], score[1]);
+        if (step + 1 == steps) break;
+        work(step + 1, score[1], score[0]);
     }
     z.l = sum_halves(z.l);
     if constexpr (KW > 1) {
@@ -819,8 +838,7 @@ __global__ void __launch_bounds__(64 * CW, 2) k_gqa_rest(RowsArgs a, uint32_t bl
 // k_gqa_prompt loads, f16 terms under one power of two for the tile's keys and one for its
 // values.  Where a tile's rows differ by more than 2^8 in their largest magnitudes, the lower terms
 // of some would fall so far below f16's normal numbers that more than 2^-21 of a row were lost to
-// the rows beside it; and a value that is not finite has to be kept from rows that do not see it.
-// The blocks of such a (sequence, kv head) are k_gqa_rest's, in a launch behind k_gqa_prompt's (in the
+// the rows beside it.  The blocks of such a (sequence, kv head) are k_gqa_rest's, in a launch behind k_gqa_prompt's (in the
 // same kernel, its registers were spilled from those of the hot loop: 16 prompts of up to 1000 rows 76 us
 // and 70 without).
 template <int W>
@@ -829,7 +847,8 @@ struct Packed {
     _Float16 v[W / 32][2][2][64][8];
 };
 struct TileInfo {
-    float kdown, vexp, vup, pad;  // 2^-e of the keys; -e and 2^e of the values
+    float kdown, vexp, vup;  // 2^-e of the keys; -e and 2^e of the values
+    uint32_t poison;         // keys with a value that is not finite
 };
 constexpr int kApart = 8;
 
@@ -895,7 +914,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
     // what lane l of every wave holds of row l % 32: keys' in the lower half, values' in the upper one
     const int lane = threadIdx.x & 63, of = lane >> 5;
     const uint32_t mine = top[of][lane & 31];
-    const bool used = tile * kKeys + (lane & 31) < keys && mine > 0;
+    const bool used = tile * kKeys + (lane & 31) < keys && mine > 0 && mine < kInf;
     int hi = used ? static_cast<int>(mine >> 23) : 0, lo = used ? static_cast<int>(mine >> 23) : 255;
     hi = static_cast<int>(group_max<32>(static_cast<uint32_t>(hi)));
     lo = 255 - static_cast<int>(group_max<32>(static_cast<uint32_t>(255 - lo)));
@@ -908,7 +927,9 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
             info.vexp = static_cast<float>(-e);
             info.vup = pow2f(e);
         }
-        if (__any(hi - lo > kApart || (of == 1 && mine >= kInf)) && lane == 0) {
+        const uint64_t bad = __ballot(of == 1 && mine >= kInf);
+        if (lane == 0) info.poison = static_cast<uint32_t>(bad >> 32);
+        if (__any(hi - lo > kApart) && lane == 0) {
             atomicOr(a.apart + pair, 1u);
             atomicOr(a.apart + static_cast<uint32_t>(a.n_kv) * a.seqs, 1u);
         }
@@ -932,7 +953,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
         }
         float z[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) z[j] = y[i][j] * vup;
+        for (int j = 0; j < 8; j++) z[j] = q < 8 && top[1][4 * (q & 7) + (j & 3)] >= kInf ? 0.0f : y[i][j] * vup;
         if (q < 8) {
             // keys 4 q .. + 3 are steps 4 (q / 2 % 2) .. + 3 of lane half q % 2 in product q / 4
 #pragma unroll
@@ -1047,6 +1068,10 @@ __global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const 
 #pragma unroll
                 for (int v = 0; v < 16; v++) now[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? now[v] : -INFINITY;
             }
+            if (__builtin_expect(of.poison != 0, 0)) {
+                const uint32_t seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;
+                z.l = seen & of.poison ? __builtin_nanf("") : z.l;
+            }
             const float sc = of.kdown * qscale;
             float top = now[0];
 #pragma unroll
@@ -1127,9 +1152,8 @@ int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p) {
 template <int W, bool TREE>
 int launch_width(fh_ctx* ctx, const RowsArgs& a, int cw) {
     if (cw == 8) return launch_rows<W, 8, 1, TREE>(ctx, a);
-    if (cw == 4) return launch_rows<W, 4, 1, TREE>(ctx, a);
-    if constexpr (W == 128) return launch_rows<W, 2, 1, TREE>(ctx, a);
-    else return launch_rows<W, 2, 2, TREE>(ctx, a);
+    if constexpr (W == 128) return launch_rows<W, 4, 1, TREE>(ctx, a);
+    else return cw == 4 ? launch_rows<W, 4, 1, TREE>(ctx, a) : launch_rows<W, 2, 2, TREE>(ctx, a);
 }
 
 }  // namespace
@@ -1140,13 +1164,13 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const int w = g.hd <= 32 ? 32 : static_cast<int>(g.hd);
     const size_t tiles = (g.limit + kKeys - 1) / kKeys, pack = heads * tiles * (static_cast<size_t>(w) * 256);
     const bool prompt = !g.parent && cols > 512 && pack < (size_t(1) << 31);
-    const int cw = prompt ? (w == 128 ? 8 : 4) : cols > 128 ? 8 : cols > 64 ? 4 : 2;
+    const int cw = prompt ? (w == 128 ? 8 : 4) : cols > 128 ? 8 : cols > 64 || w == 128 ? 4 : 2;
     const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
-    // Keys of few columns are dealt over several workgroups, four tiles of keys each at least.
+    // Keys of few columns are dealt over several workgroups, two tiles of keys each at least.
     const size_t cus = static_cast<size_t>(ctx->num_cus), places = cus;
     int splits_log2 = 0;
-    while (splits_log2 < 6 && heads * blocks << (splits_log2 + 1) <= places && size_t(8) << splits_log2 <= tiles) splits_log2++;
+    while (splits_log2 < 6 && heads * blocks << (splits_log2 + 1) <= places && size_t(4) << splits_log2 <= tiles) splits_log2++;
     if (heads * blocks > kUnits) splits_log2 = 0;
     const size_t splits = size_t(1) << splits_log2;
     unsigned* counters = nullptr;
