@@ -1115,7 +1115,8 @@ __global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const 
     if (b.on) store_out<W>(z, a, b.row, b.head, half, b.bad);
 }
 
-constexpr size_t kUnits = 8192;  // column blocks whose keys may be split
+constexpr size_t kUnits = 65536;  // counters: sequences of a tree's acceptance, or
+constexpr size_t kShared = 8192;   // column blocks whose keys may be split
 
 template <int W, int CW, int KW, bool TREE>
 int launch_rows(fh_ctx* ctx, const RowsArgs& a) {
@@ -1171,7 +1172,7 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const size_t cus = static_cast<size_t>(ctx->num_cus), places = cus;
     int splits_log2 = 0;
     while (splits_log2 < 6 && heads * blocks << (splits_log2 + 1) <= places && size_t(4) << splits_log2 <= tiles) splits_log2++;
-    if (heads * blocks > kUnits) splits_log2 = 0;
+    if (heads * blocks > kShared) splits_log2 = 0;
     const size_t splits = size_t(1) << splits_log2;
     unsigned* counters = nullptr;
     if (splits > 1) {
@@ -1293,30 +1294,41 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
 
 namespace {
 
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // (the planes' addresses are not known here)
+
 struct AcceptArgs {
     const uint32_t *parent, *tokens, *chosen, *off, *len;
     uint32_t seqs, total, max_rows;
     uint32_t *path, *count, *next, *new_len;
     const uint64_t* planes;
-    size_t kv_dim, capacity;
+    size_t n_planes, kv_dim, capacity;
 };
 
-// A workgroup a sequence: every row finds out whether it is the first that continues its parent
-// with the token chosen there, then one thread follows them from row 0.
-__global__ void __launch_bounds__(kThreads) k_tree_walk(AcceptArgs a) {
-    __shared__ uint32_t up[kMaxTree], child[kMaxTree], way[kMaxTree];
+// A workgroup a sequence and cache plane (without planes, a sequence): every row finds out whether it
+// continues its parent with the token chosen there, the first such is its parent's child, and one thread
+// follows the children from row 0; then the plane's accepted rows move to their places, as many at a
+// time as 256 threads hold.  A row moves down only, and all of a batch is read before any of it is
+// written: what a write overwrites has moved or is left behind.  Latency: a chain of three loads, the
+// walk and the move (one sequence of 16 rows and 48 planes 3.8 us, 32 of up to 32 rows 5.1; the walk and the move in
+// launches of their own 5.9 and 6.4 and the time between).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_tree_accept(AcceptArgs a, unsigned* arrived) {
+    constexpr int HOLD = 4;
+    __shared__ uint32_t up[kMaxTree], child[kMaxTree], way[kMaxTree], chosen[kMaxTree];
     __shared__ uint32_t steps;
     const uint32_t s = blockIdx.x;
-    const Rows r = rows_of(a.off, nullptr, a.total, a.max_rows, a.seqs, s);
-    const uint32_t len = a.len ? a.len[s] : 0;
+    const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+    const uint64_t base = a.n_planes ? a.planes[blockIdx.y] : 0;
+    const uint32_t len = static_cast<uint32_t>(r.at);
     for (uint32_t t = threadIdx.x; t < r.count; t += kThreads) {
-        const uint32_t p = a.parent[r.begin + t];
-        up[t] = p < t && a.tokens[r.begin + t] == a.chosen[r.begin + p] ? p : ~0u;
+        up[t] = a.parent[r.begin + t];
+        way[t] = a.tokens[r.begin + t];
+        chosen[t] = a.chosen[r.begin + t];
         child[t] = ~0u;
     }
     __syncthreads();
     for (uint32_t t = threadIdx.x; t < r.count; t += kThreads)
-        if (up[t] != ~0u) atomicMin(&child[up[t]], t);
+        if (up[t] < t && way[t] == chosen[up[t]]) atomicMin(&child[up[t]], t);
     __syncthreads();
     if (threadIdx.x == 0) {
         uint32_t n = 0;
@@ -1325,27 +1337,48 @@ __global__ void __launch_bounds__(kThreads) k_tree_walk(AcceptArgs a) {
     }
     __syncthreads();
     const uint32_t n = steps;
-    for (uint32_t t = threadIdx.x; t < r.count; t += kThreads) a.path[r.begin + t] = t < n ? way[t] : ~0u;
-    if (threadIdx.x == 0) {
-        a.count[s] = n;
-        if (n) a.next[s] = a.chosen[r.begin + way[n - 1]];
-        a.new_len[s] = len + n;
-    }
-}
-
-// A workgroup a sequence and plane: its accepted rows, each to its place, in order (a row
-// moves down only, so what it overwrites has moved before or is left behind).
-__global__ void __launch_bounds__(kThreads) k_tree_move(AcceptArgs a) {
-    const uint32_t s = blockIdx.x;
-    const Rows r = rows_of(a.off, nullptr, a.total, a.max_rows, a.seqs, s);
-    const uint32_t n = min(a.count[s], r.count);
-    const uint64_t at = a.new_len[s] - a.count[s];
-    float* plane = reinterpret_cast<float*>(a.planes[blockIdx.y]) + static_cast<size_t>(s) * a.capacity * a.kv_dim;
-    for (size_t c = threadIdx.x; c < a.kv_dim; c += kThreads)
-        for (uint32_t i = 1; i < n; i++) {
-            const uint32_t p = a.path[r.begin + i];
-            if (p != i && at + p < a.capacity) plane[(at + i) * a.kv_dim + c] = plane[(at + p) * a.kv_dim + c];
+    if (blockIdx.y == 0) {
+        for (uint32_t t = threadIdx.x; t < r.count; t += kThreads) a.path[r.begin + t] = t < n ? way[t] : ~0u;
+        if (threadIdx.x == 0) {
+            a.count[s] = n;
+            if (n) a.next[s] = chosen[way[n - 1]];
         }
+    }
+    // The new length goes out when every workgroup of the sequence has read the old one, which it may replace.
+    if (threadIdx.x == 0) {
+        const bool last = !arrived || atomicAdd(arrived + s, 1u) == gridDim.y - 1;
+        if (arrived ? last : blockIdx.y == 0) {
+            a.new_len[s] = len + n;
+            if (arrived) __hip_atomic_store(arrived + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (!a.n_planes) return;
+    const size_t width = a.kv_dim / (sizeof(T) / sizeof(float));
+    T* plane = reinterpret_cast<T*>(base) + static_cast<size_t>(s) * a.capacity * width;
+    for (size_t c0 = 0; c0 < width; c0 += kThreads * HOLD) {
+        const uint32_t wide = static_cast<uint32_t>(min(width - c0, static_cast<size_t>(kThreads * HOLD)));
+        const uint32_t rows = kThreads * HOLD / wide;  // of a batch
+        for (uint32_t i0 = 1; i0 < n; i0 += rows) {
+            T x[HOLD];
+            size_t to[HOLD];
+            bool moves[HOLD];
+#pragma unroll
+            for (int j = 0; j < HOLD; j++) {
+                const uint32_t item = static_cast<uint32_t>(j) * kThreads + threadIdx.x, i = i0 + item / wide;
+                moves[j] = item / wide < rows && i < n;
+                if (!moves[j]) continue;
+                const uint64_t p = way[i];
+                moves[j] = p != i && r.at + p < a.capacity;
+                if (!moves[j]) continue;
+                to[j] = static_cast<size_t>(r.at + i) * width + c0 + item % wide;
+                x[j] = plane[static_cast<size_t>(r.at + p) * width + c0 + item % wide];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < HOLD; j++)
+                if (moves[j]) plane[to[j]] = x[j];
+        }
+    }
 }
 
 }  // namespace
@@ -1355,11 +1388,17 @@ int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* t
                           size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
                           uint32_t* new_len) {
     AcceptArgs a{parent, tokens, chosen, off, len, static_cast<uint32_t>(seqs), static_cast<uint32_t>(total),
-                 static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, kv_dim, capacity};
-    hipLaunchKernelGGL(k_tree_walk, dim3(a.seqs), dim3(kThreads), 0, ctx->stream, a);
-    FH_HIP(ctx, hipGetLastError());
-    if (n_planes == 0 || max_rows < 2) return FH_OK;
-    hipLaunchKernelGGL(k_tree_move, dim3(a.seqs, static_cast<unsigned>(n_planes)), dim3(kThreads), 0, ctx->stream, a);
+                 static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, n_planes, kv_dim, capacity};
+    unsigned* arrived = nullptr;
+    if (new_len == len && n_planes > 1) {
+        void* area = nullptr;
+        const int rc = fh_gqa_counters(ctx, kUnits * sizeof(unsigned), &area);
+        if (rc) return rc;
+        arrived = static_cast<unsigned*>(area);
+    }
+    const dim3 grid(a.seqs, static_cast<unsigned>(std::max<size_t>(n_planes, 1)));
+    if (kv_dim % 4 == 0) hipLaunchKernelGGL(k_tree_accept<f4>, grid, dim3(kThreads), 0, ctx->stream, a, arrived);
+    else hipLaunchKernelGGL(k_tree_accept<float>, grid, dim3(kThreads), 0, ctx->stream, a, arrived);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }

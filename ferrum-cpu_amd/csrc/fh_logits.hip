@@ -26,21 +26,74 @@ struct EditArgs {
     int segs;
 };
 
-// A workgroup takes SEG ids of a row: the counts and the biases of its own ids go to LDS
-// (integer atomics: no order shows), then the logits pass through.  Bound by memory: 8 bytes
-// an id and the lists once per workgroup from the caches.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // (rows of an odd vocabulary begin anywhere)
+
+// A workgroup takes SEG ids of a row: their logits are on their way while the counts and the biases
+// of these ids gather in LDS (integer atomics: no order shows).
 template <int SEG>
 __global__ void __launch_bounds__(kThreads) k_logits_edit(EditArgs a) {
-    __shared__ uint32_t count[SEG], biased[SEG];
+    constexpr int PER = SEG / (4 * kThreads);  // float4s of a thread
+    __shared__ __align__(16) uint32_t count[SEG], biased[SEG];
+    __shared__ uint32_t up[kMaxTree], token[kMaxTree];
     const uint32_t row = blockIdx.x / a.segs, first = blockIdx.x % a.segs * SEG;
     const uint32_t n = min(static_cast<uint32_t>(SEG), a.vocab - first);
     const fh_logits_edit& e = a.e;
-    for (uint32_t i = threadIdx.x; i < SEG; i += kThreads) {
-        count[i] = 0;
-        biased[i] = 0;
+    const float* in = a.logits + static_cast<size_t>(row) * a.vocab + first;
+    float* out = a.out + static_cast<size_t>(row) * a.vocab + first;
+    const auto place = [&](int i) { return 4 * (static_cast<uint32_t>(i) * kThreads + threadIdx.x); };
+    f4 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const uint32_t v = place(i);
+        x[i] = f4{0, 0, 0, 0};
+        if (v + 4 <= n) x[i] = *reinterpret_cast<const f4*>(in + v);
+        else
+            for (uint32_t j = 0; v + j < n; j++) x[i][j] = in[v + j];
+    }
+    const float rep = e.d_repetition ? e.d_repetition[row] : 1.0f, freq = e.d_frequency ? e.d_frequency[row] : 0.0f;
+    const float pres = e.d_presence ? e.d_presence[row] : 0.0f;
+    const bool counted = e.d_ranges || e.d_tokens;
+    uint32_t mask = ~0u;
+    if (e.d_mask) {
+        mask = e.d_mask_of ? e.d_mask_of[row] : row;
+        if (mask >= e.masks) mask = ~0u;
+    }
+    uint32_t words[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        words[i] = mask != ~0u && place(i) < n ? e.d_mask[static_cast<size_t>(mask) * a.words + ((first + place(i)) >> 5)] : ~0u;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        *reinterpret_cast<uint4*>(&count[place(i)]) = make_uint4(0, 0, 0, 0);
+        if (e.d_bias_off) *reinterpret_cast<uint4*>(&biased[place(i)]) = make_uint4(0, 0, 0, 0);
+    }
+    // the row's sequence begins at `begin`; its rows up to this one
+    uint32_t begin = row;
+    if (e.d_tokens) {
+        if (e.d_off) {
+            // the last sequence that begins at or before the row
+            uint32_t last = 0;
+            for (uint32_t s = threadIdx.x & 63; s < e.seqs; s += 64) last = e.d_off[s] <= row ? s + 1 : last;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) last = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), d, 64)));
+            if (last && e.d_off[last - 1] <= row && row < e.d_off[last]) begin = e.d_off[last - 1];
+        } else {
+            begin = row - row % (a.rows / static_cast<uint32_t>(e.seqs));
+        }
+        if (row - begin >= kMaxTree) begin = row;  // (past the longest tree)
+        for (uint32_t t = threadIdx.x; t <= row - begin; t += kThreads) {
+            up[t] = e.d_parent ? e.d_parent[begin + t] : ~0u;
+            token[t] = e.d_tokens[begin + t];
+        }
     }
     __syncthreads();
-    const bool counted = e.d_ranges || e.d_tokens;
+    if (e.d_tokens && threadIdx.x == 0)
+        for (uint32_t t = row - begin, next; ; t = next) {
+            const uint32_t v = token[t] - first;
+            next = up[t];
+            if (v < n) atomicAdd(&count[v], 1u);
+            if (next >= t) break;  // (a parent is a row before)
+        }
     if (e.d_ranges) {
         const uint32_t i0 = e.d_ranges[2 * static_cast<size_t>(row)], i1 = e.d_ranges[2 * static_cast<size_t>(row) + 1];
         for (uint64_t i = i0 + static_cast<uint64_t>(threadIdx.x); i < i1; i += kThreads) {
@@ -48,61 +101,44 @@ __global__ void __launch_bounds__(kThreads) k_logits_edit(EditArgs a) {
             if (v < n) atomicAdd(&count[v], 1u);
         }
     }
-    if (e.d_tokens) {
-        // the row's sequence begins at `begin`
-        uint32_t begin;
-        if (e.d_off) {
-            uint32_t lo = 0, hi = static_cast<uint32_t>(e.seqs);  // the last s with off[s] <= row
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (e.d_off[mid] <= row) lo = mid;
-                else hi = mid;
-            }
-            begin = e.d_off[lo] <= row && row < e.d_off[lo + 1] ? e.d_off[lo] : row;
-        } else {
-            begin = row - row % (a.rows / static_cast<uint32_t>(e.seqs));
-        }
-        if (threadIdx.x == 0) {
-            uint32_t t = row - begin;
-            for (int k = 0; k < kMaxTree; k++) {
-                const uint32_t v = e.d_tokens[begin + t] - first;
-                if (v < n) atomicAdd(&count[v], 1u);
-                const uint32_t p = e.d_parent ? e.d_parent[begin + t] : ~0u;
-                if (p >= t) break;
-                t = p;
-            }
-        }
-    }
+    size_t b0 = 0;
     if (e.d_bias_off) {
-        const uint32_t i0 = e.d_bias_off[row], i1 = e.d_bias_off[row + 1];
-        for (uint64_t i = i0 + static_cast<uint64_t>(threadIdx.x); i < i1; i += kThreads) {
+        b0 = e.d_bias_off[row];
+        const uint32_t i1 = e.d_bias_off[row + 1];
+        for (uint64_t i = b0 + threadIdx.x; i < i1; i += kThreads) {
             const uint32_t v = e.d_bias_id[i] - first;
-            if (v < n) atomicMax(&biased[v], static_cast<uint32_t>(i - i0 + 1));
+            if (v < n) atomicMax(&biased[v], static_cast<uint32_t>(i - b0 + 1));
         }
     }
     __syncthreads();
-    const float rep = e.d_repetition ? e.d_repetition[row] : 1.0f, freq = e.d_frequency ? e.d_frequency[row] : 0.0f;
-    const float pres = e.d_presence ? e.d_presence[row] : 0.0f;
-    uint32_t m = ~0u;
-    if (e.d_mask) {
-        m = e.d_mask_of ? e.d_mask_of[row] : row;
-        if (m >= e.masks) m = ~0u;
-    }
-    const float* in = a.logits + static_cast<size_t>(row) * a.vocab + first;
-    float* out = a.out + static_cast<size_t>(row) * a.vocab + first;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        float x = in[i];
-        if (counted && count[i]) {
-            if (rep > 0.0f) x = x > 0.0f ? x / rep : x * rep;
-            x -= freq * static_cast<float>(count[i]);
-            x -= pres;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const uint32_t v = place(i);
+        if (counted) {
+            const uint4 c4 = *reinterpret_cast<const uint4*>(&count[v]);
+            const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (c[j]) {
+                    float y = x[i][j];
+                    if (rep > 0.0f) y = y > 0.0f ? y / rep : y * rep;
+                    y -= freq * static_cast<float>(c[j]);
+                    x[i][j] = y - pres;
+                }
         }
-        if (biased[i]) x += e.d_bias[e.d_bias_off[row] + static_cast<size_t>(biased[i] - 1)];
-        if (m != ~0u) {
-            const uint32_t v = first + i;
-            if (!(e.d_mask[static_cast<size_t>(m) * a.words + (v >> 5)] >> (v & 31) & 1)) x = -INFINITY;
+        if (e.d_bias_off) {
+            const uint4 c4 = *reinterpret_cast<const uint4*>(&biased[v]);
+            const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (c[j]) x[i][j] += e.d_bias[b0 + (c[j] - 1)];
         }
-        out[i] = x;
+        const uint32_t stays = words[i] >> (v & 31);  // (SEG and the thread's four ids begin at multiples of 32 and 4)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = stays >> j & 1 ? x[i][j] : -INFINITY;
+        if (v + 4 <= n) *reinterpret_cast<f4*>(out + v) = x[i];
+        else
+            for (uint32_t j = 0; v + j < n; j++) out[v + j] = x[i][j];
     }
 }
 
@@ -111,10 +147,15 @@ __global__ void __launch_bounds__(kThreads) k_logits_edit(EditArgs a) {
 int fh_launch_logits_edit(fh_ctx* ctx, const float* logits, size_t rows, size_t vocab, const fh_logits_edit& e, float* out) {
     EditArgs a{logits, out, static_cast<uint32_t>(rows), static_cast<uint32_t>(vocab), e,
                static_cast<uint32_t>((vocab + 31) / 32), 0};
-    constexpr int seg = 2048;
-    a.segs = static_cast<int>((vocab + seg - 1) / seg);
-    if (rows * a.segs > 0x7FFFFFFFu) return fh_fail(ctx, FH_ERR_LIMIT, "fh_logits_edit: more than 2^31 - 1 workgroups");
-    hipLaunchKernelGGL(k_logits_edit<seg>, dim3(static_cast<unsigned>(rows * a.segs)), dim3(kThreads), 0, ctx->stream, a);
-    FH_HIP(ctx, hipGetLastError());
-    return FH_OK;
+    // 1024 ids a workgroup spread one row of 50257 over 50 of them, in 3.4 us (4096: 5.2); 4096 read the lists a
+    // quarter as often: 256 rows of 151936 64 us (1024: 73), 64 rows either way 20.
+    const auto go = [&](auto kern, size_t seg) -> int {
+        const size_t segs = (vocab + seg - 1) / seg;
+        if (rows > 0x7FFFFFFFu / segs) return fh_fail(ctx, FH_ERR_LIMIT, "fh_logits_edit: more than 2^31 - 1 workgroups");
+        a.segs = static_cast<int>(segs);
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows * segs)), dim3(kThreads), 0, ctx->stream, a);
+        FH_HIP(ctx, hipGetLastError());
+        return FH_OK;
+    };
+    return rows * vocab < (size_t(1) << 24) ? go(k_logits_edit<1024>, 1024) : go(k_logits_edit<4096>, 4096);
 }
