@@ -62,6 +62,24 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float cs, float sn
 // ---- rotation and storing ------------------------------------------------------------
 
 constexpr int kMaxTree = 1024;  // nodes of a sequence's tree
+constexpr int kKeys = 32;       // keys of a tile
+
+// Division by a number of the host's: n / d = the upper half of n * (2^64 / d + 1), exact for n < 2^32.
+struct Div {
+    uint64_t m;
+    uint32_t d;
+    Div(uint32_t by = 1) : m(by > 1 ? ~uint64_t(0) / by + 1 : 0), d(by) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return m ? static_cast<uint32_t>(__umul64hi(n, m)) : n; }
+};
+
+// What a workgroup of the attention is to do where keys are dealt over several: share `split` of `shares` of
+// the tiles of column block cb of a sequence (shares 0: nothing), whose first share is workgroup `first`.
+struct Share {
+    uint32_t s, cb, split, shares;
+    uint32_t begin, count, at, first;
+};
+constexpr uint32_t kPlanned = 256;  // column blocks of a kv head
+constexpr uint32_t kJoined = 8;      // shares of a column block that are joined at once
 
 struct AppendArgs {
     const float* qkv;
@@ -81,14 +99,87 @@ struct AppendArgs {
     const float* ff;
     int heads_each, chunks;
     uint32_t* clear;  // [seqs, n_kv], 1 (NULL: nowhere): set to 0
+    Share* plan;      // [places] (NULL: none): the workgroups' shares, of every kv head alike
+    uint32_t places, col_blocks, cols;  // columns of a block
+    Div group;
     float freq[64];
 };
+
+// Shares of nearly equal length for sequences (and for prompts, blocks) of different lengths: the least number of
+// tiles q for which all blocks cut into shares of q at most are no more than the places.
+template <bool TREE>
+__device__ __forceinline__ void plan_shares(const AppendArgs& a) {
+    constexpr int PER = kPlanned / 64;
+    __shared__ uint32_t first[kPlanned + 1];
+    const uint32_t units = a.seqs * a.col_blocks;
+    if (threadIdx.x < 64) {
+        uint32_t tiles[PER];
+        int total = 0, most = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const uint32_t u = j * 64 + threadIdx.x, s = u / a.col_blocks, c0 = (u - s * a.col_blocks) * a.cols;
+            tiles[j] = 0;
+            if (u < units) {
+                const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+                const uint32_t ncols = r.count * a.group.d;
+                const uint32_t n = TREE ? r.count : a.group(min(ncols, c0 + a.cols) - 1) + 1;
+                if (c0 < ncols) tiles[j] = static_cast<uint32_t>((min(r.at + n, static_cast<uint64_t>(a.limit)) + kKeys - 1) / kKeys);
+            }
+            total += tiles[j];
+            most = max(most, static_cast<int>(tiles[j]));
+        }
+        for (int d = 32; d; d >>= 1) {
+            total += __shfl_xor(total, d);
+            most = max(most, __shfl_xor(most, d));
+        }
+        const auto shares = [&](uint32_t t, uint32_t q) { return (t + q - 1) / q; };
+        uint32_t lo = max(2u, shares(total, a.places)), hi = max(lo, static_cast<uint32_t>(most));
+        while (lo < hi) {
+            const uint32_t q = (lo + hi) / 2;
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) n += shares(tiles[j], q);
+            for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+            if (static_cast<uint32_t>(n) <= a.places) hi = q;
+            else lo = q + 1;
+        }
+        uint32_t base = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            uint32_t upto = shares(tiles[j], lo);
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t x = __shfl_up(upto, d);
+                if (static_cast<int>(threadIdx.x) >= d) upto += x;
+            }
+            first[j * 64 + threadIdx.x + 1] = base + upto;
+            base += __shfl(upto, 63);
+        }
+        if (threadIdx.x == 0) first[0] = 0;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.places; i += kThreads) {
+        uint32_t u = 0;  // the last block whose first share is not behind i
+        for (uint32_t step = kPlanned / 2; step; step >>= 1)
+            if (first[u + step] <= i) u += step;
+        Share to{};
+        if (u < units && i < first[u + 1]) {
+            const uint32_t s = u / a.col_blocks;
+            const Rows r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
+            to = Share{s, u - s * a.col_blocks, i - first[u], first[u + 1] - first[u], r.begin, r.count, static_cast<uint32_t>(r.at), first[u]};
+        }
+        a.plan[i] = to;
+    }
+}
 
 // A workgroup takes some rows of a sequence and `heads_each` of their heads: a thread
 // keeps one pair of channels' sine and cosine for all of them.
 template <bool TREE>
 __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
     const uint32_t s = blockIdx.y;
+    if (s == a.seqs) {  // (one more, where there is a plan)
+        if (blockIdx.x == 0) plan_shares<TREE>(a);
+        return;
+    }
     const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
     const int slots = a.hd / 2, each = kThreads / slots;  // rows of a workgroup
     const uint32_t t0 = blockIdx.x / a.chunks * static_cast<uint32_t>(each);
@@ -160,16 +251,6 @@ __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
 
 // ---- attention -------------------------------------------------------------------------
 
-constexpr int kKeys = 32;  // keys of a tile
-
-// Division by a number of the host's: n / d = the upper half of n * (2^64 / d + 1), exact for n < 2^32.
-struct Div {
-    uint64_t m;
-    uint32_t d;
-    Div(uint32_t by = 1) : m(by > 1 ? ~uint64_t(0) / by + 1 : 0), d(by) {}
-    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return m ? static_cast<uint32_t>(__umul64hi(n, m)) : n; }
-};
-
 struct RowsArgs {
     const float* q;  // row r's heads at r * q_ld: rotated, or with cs to be rotated
     size_t q_ld;
@@ -184,7 +265,9 @@ struct RowsArgs {
     int words;
     float scale;  // log2(e) / sqrt(hd)
     float* out;
-    int col_blocks, splits_log2;
+    int col_blocks;
+    const Share* plan;  // (NULL: a workgroup a block)
+    uint32_t places;    // workgroups of a plan
     float2* part;
     unsigned* counters;
     const uint32_t* apart;  // [seqs, n_kv], 1: (prompt) not 0 where the blocks are k_gqa_rest's; where any are
@@ -436,42 +519,56 @@ __device__ __forceinline__ float load_query(const RowsArgs& a, uint32_t row, uin
     for (int i = 0; i < KI; i++) split8(x + 8 * i, up, any, qh[i], ql[i]);
     return pow2f(-e) * a.scale;
 }
-// A workgroup's sums to memory; the last of a block's workgroups joins all shares of the keys, in
-// order (true: it is this one).
+// A workgroup's sums to memory; the last of a group of a block's workgroups joins the group's, in order, and
+// the last of the groups' joins those (true: it is this one).  What a workgroup reads of others' sums comes at
+// about 35 GB/s, so of n shares 2 sqrt(n) are read in turn, not n.
 template <int OT, int CW>
-__device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint32_t unit, uint32_t split, int cw, bool mine, int lane) {
+__device__ __forceinline__ bool join_shares(Sums<OT>& z, const RowsArgs& a, uint32_t kv, uint32_t first, uint32_t split, uint32_t shares,
+                                            int cw, bool mine, int lane) {
     constexpr int PL = Sums<OT>::kParts;
-    float2* part = a.part + ((static_cast<size_t>(unit) << a.splits_log2) * CW + cw) * (PL * 64) + lane;
-    if (mine) {
-        float2* to = part + static_cast<size_t>(split) * CW * (PL * 64);
-        store_part(to, make_float2(z.base, z.l));
-#pragma unroll
-        for (int d = 0; d < OT; d++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) store_part(to + (1 + 8 * d + i) * 64, make_float2(z.o[d][2 * i], z.o[d][2 * i + 1]));
-    }
-    // Every thread's coherent stores complete before the arrival count moves.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __shared__ int last;
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.counters + unit, 1u) == static_cast<unsigned>((1 << a.splits_log2) - 1);
-    __syncthreads();
-    if (!last) return false;
-    if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (mine) {
-        clear(z);
-        for (int k = 0; k < 1 << a.splits_log2; k += 2) {  // (two shares' loads at once)
-            const float2* from = part + static_cast<size_t>(k) * CW * (PL * 64);
-            float2 y[2][PL];
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < PL; i++) y[j][i] = load_part(from + j * CW * (PL * 64) + i * 64);
-            add_sums(z, y[0]);
-            add_sums(z, y[1]);
-        }
+    const size_t next = static_cast<size_t>(a.kvs.d) * CW * (PL * 64);  // from share to share
+    float2* part = a.part + (static_cast<size_t>(first * a.kvs.d + kv) * CW + cw) * (PL * 64) + lane;
+    uint32_t group = shares;  // shares of a group
+    if (shares > kJoined) {
+        group = 2;
+        while (group * group < shares) group++;
     }
-    return true;
+    const uint32_t lead = split / group * group;
+    unsigned* arrived = a.counters + (first + lead) * a.kvs.d + kv;
+    for (uint32_t at = split, from0 = lead, step = 1, count = min(group, shares - lead);;) {
+        if (mine) {
+            float2* to = part + at * next;
+            store_part(to, make_float2(z.base, z.l));
+#pragma unroll
+            for (int d = 0; d < OT; d++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) store_part(to + (1 + 8 * d + i) * 64, make_float2(z.o[d][2 * i], z.o[d][2 * i + 1]));
+        }
+        // Every thread's coherent stores complete before the arrival count moves.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) last = atomicAdd(arrived, 1u) == count - 1;
+        __syncthreads();
+        if (!last) return false;
+        if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (mine) {
+            clear(z);
+            for (uint32_t k = 0; k < count; k++) {
+                const float2* from = part + (from0 + k * step) * next;
+                float2 y[PL];
+#pragma unroll
+                for (int i = 0; i < PL; i++) y[i] = load_part(from + i * 64);
+                add_sums(z, y);
+            }
+        }
+        if (group == shares || step == group) return true;
+        at = lead;  // (read by this wave alone, and done with)
+        from0 = 0;
+        step = group;
+        count = (shares + group - 1) / group;
+        arrived = a.counters + a.places + first * a.kvs.d + kv;
+    }
 }
 template <int W>
 __device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs& a, uint32_t row, uint32_t head, int half, bool bad) {
@@ -515,7 +612,7 @@ struct Stage {
 // workgroups ran for the first 40 us).
 template <int CW, bool TREE>
 struct Block {
-    uint32_t pair, cb, s, kv, split;
+    uint32_t pair, cb, s, kv, split, shares, first;  // (first: of the block's workgroups)
     Rows r;
     uint32_t ncols, c0;
     // the wave's columns, and this lane's
@@ -526,14 +623,30 @@ struct Block {
     uint32_t tile0, tile1;
 
     __device__ __forceinline__ bool place(const RowsArgs& a, uint32_t workgroup) {
+        if (a.plan) {
+            const uint32_t i = a.kvs(workgroup);
+            kv = workgroup - i * a.kvs.d;
+            const Share p = a.plan[i];
+            s = p.s;
+            pair = s * a.kvs.d + kv;
+            cb = p.cb;
+            split = p.split;
+            shares = p.shares;
+            first = p.first;
+            r = Rows{p.begin, p.count, p.at};
+            ncols = r.count * a.group.d;
+            c0 = cb * (32 * CW);
+            return shares != 0;
+        }
         const uint32_t id = a.pairs(workgroup);
         pair = workgroup - id * a.pairs.d;
         if (a.pairs.d % 8 == 0) {
             const uint32_t turned = pair + 8 * id;
             pair = turned - a.pairs(turned) * a.pairs.d;
         }
-        split = id & ((1u << a.splits_log2) - 1);
-        cb = a.col_blocks - 1 - (id >> a.splits_log2);
+        split = 0;
+        shares = 1;
+        cb = a.col_blocks - 1 - id;
         s = a.kvs(pair);
         kv = pair - s * a.kvs.d;
         r = rows_of(a.off, a.len, a.total, a.max_rows, a.seqs, s);
@@ -551,9 +664,13 @@ struct Block {
         wc = c0 + cw * 32;
         wkeys = wc >= ncols ? 0 : upto(a, wc + 32);
         wfull = TREE ? at : wc >= ncols ? 0 : min(keys, at + a.group(wc) + 1);
-        const uint64_t tiles = (keys + kKeys - 1) / kKeys;
-        tile0 = static_cast<uint32_t>(tiles * split >> a.splits_log2);
-        tile1 = static_cast<uint32_t>(tiles * (split + 1) >> a.splits_log2);
+        const uint32_t tiles = keys / kKeys + (keys % kKeys != 0);
+        tile0 = 0;
+        tile1 = tiles;
+        if (shares > 1) {
+            tile0 = tiles / shares * split + min(tiles % shares, split);
+            tile1 = tile0 + tiles / shares + (split < tiles % shares ? 1 : 0);
+        }
     }
     __device__ __forceinline__ void column(const RowsArgs& a, int col) {
         const uint32_t c = wc + col, cc = min(c, ncols - 1);
@@ -808,7 +925,7 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
         static_assert(sizeof(Stage<W, CW, KW>) >= (KW - 1) * CW * Sums<OT>::kParts * 64 * sizeof(float2), "the sums fit");
         join_waves<OT, CW, KW>(z, reinterpret_cast<float2*>(smem), cw, kw, lane);
     }
-    if (a.splits_log2 && !join_shares<OT, CW>(z, a, b.pair + a.pairs.d * b.cb, b.split, cw, kw == 0, lane)) return;
+    if (b.shares > 1 && !join_shares<OT, CW>(z, a, b.kv, b.first, b.split, b.shares, cw, kw == 0, lane)) return;
     if (kw == 0 && b.on) store_out<W>(z, a, row, b.head, half, b.bad);
 }
 
@@ -1111,50 +1228,45 @@ __global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const 
         step(tile + 1, score[1], score[0]);
     }
     z.l = sum_halves(z.l);
-    if (a.splits_log2 && !join_shares<OT, CW>(z, a, b.pair + a.pairs.d * b.cb, b.split, wave, true, lane)) return;
+    if (b.shares > 1 && !join_shares<OT, CW>(z, a, b.kv, b.first, b.split, b.shares, wave, true, lane)) return;
     if (b.on) store_out<W>(z, a, b.row, b.head, half, b.bad);
 }
 
 constexpr size_t kUnits = 65536;  // counters: sequences of a tree's acceptance, or
-constexpr size_t kShared = 8192;   // column blocks whose keys may be split
 
 template <int W, int CW, int KW, bool TREE>
-int launch_rows(fh_ctx* ctx, const RowsArgs& a) {
+int launch_rows(fh_ctx* ctx, const RowsArgs& a, uint32_t workgroups) {
     constexpr size_t lds = sizeof(Stage<W, CW, KW>);
     static_assert(lds <= 160 * 1024, "a stage fits the LDS");
     const auto kern = k_gqa_rows<W, CW, KW, TREE>;
     if (lds > 64 * 1024)
         FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    hipLaunchKernelGGL(kern, dim3(a.seqs * static_cast<uint32_t>(a.n_kv * a.col_blocks << a.splits_log2)), dim3(64 * CW * KW), lds,
-                       ctx->stream, a);
+    hipLaunchKernelGGL(kern, dim3(workgroups), dim3(64 * CW * KW), lds, ctx->stream, a);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
 
 template <int W, int NWV, int OCC>
-int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p) {
+int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p, uint32_t workgroups) {
     hipLaunchKernelGGL(k_gqa_pack<W>, dim3(p.tiles, a.kvs.d, a.seqs), dim3(kThreads), 0, ctx->stream, p);
     FH_HIP(ctx, hipGetLastError());
     constexpr size_t lds = 2 * W * 256;
     static_assert(lds <= 64 * 1024, "without a larger limit");
-    hipLaunchKernelGGL((k_gqa_prompt<W, NWV, OCC>), dim3(a.pairs.d * static_cast<uint32_t>(a.col_blocks << a.splits_log2)),
-                       dim3(64 * NWV), lds, ctx->stream, a, p.packed, p.info, p.tiles);
+    hipLaunchKernelGGL((k_gqa_prompt<W, NWV, OCC>), dim3(workgroups), dim3(64 * NWV), lds, ctx->stream, a, p.packed, p.info, p.tiles);
     FH_HIP(ctx, hipGetLastError());
     constexpr size_t rest = sizeof(Stage<W, NWV, 1>);
     const auto kern = k_gqa_rest<W, NWV>;
     if (rest > 64 * 1024)
         FH_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rest)));
-    const uint32_t blocks = a.pairs.d * static_cast<uint32_t>(a.col_blocks << a.splits_log2);
-    hipLaunchKernelGGL(kern, dim3(std::min(blocks, static_cast<uint32_t>(ctx->num_cus))), dim3(64 * NWV), rest, ctx->stream, a, blocks);
+    hipLaunchKernelGGL(kern, dim3(std::min(workgroups, static_cast<uint32_t>(ctx->num_cus))), dim3(64 * NWV), rest, ctx->stream, a, workgroups);
     FH_HIP(ctx, hipGetLastError());
     return FH_OK;
 }
 
 template <int W, bool TREE>
-int launch_width(fh_ctx* ctx, const RowsArgs& a, int cw) {
-    if (cw == 8) return launch_rows<W, 8, 1, TREE>(ctx, a);
-    if constexpr (W == 128) return launch_rows<W, 4, 1, TREE>(ctx, a);
-    else return cw == 4 ? launch_rows<W, 4, 1, TREE>(ctx, a) : launch_rows<W, 2, 2, TREE>(ctx, a);
+int launch_width(fh_ctx* ctx, const RowsArgs& a, uint32_t workgroups, int cw) {
+    if constexpr (W == 128) return cw == 8 ? launch_rows<W, 8, 1, TREE>(ctx, a, workgroups) : launch_rows<W, 4, 1, TREE>(ctx, a, workgroups);
+    else return cw == 4 ? launch_rows<W, 4, 1, TREE>(ctx, a, workgroups) : launch_rows<W, 2, 2, TREE>(ctx, a, workgroups);
 }
 
 }  // namespace
@@ -1164,18 +1276,26 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const int words = g.parent ? static_cast<int>((g.max_rows + 31) / 32) : 0;
     const int w = g.hd <= 32 ? 32 : static_cast<int>(g.hd);
     const size_t tiles = (g.limit + kKeys - 1) / kKeys, pack = heads * tiles * (static_cast<size_t>(w) * 256);
-    const bool prompt = !g.parent && cols > 512 && pack < (size_t(1) << 31);
-    const int cw = prompt ? (w == 128 ? 8 : 4) : cols > 128 ? 8 : cols > 64 || w == 128 ? 4 : 2;
+    // The launches that pack the tiles and that look for blocks apart are about 15 us, won back where many column
+    // blocks read the same tiles and there are enough of both (us packed and not, heads of width 64: 1 prompt of 1000
+    // rows, 14 and 2 heads 42 and 34, of 2000 57 and 62; 16 of up to 1000 rows 91 and 114; 8 of up to 1000, 12 and 12
+    // heads 82 and 77; of width 128, 32 and 8 heads: 1 prompt of 1000 rows 65 and 66, of 2000 168 and 211).
+    const bool prompt = !g.parent && cols > 1024 && heads * cols * tiles > (size_t(3) << 19) && pack < (size_t(1) << 31);
+    // Columns of a workgroup: as many as there are, while two workgroups fit a compute unit; of 64 columns and two waves that deal
+    // the keys for small calls (one tree of 16 nodes over 511 rows, 14 and 2 heads 16.4 us, 128 columns 18.8; 32 of up
+    // to 32 nodes 39.4 and 33.6).  Width 128: eight waves with the keys split once for 256 columns (4 trees of up to 64
+    // nodes over up to 16383 rows, 32 and 8 heads 226 us, four waves 275).
+    const int cw = w == 128 ? (cols > 128 ? 8 : 4) : cols > 128 ? 4 : 2;
     const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
-    // Keys of few columns are dealt over several workgroups, two tiles of keys each at least.
-    const size_t cus = static_cast<size_t>(ctx->num_cus), places = cus;
-    int splits_log2 = 0;
-    while (splits_log2 < 6 && heads * blocks << (splits_log2 + 1) <= places && size_t(4) << splits_log2 <= tiles) splits_log2++;
-    if (heads * blocks > kShared) splits_log2 = 0;
-    const size_t splits = size_t(1) << splits_log2;
+    // Keys of few columns are dealt over as many workgroups as the device holds at once, two tiles of keys each at
+    // least (those 4 trees: 283 us with equal numbers of shares for all sequences).
+    const size_t cus = static_cast<size_t>(ctx->num_cus), all = cus * (cw == 8 ? 1 : prompt ? 3 : 2);
+    const size_t places = all / g.n_kv, units = g.seqs * blocks;
+    const bool planned = units <= std::min<size_t>(places, kPlanned) && tiles >= 4;
+    const uint32_t workgroups = static_cast<uint32_t>(planned ? places * g.n_kv : heads * blocks);
     unsigned* counters = nullptr;
-    if (splits > 1) {
+    if (planned) {
         void* area = nullptr;
         const int rc = fh_gqa_counters(ctx, kUnits * sizeof(unsigned), &area);
         if (rc) return rc;
@@ -1189,10 +1309,11 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
                       (g.rope_dim && (g.rope_type == FH_ROPE_NEOX ? half % 16 != 0 : half % 2 != 0));
     const size_t q_bytes = fh_align256(copy ? g.total * g.n_heads * g.hd * sizeof(float) : g.total * half * sizeof(float2));
     const size_t seen_bytes = fh_align256(g.total * words * sizeof(uint32_t));
-    const size_t part = splits > 1 ? heads * blocks * splits * cw * (1 + w / 4) * 64 * sizeof(float2) : 0;
+    const size_t part = planned ? workgroups * (cw * (1 + w / 4) * 64 * sizeof(float2)) : 0;
+    const size_t plan_bytes = planned ? fh_align256(places * sizeof(Share)) : 0;
     const size_t info_bytes = prompt ? heads * tiles * sizeof(TileInfo) + (heads + 1) * sizeof(uint32_t) : 0;
     void* room = nullptr;
-    const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + fh_align256(part) + (prompt ? pack + info_bytes : 0), &room);
+    const int rc = fh_kv4_room(ctx, q_bytes + seen_bytes + plan_bytes + fh_align256(part) + (prompt ? pack + info_bytes : 0), &room);
     if (rc) return rc;
 
     AppendArgs p{};
@@ -1214,11 +1335,18 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     p.parent = g.parent;
     PackArgs k{};
     if (prompt) {
-        k.packed = static_cast<char*>(room) + q_bytes + seen_bytes + fh_align256(part);
+        k.packed = static_cast<char*>(room) + q_bytes + seen_bytes + plan_bytes + fh_align256(part);
         k.info = reinterpret_cast<TileInfo*>(k.packed + pack);
         k.apart = reinterpret_cast<uint32_t*>(k.info + heads * tiles);
         p.clear = k.apart;
     }
+    if (planned) {
+        p.plan = reinterpret_cast<Share*>(static_cast<char*>(room) + q_bytes + seen_bytes);
+        p.places = static_cast<uint32_t>(places);
+        p.col_blocks = static_cast<uint32_t>(blocks);
+        p.cols = 32 * cw;
+    }
+    p.group = Div(static_cast<uint32_t>(group));
     if (copy) p.q = static_cast<float*>(room);
     else if (half) p.cs = static_cast<float2*>(room);
     p.first = copy ? 0 : static_cast<int>(g.n_heads);
@@ -1231,12 +1359,12 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     // (the frequencies as fh_rope_async forms them: in 64 bits, then rounded)
     for (size_t i = 0; i < g.rope_dim / 2; i++)
         p.freq[i] = static_cast<float>(std::pow(static_cast<double>(g.base), -2.0 * static_cast<double>(i) / static_cast<double>(g.rope_dim)));
-    const size_t each = 2 * kThreads / g.hd, row_blocks = (g.max_rows + each - 1) / each, all = (copy ? g.n_heads : 0) + 2 * g.n_kv;
+    const size_t each = 2 * kThreads / g.hd, row_blocks = (g.max_rows + each - 1) / each, takes = (copy ? g.n_heads : 0) + 2 * g.n_kv;
     size_t chunks = 1;
-    while (chunks < all && row_blocks * g.seqs * chunks < 4 * cus) chunks *= 2;
-    p.heads_each = static_cast<int>((all + chunks - 1) / chunks);
-    p.chunks = static_cast<int>((all + p.heads_each - 1) / p.heads_each);
-    const dim3 grid(static_cast<unsigned>(row_blocks * p.chunks), static_cast<unsigned>(g.seqs));
+    while (chunks < takes && row_blocks * g.seqs * chunks < 4 * cus) chunks *= 2;
+    p.heads_each = static_cast<int>((takes + chunks - 1) / chunks);
+    p.chunks = static_cast<int>((takes + p.heads_each - 1) / p.heads_each);
+    const dim3 grid(static_cast<unsigned>(row_blocks * p.chunks), static_cast<unsigned>(g.seqs + planned));
     if (g.parent) hipLaunchKernelGGL(k_gqa_append<true>, grid, dim3(kThreads), 0, ctx->stream, p);
     else hipLaunchKernelGGL(k_gqa_append<false>, grid, dim3(kThreads), 0, ctx->stream, p);
     FH_HIP(ctx, hipGetLastError());
@@ -1267,8 +1395,9 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     a.scale = kLog2e / sqrtf(static_cast<float>(g.hd));
     a.out = g.out;
     a.col_blocks = static_cast<int>(blocks);
-    a.splits_log2 = splits_log2;
-    a.part = reinterpret_cast<float2*>(static_cast<char*>(room) + q_bytes + seen_bytes);
+    a.plan = p.plan;
+    a.places = workgroups;
+    a.part = reinterpret_cast<float2*>(static_cast<char*>(room) + q_bytes + seen_bytes + plan_bytes);
     a.counters = counters;
     if (prompt) {
         a.apart = k.apart;
@@ -1284,10 +1413,10 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
         k.limit = p.limit;
         k.off = g.off;
         k.len = g.len;
-        return w == 32 ? launch_prompt<32, 4, 3>(ctx, a, k) : w == 64 ? launch_prompt<64, 4, 3>(ctx, a, k) : launch_prompt<128, 8, 2>(ctx, a, k);
+        return w == 32 ? launch_prompt<32, 4, 3>(ctx, a, k, workgroups) : w == 64 ? launch_prompt<64, 4, 3>(ctx, a, k, workgroups) : launch_prompt<128, 8, 2>(ctx, a, k, workgroups);
     }
-    if (g.parent) return w == 32 ? launch_width<32, true>(ctx, a, cw) : w == 64 ? launch_width<64, true>(ctx, a, cw) : launch_width<128, true>(ctx, a, cw);
-    return w == 32 ? launch_width<32, false>(ctx, a, cw) : w == 64 ? launch_width<64, false>(ctx, a, cw) : launch_width<128, false>(ctx, a, cw);
+    if (g.parent) return w == 32 ? launch_width<32, true>(ctx, a, workgroups, cw) : w == 64 ? launch_width<64, true>(ctx, a, workgroups, cw) : launch_width<128, true>(ctx, a, workgroups, cw);
+    return w == 32 ? launch_width<32, false>(ctx, a, workgroups, cw) : w == 64 ? launch_width<64, false>(ctx, a, workgroups, cw) : launch_width<128, false>(ctx, a, workgroups, cw);
 }
 
 // ---- what is accepted of a tree ------------------------------------------------------------
