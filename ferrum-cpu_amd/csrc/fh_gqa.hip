@@ -965,7 +965,7 @@ struct Packed {
 };
 struct TileInfo {
     float kdown, vexp, vup;  // 2^-e of the keys; -e and 2^e of the values
-    uint32_t poison;         // keys with a value that is not finite
+    uint32_t poison;         // keys that are not finite, or their values
 };
 constexpr int kApart = 8;
 
@@ -1016,9 +1016,9 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        uint32_t m = 0;  // (the largest finite one: of keys the others keep their upper term alone)
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = mag(x[i][j]) < kInf ? max(m, mag(x[i][j])) : m;
+        for (int j = 0; j < 8; j++) m = max(m, mag(x[i][j]));
         m = group_max<W / 8>(m);
         if (ch == 0 && key_of(i) < kKeys) top[0][key_of(i)] = m;
 #pragma unroll
@@ -1044,8 +1044,8 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
             info.vexp = static_cast<float>(-e);
             info.vup = pow2f(e);
         }
-        const uint64_t bad = __ballot(of == 1 && mine >= kInf);
-        if (lane == 0) info.poison = static_cast<uint32_t>(bad >> 32);
+        const uint64_t bad = __ballot(mine >= kInf);
+        if (lane == 0) info.poison = static_cast<uint32_t>(bad >> 32 | bad);
         if (__any(hi - lo > kApart) && lane == 0) {
             atomicOr(a.apart + pair, 1u);
             atomicOr(a.apart + static_cast<uint32_t>(a.n_kv) * a.seqs, 1u);
@@ -1056,12 +1056,14 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int k = key_of(i), q = quad_of(i);
+        // (what is not finite is kept out of the products; the rows that see it are told by its bit)
         if (k < kKeys) {
+            const bool bad = top[0][k] >= kInf;
             u32x4 h, l;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 uint32_t b, c;
-                split2_any(x[i][2 * j] * kup, x[i][2 * j + 1] * kup, b, c);
+                split2(bad ? 0.0f : x[i][2 * j] * kup, bad ? 0.0f : x[i][2 * j + 1] * kup, b, c);
                 h[j] = b;
                 l[j] = c;
             }
