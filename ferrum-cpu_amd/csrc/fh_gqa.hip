@@ -9,8 +9,10 @@
 //   prompt: row t at cache row c = len + t sees j <= c;
 //   tree:   node t sees j < len, and len + a for itself and its ancestors a,
 // out_r = sum over seen j of exp(s - max) v_j / sum of exp(s - max).
-// Two launches: k_gqa_append (rotate q and k, store k and v, and of a tree the depths
-// and ancestors), k_gqa_rows (the rest).
+// k_gqa_append rotates and stores the new keys, stores the values, and leaves the rows' cosines and
+// sines (a tree's: its nodes' paths too) and, where the keys are dealt over several workgroups,
+// the plan of their shares; k_gqa_rows does the rest.  Prompts of many columns and keys have
+// k_gqa_pack, k_gqa_prompt and k_gqa_rest in its place (below).
 #include "fh_internal.hpp"
 
 #include <algorithm>
@@ -172,7 +174,8 @@ __device__ __forceinline__ void plan_shares(const AppendArgs& a) {
 }
 
 // A workgroup takes some rows of a sequence and `heads_each` of their heads: a thread
-// keeps one pair of channels' sine and cosine for all of them.
+// keeps one pair of channels' sine and cosine for all of them.  (12700 rows, 2 kv heads of width 64: 8.7 us; the
+// sines and cosines are half of it.  One tree of 16 rows: 4.6, three dependent loads and a launch.)
 template <bool TREE>
 __global__ void __launch_bounds__(kThreads) k_gqa_append(AppendArgs a) {
     const uint32_t s = blockIdx.y;
@@ -288,6 +291,25 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     if constexpr (G >= 4) v = max(v, dpp_of<0x4E>(v));
     if constexpr (G >= 8) v = max(v, dpp_of<0x141>(v));
     if constexpr (G >= 16) v = max(v, dpp_of<0x140>(v));
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    return v;
+}
+// The largest of G consecutive lanes' values of four numbers each; lane l has that of number l % 4.
+template <int G>
+__device__ __forceinline__ uint32_t quad_max(const uint32_t (&x)[4], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const uint32_t a = max(odd ? x[1] : x[0], dpp_of<0xB1>(odd ? x[0] : x[1]));
+    const uint32_t b = max(odd ? x[3] : x[2], dpp_of<0xB1>(odd ? x[2] : x[3]));
+    uint32_t v = max(high ? b : a, dpp_of<0x4E>(high ? a : b));
+    v = max(v, dpp_of<0x128>(v));
+    v = max(v, dpp_of<0x124>(v));
     if constexpr (G >= 32) {
         const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
@@ -592,8 +614,16 @@ __device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs&
 // two of that key's own, undone exactly on its score; each value row's power of two goes into
 // the weights (the running maximum is that of score - exponent), so that a row's accuracy
 // does not hang on keys beside it that it does not see, nor on how large the values are.
+// A value that is not finite would reach every column through 0 * inf: its key is staged as zeros, and
+// a bit makes NaN of the columns that see it.
 // S^T = K Q^T leaves a lane 16 keys of one column, which is where O^T += V^T P^T wants them.
 // W: the head width brought to 32, 64 or 128.
+// The vector units bound it: a tile of 32 keys of width 64 is some 300 instructions a wave (half of them for the
+// staging) beside 24 products, and the two times add up.  32 trees of up to 32 nodes over up to 1023 rows, 14 and
+// 2 heads: 33.6 us, about 6 until the first tile is staged, 2 a tile, 5 to join four shares.  4 trees of up to 64
+// nodes over up to 16383 rows, 32 and 8 heads of width 128: 211 us, 2.1 TB/s of the cache and 214 TFLOP/s (three times
+// that of f16 products).  Scores of tile t + 1 are multiplied while tile t's become weights (without: 40.7 and 399 us with
+// the splits as they were).
 template <int W, int CW, int KW>
 struct Stage {
     static constexpr int KI = W / 16, OT = W / 32;
@@ -756,19 +786,20 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
             const int p = wave - V0 + i * NW;
             if (V0 && p < 0) continue;
             const int q = p * (128 / W) + lane / (W / 2), kt = q >> 3, qq = q & 7;
-            float y[8], ex[4], up[4];
-            uint32_t bad = 0;
+            uint32_t most[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t top = group_max<W / 2>(max(mag(x[i][j]), mag(x[i][4 + j])));
-                const int e = lift(top, kValueLift);
-                up[j] = pow2f(e);
-                ex[j] = static_cast<float>(-e);
-                y[j] = x[i][j] * up[j];
-                y[4 + j] = x[i][4 + j] * up[j];
-                bad |= (top >= kInf ? 1u : 0u) << j;
-            }
-            if (__builtin_expect(__any(bad != 0), 0)) {  // (kept out of the sums; the rows that see it are told by its bit)
+            for (int j = 0; j < 4; j++) most[j] = max(mag(x[i][j]), mag(x[i][4 + j]));
+            const uint32_t top = quad_max<W / 2>(most, lane);  // of key lane % 4
+            const int e = lift(top, kValueLift);
+            const uint32_t scale = __builtin_bit_cast(uint32_t, pow2f(e));
+            const float up[4] = {__builtin_bit_cast(float, dpp_of<0x00>(scale)), __builtin_bit_cast(float, dpp_of<0x55>(scale)),
+                                 __builtin_bit_cast(float, dpp_of<0xAA>(scale)), __builtin_bit_cast(float, dpp_of<0xFF>(scale))};
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = x[i][j] * up[j & 3];
+            const uint64_t wrong = __ballot(top >= kInf);
+            if (__builtin_expect(wrong != 0, 0)) {  // (kept out of the sums; the rows that see it are told by its bit)
+                const uint32_t bad = static_cast<uint32_t>(wrong >> (lane / (W / 2) * (W / 2))) & 15;
 #pragma unroll
                 for (int j = 0; j < 8; j++) y[j] = bad >> (j & 3) & 1 ? 0.0f : y[j];
                 if (vd == 0 && bad) atomicOr(&st.poison[step % 3][kt], bad << (4 * qq));
@@ -789,9 +820,9 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
                 *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][0][hq * 32 + (dd & 31)][4 * jq]) = hi;
                 *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][1][hq * 32 + (dd & 31)][4 * jq]) = lo;
             }
-            if (vd == 0) {
-                *reinterpret_cast<float4*>(&st.vexp[step & 1][kt][4 * qq]) = make_float4(ex[0], ex[1], ex[2], ex[3]);
-                *reinterpret_cast<float4*>(&st.vup[step & 1][kt][4 * qq]) = make_float4(up[0], up[1], up[2], up[3]);
+            if (vd < 8) {
+                st.vexp[step & 1][kt][4 * qq + (lane & 3)] = static_cast<float>(-e);
+                st.vup[step & 1][kt][4 * qq + (lane & 3)] = __builtin_bit_cast(float, scale);
             }
         }
     };
@@ -872,8 +903,9 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
                 } else {
                     seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;
                 }
+                const uint32_t mine = seen >> (half * 4);  // (against constants: 16 shifted bits would stay in registers)
 #pragma unroll
-                for (int v = 0; v < 16; v++) u[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? u[v] : -INFINITY;
+                for (int v = 0; v < 16; v++) u[v] = mine & 1u << acc_row(v, 0) ? u[v] : -INFINITY;
             }
             if (__builtin_expect(poison != 0, 0)) z.l = seen & poison ? __builtin_nanf("") : z.l;
             float top = u[0];
@@ -1184,8 +1216,9 @@ __global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const 
             const TileInfo of = info[tile];
             if (k0 + kKeys > b.wfull) {
                 const uint32_t seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;
+                const uint32_t mine = seen >> (half * 4);
 #pragma unroll
-                for (int v = 0; v < 16; v++) now[v] = seen >> (half * 4 + acc_row(v, 0)) & 1 ? now[v] : -INFINITY;
+                for (int v = 0; v < 16; v++) now[v] = mine & 1u << acc_row(v, 0) ? now[v] : -INFINITY;
             }
             if (__builtin_expect(of.poison != 0, 0)) {
                 const uint32_t seen = b.own > k0 ? (b.own - k0 >= 32 ? ~0u : (1u << (b.own - k0)) - 1) : 0u;

@@ -569,8 +569,10 @@ int fh_kv4_read_async(fh_ctx* ctx, const fh_kv4_cache* cache, const uint32_t* d_
  * head_dim 8, 16, 32, 64 or 128, else FH_ERR_LIMIT; caches and d_out 16-byte aligned.
  * Within 1e-5 of float64 over the same rotated rows, against each output's sum of
  * weight * the value row's largest magnitude (operands as two f16 terms under a power of
- * two of each row's own: value rows from 2^-86 to 2^27 may be mixed freely).  A key or
- * value that is not finite reaches the rows that see it and no others.  Errors otherwise
+ * two of each row's own: value rows from 2^-86 to 2^27 may be mixed freely).  A query, a
+ * key or a value row with a number that is not finite makes NaN of every channel of the
+ * outputs that see it, and of no others.  A call of the same arguments gives the same bits;
+ * another max_rows or max_keys may share the keys out differently.  Errors otherwise
  * as fh_gqa_attention_rope_decode_async's.  The context's workspace for these calls grows
  * outside graph capture only and is never freed before the context ends, so captured
  * graphs stay valid; calls of one context must not overlap, replayed graphs included. */
