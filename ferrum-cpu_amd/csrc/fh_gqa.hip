@@ -627,8 +627,11 @@ __device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs&
 template <int W, int CW, int KW>
 struct Stage {
     static constexpr int KI = W / 16, OT = W / 32;
-    _Float16 k[2][KW][KI][2][64][8];
-    _Float16 v[2][KW][OT][2][2][64][8];
+    // A half of 16 channels has 32 keys of eight channels, and room between them for the W / 8 lanes that store one
+    // key's to have banks of their own.
+    _Float16 k[2][KW][2][KI][2][kKeys + 128 / W][8];
+    _Float16 v[2][KW][OT][2][2][64][8];  // (channel c at place of(c))
+    static __device__ __forceinline__ int of(int c) { return c ^ (c >> 4 & 1); }  // (so have the lanes that store every other)
     float kdown[4][KW][kKeys];  // 2^-e of a key (step st: st % 4)
     float vexp[2][KW][kKeys];   // -e of a value row
     float vup[2][KW][kKeys];    // 2^e of it
@@ -775,8 +778,8 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
             const int e = lift(group_max<W / 8>(mag(most)), kLiftMost);
             h8f hi, lo;
             split8(x[i], pow2f(e), hi, lo);
-            *reinterpret_cast<h8f*>(st.k[step & 1][kt][kd >> 4][0][(kd & 8) * 4 + kk]) = hi;
-            *reinterpret_cast<h8f*>(st.k[step & 1][kt][kd >> 4][1][(kd & 8) * 4 + kk]) = lo;
+            *reinterpret_cast<h8f*>(st.k[step & 1][kt][0][kd >> 4][kd >> 3 & 1][kk]) = hi;
+            *reinterpret_cast<h8f*>(st.k[step & 1][kt][1][kd >> 4][kd >> 3 & 1][kk]) = lo;
             if (kd == 0) st.kdown[step & 3][kt][kk] = pow2f(-e);
         }
     };
@@ -817,8 +820,8 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
                 hi[1] = h;
                 lo[1] = l;
                 const int dd = vd + ch;
-                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][0][hq * 32 + (dd & 31)][4 * jq]) = hi;
-                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][1][hq * 32 + (dd & 31)][4 * jq]) = lo;
+                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][0][hq * 32 + st.of(dd & 31)][4 * jq]) = hi;
+                *reinterpret_cast<u32x2*>(&st.v[step & 1][kt][dd >> 5][s2][1][hq * 32 + st.of(dd & 31)][4 * jq]) = lo;
             }
             if (vd < 8) {
                 st.vexp[step & 1][kt][4 * qq + (lane & 3)] = static_cast<float>(-e);
@@ -853,12 +856,13 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
         }
     }
     const uint32_t row = b.row;
+    const int vplace = half * 32 + st.of(col);
     const auto scores = [&](uint32_t step) __attribute__((always_inline)) {
         f32x16 x = f32x16{};
 #pragma unroll
         for (int i = 0; i < KI; i++) {
-            const h8f kh = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][i][0][lane]);
-            const h8f kl = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][i][1][lane]);
+            const h8f kh = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][0][i][half][col]);
+            const h8f kl = *reinterpret_cast<const h8f*>(st.k[step & 1][kw][1][i][half][col]);
             x = mfma(kl, qh[i], x);
             x = mfma(kh, ql[i], x);
             x = mfma(kh, qh[i], x);
@@ -930,8 +934,8 @@ __device__ __forceinline__ void rows_block(const RowsArgs& a, char* smem, Block<
                 split8(w + 8 * s2, ph, pl);
 #pragma unroll
                 for (int d = 0; d < OT; d++) {
-                    const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][lane]);
-                    const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][lane]);
+                    const h8f vh = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][0][vplace]);
+                    const h8f vl = *reinterpret_cast<const h8f*>(st.v[buf][kw][d][s2][1][vplace]);
                     z.o[d] = mfma(vl, ph, z.o[d]);
                     z.o[d] = mfma(vh, pl, z.o[d]);
                     z.o[d] = mfma(vh, ph, z.o[d]);
