@@ -620,10 +620,10 @@ __device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs&
 // W: the head width brought to 32, 64 or 128.
 // The vector units bound it: a tile of 32 keys of width 64 is some 300 instructions a wave (half of them for the
 // staging) beside 24 products, and the two times add up.  32 trees of up to 32 nodes over up to 1023 rows, 14 and
-// 2 heads: 33.6 us, about 6 until the first tile is staged, 2 a tile, 5 to join four shares.  4 trees of up to 64
-// nodes over up to 16383 rows, 32 and 8 heads of width 128: 211 us, 2.1 TB/s of the cache and 214 TFLOP/s (three times
-// that of f16 products).  Scores of tile t + 1 are multiplied while tile t's become weights (without: 40.7 and 399 us with
-// the splits as they were).
+// 2 heads: 30.1 us, about 6 until the first tile is staged, 2 a tile, 5 to join four shares.  4 trees of up to 64
+// nodes over up to 16383 rows, 32 and 8 heads of width 128: 203 us a call, 2.2 TB/s of the cache and 222 TFLOP/s (three
+// times that of f16 products).  Scores of tile t + 1 are multiplied while tile t's become weights (when this was added 40.7
+// to 34.5 and 399 to 283 us).
 template <int W, int CW, int KW>
 struct Stage {
     static constexpr int KI = W / 16, OT = W / 32;
@@ -1135,7 +1135,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
 // rows of 32 and 8 heads 1460 us, 377 TFLOP/s or 1130 of f16 products; the clock falls as the matrix
 // units fill: 2.1 GHz where they were busy 40 % of the time, 1.7 at 60 %; four waves, each tile read
 // twice as often, 1557); 64: four, three to a SIMD (16 prompts of up to 1000 rows, 14 and 2 heads, 73
-// us; two to a SIMD 77, eight waves 90).  64 columns a wave with a SIMD to itself: 2000 and 125.
+// us, two to a SIMD 77, eight waves 90).  64 columns a wave with a SIMD to itself: 2000 and 125.
 template <int W, int NWV, int OCC>
 __global__ void __launch_bounds__(64 * NWV, OCC) k_gqa_prompt(RowsArgs a, const char* packed, const TileInfo* infos,
                                                                      int room) {
@@ -1317,18 +1317,20 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     const size_t tiles = (g.limit + kKeys - 1) / kKeys, pack = heads * tiles * (static_cast<size_t>(w) * 256);
     // The launches that pack the tiles and that look for blocks apart are about 15 us, won back where many column
     // blocks read the same tiles and there are enough of both (us packed and not, heads of width 64: 1 prompt of 1000
-    // rows, 14 and 2 heads 42 and 34, of 2000 57 and 62; 16 of up to 1000 rows 91 and 114; 8 of up to 1000, 12 and 12
-    // heads 82 and 77; of width 128, 32 and 8 heads: 1 prompt of 1000 rows 65 and 66, of 2000 168 and 211).
+    // rows, 14 and 2 heads 41 and 32, of 2000 55 and 56; 16 of up to 1000 rows 91 and 107; 8 of up to 1000, 12 and 12
+    // heads 81 and 72; of width 128, 32 and 8 heads: 1 prompt of 1000 rows 66 and 63, of 1500 106 and 112, of 2000 168
+    // and 190).
     const bool prompt = !g.parent && cols > 1024 && heads * cols * tiles > (size_t(3) << 19) && pack < (size_t(1) << 31);
     // Columns of a workgroup: as many as there are, while two workgroups fit a compute unit; of 64 columns and two waves that deal
-    // the keys for small calls (one tree of 16 nodes over 511 rows, 14 and 2 heads 16.4 us, 128 columns 18.8; 32 of up
-    // to 32 nodes 39.4 and 33.6).  Width 128: eight waves with the keys split once for 256 columns (4 trees of up to 64
-    // nodes over up to 16383 rows, 32 and 8 heads 226 us, four waves 275).
+    // the keys for small calls (us of 64 and of 128: one tree of 100 nodes over 4000 rows, 4 heads of width 32 24.4 and
+    // 26.3, one of 16 nodes over 511, 14 and 2 heads of 64 20.6 and 20.9, 32 of up to 32 nodes over up to 1023 39.8 and
+    // 36.4).  Width 128: eight waves with the keys split once for 256 columns (4 trees of up to 64 nodes over up to 16383
+    // rows, 32 and 8 heads 208 us, four waves 234).
     const int cw = w == 128 ? (cols > 128 ? 8 : 4) : cols > 128 ? 4 : 2;
     const size_t blocks = (cols + 32 * cw - 1) / (32 * cw);
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
     // Keys of few columns are dealt over as many workgroups as the device holds at once, two tiles of keys each at
-    // least (those 4 trees: 283 us with equal numbers of shares for all sequences).
+    // least (those 4 trees, when this was added: 215 us, 283 with equal numbers of shares for all sequences).
     const size_t cus = static_cast<size_t>(ctx->num_cus), all = cus * (cw == 8 ? 1 : prompt ? 3 : 2);
     const size_t places = all / g.n_kv, units = g.seqs * blocks;
     const bool planned = units <= std::min<size_t>(places, kPlanned) && tiles >= 4;
