@@ -148,7 +148,7 @@ int fh_kv4_room(fh_ctx* ctx, size_t bytes, void** out) {
         FH_HIP(ctx, hipStreamIsCapturing(ctx->stream, &cs));
         if (cs != hipStreamCaptureStatusNone)
             return fh_fail(ctx, FH_ERR_INVALID,
-                           "the 4-bit cache's workspace must grow, which cannot happen during graph capture: "
+                           "the cached attention's workspace must grow, which cannot happen during graph capture: "
                            "run the same call once outside capture first");
         bytes = fh_align256(std::max(bytes, 2 * ctx->kv4_room_bytes));
         void* room = nullptr;

@@ -1803,7 +1803,7 @@ class LlamaDevice:
         from self.zt) at the node before.  The accepted nodes' cache rows move together in every
         layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
         last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
-        many they were."""
+        many they were.  (forward_one goes on from next_pos: set it to self.pos first.)"""
         if self._tree is None:
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
         n, tokens, parents = self._tree
@@ -1812,6 +1812,7 @@ class LlamaDevice:
         tree_accept_async(self.ctx, parents, tokens, chosen, total, None, self.rows, n, self.pos, self._planes,
                           2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos)
         self.path, self.count, self._tree = w["path"].view(self.rows, n), w["count"], None
+        self._keep = (tokens, parents, chosen)  # alive until the stream has used them
 
     def evict_async(self, keep: int, recent: int):
         """Cuts every row's caches that hold more than `keep` keys to the last

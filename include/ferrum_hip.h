@@ -600,8 +600,10 @@ int fh_gqa_attention_rope_tree_async(fh_ctx* ctx, const float* d_qkv, size_t ld,
  * d_new_len [seqs] (it may be d_len) d_len + the number.  In each of the n_planes caches
  * whose device addresses d_planes holds ([seqs, capacity, kv_dim] floats each; every layer's
  * keys and values), cache row d_len[s] + path[i] goes to d_len[s] + i; rows past the
- * capacity are not touched.  A sequence without rows: d_count 0, d_next left as it is.  At
- * most 1024 rows a sequence, 65535 sequences, else FH_ERR_LIMIT. */
+ * capacity are not touched.  A sequence without rows: d_count 0, d_next left as it is.  No
+ * other output may overlap an input, and the caches do not overlap.  At most 1024 rows a
+ * sequence, 65535 sequences, 65535 caches, else FH_ERR_LIMIT.  Calls of one context must not
+ * overlap, replayed graphs included. */
 int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
                          size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
                          const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
@@ -642,7 +644,7 @@ typedef struct {
     const uint32_t* d_mask_of;
     size_t masks;
 } fh_logits_edit;
-/* d_out [rows, vocab] gets the edited logits; it may be d_logits. */
+/* d_out [rows, vocab] gets the edited logits; it may be d_logits, else nothing that is read. */
 int fh_logits_edit_async(fh_ctx* ctx, const float* d_logits, size_t rows, size_t vocab, const fh_logits_edit* edit,
                          float* d_out);
 
