@@ -385,14 +385,13 @@ __device__ __forceinline__ void clear(Sums<OT>& z) {
 #pragma unroll
     for (int d = 0; d < OT; d++) z.o[d] = f32x16{};
 }
-// Weights lie at 2^10 of the largest so far, and up to 2^14 before the sums are brought to a
-// new one: their lower terms stay normal numbers of f16 far below it.
+// Weights lie at 2^10 of the largest so far, and up to 2^14 before a column's sums are brought to a
+// new one (its own scores decide, not its neighbours'): their lower terms stay normal numbers of f16 far below it.
 constexpr float kRaise = 14.0f;
 template <int OT>
 __device__ __forceinline__ void raise_base(Sums<OT>& z, float top) {
     if (__any(top > z.base + kRaise)) {
-        const float m = fmaxf(z.base == -FLT_MAX ? -FLT_MAX : z.base + 10.0f, max_halves(top));
-        const float nb = m == -FLT_MAX ? -FLT_MAX : m - 10.0f, f = __builtin_amdgcn_exp2f(z.base - nb);
+        const float m = max_halves(top), nb = m > z.base + kRaise ? m - 10.0f : z.base, f = __builtin_amdgcn_exp2f(z.base - nb);
         z.l *= f;
 #pragma unroll
         for (int d = 0; d < OT; d++) z.o[d] *= f;

@@ -163,3 +163,29 @@ def test_acceptance_in_caches_at_odd_addresses(fh, kv_dim):
             np.testing.assert_array_equal(v[s].cpu().numpy(), want)
     for p in planes:
         assert p.isfinite().all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (32, 2, 64), (4, 2, 128), (80, 2, 128), (4, 4, 32), (2, 1, 8)])
+@pytest.mark.parametrize("where", ["q", "k", "v", "cached k", "cached v"])
+def test_every_channel_of_a_row_that_sees_what_is_not_finite(fh, bad, heads, where):
+    """And no bit of the others, at every number of columns of a workgroup."""
+    for parents in (None, trees([40], 67)):
+        a = Call(heads, [50], [40], 68, parents=parents, rope=(None, None))
+        plain = a.run(fh)
+        at, group = 29, a.h // a.g
+        if where == "cached k":
+            a.k[0, at, 2] = bad
+        elif where == "cached v":
+            a.v[0, at, 2] = bad
+        else:
+            a.qkv[at, {"q": group - 1, "k": a.h, "v": a.h + a.g}[where] * a.hd + 3] = bad
+        got = a.run(fh)
+        ways = [list(range(t + 1)) if parents is None else ref.path(parents[0], t) for t in range(40)]
+        hit = np.zeros((40, a.h), bool)
+        if where == "q":
+            hit[at, group - 1] = True
+        else:
+            hit[["cached" in where or at in w for w in ways], :group] = True
+        assert np.isnan(got[hit]).all()
+        np.testing.assert_array_equal(got[~hit], plain[~hit])
