@@ -1330,8 +1330,12 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     if (heads * blocks > 0x7FFFFFFFu / 64) return fh_fail(ctx, FH_ERR_LIMIT, "fh_gqa_attention: more than 2^25 workgroups");
     // Keys of few columns are dealt over as many workgroups as the device holds at once, two tiles of keys each at
     // least (those 4 trees, when this was added: 215 us, 283 with equal numbers of shares for all sequences).
-    const size_t cus = static_cast<size_t>(ctx->num_cus), all = cus * (cw == 8 ? 1 : prompt ? 3 : 2);
-    const size_t places = all / g.n_kv, units = g.seqs * blocks;
+    const size_t cus = static_cast<size_t>(ctx->num_cus), units = g.seqs * blocks;
+    // Where a compute unit has 16 tiles at most, one workgroup on each: two would meet on some while others had none (us
+    // with one and with two: a tree of 16 nodes over 16000 rows, 14 and 2 heads 33 and 39, a prompt of 64 rows over 4000
+    // 31 and 39; 32 trees of up to 32 nodes over up to 1023, 17 tiles each, 40 and 36).
+    const bool few = units * tiles * g.n_kv <= 16 * cus;
+    const size_t all = cus * (cw == 8 || few ? 1 : prompt ? 3 : 2), places = all / g.n_kv;
     const bool planned = units <= std::min<size_t>(places, kPlanned) && tiles >= 4;
     const uint32_t workgroups = static_cast<uint32_t>(planned ? places * g.n_kv : heads * blocks);
     unsigned* counters = nullptr;
