@@ -1475,11 +1475,13 @@ struct AcceptArgs {
     uint32_t *path, *count, *next, *new_len;
     const uint64_t* planes;
     size_t n_planes, kv_dim, capacity;
+    uint64_t stored;  // cache rows of a sequence: nothing is accepted from there on
 };
 
 // A workgroup a sequence and cache plane (without planes, a sequence): every row finds out whether it
 // continues its parent with the token chosen there, the first such is its parent's child, and one thread
-// follows the children from row 0; then the plane's accepted rows move to their places, as many at a
+// follows the children from row 0, as far as their keys and values were stored (a row that was not has scores
+// that are no numbers, and rows of a path rise: none behind it was); then the plane's accepted rows move to their places, as many at a
 // time as 256 threads hold.  A row moves down only, and all of a batch is read before any of it is
 // written: what a write overwrites has moved or is left behind.  Latency: a chain of three loads, the
 // walk and the move (one sequence of 16 rows and 48 planes 3.8 us, 32 of up to 32 rows 5.1; the walk and the move in
@@ -1505,7 +1507,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_accept(AcceptArgs a, unsigned
     __syncthreads();
     if (threadIdx.x == 0) {
         uint32_t n = 0;
-        for (uint32_t t = 0; t < r.count; t = child[t]) way[n++] = t;  // (rows of a path rise; ~0 ends it)
+        for (uint32_t t = 0; t < r.count && r.at + t < a.stored; t = child[t]) way[n++] = t;  // (~0 ends it)
         steps = n;
     }
     __syncthreads();
@@ -1541,7 +1543,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_accept(AcceptArgs a, unsigned
                 moves[j] = item / wide < rows && i < n;
                 if (!moves[j]) continue;
                 const uint64_t p = way[i];
-                moves[j] = p != i && r.at + p < a.capacity;
+                moves[j] = p != i;
                 if (!moves[j]) continue;
                 to[j] = static_cast<size_t>(r.at + i) * width + c0 + item % wide;
                 x[j] = plane[static_cast<size_t>(r.at + p) * width + c0 + item % wide];
@@ -1561,7 +1563,8 @@ int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* t
                           size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
                           uint32_t* new_len) {
     AcceptArgs a{parent, tokens, chosen, off, len, static_cast<uint32_t>(seqs), static_cast<uint32_t>(total),
-                 static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, n_planes, kv_dim, capacity};
+                 static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, n_planes, kv_dim, capacity,
+                 n_planes ? capacity : ~uint64_t(0)};
     unsigned* arrived = nullptr;
     if (new_len == len && n_planes > 1) {
         void* area = nullptr;

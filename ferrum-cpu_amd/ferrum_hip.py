@@ -1222,9 +1222,10 @@ def gqa_attention_rope_tree_async(ctx: Context, qkv, ld: int, total: int, n_head
 def tree_accept_async(ctx: Context, parent, tokens, chosen, total: int, off, seqs: int, max_rows: int, len_, planes,
                       n_planes: int, kv_dim: int, capacity: int, path, count, next_, new_len):
     """Follows each sequence's tree from its row 0 along the drafted tokens that the model
-    chose itself (chosen [total]): path [total] (-1 behind the last), count, next_ (the id
-    chosen behind it) and new_len [seqs]; the accepted rows move together in the caches
-    whose device addresses planes (int64) holds."""
+    chose itself (chosen [total]), as far as the caches have places for them: path [total]
+    (-1 behind the last), count, next_ (the id chosen behind it; left as it is where count is 0)
+    and new_len [seqs]; the accepted rows move together in the caches whose device addresses
+    planes (int64) holds."""
     ctx.check(lib().fh_tree_accept_async(ctx.h, _ptr(parent), _ptr(tokens), _ptr(chosen), total, _ptr(off), seqs, max_rows,
                                          _ptr(len_), _ptr(planes), n_planes, kv_dim, capacity, _ptr(path), _ptr(count),
                                          _ptr(next_), _ptr(new_len)))
@@ -1803,7 +1804,8 @@ class LlamaDevice:
         from self.zt) at the node before.  The accepted nodes' cache rows move together in every
         layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
         last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
-        many they were.  (forward_one goes on from next_pos: set it to self.pos first.)"""
+        many they were.  Nodes past the cache are not accepted: a count of 0 is a full cache.
+        (forward_one goes on from next_pos: set it to self.pos first.)"""
         if self._tree is None:
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
         n, tokens, parents = self._tree

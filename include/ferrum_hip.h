@@ -595,15 +595,16 @@ int fh_gqa_attention_rope_tree_async(fh_ctx* ctx, const float* d_qkv, size_t ld,
 /* What is accepted of each sequence's tree (rows, d_off, d_len and d_parent as above; row 0 is
  * the token that the model chose last, accepted as it is): from row 0 on, the first row that
  * continues it and whose d_tokens [total] is the d_chosen [total] of the row before, until
- * there is none.  d_path [total]: the accepted rows in order, at the sequence's rows, then
- * 0xFFFFFFFF; d_count [seqs] their number; d_next [seqs] the last one's d_chosen;
- * d_new_len [seqs] (it may be d_len) d_len + the number.  In each of the n_planes caches
- * whose device addresses d_planes holds ([seqs, capacity, kv_dim] floats each; every layer's
- * keys and values), cache row d_len[s] + path[i] goes to d_len[s] + i; rows past the
- * capacity are not touched.  A sequence without rows: d_count 0, d_next left as it is.  No
- * other output may overlap an input, and the caches do not overlap.  At most 1024 rows a
- * sequence, 65535 sequences, 65535 caches, else FH_ERR_LIMIT.  Calls of one context must not
- * overlap, replayed graphs included. */
+ * there is none or it has no place in the caches (cache row d_len[s] + t at or past the
+ * capacity; where row 0 has none, nothing is accepted).  d_path [total]: the accepted rows in
+ * order, at the sequence's rows, then 0xFFFFFFFF; d_count [seqs] their number; d_next [seqs]
+ * the last one's d_chosen; d_new_len [seqs] (it may be d_len) d_len + the number.  In each of
+ * the n_planes caches whose device addresses d_planes holds ([seqs, capacity, kv_dim] floats
+ * each; every layer's keys and values; n_planes 0: no caches, and no capacity), cache row
+ * d_len[s] + path[i] goes to d_len[s] + i.  A sequence of which nothing is accepted: d_count 0,
+ * d_next left as it is.  No other output may overlap an input, and the caches do not overlap.
+ * At most 1024 rows a sequence, 65535 sequences, 65535 caches, else FH_ERR_LIMIT.  Calls of one
+ * context must not overlap, replayed graphs included. */
 int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
                          size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
                          const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,

@@ -13,6 +13,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (runs the HIP path through the C ABI)")
 
 
+# Tests that hold a value that has been shown to be wrong: they run as they are and are expected to fail.
+HOLD_WRONG_VALUES = {
+    "test_gpu_tree_accept.py::test_rows_outside_beyond_and_in_place":
+        "its third call wants 4 rows accepted behind 30 in a cache of 33 (a length of 34, rows 33 and 34 never "
+        "stored); test_gpu_tree_accept_bounds.py has what is right, and this test's other calls",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        reason = HOLD_WRONG_VALUES.get(item.nodeid.split("/")[-1])
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
+
+
 @pytest.fixture(scope="session")
 def orc():
     import oracle
