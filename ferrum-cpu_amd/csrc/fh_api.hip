@@ -1116,10 +1116,11 @@ int fh_gqa_attention_rope_tree_async(fh_ctx* ctx, const float* d_qkv, size_t ld,
     return gqa_rows(ctx, "fh_gqa_attention_rope_tree", g, max_keys, true);
 }
 
-int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
-                         size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
-                         const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
-                         uint32_t* d_count, uint32_t* d_next, uint32_t* d_new_len) {
+int fh_tree_accept_within_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
+                                size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
+                                const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity,
+                                size_t max_keys, uint32_t* d_path, uint32_t* d_count, uint32_t* d_next,
+                                uint32_t* d_new_len) {
     if (!ctx) return FH_ERR_INVALID;
     ctx->err.clear();
     if (seqs == 0) return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: no sequences");
@@ -1141,7 +1142,15 @@ int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* 
         return fh_fail(ctx, FH_ERR_INVALID, "fh_tree_accept: caches without addresses, width or capacity");
     FH_ON_DEVICE(ctx);
     return fh_launch_tree_accept(ctx, d_parent, d_tokens, d_chosen, total, d_off, seqs, max_rows, d_len, d_planes, n_planes,
-                                 kv_dim, capacity, d_path, d_count, d_next, d_new_len);
+                                 kv_dim, capacity, max_keys, d_path, d_count, d_next, d_new_len);
+}
+
+int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
+                         size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
+                         const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
+                         uint32_t* d_count, uint32_t* d_next, uint32_t* d_new_len) {
+    return fh_tree_accept_within_async(ctx, d_parent, d_tokens, d_chosen, total, d_off, seqs, max_rows, d_len, d_planes,
+                                       n_planes, kv_dim, capacity, SIZE_MAX, d_path, d_count, d_next, d_new_len);
 }
 
 int fh_logits_edit_async(fh_ctx* ctx, const float* d_logits, size_t rows, size_t vocab, const fh_logits_edit* edit,

@@ -1560,11 +1560,11 @@ __global__ void __launch_bounds__(kThreads) k_tree_accept(AcceptArgs a, unsigned
 
 int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* tokens, const uint32_t* chosen, size_t total,
                           const uint32_t* off, size_t seqs, size_t max_rows, const uint32_t* len, const uint64_t* planes,
-                          size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
-                          uint32_t* new_len) {
+                          size_t n_planes, size_t kv_dim, size_t capacity, size_t max_keys, uint32_t* path,
+                          uint32_t* count, uint32_t* next, uint32_t* new_len) {
     AcceptArgs a{parent, tokens, chosen, off, len, static_cast<uint32_t>(seqs), static_cast<uint32_t>(total),
                  static_cast<uint32_t>(max_rows), path, count, next, new_len, planes, n_planes, kv_dim, capacity,
-                 n_planes ? capacity : ~uint64_t(0)};
+                 n_planes ? std::min(capacity, max_keys) : max_keys};
     unsigned* arrived = nullptr;
     if (new_len == len && n_planes > 1) {
         void* area = nullptr;

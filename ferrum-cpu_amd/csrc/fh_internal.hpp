@@ -286,8 +286,8 @@ struct fh_gqa_call {
 int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g);
 int fh_launch_tree_accept(fh_ctx* ctx, const uint32_t* parent, const uint32_t* tokens, const uint32_t* chosen, size_t total,
                           const uint32_t* off, size_t seqs, size_t max_rows, const uint32_t* len, const uint64_t* planes,
-                          size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* path, uint32_t* count, uint32_t* next,
-                          uint32_t* new_len);
+                          size_t n_planes, size_t kv_dim, size_t capacity, size_t max_keys, uint32_t* path,
+                          uint32_t* count, uint32_t* next, uint32_t* new_len);
 int fh_launch_logits_edit(fh_ctx* ctx, const float* logits, size_t rows, size_t vocab, const fh_logits_edit& e, float* out);
 int fh_launch_dequant(fh_ctx* ctx, const uint8_t* raw, size_t n, float* out);
 int fh_launch_block_dots(fh_ctx* ctx, const fh_q8_0* w, const int8_t* qx, size_t m,

@@ -52,7 +52,7 @@ EXPORTS = (
     "fh_gpt2_stack_create", "fh_gpt2_stack_free", "fh_gpt2_stack_forward_async",
     "fh_rmsnorm_async", "fh_rope_async", "fh_gqa_attention_decode_async", "fh_gqa_attention_rope_decode_async",
     "fh_gqa_attention_rope_prefill_async", "fh_gqa_attention_rope_tree_async", "fh_tree_accept_async",
-    "fh_logits_edit_async",
+    "fh_tree_accept_within_async", "fh_logits_edit_async",
     "fh_swiglu_async", "fh_embed_rows_async",
     "fh_embed_rows_pos_async",
     "fh_gguf_open", "fh_gguf_close", "fh_gguf_error", "fh_gguf_version", "fh_gguf_tensor_count", "fh_gguf_find_tensor",
@@ -315,6 +315,7 @@ def lib():
         L.fh_gqa_attention_rope_prefill_async.argtypes = rows + [vp] + turn
         L.fh_gqa_attention_rope_tree_async.argtypes = rows + [vp, vp] + turn
         L.fh_tree_accept_async.argtypes = [vp, vp, vp, vp, sz, vp, sz, sz, vp, vp, sz, sz, sz, vp, vp, vp, vp]
+        L.fh_tree_accept_within_async.argtypes = [vp, vp, vp, vp, sz, vp, sz, sz, vp, vp, sz, sz, sz, sz, vp, vp, vp, vp]
         L.fh_logits_edit_async.argtypes = [vp, vp, sz, sz, C.POINTER(LogitsEdit), vp]
         _lib = L
     return _lib
@@ -1220,15 +1221,17 @@ def gqa_attention_rope_tree_async(ctx: Context, qkv, ld: int, total: int, n_head
 
 
 def tree_accept_async(ctx: Context, parent, tokens, chosen, total: int, off, seqs: int, max_rows: int, len_, planes,
-                      n_planes: int, kv_dim: int, capacity: int, path, count, next_, new_len):
+                      n_planes: int, kv_dim: int, capacity: int, path, count, next_, new_len, max_keys=None):
     """Follows each sequence's tree from its row 0 along the drafted tokens that the model
     chose itself (chosen [total]), as far as the caches have places for them: path [total]
     (-1 behind the last), count, next_ (the id chosen behind it; left as it is where count is 0)
     and new_len [seqs]; the accepted rows move together in the caches whose device addresses
-    planes (int64) holds."""
-    ctx.check(lib().fh_tree_accept_async(ctx.h, _ptr(parent), _ptr(tokens), _ptr(chosen), total, _ptr(off), seqs, max_rows,
-                                         _ptr(len_), _ptr(planes), n_planes, kv_dim, capacity, _ptr(path), _ptr(count),
-                                         _ptr(next_), _ptr(new_len)))
+    planes (int64) holds.  max_keys: the attention call's, where it was below the capacity."""
+    before = (ctx.h, _ptr(parent), _ptr(tokens), _ptr(chosen), total, _ptr(off), seqs, max_rows, _ptr(len_), _ptr(planes),
+              n_planes, kv_dim, capacity)
+    outs = (_ptr(path), _ptr(count), _ptr(next_), _ptr(new_len))
+    ctx.check(lib().fh_tree_accept_async(*before, *outs) if max_keys is None else
+              lib().fh_tree_accept_within_async(*before, max_keys, *outs))
 
 
 def logits_edit_async(ctx: Context, logits, rows: int, vocab: int, edit: LogitsEdit, out):
@@ -1767,8 +1770,8 @@ class LlamaDevice:
         is the token that the row goes on with (self.tokens of a plain step), node t > 0 a
         draft to follow node parents[t] < t of its tree.  Node t lies at cache row self.pos[r] + t
         and is seen by the nodes behind it; max_pos bounds self.pos.  The nodes' scores land in
-        self.zt [rows * n, vocab]; nothing is advanced (accept_async).  Nodes past the cache get
-        NaN scores."""
+        self.zt [rows * n, vocab]; nothing is advanced (accept_async).  Nodes past the cache, or at
+        row max_pos + n or past it, get NaN scores and are not accepted."""
         import torch
 
         if self.kv != "f32":
@@ -1796,7 +1799,7 @@ class LlamaDevice:
 
         self._blocks_async(tokens, total, w, attend)
         linear_forward_async(ctx, self.head, w["h"], total, self.d, None, 0, w["z"])
-        self._tree, self.zt = (n, tokens, parents), w["z"]
+        self._tree, self.zt = (n, tokens, parents, max_keys), w["z"]
 
     def accept_async(self, chosen):
         """After verify_async: follows each row's tree from node 0 along the drafts that equal
@@ -1804,15 +1807,16 @@ class LlamaDevice:
         from self.zt) at the node before.  The accepted nodes' cache rows move together in every
         layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
         last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
-        many they were.  Nodes past the cache are not accepted: a count of 0 is a full cache.
+        many they were.  Nodes that verify_async had no place for are not accepted: a count of 0
+        is a full cache (or a max_pos below self.pos - n).
         (forward_one goes on from next_pos: set it to self.pos first.)"""
         if self._tree is None:
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
-        n, tokens, parents = self._tree
+        n, tokens, parents, max_keys = self._tree
         total, w = self.rows * n, self._trees[n]
         self._ids("accept_async", "ids", chosen, total, f"{self.rows} trees of {n}")
         tree_accept_async(self.ctx, parents, tokens, chosen, total, None, self.rows, n, self.pos, self._planes,
-                          2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos)
+                          2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos, max_keys)
         self.path, self.count, self._tree = w["path"].view(self.rows, n), w["count"], None
         self._keep = (tokens, parents, chosen)  # alive until the stream has used them
 

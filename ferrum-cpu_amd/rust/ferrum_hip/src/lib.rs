@@ -193,6 +193,7 @@ pub mod sys {
         pub fn fh_gqa_attention_rope_prefill_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, seqs: usize, capacity: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
         pub fn fh_gqa_attention_rope_tree_async(ctx: *mut fh_ctx, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, n_kv: usize, head_dim: usize, d_k_cache: *mut f32, d_v_cache: *mut f32, seqs: usize, capacity: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, d_parent: *const u32, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_out: *mut f32) -> c_int;
         pub fn fh_tree_accept_async(ctx: *mut fh_ctx, d_parent: *const u32, d_tokens: *const u32, d_chosen: *const u32, total: usize, d_off: *const u32, seqs: usize, max_rows: usize, d_len: *const u32, d_planes: *const u64, n_planes: usize, kv_dim: usize, capacity: usize, d_path: *mut u32, d_count: *mut u32, d_next: *mut u32, d_new_len: *mut u32) -> c_int;
+        pub fn fh_tree_accept_within_async(ctx: *mut fh_ctx, d_parent: *const u32, d_tokens: *const u32, d_chosen: *const u32, total: usize, d_off: *const u32, seqs: usize, max_rows: usize, d_len: *const u32, d_planes: *const u64, n_planes: usize, kv_dim: usize, capacity: usize, max_keys: usize, d_path: *mut u32, d_count: *mut u32, d_next: *mut u32, d_new_len: *mut u32) -> c_int;
         pub fn fh_logits_edit_async(ctx: *mut fh_ctx, d_logits: *const f32, rows: usize, vocab: usize, edit: *const fh_logits_edit, d_out: *mut f32) -> c_int;
         pub fn fh_kv4_append_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_qkv: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, d_pos: *const u32, rope_dim: usize, base: f32, rope_type: c_int, d_freq_factors: *const f32, linear_factor: f32, d_q: *mut f32) -> c_int;
         pub fn fh_kv4_attention_async(ctx: *mut fh_ctx, cache: *const fh_kv4_cache, d_q: *const f32, ld: usize, total: usize, n_heads: usize, d_off: *const u32, max_rows: usize, d_len: *const u32, max_keys: usize, score: *const fh_attn_score, d_out: *mut f32, d_lse: *mut f32) -> c_int;

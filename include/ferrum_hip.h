@@ -609,6 +609,13 @@ int fh_tree_accept_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* 
                          size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
                          const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity, uint32_t* d_path,
                          uint32_t* d_count, uint32_t* d_next, uint32_t* d_new_len);
+/* The same after an attention call with max_keys below the capacity: rows that it had no place
+ * for (cache row d_len[s] + t at or past max_keys) are not accepted either. */
+int fh_tree_accept_within_async(fh_ctx* ctx, const uint32_t* d_parent, const uint32_t* d_tokens, const uint32_t* d_chosen,
+                                size_t total, const uint32_t* d_off, size_t seqs, size_t max_rows, const uint32_t* d_len,
+                                const uint64_t* d_planes, size_t n_planes, size_t kv_dim, size_t capacity,
+                                size_t max_keys, uint32_t* d_path, uint32_t* d_count, uint32_t* d_next,
+                                uint32_t* d_new_len);
 
 /* ---- logits before they are sampled --------------------------------------------------
  * sample_with_params (slm/sampling.rs:124-210) knows one penalty, once per occurrence;

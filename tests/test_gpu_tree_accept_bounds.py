@@ -17,7 +17,7 @@ def way_within(parent, tokens, chosen, at, limit):
     return ref.accept(parent[:stored], tokens[:stored], chosen[:stored])
 
 
-def call(fh, trees, lens, cap, planes, kv_dim, alias=False, caches=True):
+def call(fh, trees, lens, cap, planes, kv_dim, alias=False, caches=True, max_keys=None):
     """The call's outputs, and the caches before and after."""
     import ferrum_hip
     import torch
@@ -34,7 +34,8 @@ def call(fh, trees, lens, cap, planes, kv_dim, alias=False, caches=True):
     new_len = length if alias else ln
     torch.cuda.synchronize()
     ferrum_hip.tree_accept_async(fh, parent, tokens, chosen, total, doff, seqs, max(news), length, table if caches else None,
-                                 planes if caches else 0, kv_dim, cap, path, count, nxt, new_len)
+                                 planes if caches else 0, kv_dim, cap, path, count, nxt, new_len,
+                                 *([] if max_keys is None else [max_keys]))
     fh.sync()
     path = path.cpu().numpy()
     paths = [path[off[s]:off[s + 1]].tolist() for s in range(seqs)]
@@ -115,6 +116,47 @@ def test_a_step_behind_an_acceptance_at_the_end_of_the_context(fh, orc, name):
     assert m.count.tolist() == [1, 2] and m.path.tolist() == [[0, -1, -1, -1], [0, 3, -1, -1]]
     assert m.pos.tolist() == [cap - 2, cap - 7] and m.tokens.tolist() == [23, 33]
     m.feed_async(cap - 2)
+    fh.sync()
+    for r, t in enumerate((text[0] + [3, 23], text[1] + [4, 23, 33])):
+        oracle = OracleLlamaRow(orc, w, cfg)
+        assert close(m.z[r].cpu().numpy(), [oracle.feed(x) for x in t][-1]), r
+    m.free()
+
+
+@pytest.mark.parametrize("alias", [False, True])
+def test_rows_that_the_attention_had_no_place_for(fh, alias):
+    """max_keys below the capacity, above it, and without caches."""
+    rng = np.random.default_rng(43)
+    trees = [draft(n, rng, 0.9, 3) for n in (20, 40, 300)] + [(np.arange(30) - 1, np.arange(30) + 50, np.arange(30) + 51)]
+    assert check(fh, trees, [24, 27, 29, 10], 400, 30, alias=alias, max_keys=30) >= 2
+    check(fh, trees, [24, 27, 29, 10], 400, 0, alias=alias, max_keys=0)
+    check(fh, trees, [24, 27, 29, 10], 400, 400, alias=alias, max_keys=1 << 40)
+    paths, count, _, new_len, _, _ = call(fh, trees[3:], [10], 400, 1, 8, caches=False, max_keys=30)
+    assert (paths, count, new_len) == ([list(range(20)) + [-1] * 10], [20], [30])
+
+
+def test_drafts_past_max_pos_are_not_accepted(fh, orc):
+    """A step with a bound that the rows have outgrown, as a captured one replayed too often has: the
+    drafts it had no place for are left, and the next token's scores are the oracle's."""
+    import torch
+
+    cfg, w, m = build(fh, orc, "qwen", 2)
+    rng = np.random.default_rng(44)
+    text = [rng.integers(0, cfg["vocab"], n).tolist() for n in (20, 17)]
+    m.prompt_async(ints(np.concatenate(text)), [20, 17])
+    m.pos.copy_(ints([20, 17]))
+    tokens, parents = ints([3, 21, 22, 23, 4, 21, 22, 23]), ints([-1, 0, 0, 0] * 2)
+    chosen = ints([23, 31, 32, 33] * 2)
+    torch.cuda.synchronize()
+    m.verify_async(tokens, parents, 4, 18)  # rows up to 21
+    fh.sync()
+    finite = torch.isfinite(m.zt).all(dim=1).tolist()
+    assert finite == [True, True, False, False] + [True] * 4
+    m.accept_async(chosen)
+    fh.sync()
+    assert m.count.tolist() == [1, 2] and m.path.tolist() == [[0, -1, -1, -1], [0, 3, -1, -1]]
+    assert m.pos.tolist() == [21, 19] and m.tokens.tolist() == [23, 33]
+    m.feed_async(21)
     fh.sync()
     for r, t in enumerate((text[0] + [3, 23], text[1] + [4, 23, 33])):
         oracle = OracleLlamaRow(orc, w, cfg)
