@@ -180,15 +180,21 @@ class LogitsEdit(C.Structure):
     [rows, 2]: each row's list of ids; repetition, frequency, presence [rows]; tokens,
     parent [rows] of drafted trees, `seqs` sequences with rows off[s] .. off[s + 1] - 1 (off
     None: equal parts); bias_off [rows + 1], bias_id, bias; mask [masks, ceil(vocab / 32)]
-    bits of the ids that stay, mask_of [rows] (None: row r's is mask r).  Integers are
-    32-bit.  Tensors are kept alive here."""
+    bits of the ids that stay (masks None: as many as the mask has rows), mask_of [rows]
+    (None: row r's is mask r).  Integers are 32-bit.  Tensors are kept alive here."""
 
     _FIELDS = ("recent", "ranges", "repetition", "frequency", "presence", "parent", "tokens", "off", "seqs", "bias_off",
                "bias_id", "bias", "mask", "mask_of", "masks")
     _fields_ = [(n, C.c_size_t if n in ("seqs", "masks") else C.c_void_p) for n in _FIELDS]
 
     def __init__(self, recent=None, ranges=None, repetition=None, frequency=None, presence=None, parent=None, tokens=None,
-                 off=None, seqs: int = 0, bias_off=None, bias_id=None, bias=None, mask=None, mask_of=None, masks: int = 0):
+                 off=None, seqs: int = 0, bias_off=None, bias_id=None, bias=None, mask=None, mask_of=None, masks=None):
+        if masks is None:
+            shape = getattr(mask, "shape", ())
+            if mask is not None and len(shape) != 2:
+                raise FerrumHipError(FH_ERR_INVALID, "LogitsEdit: masks has to say how many rows a mask that is not "
+                                                     "[masks, words] has")
+            masks = shape[0] if shape else 0
         values = (recent, ranges, repetition, frequency, presence, parent, tokens, off, int(seqs), bias_off, bias_id, bias,
                   mask, mask_of, int(masks))
         super().__init__(*(v if n in ("seqs", "masks") else _ptr(v) for n, v in zip(self._FIELDS, values)))
