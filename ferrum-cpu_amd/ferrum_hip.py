@@ -1649,7 +1649,7 @@ class LlamaDevice:
             self.ctx.sync()
             if fed is None or int(pos[0]) == fed:
                 pos.fill_(self._next_pos)
-            torch.cuda.current_stream().synchronize()
+            torch.cuda.synchronize(pos.device)
         self._ahead = None
 
     def forward_one(self, token: int):
@@ -1738,13 +1738,14 @@ class LlamaDevice:
         total, most = int(n.sum()), int(n.max())
         self._ids(who, "tokens", tokens, total, f"{total} places")
         self._go_on(who)
-        ctx.sync()
-        torch.cuda.synchronize()
         place = self.used if self.kv == "q4" else self.pos
+        dev = place.device  # (the model's: another may be the current one)
+        ctx.sync()
+        torch.cuda.synchronize(dev)
         max_keys = int((place.cpu().numpy().astype(np.int64) + n).max())
         if max_keys > self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
-        dev, ends = "cuda", np.cumsum(n)
+        ends = np.cumsum(n)
         off = torch.from_numpy(np.concatenate([[0], ends]).astype(np.int32)).to(dev)
         w = self._row_buffers(total)
         if self.kv == "q4":
@@ -1761,11 +1762,11 @@ class LlamaDevice:
                 gqa_attention_rope_prefill_async(ctx, w["qkv"], self.qkv_dim, total, self.nh, self.nkv, self.hd, b["k"],
                                                  b["v"], B, self.cap, off, most, self.pos, max_keys, None, self.rope_dim,
                                                  self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear, w["att"])
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(dev)
         self._blocks_async(tokens, total, w, attend)
         ctx.sync()
         last = w["h"][torch.from_numpy(ends - 1).to(dev)].contiguous()
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(dev)
         linear_forward_async(ctx, self.head, last, B, self.d, None, 0, self.z)
         self._keep = last  # alive until the stream has used it
 
@@ -1775,7 +1776,7 @@ class LlamaDevice:
 
         widths = {"x": self.d, "x2": self.d, "h": self.d, "proj": self.d, "qkv": self.qkv_dim, "att": self.q_dim,
                   "gu": 2 * self.ffn, "mid": self.ffn}
-        return {name: torch.empty((total, wide), device="cuda") for name, wide in widths.items()}
+        return {name: torch.empty((total, wide), device=self.pos.device) for name, wide in widths.items()}
 
     def _blocks_async(self, tokens, total: int, w: dict, attend):
         """The blocks over `total` rows of any sequences (attend: a block's attention, from
@@ -1823,14 +1824,15 @@ class LlamaDevice:
         for what, ids in (("tokens", tokens), ("parents", parents)):
             self._ids("verify_async", what, ids, total, f"{B} trees of {n}")
         self._go_on("verify_async")
+        dev = self.pos.device
         if n not in self._trees:
-            ints = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
-            self._trees[n] = dict(self._row_buffers(total), z=torch.empty((total, self.vocab), device="cuda"),
+            ints = lambda m: torch.zeros(m, dtype=torch.int32, device=dev)  # noqa: E731
+            self._trees[n] = dict(self._row_buffers(total), z=torch.empty((total, self.vocab), device=dev),
                                   path=ints(total), count=ints(B))
             if self._planes is None:
                 self._planes = torch.tensor([b[c].data_ptr() for b in self.blocks for c in "kv"], dtype=torch.int64,
-                                            device="cuda")
-            torch.cuda.synchronize()
+                                            device=dev)
+            torch.cuda.synchronize(dev)
         w = self._trees[n]
         max_keys = min(max_pos + n, self.cap)
 

@@ -1,0 +1,71 @@
+"""What LlamaDevice keeps between verify_async and accept_async, on the CPU: the calls into the
+library are recorded, not made."""
+import gc
+import types
+import weakref
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import ferrum_hip as F  # noqa: E402
+
+CALLS = ("embed_rows_async", "rmsnorm_async", "linear_forward_async", "swiglu_async", "gqa_attention_rope_tree_async",
+         "gqa_attention_rope_prefill_async", "tree_accept_async", "gqa_attention_decode_async", "rope_async")
+
+
+class Ctx:
+    def __init__(self):
+        self.waits = 0
+
+    def sync(self):
+        self.waits += 1
+
+
+@pytest.fixture
+def model(monkeypatch):
+    """rows, device -> a LlamaDevice without weights; its calls gather in m.calls."""
+    calls = []
+    for name in CALLS:
+        monkeypatch.setattr(F, name, lambda *a, _n=name, **k: calls.append((_n, a)))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a, **k: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a, **k: types.SimpleNamespace(synchronize=lambda: None))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(F.LlamaDevice, "_ids", lambda *a: None)
+    empty = torch.empty
+
+    def make(rows, device="cpu", vocab=64):
+        cfg = dict(vocab=vocab, d=8, n_heads=2, n_kv=1, head_dim=8, layers=1, ffn=16, context=64)
+        with monkeypatch.context() as patch:
+            patch.setattr(torch, "device", lambda *a: device)
+            m = F.LlamaDevice(Ctx(), cfg, rows)
+        m.blocks = [dict.fromkeys(("qkv", "qkv_b", "o", "gate_up", "down", "attn_norm", "ffn_norm"),) |
+                    {"k": empty(8, device=device), "v": empty(8, device=device), "glu": False}]
+        m.head = m.tok_w = m.out_norm = None
+        m.calls = calls
+        return m
+
+    return make
+
+
+def ids(rows, n):
+    return torch.zeros((rows, n), dtype=torch.int32)
+
+
+def test_buffers_lie_on_the_models_device(model):
+    """(meta stands for a device that is not the current one)"""
+    m = model(2, device="meta")
+    m.verify_async(ids(2, 4), ids(2, 4), 4, 0)
+    assert m.zt.device.type == "meta"
+    for name, args in m.calls:
+        for t in args:
+            if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
+                assert t.device.type == "meta", name
+
+
+def test_a_prompts_buffers_lie_on_the_models_device(model):
+    m = model(2)
+    m.z = torch.zeros((2, 64))
+    m.prompt_async(ids(1, 5), [2, 3])
+    tensors = [t for _, args in m.calls for t in args if isinstance(t, torch.Tensor)]
+    assert len(tensors) > 20 and all(t.device.type == "cpu" for t in tensors)
