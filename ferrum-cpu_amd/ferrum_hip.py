@@ -1372,7 +1372,8 @@ class LlamaDevice:
         self._next_pos = self._next_used = 0
         self._used_given = False  # next_used was set since forward_one last went on
         self._ahead = None  # self.pos as forward_one or next_pos found it: prompts and trees go on at next_pos
-        self._trees, self._tree, self._planes = {}, None, None  # verify_async's buffers by size; the last call's
+        # verify_async's buffers, their first rows by a tree's size, and what its last call leaves for accept_async
+        self._tree_sets, self._tree_nodes, self._tree_views, self._tree, self._planes = [], 0, {}, None, None
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
         self.fused = 3 <= B <= 64 and self.d % 32 == 0
@@ -1810,10 +1811,11 @@ class LlamaDevice:
         parents (int32, [rows, n], on the device) hold the rows' trees one after the other.  Node 0
         is the token that the row goes on with (self.tokens of a plain step), node t > 0 a
         draft to follow node parents[t] < t of its tree.  Node t lies at cache row self.pos[r] + t
-        (a single row's self.pos goes to next_pos first, as for prompt_async)
-        and is seen by the nodes behind it; max_pos bounds self.pos.  The nodes' scores land in
-        self.zt [rows * n, vocab]; nothing is advanced (accept_async).  Nodes past the cache, or at
-        row max_pos + n or past it, get NaN scores and are not accepted."""
+        (a single row's self.pos goes to next_pos first, as for prompt_async) and is seen by the
+        nodes behind it; max_pos bounds self.pos.  The nodes' scores land in self.zt [rows * n,
+        vocab], which stays until the next call; nothing is advanced (accept_async).  Nodes past the
+        cache, or at row max_pos + n or past it, get NaN scores and are not accepted.  Run the
+        largest tree once before capturing any."""
         import torch
 
         if self.kv != "f32":
@@ -1824,16 +1826,7 @@ class LlamaDevice:
         for what, ids in (("tokens", tokens), ("parents", parents)):
             self._ids("verify_async", what, ids, total, f"{B} trees of {n}")
         self._go_on("verify_async")
-        dev = self.pos.device
-        if n not in self._trees:
-            ints = lambda m: torch.zeros(m, dtype=torch.int32, device=dev)  # noqa: E731
-            self._trees[n] = dict(self._row_buffers(total), z=torch.empty((total, self.vocab), device=dev),
-                                  path=ints(total), count=ints(B))
-            if self._planes is None:
-                self._planes = torch.tensor([b[c].data_ptr() for b in self.blocks for c in "kv"], dtype=torch.int64,
-                                            device=dev)
-            torch.cuda.synchronize(dev)
-        w = self._trees[n]
+        w = self._tree_views.get(n) or self._tree_buffers(n)
         max_keys = min(max_pos + n, self.cap)
 
         def attend(b):
@@ -1843,7 +1836,27 @@ class LlamaDevice:
 
         self._blocks_async(tokens, total, w, attend)
         linear_forward_async(ctx, self.head, w["h"], total, self.d, None, 0, w["z"])
-        self._tree, self.zt = (n, tokens, parents, max_keys), w["z"]
+        self._tree, self.zt = (n, tokens, parents, max_keys, w), w["z"]
+
+    def _tree_buffers(self, n: int) -> dict:
+        """Room for a tree of n nodes a row: the first rows of one set for all sizes, which grows
+        to twice its size at least.  What it grows out of stays: a captured graph may hold it."""
+        import torch
+
+        B, dev = self.rows, self.pos.device
+        if n > self._tree_nodes:
+            most = max(n, min(2 * self._tree_nodes, 1024))
+            ints = lambda m: torch.zeros(m, dtype=torch.int32, device=dev)  # noqa: E731
+            self._tree_sets.append(dict(self._row_buffers(B * most), z=torch.empty((B * most, self.vocab), device=dev),
+                                        path=ints(B * most), count=ints(B)))
+            if self._planes is None:
+                self._planes = torch.tensor([b[c].data_ptr() for b in self.blocks for c in "kv"], dtype=torch.int64,
+                                            device=dev)
+            torch.cuda.synchronize(dev)
+            self._tree_nodes, self._tree_views = most, {}
+        w = {name: t if name == "count" else t[:B * n] for name, t in self._tree_sets[-1].items()}
+        self._tree_views[n] = w
+        return w
 
     def accept_async(self, chosen):
         """After verify_async: follows each row's tree from node 0 along the drafts that equal
@@ -1856,8 +1869,8 @@ class LlamaDevice:
         (forward_one goes on from next_pos: set it to self.pos first.)"""
         if self._tree is None:
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
-        n, tokens, parents, max_keys = self._tree
-        total, w = self.rows * n, self._trees[n]
+        n, tokens, parents, max_keys, w = self._tree
+        total = self.rows * n
         self._ids("accept_async", "ids", chosen, total, f"{self.rows} trees of {n}")
         tree_accept_async(self.ctx, parents, tokens, chosen, total, None, self.rows, n, self.pos, self._planes,
                           2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos, max_keys)

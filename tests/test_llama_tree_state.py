@@ -52,6 +52,31 @@ def ids(rows, n):
     return torch.zeros((rows, n), dtype=torch.int32)
 
 
+def test_trees_of_every_size_share_one_set_of_buffers(model):
+    m = model(2)
+    seen = {}
+    for n in list(range(1, 65)) + list(range(64, 0, -1)):
+        m.verify_async(ids(2, n), ids(2, n), n, 0)
+        assert m.zt.shape == (2 * n, 64) and m.zt.is_contiguous()
+        m.accept_async(ids(2, n))
+        assert m.path.shape == (2, n) and m.count.shape == (2,)
+        seen[m.zt.untyped_storage().data_ptr()] = m.zt.untyped_storage().nbytes()
+    # sets that were grown out of stay (a captured graph may hold them): no more than the last one again
+    assert sum(seen.values()) <= 2 * max(seen.values())
+    assert max(seen.values()) <= 2 * 2 * 64 * 64 * 4
+    last = m.zt.untyped_storage().data_ptr()
+    m.verify_async(ids(2, 33), ids(2, 33), 33, 0)
+    assert m.zt.untyped_storage().data_ptr() == last
+
+
+def test_a_first_tree_has_what_it_needs_and_no_more(model):
+    m = model(2)
+    m.verify_async(ids(2, 5), ids(2, 5), 5, 0)
+    assert m.zt.untyped_storage().nbytes() == 2 * 5 * 64 * 4
+    m.verify_async(ids(2, 1024), ids(2, 1024), 1024, 0)
+    assert m.zt.untyped_storage().nbytes() == 2 * 1024 * 64 * 4
+
+
 def test_buffers_lie_on_the_models_device(model):
     """(meta stands for a device that is not the current one)"""
     m = model(2, device="meta")
