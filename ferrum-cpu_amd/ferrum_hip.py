@@ -1374,6 +1374,7 @@ class LlamaDevice:
         self._ahead = None  # self.pos as forward_one or next_pos found it: prompts and trees go on at next_pos
         # verify_async's buffers, their first rows by a tree's size, and what its last call leaves for accept_async
         self._tree_sets, self._tree_nodes, self._tree_views, self._tree, self._planes = [], 0, {}, None, None
+        self._held = []  # inputs of theirs that the stream may not have used yet
         self.blocks = []
         # the residual stream's row statistics between a projection and the next RmsNorm
         self.fused = 3 <= B <= 64 and self.d % 32 == 0
@@ -1743,6 +1744,7 @@ class LlamaDevice:
         dev = place.device  # (the model's: another may be the current one)
         ctx.sync()
         torch.cuda.synchronize(dev)
+        self._held.clear()
         max_keys = int((place.cpu().numpy().astype(np.int64) + n).max())
         if max_keys > self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
@@ -1815,7 +1817,9 @@ class LlamaDevice:
         nodes behind it; max_pos bounds self.pos.  The nodes' scores land in self.zt [rows * n,
         vocab], which stays until the next call; nothing is advanced (accept_async).  Nodes past the
         cache, or at row max_pos + n or past it, get NaN scores and are not accepted.  Run the
-        largest tree once before capturing any."""
+        largest tree once before capturing any.  The tokens and parents (and what accept_async
+        is given) have to be there for the context's stream: where another one writes them,
+        wait for it first."""
         import torch
 
         if self.kv != "f32":
@@ -1834,9 +1838,20 @@ class LlamaDevice:
                                           self.cap, None, n, self.pos, max_keys, parents, None, self.rope_dim, self.rope_base,
                                           self.rope_type, self.rope_freqs, self.rope_linear, w["att"])
 
+        self._hold(tokens, parents)
         self._blocks_async(tokens, total, w, attend)
         linear_forward_async(ctx, self.head, w["h"], total, self.d, None, 0, w["z"])
         self._tree, self.zt = (n, tokens, parents, max_keys, w), w["z"]
+
+    def _hold(self, *inputs):
+        """Keeps a call's inputs alive until the device has used them: until it has been waited for,
+        which every 64th such call does (a captured one's are the program's to keep)."""
+        import torch
+
+        if len(self._held) >= 64 and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.synchronize(self.pos.device)
+            self._held.clear()
+        self._held.append(inputs)
 
     def _tree_buffers(self, n: int) -> dict:
         """Room for a tree of n nodes a row: the first rows of one set for all sizes, which grows
@@ -1875,7 +1890,7 @@ class LlamaDevice:
         tree_accept_async(self.ctx, parents, tokens, chosen, total, None, self.rows, n, self.pos, self._planes,
                           2 * self.layers, self.kv_dim, self.cap, w["path"], w["count"], self.tokens, self.pos, max_keys)
         self.path, self.count, self._tree = w["path"].view(self.rows, n), w["count"], None
-        self._keep = (tokens, parents, chosen)  # alive until the stream has used them
+        self._hold(chosen)
 
     def evict_async(self, keep: int, recent: int):
         """Cuts every row's caches that hold more than `keep` keys to the last

@@ -15,11 +15,8 @@ CALLS = ("embed_rows_async", "rmsnorm_async", "linear_forward_async", "swiglu_as
 
 
 class Ctx:
-    def __init__(self):
-        self.waits = 0
-
     def sync(self):
-        self.waits += 1
+        pass
 
 
 @pytest.fixture
@@ -28,7 +25,8 @@ def model(monkeypatch):
     calls = []
     for name in CALLS:
         monkeypatch.setattr(F, name, lambda *a, _n=name, **k: calls.append((_n, a)))
-    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a, **k: None)
+    waits = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a, **k: waits.append(a))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a, **k: types.SimpleNamespace(synchronize=lambda: None))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(F.LlamaDevice, "_ids", lambda *a: None)
@@ -42,7 +40,7 @@ def model(monkeypatch):
         m.blocks = [dict.fromkeys(("qkv", "qkv_b", "o", "gate_up", "down", "attn_norm", "ffn_norm"),) |
                     {"k": empty(8, device=device), "v": empty(8, device=device), "glu": False}]
         m.head = m.tok_w = m.out_norm = None
-        m.calls = calls
+        m.calls, m.waits = calls, waits
         return m
 
     return make
@@ -75,6 +73,48 @@ def test_a_first_tree_has_what_it_needs_and_no_more(model):
     assert m.zt.untyped_storage().nbytes() == 2 * 5 * 64 * 4
     m.verify_async(ids(2, 1024), ids(2, 1024), 1024, 0)
     assert m.zt.untyped_storage().nbytes() == 2 * 1024 * 64 * 4
+
+
+def test_inputs_live_until_the_device_has_been_waited_for(model, monkeypatch):
+    m = model(2)
+    alive = []
+
+    def step():
+        given = [ids(2, 4) for _ in range(3)]
+        alive.extend(weakref.ref(t) for t in given)
+        m.verify_async(given[0], given[1], 4, 0)
+        m.accept_async(given[2])
+
+    step()
+    m.waits.clear()  # (the buffers')
+    for _ in range(20):
+        step()
+    m.calls.clear()
+    gc.collect()
+    assert not m.waits and all(r() is not None for r in alive)
+    for _ in range(500):
+        step()
+        m.calls.clear()
+    gc.collect()
+    # not for ever: what was kept goes when the device has been waited for
+    assert m.waits and sum(r() is not None for r in alive) <= 3 * 64
+    before = len(m.waits)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for _ in range(100):  # (in a capture nothing waits)
+        step()
+    assert len(m.waits) == before
+
+
+def test_a_tree_that_is_verified_again_keeps_the_first_ones_inputs(model):
+    m = model(1)
+    first = ids(1, 4)
+    ref = weakref.ref(first)
+    m.verify_async(first, ids(1, 4), 4, 0)
+    del first
+    m.verify_async(ids(1, 4), ids(1, 4), 4, 0)
+    m.calls.clear()
+    gc.collect()
+    assert ref() is not None
 
 
 def test_buffers_lie_on_the_models_device(model):
