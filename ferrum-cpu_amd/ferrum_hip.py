@@ -1607,7 +1607,7 @@ class LlamaDevice:
         """The next token of every row starts another text, in an empty cache."""
         import torch
 
-        self._used_given = False
+        self._used_given, self._tree = False, None
         self.next_pos = 0
         self.ctx.sync()
         self.pos.zero_()
@@ -1668,6 +1668,7 @@ class LlamaDevice:
         used = self._next_used if self.kv == "q4" else nxt
         if used >= self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
+        self._tree = None
         self.ctx.sync()
         self.tokens.fill_(int(token))
         self.pos.fill_(nxt)
@@ -1748,6 +1749,7 @@ class LlamaDevice:
         max_keys = int((place.cpu().numpy().astype(np.int64) + n).max())
         if max_keys > self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
+        self._tree = None
         ends = np.cumsum(n)
         off = torch.from_numpy(np.concatenate([[0], ends]).astype(np.int32)).to(dev)
         w = self._row_buffers(total)
@@ -1880,8 +1882,9 @@ class LlamaDevice:
         layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
         last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
         many they were.  Nodes that verify_async had no place for are not accepted: a count of 0
-        is a full cache (or a max_pos below self.pos - n).
-        (forward_one goes on from next_pos: set it to self.pos first.)"""
+        is a full cache (or a max_pos below self.pos - n).  A tree is left unaccepted where a
+        prompt, forward_one or reset comes between.  (forward_one goes on from next_pos: set it to
+        self.pos first.)"""
         if self._tree is None:
             raise FerrumHipError(FH_ERR_INVALID, "LlamaDevice.accept_async follows verify_async")
         n, tokens, parents, max_keys, w = self._tree

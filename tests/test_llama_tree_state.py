@@ -117,6 +117,22 @@ def test_a_tree_that_is_verified_again_keeps_the_first_ones_inputs(model):
     assert ref() is not None
 
 
+@pytest.mark.parametrize("between", ["reset", "forward_one", "prompt_async"])
+def test_what_moves_the_rows_ends_a_verified_tree(model, between, monkeypatch):
+    m = model(1)
+    m.z = torch.zeros((1, 64))
+    m.verify_async(ids(1, 4), ids(1, 4), 4, 0)
+    if between == "reset":
+        m.reset()
+    elif between == "forward_one":
+        m.forward_one(3)
+    else:
+        monkeypatch.setattr(torch.Tensor, "cuda", lambda t: t)
+        m.prompt_async(ids(1, 4), [4])
+    with pytest.raises(F.FerrumHipError, match="follows verify_async"):
+        m.accept_async(ids(1, 4))
+
+
 def test_buffers_lie_on_the_models_device(model):
     """(meta stands for a device that is not the current one)"""
     m = model(2, device="meta")
