@@ -1768,8 +1768,10 @@ class LlamaDevice:
                                                  b["v"], B, self.cap, off, most, self.pos, max_keys, None, self.rope_dim,
                                                  self.rope_base, self.rope_type, self.rope_freqs, self.rope_linear, w["att"])
         torch.cuda.synchronize(dev)
-        self._blocks_async(tokens, total, w, attend)
-        ctx.sync()
+        try:
+            self._blocks_async(tokens, total, w, attend)
+        finally:
+            ctx.sync()  # (the buffers end with this call, also where a block was refused)
         last = w["h"][torch.from_numpy(ends - 1).to(dev)].contiguous()
         torch.cuda.synchronize(dev)
         linear_forward_async(ctx, self.head, last, B, self.d, None, 0, self.z)

@@ -15,8 +15,11 @@ CALLS = ("embed_rows_async", "rmsnorm_async", "linear_forward_async", "swiglu_as
 
 
 class Ctx:
+    def __init__(self, calls):
+        self.calls = calls
+
     def sync(self):
-        pass
+        self.calls.append(("sync", ()))
 
 
 @pytest.fixture
@@ -36,7 +39,7 @@ def model(monkeypatch):
         cfg = dict(vocab=vocab, d=8, n_heads=2, n_kv=1, head_dim=8, layers=1, ffn=16, context=64)
         with monkeypatch.context() as patch:
             patch.setattr(torch, "device", lambda *a: device)
-            m = F.LlamaDevice(Ctx(), cfg, rows)
+            m = F.LlamaDevice(Ctx(calls), cfg, rows)
         m.blocks = [dict.fromkeys(("qkv", "qkv_b", "o", "gate_up", "down", "attn_norm", "ffn_norm"),) |
                     {"k": empty(8, device=device), "v": empty(8, device=device), "glu": False}]
         m.head = m.tok_w = m.out_norm = None
@@ -150,3 +153,19 @@ def test_a_prompts_buffers_lie_on_the_models_device(model):
     m.prompt_async(ids(1, 5), [2, 3])
     tensors = [t for _, args in m.calls for t in args if isinstance(t, torch.Tensor)]
     assert len(tensors) > 20 and all(t.device.type == "cpu" for t in tensors)
+
+
+@pytest.mark.parametrize("where", ["gqa_attention_rope_prefill_async", "swiglu_async"])
+def test_a_prompt_that_a_block_refuses_waits_for_what_runs(model, monkeypatch, where):
+    """(its buffers go back to torch when it ends)"""
+    m = model(2)
+    m.z = torch.zeros((2, 64))
+
+    def refuse(*a):
+        raise F.FerrumHipError(F.FH_ERR_LIMIT, "no")
+
+    monkeypatch.setattr(F, where, refuse)
+    with pytest.raises(F.FerrumHipError, match="no"):
+        m.prompt_async(ids(1, 5), [2, 3])
+    names = [name for name, _ in m.calls]
+    assert "embed_rows_async" in names and names[-1] == "sync"
