@@ -1628,28 +1628,31 @@ class LlamaDevice:
             self.pos.fill_(pos)
             self.used.fill_(used)
             torch.cuda.current_stream().synchronize()
-        self._leave()
+        elif self.kv == "f32" and self.rows == 1:
+            self._ahead = None
+            if not torch.cuda.is_current_stream_capturing():
+                self.ctx.sync()
+                self._leave(int(self.pos[0]))
 
-    def _leave(self, fed=None):
-        """Over an f32 cache self.pos is left to the program (where it steps by it, forward_one's
-        last place, `fed`, is the one that it counts from)."""
+    def _leave(self, pos: int):
+        """Over an f32 cache self.pos, which is at `pos`, is left to the program that steps by it."""
         ours = self.kv == "f32" and self.rows == 1 and not self.pos.is_inference()
-        self._ahead = (self.pos, self.pos._version, fed) if ours else None
+        self._ahead = (self.pos, self.pos._version, pos) if ours else None
 
     def _go_on(self, who: str):
-        """self.pos at next_pos, where forward_one or next_pos came last and it was not written since
-        (by torch; or by a replayed graph, behind forward_one)."""
+        """self.pos at next_pos, where forward_one or next_pos came last and it was not written since,
+        by torch or (which its value alone shows) by a replayed graph."""
         import torch
 
         if self._ahead is None:
             return
-        pos, version, fed = self._ahead
+        pos, version, at = self._ahead
         if self.pos is pos and pos._version == version:
             if torch.cuda.is_current_stream_capturing():
                 raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: forward_one or next_pos came last: write self.pos "
                                                      "before the capture")
             self.ctx.sync()
-            if fed is None or int(pos[0]) == fed:
+            if int(pos[0]) == at:
                 pos.fill_(self._next_pos)
             torch.cuda.synchronize(pos.device)
         self._ahead = None

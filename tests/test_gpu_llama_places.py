@@ -146,3 +146,69 @@ def test_a_place_that_a_graph_moved_counts(fh, orc):
     fh.sync()
     assert close(m.z[0].cpu().numpy(), want[11])
     m.free()
+
+
+@pytest.mark.parametrize("how", ["forward_one", "next_pos"])
+def test_a_place_that_replayed_trees_moved_counts(fh, orc, how):
+    """A captured step of trees, replayed behind forward_one or next_pos: a prompt goes on where it left off."""
+    import torch
+
+    cfg, w, m = build(fh, orc, "qwen", 1)
+    ids = np.random.default_rng(55).integers(0, cfg["vocab"], 24)
+    want = fed(orc, w, cfg, ids)
+    tokens, parents, chosen = ints([0, 0]), ints([-1, 0]), ints([0, 0])
+    m.verify_async(tokens, parents, 2, 30)
+    m.accept_async(chosen)
+    fh.sync()
+    m.reset()
+    for t in range(4):
+        m.forward_one(int(ids[t]))
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    m.pos.fill_(4)
+    torch.cuda.synchronize()
+    fh.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            m.verify_async(tokens, parents, 2, 30)
+            m.accept_async(chosen)
+    finally:
+        fh.set_stream(None)
+    if how == "forward_one":
+        m.next_pos = 3
+        m.forward_one(int(ids[3]))
+        m.pos.fill_(4)
+    else:
+        m.pos.fill_(4)
+        torch.cuda.synchronize()
+        m.next_pos = 2
+    for t in (4, 6, 8):
+        tokens.copy_(ints(ids[t:t + 2]))
+        chosen.copy_(ints([ids[t + 1], ids[t + 2]]))
+        graph.replay()
+        torch.cuda.synchronize()
+    assert m.pos.tolist() == [10]
+    m.prompt_async(ints(ids[10:16]), [6])
+    fh.sync()
+    assert close(m.z[0].cpu().numpy(), want[15])
+    m.free()
+
+
+def test_a_capture_refuses_a_place_that_is_not_written(fh, orc):
+    import ferrum_hip
+    import torch
+
+    cfg, w, m = build(fh, orc, "qwen", 1)
+    ids = ints([1, 2])
+    m.verify_async(ids, ints([-1, 0]), 2, 10)
+    fh.sync()
+    m.forward_one(3)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    fh.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            torch.zeros(1, device="cuda")
+            with pytest.raises(ferrum_hip.FerrumHipError, match="before the capture"):
+                m.verify_async(ids, ids, 2, 10)
+    finally:
+        fh.set_stream(None)
+    m.free()

@@ -169,3 +169,16 @@ def test_a_prompt_that_a_block_refuses_waits_for_what_runs(model, monkeypatch, w
         m.prompt_async(ids(1, 5), [2, 3])
     names = [name for name, _ in m.calls]
     assert "embed_rows_async" in names and names[-1] == "sync"
+
+
+def test_a_model_made_in_inference_mode_sees_what_is_written(model):
+    with torch.inference_mode():
+        m = model(1)
+        m.z = torch.zeros((1, 64))
+        m.forward_one(5)
+        m.pos.fill_(7)
+        m.verify_async(ids(1, 2), ids(1, 2), 2, 9)
+        assert m.pos.tolist() == [7]
+        m.next_pos = 3
+        m.verify_async(ids(1, 2), ids(1, 2), 2, 9)
+        assert m.pos.tolist() == [3]
