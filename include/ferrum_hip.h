@@ -567,12 +567,20 @@ int fh_kv4_read_async(fh_ctx* ctx, const fh_kv4_cache* cache, const uint32_t* d_
  * gets NaN and is not stored.  Positions are below 2^31.
  *
  * head_dim 8, 16, 32, 64 or 128, else FH_ERR_LIMIT; caches and d_out 16-byte aligned.
- * Within 1e-5 of float64 over the same rotated rows, against each output's sum of
- * weight * the value row's largest magnitude (operands as two f16 terms under a power of
- * two of each row's own: value rows from 2^-86 to 2^27 may be mixed freely).  A query, a
- * key or a value row with a number that is not finite makes NaN of every channel of the
- * outputs that see it, and of no others.  A call of the same arguments gives the same bits;
- * another max_rows or max_keys may share the keys out differently.  Errors otherwise
+ * Accuracy: operands are two f16 terms (22 bits) under a power of two of each row's own, the
+ * product of the lower terms is left out, sums are f32.  Against float64 over the same
+ * rotated rows an output is off by no more than
+ *   m (2 d + 3 * 2^-22 + (6 ceil(keys / 32) + 16 + min(keys, 64)) 2^-24),
+ *   d = S (2^-20 + (3 head_dim / 16 + 4) 2^-24),
+ * m its sum of weight * the value row's largest magnitude (a channel far below that is held to
+ * it, not to itself), S the largest sum of |q k| / sqrt(head_dim) of a key that it sees: every
+ * rounding at its worst.  Rows of unit normal numbers are within 1e-5 of m.  This is for queries
+ * and keys from 2^-46 (lower ones lose bits) to 2^100 whose scores f32 holds, and for value rows
+ * from 2^-86 to 2^27 and zeros, which may be mixed freely; where value rows meet that differ by
+ * more than 2^113 (zeros count as 2^-86), the weights of the smaller underflow and are missing
+ * from the sums.  A query, a key or a value row with a number that is not finite makes NaN of
+ * every channel of the outputs that see it, and of no others.  A call of the same arguments
+ * gives the same bits; another max_rows or max_keys may share the keys out differently.  Errors otherwise
  * as fh_gqa_attention_rope_decode_async's.  The context's workspace for these calls grows
  * outside graph capture only and is never freed before the context ends, so captured
  * graphs stay valid; calls of one context must not overlap, replayed graphs included. */
