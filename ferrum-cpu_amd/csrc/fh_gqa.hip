@@ -620,7 +620,7 @@ __device__ __forceinline__ void store_out(const Sums<W / 32>& z, const RowsArgs&
 // The vector units bound it: a tile of 32 keys of width 64 is some 300 instructions a wave (half of them for the
 // staging) beside 24 products, and the two times add up.  32 trees of up to 32 nodes over up to 1023 rows, 14 and
 // 2 heads: 30.1 us, about 6 until the first tile is staged, 2 a tile, 5 to join four shares.  4 trees of up to 64
-// nodes over up to 16383 rows, 32 and 8 heads of width 128: 203 us a call, 2.2 TB/s of the cache and 222 TFLOP/s (three
+// nodes over up to 16383 rows, 32 and 8 heads of width 128: 198 us a call, 2.2 TB/s of the cache and 228 TFLOP/s (three
 // times that of f16 products).  Scores of tile t + 1 are multiplied while tile t's become weights (when this was added 40.7
 // to 34.5 and 399 to 283 us).
 template <int W, int CW, int KW>
@@ -971,7 +971,10 @@ __global__ void __launch_bounds__(64 * CW * KW, 2) k_gqa_rows(RowsArgs a) {
     if (b.place(a, blockIdx.x)) rows_block<W, CW, KW, TREE>(a, smem, b);
 }
 
-// The blocks that k_gqa_prompt leaves out, if there are any.
+// The blocks that k_gqa_prompt leaves out, if there are any: slower than if nothing had been packed, since a workgroup
+// takes every num_cus-th block and a kv head's are every n_kv-th, so that one head keeps one workgroup in n_kv busy (us with no
+// row apart, a row of one kv head, rows of all, and nothing packed: 1 x 8192 rows, 32 and 8 heads of width 128 1442, 3300,
+// 2000 and 1655 to 1860; 16 x <= 1000, 14 and 2 heads of 64 90, 305, 260 and 107 to 114).
 template <int W, int CW>
 __global__ void __launch_bounds__(64 * CW, 2) k_gqa_rest(RowsArgs a, uint32_t blocks) {
     extern __shared__ __align__(16) char smem[];
@@ -1131,7 +1134,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_pack(PackArgs a) {
 // NWV waves of 32 columns a workgroup.  Step t multiplies tile t + 1's scores while tile t's become
 // weights, and stages tile t + 2's keys and t + 1's values, so that a wave has work for the matrix and
 // for the vector units side by side.  Width 128: eight waves, near the rate of a large f16 product (1 x 8192
-// rows of 32 and 8 heads 1460 us, 377 TFLOP/s or 1130 of f16 products; the clock falls as the matrix
+// rows of 32 and 8 heads 1420 us, 387 TFLOP/s or 1160 of f16 products; the clock falls as the matrix
 // units fill: 2.1 GHz where they were busy 40 % of the time, 1.7 at 60 %; four waves, each tile read
 // twice as often, 1557); 64: four, three to a SIMD (16 prompts of up to 1000 rows, 14 and 2 heads, 73
 // us, two to a SIMD 77, eight waves 90).  64 columns a wave with a SIMD to itself: 2000 and 125.
@@ -1301,6 +1304,8 @@ int launch_prompt(fh_ctx* ctx, const RowsArgs& a, const PackArgs& p, uint32_t wo
     return FH_OK;
 }
 
+// (k_gqa_rows<128, 4, 1, ..> keeps 8 registers in scratch, 36 bytes a thread, since keys' pieces and values' groups have
+// banks of their own; <128, 8, 1, ..> and the narrower ones none.)
 template <int W, bool TREE>
 int launch_width(fh_ctx* ctx, const RowsArgs& a, uint32_t workgroups, int cw) {
     if constexpr (W == 128) return cw == 8 ? launch_rows<W, 8, 1, TREE>(ctx, a, workgroups) : launch_rows<W, 4, 1, TREE>(ctx, a, workgroups);
@@ -1318,7 +1323,9 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     // blocks read the same tiles and there are enough of both (us packed and not, heads of width 64: 1 prompt of 1000
     // rows, 14 and 2 heads 41 and 32, of 2000 55 and 56; 16 of up to 1000 rows 91 and 107; 8 of up to 1000, 12 and 12
     // heads 81 and 72; of width 128, 32 and 8 heads: 1 prompt of 1000 rows 66 and 63, of 1500 106 and 112, of 2000 168
-    // and 190).
+    // and 190).  Not in a room of 2 GiB and more, which would stay with the context, and be twice as large where it grows, for
+    // little (ms packed and not, those heads: 24 prompts of 512 rows behind 15872, 3 GiB, 10.4 and 10.4, 32 of 1024 behind
+    // 7168, 2 GiB, 12.9 and 13.8, 16 of 2048 behind 14336, 2 GiB, 23.0 and 25.6).
     const bool prompt = !g.parent && cols > 1024 && heads * cols * tiles > (size_t(3) << 19) && pack < (size_t(1) << 31);
     // Columns of a workgroup: as many as there are, while two workgroups fit a compute unit; of 64 columns and two waves that deal
     // the keys for small calls (us of 64 and of 128: one tree of 100 nodes over 4000 rows, 4 heads of width 32 24.4 and
@@ -1332,8 +1339,12 @@ int fh_launch_gqa_rows(fh_ctx* ctx, const fh_gqa_call& g) {
     // least (those 4 trees, when this was added: 215 us, 283 with equal numbers of shares for all sequences).
     const size_t cus = static_cast<size_t>(ctx->num_cus), units = g.seqs * blocks;
     // Where a compute unit has 16 tiles at most, one workgroup on each: two would meet on some while others had none (us
-    // with one and with two: a tree of 16 nodes over 16000 rows, 14 and 2 heads 33 and 39, a prompt of 64 rows over 4000
-    // 31 and 39; 32 trees of up to 32 nodes over up to 1023, 17 tiles each, 40 and 36).
+    // with one and with two, 14 and 2 heads of width 64: a tree of 16 nodes over 16000 rows, 8 tiles each, 34 and 39,
+    // over 30000, 15 tiles, 41 and 44, over 36000, 18 tiles, 44 and 47; 8 trees of 32 nodes over up to 2000, 8 tiles, 30 and
+    // 33, over up to 4000, 16 tiles, 39 and 40, over up to 5000, 20 tiles, 44 and 43; 32 and 8 heads of 128: 4 of 32 over up
+    // to 3000, 12 tiles, 58 and 64, over up to 5000, 20 tiles, 72 and 74).  With as many blocks as fill half of the device
+    // by themselves the two meet sooner: 32 trees of up to 32 nodes over up to 511, 8 tiles, 29 and 29, over up to 767, 12
+    // tiles, 35 and 33, over up to 960, 15 tiles, 39 and 35, over up to 1023, 17 tiles, 40 and 36.
     const bool few = units * tiles * g.n_kv <= 16 * cus;
     const size_t all = cus * (cw == 8 || few ? 1 : prompt ? 3 : 2), places = all / g.n_kv;
     const bool planned = units <= std::min<size_t>(places, kPlanned) && tiles >= 4;
