@@ -1639,22 +1639,31 @@ class LlamaDevice:
         ours = self.kv == "f32" and self.rows == 1 and not self.pos.is_inference()
         self._ahead = (self.pos, self.pos._version, pos) if ours else None
 
-    def _go_on(self, who: str):
-        """self.pos at next_pos, where forward_one or next_pos came last and it was not written since,
-        by torch or (which its value alone shows) by a replayed graph."""
+    def _goes_on(self, who: str) -> bool:
+        """Whether a prompt or tree goes on at next_pos: forward_one or next_pos came last and
+        self.pos was not written since, by torch or (which its value alone shows) by a replayed
+        graph."""
         import torch
 
         if self._ahead is None:
-            return
+            return False
         pos, version, at = self._ahead
-        if self.pos is pos and pos._version == version:
-            if torch.cuda.is_current_stream_capturing():
-                raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: forward_one or next_pos came last: write self.pos "
-                                                     "before the capture")
-            self.ctx.sync()
-            if int(pos[0]) == at:
-                pos.fill_(self._next_pos)
-            torch.cuda.synchronize(pos.device)
+        if self.pos is not pos or pos._version != version:
+            self._ahead = None
+            return False
+        if torch.cuda.is_current_stream_capturing():
+            raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: forward_one or next_pos came last: write self.pos "
+                                                 "before the capture")
+        self.ctx.sync()
+        return int(pos[0]) == at
+
+    def _go_on(self, who: str):
+        """self.pos at next_pos, where the call goes on there."""
+        import torch
+
+        if self._goes_on(who):
+            self.pos.fill_(self._next_pos)
+            torch.cuda.synchronize(self.pos.device)
         self._ahead = None
 
     def forward_one(self, token: int):
@@ -1743,16 +1752,17 @@ class LlamaDevice:
             raise FerrumHipError(FH_ERR_INVALID, f"LlamaDevice.{who}: {B} lengths of at least 1")
         total, most = int(n.sum()), int(n.max())
         self._ids(who, "tokens", tokens, total, f"{total} places")
-        self._go_on(who)
         place = self.used if self.kv == "q4" else self.pos
         dev = place.device  # (the model's: another may be the current one)
         ctx.sync()
         torch.cuda.synchronize(dev)
         self._held.clear()
-        max_keys = int((place.cpu().numpy().astype(np.int64) + n).max())
+        at = self._next_pos if self._goes_on(who) else place.cpu().numpy().astype(np.int64)
+        max_keys = int((at + n).max())
         if max_keys > self.cap:
             raise DimMismatch(FH_ERR_DIM, f"KvCache full ({self.cap} positions): clear and re-prime to continue")
         self._tree = None
+        self._go_on(who)
         ends = np.cumsum(n)
         off = torch.from_numpy(np.concatenate([[0], ends]).astype(np.int32)).to(dev)
         w = self._row_buffers(total)
@@ -1836,8 +1846,8 @@ class LlamaDevice:
         ctx, B, total = self.ctx, self.rows, self.rows * n
         for what, ids in (("tokens", tokens), ("parents", parents)):
             self._ids("verify_async", what, ids, total, f"{B} trees of {n}")
-        self._go_on("verify_async")
         w = self._tree_views.get(n) or self._tree_buffers(n)
+        self._go_on("verify_async")
         max_keys = min(max_pos + n, self.cap)
 
         def attend(b):
@@ -1887,7 +1897,7 @@ class LlamaDevice:
         layer, self.pos advances by their number, self.tokens becomes the id chosen behind the
         last; self.path [rows, n] (-1 behind the last) and self.count [rows] say which and how
         many they were.  Nodes that verify_async had no place for are not accepted: a count of 0
-        is a full cache (or a max_pos below self.pos - n).  A tree is left unaccepted where a
+        is a full cache (or a max_pos of self.pos - n or less).  A tree is left unaccepted where a
         prompt, forward_one or reset comes between.  (forward_one goes on from next_pos: set it to
         self.pos first.)"""
         if self._tree is None:

@@ -182,3 +182,18 @@ def test_a_model_made_in_inference_mode_sees_what_is_written(model):
         m.next_pos = 3
         m.verify_async(ids(1, 2), ids(1, 2), 2, 9)
         assert m.pos.tolist() == [3]
+
+
+def test_a_prompt_that_does_not_fit_leaves_the_place(model):
+    """forward_one's place is the program's to step by, also behind a prompt that was refused."""
+    m = model(1)
+    m.z = torch.zeros((1, 64))
+    for t in range(60):
+        m.forward_one(t)
+    with pytest.raises(F.DimMismatch, match="KvCache full"):
+        m.prompt_async(ids(1, 5), [5])  # (4 places are left)
+    assert m.pos.tolist() == [59] and m.next_pos == 60
+    m.prompt_async(ids(1, 4), [4])
+    assert m.pos.tolist() == [60]
+    prompts = [args for name, args in m.calls if name == "gqa_attention_rope_prefill_async"]
+    assert len(prompts) == 1 and prompts[0][14] == 64  # (max_keys)
